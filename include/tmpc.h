@@ -587,6 +587,99 @@ int tmpc_linesearch_choose_f64(hipStream_t stream, int32_t B, int32_t A, const d
                                const double* iq_a, const double* alphas, double eta, double mu_min,
                                double mu_max, double floor_, double* alpha_out, double* mu_out);
 
+/* --- operators of a learned model upstream of the differentiable solve ---
+ * A history model (turbompc_amd.learning) turns what a problem's vehicle has
+ * seen into the tracking weights of its solve.  Its arrays are fp32 (*_f32) or
+ * bfloat16 (*_bf16), row-major with contiguous rows; states, statistics and
+ * sums are fp32 in both.  Pointers are aligned to their element.  Nothing is
+ * read from masked places (steps past a length, idle problems), whatever they
+ * hold.  Sums run in a fixed order: equal inputs give equal bits. */
+
+/* Root-mean-square norm with the residual's addition, over rows of 1 <= width <= 8192:
+ * s = x + residual, rstd = (mean s^2 + eps)^-1/2, y = s rstd weight.  x and
+ * residual (or NULL: zero) have row pitches ldx, ldr; y and s (or NULL) are
+ * contiguous; rstd (rows, or NULL) is what the backward pass reads. */
+int tmpc_rms_norm_forward_f32(hipStream_t stream, int64_t rows, int32_t width, const void* x, int64_t ldx,
+                              const void* residual, int64_t ldr, const void* weight, double eps, void* y, void* s,
+                              float* rstd);
+int tmpc_rms_norm_forward_bf16(hipStream_t stream, int64_t rows, int32_t width, const void* x, int64_t ldx,
+                               const void* residual, int64_t ldr, const void* weight, double eps, void* y, void* s,
+                               float* rstd);
+/* Its gradients from dy (pitch lddy), ds (pitch ldds, or NULL: zero), s (pitch
+ * lds) and rstd: dx (rows, width), also the residual's, and dweight (width). */
+size_t tmpc_rms_norm_backward_workspace_bytes(int elem_bytes, int64_t rows, int32_t width);
+int tmpc_rms_norm_backward_f32(hipStream_t stream, int64_t rows, int32_t width, const void* dy, int64_t lddy,
+                               const void* ds, int64_t ldds, const void* s, int64_t lds, const void* weight,
+                               const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes);
+int tmpc_rms_norm_backward_bf16(hipStream_t stream, int64_t rows, int32_t width, const void* dy, int64_t lddy,
+                                const void* ds, int64_t ldds, const void* s, int64_t lds, const void* weight,
+                                const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes);
+
+/* Linear attention with a decay for each head: for problem b and head h, with
+ * g = log_decay[h] <= 0 and t < lengths[b] (clamped to 0..T; NULL: T)
+ *   S_t = e^g S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,  S_{-1} = state_in (or zero);
+ * steps past the length give o = 0 and leave the state.  H is a multiple of
+ * Hk; head h reads key/value head h / (H / Hk).  1 <= dk, dv <= 128.  q (B, T,
+ * H, dk), k (B, T, Hk, dk), v (B, T, Hk, dv) have contiguous rows and the given
+ * strides (elements) of problem, step and head. */
+typedef struct tmpc_decay_attention {
+  int32_t B, T, H, Hk, dk, dv;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const float* log_decay;  /* (H) */
+  const int32_t* lengths;  /* (B) or NULL */
+  const float* state_in;   /* (B, H, dk, dv) or NULL */
+  double scale;
+} tmpc_decay_attention;
+size_t tmpc_decay_attention_workspace_bytes(int elem_bytes, const tmpc_decay_attention* args, int backward);
+/* o (B, T, H, dv) and state_out (B, H, dk, dv, or NULL), contiguous. */
+int tmpc_decay_attention_forward_f32(hipStream_t stream, const tmpc_decay_attention* args, void* o, float* state_out,
+                                     void* workspace, size_t workspace_bytes);
+int tmpc_decay_attention_forward_bf16(hipStream_t stream, const tmpc_decay_attention* args, void* o,
+                                      float* state_out, void* workspace, size_t workspace_bytes);
+/* Gradients from those of o (d_o, strides d_o_stride) and of the final state
+ * (d_state_out, or NULL: zero): dq (B, T, H, dk), dk (B, T, Hk, dk), dv (B, T,
+ * Hk, dv) and d_state_in (B, H, dk, dv, or NULL), contiguous.  log_decay is a
+ * constant.  The state is formed again; nothing of the forward call is kept. */
+int tmpc_decay_attention_backward_f32(hipStream_t stream, const tmpc_decay_attention* args, const void* d_o,
+                                      const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,
+                                      void* dv, float* d_state_in, void* workspace, size_t workspace_bytes);
+int tmpc_decay_attention_backward_bf16(hipStream_t stream, const tmpc_decay_attention* args, const void* d_o,
+                                       const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,
+                                       void* dv, float* d_state_in, void* workspace, size_t workspace_bytes);
+/* One step (T = 1; lengths and state_in are not read): state (B, H, dk, dv) is
+ * updated in place, o (B, H, dv).  Where active (B bytes, or NULL: all) is 0, o
+ * is 0 and the state stays. */
+int tmpc_decay_attention_step_f32(hipStream_t stream, const tmpc_decay_attention* args, const uint8_t* active,
+                                  float* state, void* o);
+int tmpc_decay_attention_step_bf16(hipStream_t stream, const tmpc_decay_attention* args, const uint8_t* active,
+                                   float* state, void* o);
+
+/* Gated feed-forward block: y = (act(x w_gate^T) o (x w_up^T)) w_down^T for
+ * rows x (M, D) of pitch ldx, w_gate, w_up (F, D), w_down (Dout, F) contiguous;
+ * activation 0: silu, 1: gelu (exact). */
+typedef struct tmpc_gated_ff {
+  int64_t M;
+  int32_t D, F, Dout, activation;
+  const void* x;
+  int64_t ldx;
+  const void *w_gate, *w_up, *w_down;
+} tmpc_gated_ff;
+size_t tmpc_gated_ff_workspace_bytes(int elem_bytes, const tmpc_gated_ff* args, int backward);
+/* y (M, Dout); gate, up (M, F), fp32: the projections, which the backward pass
+ * reads (both or neither NULL). */
+int tmpc_gated_ff_forward_f32(hipStream_t stream, const tmpc_gated_ff* args, void* y, float* gate, float* up,
+                              void* workspace, size_t workspace_bytes);
+int tmpc_gated_ff_forward_bf16(hipStream_t stream, const tmpc_gated_ff* args, void* y, float* gate, float* up,
+                               void* workspace, size_t workspace_bytes);
+/* Gradients from dy (pitch lddy): dx (M, D), dw_gate, dw_up (F, D), dw_down (Dout, F). */
+int tmpc_gated_ff_backward_f32(hipStream_t stream, const tmpc_gated_ff* args, const float* gate, const float* up,
+                               const void* dy, int64_t lddy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                               void* workspace, size_t workspace_bytes);
+int tmpc_gated_ff_backward_bf16(hipStream_t stream, const tmpc_gated_ff* args, const float* gate, const float* up,
+                                const void* dy, int64_t lddy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                                void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

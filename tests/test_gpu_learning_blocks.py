@@ -1,0 +1,210 @@
+"""The gated feed-forward block and the root-mean-square norm (turbompc_amd.learning)
+against their definitions in 64 bits."""
+import pytest
+import torch
+
+import learning_reference as ref
+from turbompc_amd import learning
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def ff_inputs(M, D, F, Dout, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s, std=1.0: (torch.randn(s, generator=gen) * std).to(dtype).to(DEV)  # noqa: E731
+    return dict(x=r(M, D), wg=r(F, D, std=D ** -0.5), wu=r(F, D, std=D ** -0.5), wd=r(Dout, F, std=F ** -0.5),
+                dy=r(M, Dout))
+
+
+def ff_run(x, act):
+    leaf = {k: x[k].detach().requires_grad_(True) for k in ("x", "wg", "wu", "wd")}
+    y = learning.gated_feed_forward(*leaf.values(), act)
+    out = {"y": y.detach()}
+    out.update({"d" + k: t for k, t in zip(leaf, torch.autograd.grad(y, list(leaf.values()), x["dy"]))})
+    return out
+
+
+FF = [  # M, D, F, Dout
+    (1, 1, 1, 1), (1, 64, 96, 64), (5, 33, 57, 33), (16, 128, 64, 40), (64, 256, 683, 256), (130, 72, 200, 72),
+    (129, 129, 130, 131), (200, 64, 128, 17), (1500, 40, 72, 40), (300, 520, 260, 520),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("shape", FF, ids=lambda s: "x".join(map(str, s)))
+def test_feed_forward(shape, act, dtype):
+    x = ff_inputs(*shape, dtype, seed=sum(shape))
+    got = ff_run(x, act)
+    for k, (v, tol) in ref.feed_forward(x["x"], x["wg"], x["wu"], x["wd"], act, x["dy"]).items():
+        ref.assert_within(k, got[k], v, tol)
+    with torch.no_grad():  # without the saved projections: the same numbers
+        assert torch.equal(learning.gated_feed_forward(x["x"], x["wg"], x["wu"], x["wd"], act), got["y"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_feed_forward_large_activations(dtype):
+    """Gates far on either side, where the exponential over- or underflows."""
+    x = ff_inputs(40, 16, 48, 16, dtype, seed=1)
+    x["wg"] = x["wg"] * 100
+    for act in ("silu", "gelu"):
+        got = ff_run(x, act)
+        for k, (v, tol) in ref.feed_forward(x["x"], x["wg"], x["wu"], x["wd"], act, x["dy"]).items():
+            ref.assert_within(k, got[k], v, tol)
+
+
+def test_feed_forward_strides_and_leading_axes():
+    x = ff_inputs(24, 40, 72, 40, torch.bfloat16, seed=2)
+    wide = torch.zeros((2, 12, 90), dtype=torch.bfloat16, device=DEV)
+    wide[..., 3:43] = x["x"].view(2, 12, 40)
+    want = ff_run(x, "silu")
+    got = ff_run(dict(x, x=wide[..., 3:43], wg=x["wg"].t().contiguous().t(), dy=x["dy"].view(2, 12, 40)), "silu")
+    assert got["y"].shape == (2, 12, 40) and got["dx"].shape == (2, 12, 40)
+    for k in want:
+        assert torch.equal(got[k].reshape(want[k].shape), want[k]), k
+    # a broadcast gradient (the sum of y) as a full one
+    ones = dict(x, dy=torch.ones((), dtype=torch.bfloat16, device=DEV).expand(24, 40))
+    a, b = ff_run(ones, "gelu"), ff_run(dict(x, dy=torch.ones_like(x["dy"])), "gelu")
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+
+
+def test_feed_forward_gradients_against_differences():
+    """y is linear in w_up and w_down: differences of any width are exact up to rounding."""
+    x = ff_inputs(60, 48, 80, 48, torch.float32, seed=3)
+    got = ff_run(x, "silu")
+    loss = lambda y: float((learning.gated_feed_forward(y["x"], y["wg"], y["wu"], y["wd"]).double()  # noqa: E731
+                            * x["dy"].double()).sum())
+    want = ref.feed_forward(x["x"], x["wg"], x["wu"], x["wd"], "silu")["y"]
+    noise = float((want[1] * ref.cpu64(x["dy"]).abs()).sum())
+    for k in ("wu", "wd"):
+        d = torch.randn(x[k].shape, generator=torch.Generator().manual_seed(4)).to(DEV) * x[k].std()
+        diff = (loss(dict(x, **{k: x[k] + d})) - loss(dict(x, **{k: x[k] - d}))) / 2
+        exact = float((got["d" + k].double() * d.double()).sum())
+        assert abs(diff - exact) <= 4 * noise, (k, diff, exact)
+    for k in ("x", "wg"):  # width h: the truncation falls with h^2, so a third of it with h / sqrt 3
+        d = torch.randn(x[k].shape, generator=torch.Generator().manual_seed(5)).to(DEV) * x[k].std()
+        exact = float((got["d" + k].double() * d.double()).sum())
+        diff = [(loss(dict(x, **{k: x[k] + h * d})) - loss(dict(x, **{k: x[k] - h * d}))) / (2 * h) for h in (0.04, 0.02)]
+        extrapolated = (4 * diff[1] - diff[0]) / 3
+        assert abs(extrapolated - exact) <= 4 * noise / 0.02 + abs(diff[1] - diff[0]), (k, diff, exact)
+
+
+def test_feed_forward_empty_batch():
+    x = ff_inputs(0, 16, 24, 16, torch.bfloat16)
+    got = ff_run(x, "silu")
+    assert got["y"].shape == (0, 16) and not got["dwg"].any() and not got["dwu"].any() and not got["dwd"].any()
+
+
+def test_feed_forward_bits_and_graph():
+    x = ff_inputs(700, 64, 96, 64, torch.bfloat16, seed=6)
+    a, b = ff_run(x, "silu"), ff_run(x, "silu")
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+    xs = x["x"].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = learning.gated_feed_forward(xs, x["wg"], x["wu"], x["wd"])
+        n, s = learning.rms_norm_residual(xs, y, torch.ones_like(xs[0]))
+    for i in range(4):
+        xs.copy_(x["x"].roll(i, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            ye = learning.gated_feed_forward(xs, x["wg"], x["wu"], x["wd"])
+            ne, se = learning.rms_norm_residual(xs, ye, torch.ones_like(xs[0]))
+        assert torch.equal(y, ye) and torch.equal(n, ne) and torch.equal(s, se)
+
+
+def norm_inputs(M, D, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=gen).to(dtype).to(DEV)  # noqa: E731
+    return dict(x=r(M, D), r=2 * r(M, D), w=1 + r(D) / 8, dy=r(M, D), ds=r(M, D))
+
+
+def norm_run(x, eps=1e-6):
+    leaf = {k: x[k].detach().requires_grad_(True) for k in ("x", "r", "w") if x[k] is not None}
+    y, s = learning.rms_norm_residual(leaf["x"], leaf.get("r"), leaf["w"], eps)
+    grads = torch.autograd.grad((y, s), list(leaf.values()), (x["dy"], x["ds"]))
+    return {"y": y.detach(), "s": s.detach(), **{"d" + k: t for k, t in zip(leaf, grads)}}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("M,D", [(1, 1), (1, 8192), (3, 7), (17, 16), (5, 128), (200, 129), (33, 512), (70, 1000),
+                                 (9, 2049), (4, 4096), (6000, 24), (4100, 300)])
+def test_norm(M, D, residual, dtype):
+    x = norm_inputs(M, D, dtype, seed=M + D)
+    if not residual:
+        x["r"] = None
+    got = norm_run(x)
+    want = ref.norm(x["x"], x["r"], x["w"], 1e-6, x["dy"], x["ds"])
+    for k, (v, tol) in want.items():
+        ref.assert_within(k, got[k], v, tol)
+    if residual:
+        assert torch.equal(got["dr"], got["dx"])
+
+
+def test_norm_partial_gradients_strides_and_zero_rows():
+    x = norm_inputs(12, 40, torch.float32, seed=1)
+    x["x"][3], x["r"][3] = 0.0, 0.0  # a row of zeros: eps alone under the root
+    full = norm_run(x)
+    assert all(bool(torch.isfinite(t).all()) for t in full.values())
+    leaf = [x[k].detach().requires_grad_(True) for k in ("x", "r", "w")]
+    y, s = learning.rms_norm_residual(*leaf)
+    gy = torch.autograd.grad(y, leaf, x["dy"])  # no gradient reaches s
+    zero = norm_run(dict(x, ds=torch.zeros_like(x["ds"])))
+    for a, k in zip(gy, ("dx", "dr", "dw")):
+        assert torch.equal(a, zero[k]), k
+    y, s = learning.rms_norm_residual(*leaf)
+    gs = torch.autograd.grad(s, leaf[:2], x["ds"])  # nor y
+    assert torch.equal(gs[0], x["ds"]) and torch.equal(gs[1], x["ds"])
+    wide = torch.zeros((12, 3, 50), device=DEV)
+    wide[:, 1, 5:45] = x["x"]
+    got = norm_run(dict(x, x=wide[:, 1, 5:45], r=x["r"].t().contiguous().t(),
+                        dy=x["dy"].repeat_interleave(2, 0)[::2]))
+    for k in full:
+        assert torch.equal(got[k], full[k]), k
+
+
+def test_norm_gradient_against_differences():
+    x = norm_inputs(20, 64, torch.float32, seed=2)
+    got = norm_run(x)
+
+    def loss(z):
+        y, s = learning.rms_norm_residual(z["x"], z["r"], z["w"])
+        return float((y.double() * x["dy"].double()).sum() + (s.double() * x["ds"].double()).sum())
+
+    want = ref.norm(x["x"], x["r"], x["w"], 1e-6)
+    noise = float((want["y"][1] * ref.cpu64(x["dy"]).abs()).sum() + (want["s"][1] * ref.cpu64(x["ds"]).abs()).sum())
+    for k in ("x", "w"):
+        d = torch.randn(x[k].shape, generator=torch.Generator().manual_seed(3)).to(DEV)
+        exact = float((got["d" + k].double() * d.double()).sum())
+        diff = [(loss(dict(x, **{k: x[k] + h * d})) - loss(dict(x, **{k: x[k] - h * d}))) / (2 * h) for h in (0.04, 0.02)]
+        extrapolated = (4 * diff[1] - diff[0]) / 3
+        assert abs(extrapolated - exact) <= 4 * noise / 0.02 + abs(diff[1] - diff[0]), (k, diff, exact)
+
+
+def test_refusals():
+    x = ff_inputs(4, 16, 24, 16, torch.float32)
+    w = [x["wg"], x["wu"], x["wd"]]
+    for err, args in [
+        (TypeError, (x["x"].double(), *w)), (TypeError, (x["x"].bfloat16(), *w)), (ValueError, (x["x"].cpu(), *w)),
+        (ValueError, (x["x"][:, :8], *w)), (ValueError, (x["x"], w[0][:5], *w[1:])),
+        (ValueError, (x["x"], w[0], w[1], w[2][:, :5])), (ValueError, (x["x"], *w, "tanh")),
+        (ValueError, (x["x"], w[0].cpu(), *w[1:])),
+    ]:
+        with pytest.raises(err):
+            learning.gated_feed_forward(*args)
+    n = norm_inputs(4, 16, torch.float32)
+    for err, args in [
+        (TypeError, (n["x"].half(), None, n["w"])), (TypeError, (n["x"], n["r"], n["w"].bfloat16())),
+        (ValueError, (n["x"], n["r"][:2], n["w"])), (ValueError, (n["x"], n["r"], n["w"][:3])),
+        (ValueError, (n["x"], n["r"], n["w"], -1.0)), (ValueError, (n["x"].cpu(), None, n["w"].cpu())),
+        (ValueError, (torch.zeros(2, 8193, device=DEV), None, torch.zeros(8193, device=DEV))),
+    ]:
+        with pytest.raises(err):
+            learning.rms_norm_residual(*args)

@@ -147,8 +147,24 @@ class MeritTerms(ctypes.Structure):
     ]
 
 
+class DecayAttention(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int32) for k in ("B", "T", "H", "Hk", "dk", "dv")] + [
+        (k, ctypes.c_void_p) for k in ("q", "k", "v")
+    ] + [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride")] + [
+        (k, ctypes.c_void_p) for k in ("log_decay", "lengths", "state_in")
+    ] + [("scale", ctypes.c_double)]
+
+
+class GatedFF(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int64)] + [(k, ctypes.c_int32) for k in ("D", "F", "Dout", "activation")] + [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64)
+    ] + [(k, ctypes.c_void_p) for k in ("w_gate", "w_up", "w_down")]
+
+
 # name -> argtypes (restype is int unless listed in _SIZE_FNS)
 _VP, _I32, _U32, _F64, _SZ = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_double, ctypes.c_size_t
+_I64 = ctypes.c_int64
+_PDA, _PFF = ctypes.POINTER(DecayAttention), ctypes.POINTER(GatedFF)
 _PD, _PQ, _PS, _PC, _PSQ = (ctypes.POINTER(t) for t in (Dims, QP, State, AdmmCfg, SqpStep))
 SIGNATURES = {
     "tmpc_version": [],
@@ -207,13 +223,30 @@ SIGNATURES = {
     "tmpc_obstacle_linearize_f64": [_VP] + [_I32] * 6 + [_VP] * 3 + [_I32, _I32] + [_VP] * 3,
     "tmpc_obstacle_lagrangian_hessian_f32": [_VP] + [_I32] * 6 + [_VP] * 3 + [_I32, _I32] + [_VP] * 2,
     "tmpc_obstacle_lagrangian_hessian_f64": [_VP] + [_I32] * 6 + [_VP] * 3 + [_I32, _I32] + [_VP] * 2,
+    "tmpc_rms_norm_backward_workspace_bytes": [ctypes.c_int, _I64, _I32],
+    "tmpc_decay_attention_workspace_bytes": [ctypes.c_int, _PDA, ctypes.c_int],
+    "tmpc_gated_ff_workspace_bytes": [ctypes.c_int, _PFF, ctypes.c_int],
 }
+for _sfx in ("f32", "bf16"):
+    SIGNATURES.update({
+        f"tmpc_rms_norm_forward_{_sfx}": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _VP, _F64, _VP, _VP, _VP],
+        f"tmpc_rms_norm_backward_{_sfx}": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP,
+                                           _SZ],
+        f"tmpc_decay_attention_forward_{_sfx}": [_VP, _PDA, _VP, _VP, _VP, _SZ],
+        f"tmpc_decay_attention_backward_{_sfx}": [_VP, _PDA, _VP, ctypes.POINTER(_I64)] + [_VP] * 6 + [_SZ],
+        f"tmpc_decay_attention_step_{_sfx}": [_VP, _PDA, _VP, _VP, _VP],
+        f"tmpc_gated_ff_forward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _VP, _SZ],
+        f"tmpc_gated_ff_backward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _I64] + [_VP] * 5 + [_SZ],
+    })
 _SIZE_FNS = {
     "tmpc_admm_direct_workspace_bytes",
     "tmpc_admm_pcg_workspace_bytes",
     "tmpc_blktri_workspace_bytes",
     "tmpc_schur_pcg_workspace_bytes",
     "tmpc_adjoint_kkt_workspace_bytes",
+    "tmpc_rms_norm_backward_workspace_bytes",
+    "tmpc_decay_attention_workspace_bytes",
+    "tmpc_gated_ff_workspace_bytes",
 }
 
 _LIB: Optional[ctypes.CDLL] = None

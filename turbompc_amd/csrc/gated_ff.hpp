@@ -1,0 +1,264 @@
+// Gated feed-forward block  y = (act(x Wg^T) o (x Wu^T)) Wd^T  and its backward pass:
+//   dh = dy Wd;  dG = dh o U o act'(G);  dU = dh o act(G);
+//   dx = dG Wg + dU Wu;  dWg = dG^T x;  dWu = dU^T x;  dWd = dy^T h.
+// Both projections, the activation and the product are one kernel: a column tile of
+// the product holds 16 columns of the gate next to the same 16 of the other
+// projection, so a lane has both values of a feature.  The product dy Wd ends in the
+// derivatives, so dh is never written; h is formed again there from the saved G, U.
+// Every matrix here is multiplied in the layout it is stored in: an operand whose
+// contracted index is its row (W in dx, every operand of the weight gradients) is
+// staged as it lies and read from LDS transposed.
+#pragma once
+#include "learn_common.hpp"
+
+namespace tmpc {
+
+enum { ACT_SILU = 0, ACT_GELU = 1 };
+
+// act(g) and its derivative
+template <int ACT>
+__device__ inline void act_both(float g, float& a, float& d) {
+  if constexpr (ACT == ACT_SILU) {
+    const float sg = 1.0f / (1.0f + __expf(-g));
+    a = g * sg;
+    d = sg * (1.0f + g * (1.0f - sg));
+  } else {
+    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    a = g * phi;
+    d = phi + g * (0.39894228040143268f * __expf(-0.5f * g * g));
+  }
+}
+template <int ACT>
+__device__ inline float act_only(float g) {
+  if constexpr (ACT == ACT_SILU) return g / (1.0f + __expf(-g));
+  return g * (0.5f * erfcf(-0.70710678118654752f * g));
+}
+
+// out (M, N) = sum over segments s of A_s B_s, K contracted entries each.
+//   A_s (M, K) of pitch lda, or (K, M) with AT; B_s (N, K) of pitch ldb, or (K, N) with BT.
+// DUAL: B_0, B_1 are the two projections (no segments).
+template <typename E>
+struct GemmArgs {
+  int64_t M;
+  int N, nseg;
+  int64_t K;
+  const E *A[2], *B[2];
+  int64_t lda, ldb;
+  // outputs; pitches in elements
+  E *o0, *o1, *o2;
+  float *g, *u;      // the saved projections: fp32, for rounding them would double the gradients' error
+  int64_t ldo, ldg;  // pitches of o* and of g, u
+  float* part;       // split over K: (splits, M, N) partial sums
+  int64_t k_split;   // contracted entries of a split (a multiple of the K tile)
+};
+
+enum GemmEpi {
+  EPI_STORE = 0,     // o0 = acc
+  EPI_GATE = 1,      // DUAL: o0 = act(G) o U
+  EPI_GATE_SAVE = 2, // and g = G, u = U
+  EPI_DGATE = 3,     // acc = dh: o0 = dG, o1 = dU, o2 = h from the saved g, u
+  EPI_PART = 4       // part[split] = acc
+};
+
+template <typename E>
+struct GemmTile {
+  static constexpr int BK = sizeof(E) == 2 ? 64 : 32;
+  static constexpr int PAD = 16 / sizeof(E);
+};
+
+// The operand tile of one K step: global memory -> registers -> LDS.
+template <typename E, int BR, int THREADS, bool TR, bool DUAL>
+struct Stage {
+  static constexpr int BK = GemmTile<E>::BK, P = Elem<E>::PIECE, PAD = GemmTile<E>::PAD;
+  static constexpr int LD = TR ? BR + PAD : BK + PAD;
+  static constexpr int ELEMS = TR ? BK * LD : BR * LD;
+  static constexpr int PIECES = BR * BK / P, NP = (PIECES + THREADS - 1) / THREADS;
+  piece_t<E> r[NP];
+
+  // rows r0 .. of an operand with `rows` rows (outer index) and K contracted entries
+  __device__ void load(const E* const* src, int seg, int64_t ld, int64_t r0, int64_t rows, int64_t k0, int64_t K, int tid) {
+    const bool k_in = k0 + BK <= K, r_in = r0 + BR <= rows;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int e = tid + i * THREADS;
+      if (PIECES % THREADS != 0 && e >= PIECES) break;
+      if constexpr (!TR) {
+        const int row = e / (BK / P), c = (e - row * (BK / P)) * P;
+        int64_t gr;
+        const E* base;
+        if constexpr (DUAL) {  // 16 rows of the one, 16 of the other
+          gr = r0 + (row >> 5) * 16 + (row & 15);
+          base = src[(row >> 4) & 1];
+        } else {
+          gr = r0 + row;
+          base = src[seg];
+        }
+        gr = gr < rows ? gr : rows - 1;  // past the edge: any row, its results are not stored
+        const E* rp = base + gr * ld;
+        if (k_in)
+          r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(rp + k0 + c);
+        else
+          r[i] = load_piece(rp + k0, c, (int)(K - k0), true);
+      } else {
+        const int kr = e / (BR / P), c = (e - kr * (BR / P)) * P;
+        const E* rp = src[seg] + (k0 + kr) * ld + r0;
+        if (k_in && r_in)
+          r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(rp + c);
+        else
+          r[i] = load_piece(rp, c, (int)(rows - r0 < BR ? rows - r0 : BR), k0 + kr < K);
+      }
+    }
+  }
+  __device__ void store(E* t, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int e = tid + i * THREADS;
+      if (PIECES % THREADS != 0 && e >= PIECES) break;
+      const int w = TR ? BR / P : BK / P;
+      const int row = e / w, c = (e - row * w) * P;
+      *reinterpret_cast<piece_t<E>*>(t + row * LD + c) = r[i];
+    }
+  }
+  // the quad of outer rows 16 o .., contracted entries 16 k ..
+  __device__ static quad_t<E> quad(const E* t, int row0, int k0, int lane) {
+    if constexpr (TR)
+      return lds_quad_t(t, LD, k0, row0, lane);
+    else
+      return lds_quad(t, LD, row0, k0, lane);
+  }
+};
+
+// BM x BN tile by WM x WN waves; BN counts both projections' columns with DUAL.
+template <typename E, int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI, int ACT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs<E> p) {
+  constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
+  constexpr int THREADS = 64 * WM * WN, BK = GemmTile<E>::BK;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int BF = DUAL ? BN / 2 : BN;  // output columns of the tile
+  using SA = Stage<E, BM, THREADS, AT, false>;
+  using SB = Stage<E, BN, THREADS, BT, DUAL>;
+  extern __shared__ __align__(16) char smem[];
+  E* ta = reinterpret_cast<E*>(smem);
+  E* tb = ta + 2 * SA::ELEMS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int wm = wave / WN, wn = wave - wm * WN;
+  const int64_t m0 = (int64_t)blockIdx.x * BM;
+  const int64_t n0 = (int64_t)blockIdx.y * BF;
+  const int64_t kb = (int64_t)blockIdx.z * p.k_split;
+  const int64_t ke = EPI == EPI_PART ? (kb + p.k_split < p.K ? kb + p.k_split : p.K) : p.K;
+  const int tiles = (int)((ke - kb + BK - 1) / BK), total = tiles * (DUAL ? 1 : p.nseg);
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  SA sa;
+  SB sb;
+  int seg = 0;
+  int64_t k = kb;
+  if (total > 0) {
+    sa.load(p.A, 0, p.lda, m0, p.M, k, ke, tid);
+    sb.load(p.B, 0, p.ldb, n0, p.N, k, ke, tid);
+    sa.store(ta, tid);
+    sb.store(tb, tid);
+  }
+  __syncthreads();
+  for (int it = 0; it < total; ++it) {
+    const E* ca = ta + (it & 1) * SA::ELEMS;
+    const E* cb = tb + (it & 1) * SB::ELEMS;
+    const bool more = it + 1 < total;
+    if (more) {
+      k += BK;
+      if (k >= ke) k = kb, ++seg;
+      sa.load(p.A, seg, p.lda, m0, p.M, k, ke, tid);
+      sb.load(p.B, seg, p.ldb, n0, p.N, k, ke, tid);
+    }
+#pragma unroll
+    for (int kk = 0; kk < BK; kk += 32) {
+      quad_t<E> a0[TM], a1[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        a0[i] = SA::quad(ca, (wm * TM + i) * 16, kk, lane);
+        a1[i] = SA::quad(ca, (wm * TM + i) * 16, kk + 16, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const quad_t<E> b0 = SB::quad(cb, (wn * TN + j) * 16, kk, lane);
+        const quad_t<E> b1 = SB::quad(cb, (wn * TN + j) * 16, kk + 16, lane);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = mma2(b0, b1, a0[i], a1[i], acc[i][j]);
+      }
+    }
+    if (more) {  // the other buffer was last read before the previous barrier
+      sa.store(ta + ((it + 1) & 1) * SA::ELEMS, tid);
+      sb.store(tb + ((it + 1) & 1) * SB::ELEMS, tid);
+    }
+    __syncthreads();
+  }
+
+  // lane: row m, 4 consecutive columns
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t m = m0 + (wm * TM + i) * 16 + lo;
+    if (m >= p.M) continue;
+    if constexpr (DUAL) {
+      static_assert(TN % 2 == 0, "a wave holds both projections of its features");
+#pragma unroll
+      for (int j = 0; j < TN; j += 2) {
+        const int64_t c = n0 + (wn * TN + j) * 8 + 4 * hi;
+        f32x4 hv;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) hv[r] = act_only<ACT>(acc[i][j][r]) * acc[i][j + 1][r];
+        if (c >= p.N) continue;
+        store_quad(p.o0 + m * p.ldo, (int)c, p.N, hv);
+        if constexpr (EPI == EPI_GATE_SAVE) {
+          store_quad(p.g + m * p.ldg, (int)c, p.N, acc[i][j]);
+          store_quad(p.u + m * p.ldg, (int)c, p.N, acc[i][j + 1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t c = n0 + (wn * TN + j) * 16 + 4 * hi;
+        if (c >= p.N) continue;
+        if constexpr (EPI == EPI_STORE) {
+          store_quad(p.o0 + m * p.ldo, (int)c, p.N, acc[i][j]);
+        } else if constexpr (EPI == EPI_PART) {
+          store_quad(p.part + ((int64_t)blockIdx.z * p.M + m) * p.N, (int)c, p.N, acc[i][j]);
+        } else {
+          const f32x4 gv = load_quad_f32(p.g + m * p.ldg, (int)c, p.N), uv = load_quad_f32(p.u + m * p.ldg, (int)c, p.N);
+          f32x4 dg, du, hv;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float a, d;
+            act_both<ACT>(gv[r], a, d);
+            dg[r] = acc[i][j][r] * uv[r] * d, du[r] = acc[i][j][r] * a, hv[r] = a * uv[r];
+          }
+          store_quad(p.o0 + m * p.ldo, (int)c, p.N, dg);
+          store_quad(p.o1 + m * p.ldo, (int)c, p.N, du);
+          store_quad(p.o2 + m * p.ldo, (int)c, p.N, hv);
+        }
+      }
+    }
+  }
+}
+
+// out = sum of the partial sums over the splits, in order
+template <typename E>
+__global__ __launch_bounds__(256) void gemm_reduce_kernel(const float* __restrict__ part, int64_t n, int splits,
+                                                          E* __restrict__ out) {
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += part[(int64_t)s * n + e];
+    out[e] = (E)v;
+  }
+}
+
+template <typename E, int BM, int BN, bool AT, bool BT, int THREADS, bool DUAL>
+constexpr size_t gemm_lds() {
+  return 2 * sizeof(E) * (size_t)(Stage<E, BM, THREADS, AT, false>::ELEMS + Stage<E, BN, THREADS, BT, DUAL>::ELEMS);
+}
+
+}  // namespace tmpc

@@ -1,0 +1,416 @@
+// C ABI of the history model's operators (include/tmpc.h): argument checks, the
+// choice of tile and workspace, launches.
+#include <algorithm>
+
+#include "../../include/tmpc.h"
+#include "decay_attention.hpp"
+#include "gated_ff.hpp"
+#include "rms_norm.hpp"
+
+namespace tmpc {
+namespace {
+
+constexpr int kCUs = 256;
+
+inline size_t align_up(size_t n) { return (n + 255) & ~size_t(255); }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int launch_status() { return hipGetLastError() == hipSuccess ? TMPC_OK : TMPC_ELAUNCH; }
+
+// Dynamic LDS above the 64 KiB default needs an explicit opt-in per kernel.
+template <typename K>
+void lds_optin(K kernel, size_t bytes) {
+  if (bytes > 65536)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)bytes);
+}
+
+// ---------------------------------------------------------------- rms norm --
+constexpr int kMaxWidth = 8192;
+constexpr int kRmsBlocks = 1024;  // of the backward pass: rows meet in its blocks' partial sums
+
+// f(threads per row, pieces per thread) of the smallest form that holds `width`
+template <typename E, typename F>
+void with_row(int width, F f) {
+  const int pieces = (width + Elem<E>::PIECE - 1) / Elem<E>::PIECE;
+  using std::integral_constant;
+  if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+  else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else if (pieces <= 128) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else if (pieces <= 256) f(integral_constant<int, 256>(), integral_constant<int, 1>());
+  else if (pieces <= 512) f(integral_constant<int, 256>(), integral_constant<int, 2>());
+  else if (pieces <= 1024) f(integral_constant<int, 256>(), integral_constant<int, 4>());
+  else f(integral_constant<int, 256>(), integral_constant<int, 8>());
+}
+
+inline int64_t rms_rows_per_block(int width, int elem_bytes) {
+  const int pieces = (width * elem_bytes + 15) / 16;
+  return pieces <= 16 ? 16 : pieces <= 128 ? 4 : 1;
+}
+inline int64_t rms_backward_blocks(int64_t rows, int width, int elem_bytes) {
+  return std::min<int64_t>(ceil_div(rows, rms_rows_per_block(width, elem_bytes)), kRmsBlocks);
+}
+
+bool rms_shape_ok(int64_t rows, int width) { return rows >= 0 && width >= 1 && width <= kMaxWidth; }
+
+template <typename E>
+int rms_forward_impl(hipStream_t st, int64_t rows, int32_t width, const void* x, int64_t ldx, const void* r,
+                     int64_t ldr, const void* w, double eps, void* y, void* s, float* rstd) {
+  if (!rms_shape_ok(rows, width)) return TMPC_EBADSHAPE;
+  if (rows == 0) return TMPC_OK;
+  if (!x || !w || !y || !(eps >= 0.0) || ldx < 0 || ldr < 0) return TMPC_EBADARG;
+  const RmsArgs<E> a{rows, width, (const E*)x, (const E*)r, (const E*)w, ldx, ldr, (float)eps, (E*)y, (E*)s, rstd};
+  with_row<E>(width, [&](auto tpr, auto np) {
+    const int64_t blocks = ceil_div(rows, 256 / tpr());
+    hipLaunchKernelGGL((rms_forward_kernel<E, tpr(), np()>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)),
+                       dim3(256), 0, st, a);
+  });
+  return launch_status();
+}
+
+template <typename E>
+int rms_backward_impl(hipStream_t st, int64_t rows, int32_t width, const void* dy, int64_t lddy, const void* ds,
+                      int64_t ldds, const void* s, int64_t lds, const void* w, const float* rstd, void* dx, void* dw,
+                      void* ws, size_t wsb) {
+  if (!rms_shape_ok(rows, width)) return TMPC_EBADSHAPE;
+  if (!dw || (rows > 0 && (!dy || !s || !w || !rstd || !dx)) || lddy < 0 || ldds < 0 || lds < 0) return TMPC_EBADARG;
+  const int64_t blocks = rms_backward_blocks(rows, width, sizeof(E));
+  const size_t need = (size_t)blocks * width * sizeof(float);
+  if (wsb < need) return TMPC_EWORKSPACE;
+  if (need > 0 && !ws) return TMPC_EBADARG;
+  float* part = (float*)ws;
+  if (rows > 0) {
+    const RmsBwdArgs<E> a{rows, width, (const E*)dy, (const E*)ds, (const E*)s, (const E*)w, lddy, ldds, lds, rstd, (E*)dx, part};
+    with_row<E>(width, [&](auto tpr, auto np) {
+      hipLaunchKernelGGL((rms_backward_kernel<E, tpr(), np()>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    });
+  }
+  hipLaunchKernelGGL((rms_dweight_kernel<E>), dim3((unsigned)ceil_div(width, 16)), dim3(256), 0, st, part, (int)blocks,
+                     width, (E*)dw);
+  return launch_status();
+}
+
+// --------------------------------------------------------- decay attention --
+bool attn_shape_ok(const tmpc_decay_attention* a) {
+  return a && a->B >= 0 && a->T >= 0 && a->H >= 1 && a->Hk >= 1 && a->H % a->Hk == 0 && a->dk >= 1 && a->dk <= 128 &&
+         a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 0x7fffffff;
+}
+
+template <typename E>
+void launch_attn(hipStream_t st, const AttnArgs<E>& p) {
+  auto go = [&](auto da, auto dc) {
+    using S = AttnShape<E, da(), dc()>;
+    auto k = attn_chunk_kernel<E, da(), dc()>;
+    lds_optin(k, S::LDS);
+    hipLaunchKernelGGL(k, dim3((unsigned)(p.B * p.H)), dim3(S::THREADS), S::LDS, st, p);
+  };
+  using std::integral_constant;
+  auto with_c = [&](auto da) {
+    if (p.dc <= 32) go(da, integral_constant<int, 32>());
+    else if (p.dc <= 64) go(da, integral_constant<int, 64>());
+    else go(da, integral_constant<int, 128>());
+  };
+  if (p.da <= 32) with_c(integral_constant<int, 32>());
+  else if (p.da <= 64) with_c(integral_constant<int, 64>());
+  else with_c(integral_constant<int, 128>());
+}
+
+template <typename E>
+AttnArgs<E> attn_args(const tmpc_decay_attention* x) {
+  AttnArgs<E> p{};
+  p.B = x->B, p.T = x->T, p.H = x->H, p.da = x->dk, p.dc = x->dv;
+  p.log_decay = x->log_decay, p.lengths = x->lengths;
+  p.ga = p.gb = p.gc = 1;
+  return p;
+}
+
+template <typename E>
+size_t attn_ws_bytes(const tmpc_decay_attention* x, bool backward) {
+  if (!backward || x->H == x->Hk) return 0;
+  const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
+  return align_up(tok * x->dk) + align_up(tok * x->dv);
+}
+
+template <typename E>
+int attn_forward_impl(hipStream_t st, const tmpc_decay_attention* x, void* o, float* state_out, void* ws, size_t wsb) {
+  if (!attn_shape_ok(x)) return TMPC_EBADSHAPE;
+  if (x->B == 0) return TMPC_OK;
+  if (!x->log_decay || (x->T > 0 && (!x->q || !x->k || !x->v || !o))) return TMPC_EBADARG;
+  if (wsb < attn_ws_bytes<E>(x, false)) return TMPC_EWORKSPACE;
+  AttnArgs<E> p = attn_args<E>(x);
+  p.a = (const E*)x->q, p.b = (const E*)x->k, p.c = (const E*)x->v;
+  std::copy_n(x->q_stride, 3, p.as), std::copy_n(x->k_stride, 3, p.bs), std::copy_n(x->v_stride, 3, p.cs);
+  p.gb = p.gc = x->H / x->Hk;
+  p.ss = p.si = (float)x->scale, p.su = 1.0f;
+  p.s_in = x->state_in, p.s_out = state_out, p.o = o;
+  launch_attn(st, p);
+  return launch_status();
+}
+
+template <typename E>
+int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void* d_o, const int64_t* dos,
+                       const float* d_state_out, void* dq, void* dk, void* dv, float* d_state_in, void* ws,
+                       size_t wsb) {
+  if (!attn_shape_ok(x)) return TMPC_EBADSHAPE;
+  if (x->B == 0) return TMPC_OK;
+  if (!x->log_decay || !dos || (x->T > 0 && (!x->q || !x->k || !x->v || !d_o || !dq || !dk || !dv)))
+    return TMPC_EBADARG;
+  if (wsb < attn_ws_bytes<E>(x, true)) return TMPC_EWORKSPACE;
+  if (attn_ws_bytes<E>(x, true) > 0 && !ws) return TMPC_EBADARG;
+  const int G = x->H / x->Hk;
+  const float scale = (float)x->scale;
+  {  // dq: (do, v, k) from the transposed state
+    AttnArgs<E> p = attn_args<E>(x);
+    p.da = x->dv, p.dc = x->dk;
+    p.a = (const E*)d_o, p.b = (const E*)x->v, p.c = (const E*)x->k;
+    std::copy_n(dos, 3, p.as), std::copy_n(x->v_stride, 3, p.bs), std::copy_n(x->k_stride, 3, p.cs);
+    p.gb = p.gc = G;
+    p.ss = p.si = scale, p.su = 1.0f;
+    p.s_in = x->state_in, p.s_in_t = 1, p.o = dq;
+    launch_attn(st, p);
+  }
+  const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
+  float* gk = G > 1 ? (float*)ws : nullptr;
+  float* gv = G > 1 ? (float*)((char*)ws + align_up(tok * x->dk)) : nullptr;
+  {  // dk: backwards, (v, do, q) from the transposed gradient of the state
+    AttnArgs<E> p = attn_args<E>(x);
+    p.da = x->dv, p.dc = x->dk, p.rev = 1;
+    p.a = (const E*)x->v, p.b = (const E*)d_o, p.c = (const E*)x->q;
+    std::copy_n(x->v_stride, 3, p.as), std::copy_n(dos, 3, p.bs), std::copy_n(x->q_stride, 3, p.cs);
+    p.ga = G;
+    p.ss = p.su = scale, p.si = 1.0f;
+    p.s_in = d_state_out, p.s_in_t = 1;
+    p.o = gk ? (void*)gk : dk, p.o_f32 = gk != nullptr;
+    launch_attn(st, p);
+  }
+  {  // dv: backwards, (k, q, do)
+    AttnArgs<E> p = attn_args<E>(x);
+    p.rev = 1;
+    p.a = (const E*)x->k, p.b = (const E*)x->q, p.c = (const E*)d_o;
+    std::copy_n(x->k_stride, 3, p.as), std::copy_n(x->q_stride, 3, p.bs), std::copy_n(dos, 3, p.cs);
+    p.ga = G;
+    p.ss = p.su = scale, p.si = 1.0f;
+    p.s_in = d_state_out, p.s_out = d_state_in;
+    p.o = gv ? (void*)gv : dv, p.o_f32 = gv != nullptr;
+    launch_attn(st, p);
+  }
+  if (G > 1 && x->T > 0) {
+    auto sum = [&](const float* in, int d, void* out) {
+      const int64_t n = (int64_t)x->B * x->T * x->Hk * d;
+      hipLaunchKernelGGL((attn_head_sum_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 16 * kCUs)),
+                         dim3(256), 0, st, in, n, G, d, (E*)out);
+    };
+    sum(gk, x->dk, dk);
+    sum(gv, x->dv, dv);
+  }
+  return launch_status();
+}
+
+template <typename E>
+int attn_step_impl(hipStream_t st, const tmpc_decay_attention* x, const uint8_t* active, float* state, void* o) {
+  if (!attn_shape_ok(x) || x->T != 1) return TMPC_EBADSHAPE;
+  if (x->B == 0) return TMPC_OK;
+  if (!x->q || !x->k || !x->v || !x->log_decay || !state || !o) return TMPC_EBADARG;
+  AttnStepArgs<E> p{x->B, x->H, x->H / x->Hk, x->dk, x->dv, (const E*)x->q, (const E*)x->k, (const E*)x->v};
+  p.qs[0] = x->q_stride[0], p.qs[1] = x->q_stride[2];
+  p.ks[0] = x->k_stride[0], p.ks[1] = x->k_stride[2];
+  p.vs[0] = x->v_stride[0], p.vs[1] = x->v_stride[2];
+  p.log_decay = x->log_decay, p.active = active, p.scale = (float)x->scale, p.state = state, p.o = (E*)o;
+  hipLaunchKernelGGL((attn_step_kernel<E>), dim3((unsigned)(x->B * x->H)), dim3(256), 0, st, p);
+  return launch_status();
+}
+
+// ------------------------------------------------------ gated feed-forward --
+bool ff_shape_ok(const tmpc_gated_ff* a) {
+  return a && a->M >= 0 && a->D >= 1 && a->F >= 1 && a->Dout >= 1 && a->M <= 0x7fffffff;
+}
+// pitch of the block's own (M, F) arrays: rows of whole 16-byte pieces
+template <typename E>
+int64_t ff_pitch(const tmpc_gated_ff* a) {
+  return ceil_div(a->F, Elem<E>::PIECE) * Elem<E>::PIECE;
+}
+
+template <typename E, bool AT, bool BT, int EPI, int ACT = 0>
+void launch_gemm(hipStream_t st, GemmArgs<E> p, int splits = 1) {
+  constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
+  auto go = [&](auto bm, auto bn, auto wm, auto wn) {
+    constexpr int BM = bm(), BN = bn(), THREADS = 64 * wm() * wn();
+    constexpr size_t lds = gemm_lds<E, BM, BN, AT, BT, THREADS, DUAL>();
+    auto k = gemm_kernel<E, BM, BN, wm(), wn(), AT, BT, EPI, ACT>;
+    lds_optin(k, lds);
+    const dim3 grid((unsigned)ceil_div(p.M, BM), (unsigned)ceil_div(p.N, DUAL ? BN / 2 : BN), (unsigned)splits);
+    hipLaunchKernelGGL(k, grid, dim3(THREADS), lds, st, p);
+  };
+  using std::integral_constant;
+  if (splits == 1) p.k_split = std::max<int64_t>(p.K, 1);
+  go(integral_constant<int, 128>(), integral_constant<int, 128>(), integral_constant<int, 2>(),
+     integral_constant<int, 2>());
+}
+
+// the weight gradients' rows are few and their contracted index is every row of the
+// batch: it is split until the tiles fill the chip
+template <typename E>
+int ff_splits(int64_t rows, int64_t cols, int64_t K) {
+  const int64_t tiles = ceil_div(rows, 128) * ceil_div(cols, 128);
+  const int64_t want = std::max<int64_t>(1, 2 * kCUs / tiles);
+  return (int)std::min<int64_t>(want, std::max<int64_t>(1, K / (8 * GemmTile<E>::BK)));
+}
+
+template <typename E>
+size_t ff_part_bytes(int64_t rows, int64_t cols, int64_t K) {
+  const int s = ff_splits<E>(rows, cols, K);
+  return s > 1 ? align_up((size_t)s * rows * cols * sizeof(float)) : 0;
+}
+
+template <typename E>
+size_t ff_ws_bytes(const tmpc_gated_ff* a, bool backward) {
+  const size_t act = align_up((size_t)a->M * ff_pitch<E>(a) * sizeof(E));
+  if (!backward) return act;
+  return 3 * act + std::max(ff_part_bytes<E>(a->F, a->D, a->M), ff_part_bytes<E>(a->Dout, a->F, a->M));
+}
+
+// dW (rows, cols) = P^T X over the batch's M rows
+template <typename E>
+void launch_weight_grad(hipStream_t st, int64_t M, int rows, int cols, const E* P, int64_t ldp, const E* X, int64_t ldx,
+                        E* out, float* part) {
+  GemmArgs<E> p{};
+  p.M = rows, p.N = cols, p.nseg = 1, p.K = M;
+  p.A[0] = P, p.lda = ldp, p.B[0] = X, p.ldb = ldx;
+  p.o0 = out, p.ldo = cols;
+  const int splits = ff_splits<E>(rows, cols, M);
+  if (splits == 1) {
+    launch_gemm<E, true, true, EPI_STORE>(st, p);
+    return;
+  }
+  p.part = part;
+  p.k_split = ceil_div(ceil_div(M, GemmTile<E>::BK), splits) * GemmTile<E>::BK;
+  launch_gemm<E, true, true, EPI_PART>(st, p, splits);
+  const int64_t n = (int64_t)rows * cols;
+  hipLaunchKernelGGL((gemm_reduce_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 16 * kCUs)), dim3(256),
+                     0, st, part, n, splits, out);
+}
+
+template <typename E>
+int ff_forward_impl(hipStream_t st, const tmpc_gated_ff* a, void* y, float* gate, float* up, void* ws, size_t wsb) {
+  if (!ff_shape_ok(a)) return TMPC_EBADSHAPE;
+  if (a->M == 0) return TMPC_OK;
+  if (!a->x || !a->w_gate || !a->w_up || !a->w_down || !y || !gate != !up || a->ldx < 0 ||
+      (a->activation != ACT_SILU && a->activation != ACT_GELU))
+    return TMPC_EBADARG;
+  if (wsb < ff_ws_bytes<E>(a, false)) return TMPC_EWORKSPACE;
+  if (!ws) return TMPC_EBADARG;
+  const int64_t ldh = ff_pitch<E>(a);
+  E* h = (E*)ws;
+  GemmArgs<E> p{};
+  p.M = a->M, p.N = a->F, p.nseg = 1, p.K = a->D;
+  p.A[0] = (const E*)a->x, p.lda = a->ldx;
+  p.B[0] = (const E*)a->w_gate, p.B[1] = (const E*)a->w_up, p.ldb = a->D;
+  p.o0 = h, p.ldo = ldh, p.g = gate, p.u = up, p.ldg = a->F;
+  if (a->activation == ACT_SILU) {
+    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_SILU>(st, p);
+    else launch_gemm<E, false, false, EPI_GATE, ACT_SILU>(st, p);
+  } else {
+    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_GELU>(st, p);
+    else launch_gemm<E, false, false, EPI_GATE, ACT_GELU>(st, p);
+  }
+  GemmArgs<E> d{};
+  d.M = a->M, d.N = a->Dout, d.nseg = 1, d.K = a->F;
+  d.A[0] = h, d.lda = ldh, d.B[0] = (const E*)a->w_down, d.ldb = a->F, d.o0 = (E*)y, d.ldo = a->Dout;
+  launch_gemm<E, false, false, EPI_STORE>(st, d);
+  return launch_status();
+}
+
+template <typename E>
+int ff_backward_impl(hipStream_t st, const tmpc_gated_ff* a, const float* gate, const float* up, const void* dy,
+                     int64_t lddy, void* dx, void* dwg, void* dwu, void* dwd, void* ws, size_t wsb) {
+  if (!ff_shape_ok(a)) return TMPC_EBADSHAPE;
+  if (!a->w_gate || !a->w_up || !a->w_down || !dwg || !dwu || !dwd || a->ldx < 0 || lddy < 0 ||
+      (a->M > 0 && (!a->x || !gate || !up || !dy || !dx)) ||
+      (a->activation != ACT_SILU && a->activation != ACT_GELU))
+    return TMPC_EBADARG;
+  const size_t need = ff_ws_bytes<E>(a, true);
+  if (wsb < need) return TMPC_EWORKSPACE;
+  if (need > 0 && !ws) return TMPC_EBADARG;
+  const int64_t ldh = ff_pitch<E>(a);
+  const size_t act = align_up((size_t)a->M * ldh * sizeof(E));
+  E* dg = (E*)ws;
+  E* du = (E*)((char*)ws + act);
+  E* h = (E*)((char*)ws + 2 * act);
+  float* part = (float*)((char*)ws + 3 * act);
+  if (a->M > 0) {
+    GemmArgs<E> p{};
+    p.M = a->M, p.N = a->F, p.nseg = 1, p.K = a->Dout;
+    p.A[0] = (const E*)dy, p.lda = lddy, p.B[0] = (const E*)a->w_down, p.ldb = a->F;
+    p.o0 = dg, p.o1 = du, p.o2 = h, p.ldo = ldh, p.g = const_cast<float*>(gate), p.u = const_cast<float*>(up), p.ldg = a->F;
+    if (a->activation == ACT_SILU) launch_gemm<E, false, true, EPI_DGATE, ACT_SILU>(st, p);
+    else launch_gemm<E, false, true, EPI_DGATE, ACT_GELU>(st, p);
+    GemmArgs<E> d{};
+    d.M = a->M, d.N = a->D, d.nseg = 2, d.K = a->F;
+    d.A[0] = dg, d.A[1] = du, d.lda = ldh;
+    d.B[0] = (const E*)a->w_gate, d.B[1] = (const E*)a->w_up, d.ldb = a->D;
+    d.o0 = (E*)dx, d.ldo = a->D;
+    launch_gemm<E, false, true, EPI_STORE>(st, d);
+  }
+  launch_weight_grad<E>(st, a->M, a->F, a->D, dg, ldh, (const E*)a->x, a->ldx, (E*)dwg, part);
+  launch_weight_grad<E>(st, a->M, a->F, a->D, du, ldh, (const E*)a->x, a->ldx, (E*)dwu, part);
+  launch_weight_grad<E>(st, a->M, a->Dout, a->F, (const E*)dy, lddy, h, ldh, (E*)dwd, part);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace tmpc
+
+using namespace tmpc;
+
+extern "C" {
+
+size_t tmpc_rms_norm_backward_workspace_bytes(int elem_bytes, int64_t rows, int32_t width) {
+  if (!rms_shape_ok(rows, width) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  return align_up((size_t)rms_backward_blocks(rows, width, elem_bytes) * width * sizeof(float));
+}
+size_t tmpc_decay_attention_workspace_bytes(int elem_bytes, const tmpc_decay_attention* a, int backward) {
+  if (!attn_shape_ok(a) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  return elem_bytes == 2 ? attn_ws_bytes<bf16>(a, backward != 0) : attn_ws_bytes<float>(a, backward != 0);
+}
+size_t tmpc_gated_ff_workspace_bytes(int elem_bytes, const tmpc_gated_ff* a, int backward) {
+  if (!ff_shape_ok(a) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  return elem_bytes == 2 ? ff_ws_bytes<bf16>(a, backward != 0) : ff_ws_bytes<float>(a, backward != 0);
+}
+
+#define TMPC_LEARNING(SFX, E)                                                                                          \
+  int tmpc_rms_norm_forward_##SFX(hipStream_t s, int64_t rows, int32_t width, const void* x, int64_t ldx,              \
+                                  const void* r, int64_t ldr, const void* w, double eps, void* y, void* sum,           \
+                                  float* rstd) {                                                                       \
+    return rms_forward_impl<E>(s, rows, width, x, ldx, r, ldr, w, eps, y, sum, rstd);                                  \
+  }                                                                                                                    \
+  int tmpc_rms_norm_backward_##SFX(hipStream_t s, int64_t rows, int32_t width, const void* dy, int64_t lddy,           \
+                                   const void* ds, int64_t ldds, const void* sum, int64_t lds, const void* w,          \
+                                   const float* rstd, void* dx, void* dw, void* ws, size_t wsb) {                      \
+    return rms_backward_impl<E>(s, rows, width, dy, lddy, ds, ldds, sum, lds, w, rstd, dx, dw, ws, wsb);               \
+  }                                                                                                                    \
+  int tmpc_decay_attention_forward_##SFX(hipStream_t s, const tmpc_decay_attention* a, void* o, float* state_out,      \
+                                         void* ws, size_t wsb) {                                                       \
+    return attn_forward_impl<E>(s, a, o, state_out, ws, wsb);                                                          \
+  }                                                                                                                    \
+  int tmpc_decay_attention_backward_##SFX(hipStream_t s, const tmpc_decay_attention* a, const void* d_o,               \
+                                          const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,     \
+                                          void* dv, float* d_state_in, void* ws, size_t wsb) {                         \
+    return attn_backward_impl<E>(s, a, d_o, d_o_stride, d_state_out, dq, dk, dv, d_state_in, ws, wsb);                 \
+  }                                                                                                                    \
+  int tmpc_decay_attention_step_##SFX(hipStream_t s, const tmpc_decay_attention* a, const uint8_t* active,             \
+                                      float* state, void* o) {                                                         \
+    return attn_step_impl<E>(s, a, active, state, o);                                                                  \
+  }                                                                                                                    \
+  int tmpc_gated_ff_forward_##SFX(hipStream_t s, const tmpc_gated_ff* a, void* y, float* gate, float* up, void* ws,      \
+                                  size_t wsb) {                                                                        \
+    return ff_forward_impl<E>(s, a, y, gate, up, ws, wsb);                                                             \
+  }                                                                                                                    \
+  int tmpc_gated_ff_backward_##SFX(hipStream_t s, const tmpc_gated_ff* a, const float* gate, const float* up,            \
+                                   const void* dy, int64_t lddy, void* dx, void* dwg, void* dwu, void* dwd, void* ws,  \
+                                   size_t wsb) {                                                                       \
+    return ff_backward_impl<E>(s, a, gate, up, dy, lddy, dx, dwg, dwu, dwd, ws, wsb);                                  \
+  }
+TMPC_LEARNING(f32, float)
+TMPC_LEARNING(bf16, bf16)
+
+}  // extern "C"
