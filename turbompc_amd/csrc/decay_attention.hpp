@@ -36,7 +36,15 @@ struct AttnArgs {
   float* s_out;              // (B, H, da, dc) or NULL
   void* o;                   // (B, T, H, dc): E, or fp32 with o_f32
   int o_f32;
+  int segs, seg_len;         // the steps in segs runs of seg_len (a multiple of the chunk)
+  float* seg_state;          // segs > 1: (B, H, segs, da, dc): each run's own sum, then its start
 };
+
+// live steps of problem b
+template <typename E>
+__device__ inline int attn_length(const AttnArgs<E>& p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+}
 
 template <typename E>
 struct AttnTile {
@@ -57,31 +65,60 @@ struct AttnShape {
   static constexpr int THREADS = 64 * W;
   static constexpr int C = AttnTile<E>::C;
   static constexpr int LDA = DA + AttnTile<E>::PAD, LDC = DC + AttnTile<E>::PAD, LDP = C + AttnTile<E>::PAD;
-  static constexpr size_t LDS = sizeof(E) * (size_t)(2 * C * LDA + C * LDC + C * LDP);
+  static constexpr size_t LDS_STATE = sizeof(E) * (size_t)(C * LDA + C * LDC);
+  static constexpr size_t LDS = LDS_STATE + sizeof(E) * (size_t)(C * LDA + C * LDP);
 };
 
-template <typename E, int DA, int DC>
-__global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_kernel(AttnArgs<E> p) {
+// A chunk's rows of one operand on their way from memory through registers to LDS: the
+// next chunk's are in flight while this one's are multiplied.
+template <typename E, int C, int D, int THREADS>
+struct AttnRows {
+  static constexpr int P = Elem<E>::PIECE, W = D / P, N = (C * W + THREADS - 1) / THREADS, LD = D + AttnTile<E>::PAD;
+  static_assert(C * W % THREADS == 0, "a whole number of pieces a thread");
+  piece_t<E> r[N];
+  // rows t0 .. of `base`, which points at the first live step; n live ones
+  __device__ void load(const E* base, int64_t stride, int t0, int n, int width, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * THREADS, row = e / W, c = (e - row * W) * P;
+      r[i] = load_piece(base + (t0 + row) * stride, c, width, row < n);
+    }
+  }
+  __device__ void store(E* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * THREADS, row = e / W, c = (e - row * W) * P;
+      *reinterpret_cast<piece_t<E>*>(tile + row * LD + c) = r[i];
+    }
+  }
+};
+
+// FULL: outputs and the carried state; else the run's own sum alone, into seg_state.
+template <typename E, int DA, int DC, bool FULL>
+__global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk_kernel(AttnArgs<E> p) {
   using S = AttnShape<E, DA, DC>;
   constexpr int C = S::C, W = S::W, NV = S::NV, LDA = S::LDA, LDC = S::LDC, LDP = S::LDP;
-  constexpr int P = Elem<E>::PIECE, CT = C / 16, KA = DA / 16;
+  constexpr int CT = C / 16, KA = DA / 16;
   extern __shared__ __align__(16) char smem[];
-  E* ta = reinterpret_cast<E*>(smem);
-  E* tb = ta + C * LDA;
+  E* tb = reinterpret_cast<E*>(smem);
   E* tc = tb + C * LDA;
-  E* tp = tc + C * LDC;
+  E* ta = tc + C * LDC;
+  E* tp = ta + C * LDA;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
-  const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs;
+  const int b = bh / p.H, h = bh - b * p.H;
   const float g = p.log_decay[h];
-  int L = p.T;
-  if (p.lengths) L = min(max(p.lengths[b], 0), p.T);
+  const int L = attn_length(p, b);
   const int64_t first = p.rev ? L - 1 : 0, dir = p.rev ? -1 : 1;
-  const E* pa = p.a + b * p.as[0] + (h / p.ga) * p.as[2];
-  const E* pb = p.b + b * p.bs[0] + (h / p.gb) * p.bs[2];
-  const E* pc = p.c + b * p.cs[0] + (h / p.gc) * p.cs[2];
+  const E* pa = p.a + b * p.as[0] + (h / p.ga) * p.as[2] + first * p.as[1];
+  const E* pb = p.b + b * p.bs[0] + (h / p.gb) * p.bs[2] + first * p.bs[1];
+  const E* pc = p.c + b * p.cs[0] + (h / p.gc) * p.cs[2] + first * p.cs[1];
   const int64_t orow = (int64_t)p.H * p.dc;
   const int64_t obase = ((int64_t)b * p.T * p.H + h) * p.dc;
   const int col0 = wave * NV * 16;
+  const int begin = seg * p.seg_len, end = min(L, begin + p.seg_len);
+  const int64_t sbase = (int64_t)bh * p.da * p.dc;
+  float* seg_state = p.segs > 1 ? p.seg_state + (int64_t)blockIdx.x * p.da * p.dc : nullptr;
 
   // S[m][n]: rows 16 m + 4 hi + r, column col0 + 16 n + lo
   f32x4 s[KA][NV];
@@ -93,28 +130,33 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * m + 4 * hi + r, col = col0 + 16 * n + lo;
         float v = 0.0f;
-        if (p.s_in && row < p.da && col < p.dc) {
-          const float* base = p.s_in + (int64_t)blockIdx.x * p.da * p.dc;
-          v = p.s_in_t ? base[(int64_t)col * p.da + row] : base[(int64_t)row * p.dc + col];
+        if (FULL && row < p.da && col < p.dc) {
+          if (seg_state)
+            v = seg_state[(int64_t)row * p.dc + col];
+          else if (p.s_in)
+            v = p.s_in_t ? p.s_in[sbase + (int64_t)col * p.da + row] : p.s_in[sbase + (int64_t)row * p.dc + col];
         }
         s[m][n][r] = v;
       }
 
-  for (int t0 = 0; t0 < L; t0 += C) {
-    const int n = min(C, L - t0);  // live steps
-    for (int e = tid; e < C * (DA / P); e += S::THREADS) {
-      const int row = e / (DA / P), c = (e - row * (DA / P)) * P;
-      const int64_t t = first + dir * (t0 + row);
-      *reinterpret_cast<piece_t<E>*>(ta + row * LDA + c) = load_piece(pa + t * p.as[1], c, p.da, row < n);
-      *reinterpret_cast<piece_t<E>*>(tb + row * LDA + c) = load_piece(pb + t * p.bs[1], c, p.da, row < n);
-    }
-    for (int e = tid; e < C * (DC / P); e += S::THREADS) {
-      const int row = e / (DC / P), c = (e - row * (DC / P)) * P;
-      const int64_t t = first + dir * (t0 + row);
-      *reinterpret_cast<piece_t<E>*>(tc + row * LDC + c) = load_piece(pc + t * p.cs[1], c, p.dc, row < n);
-    }
+  AttnRows<E, C, DA, S::THREADS> ra, rb;
+  AttnRows<E, C, DC, S::THREADS> rc;
+  auto fetch = [&](int t0) {
+    const int n = end - t0;
+    rb.load(pb, dir * p.bs[1], t0, n, p.da, tid);
+    rc.load(pc, dir * p.cs[1], t0, n, p.dc, tid);
+    if constexpr (FULL) ra.load(pa, dir * p.as[1], t0, n, p.da, tid);
+  };
+  if (begin < end) fetch(begin);
+  for (int t0 = begin; t0 < end; t0 += C) {
+    const int n = min(C, end - t0);  // live steps
+    rb.store(tb, tid);
+    rc.store(tc, tid);
+    if constexpr (FULL) ra.store(ta, tid);
     __syncthreads();
+    if (t0 + C < end) fetch(t0 + C);
 
+    if constexpr (FULL) {
     // scores: tile (it, jt <= it) as its transpose, so that a lane holds 4 consecutive j of
     // one i; rounded to E for the product with V (the output is E as well)
     for (int q = wave; q < CT * (CT + 1) / 2; q += W) {
@@ -133,6 +175,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
       *reinterpret_cast<quad_t<E>*>(tp + (16 * it + lo) * LDP + 16 * jt + 4 * hi) = to_quad<E>(acc);
     }
     __syncthreads();
+    }
 
     // the wave's values, contracted over the steps
     quad_t<E> v[CT][NV];
@@ -142,6 +185,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
       for (int x = 0; x < NV; ++x) v[j][x] = lds_quad_t(tc, LDC, 16 * j, col0 + 16 * x, lane);
 
     // O^T tiles: columns i, rows the values
+    if constexpr (FULL) {
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
       const int i = 16 * it + lo;
@@ -178,6 +222,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
             store_quad(reinterpret_cast<E*>(p.o) + row, c, p.dc, acc[x]);
         }
       }
+    }
     }
 
     // S update.  The decayed values are not exact in bf16: they enter as a sum of three bf16
@@ -220,16 +265,20 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
     __syncthreads();  // the tiles are free
   }
 
-  // steps past the end
-  for (int64_t e = (int64_t)L * p.dc + tid; e < (int64_t)p.T * p.dc; e += S::THREADS) {
-    const int64_t t = e / p.dc, c = e - t * p.dc;
-    if (p.o_f32)
-      reinterpret_cast<float*>(p.o)[obase + t * orow + c] = 0.0f;
-    else
-      reinterpret_cast<E*>(p.o)[obase + t * orow + c] = E(0.0f);
+  if constexpr (FULL) {
+    // this run's steps past the end
+    const int64_t z0 = max(L, begin), z1 = min(p.T, begin + p.seg_len);
+    for (int64_t e = z0 * p.dc + tid; e < z1 * p.dc; e += S::THREADS) {
+      const int64_t t = e / p.dc, c = e - t * p.dc;
+      if (p.o_f32)
+        reinterpret_cast<float*>(p.o)[obase + t * orow + c] = 0.0f;
+      else
+        reinterpret_cast<E*>(p.o)[obase + t * orow + c] = E(0.0f);
+    }
   }
-  if (p.s_out) {
-    float* out = p.s_out + (int64_t)blockIdx.x * p.da * p.dc;
+  // the run that holds the last live step has the final state
+  float* out = FULL ? (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0) ? p.s_out + sbase : nullptr) : seg_state;
+  if (out) {
 #pragma unroll
     for (int m = 0; m < KA; ++m)
 #pragma unroll
@@ -239,6 +288,39 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS)) void attn_chunk_ke
           const int row = 16 * m + 4 * hi + r, col = col0 + 16 * n + lo;
           if (row < p.da && col < p.dc) out[(int64_t)row * p.dc + col] = s[m][n][r];
         }
+  }
+}
+
+// Between the passes of a split history: each run's own sum becomes the state it starts
+// from.  A thread an element of the state; the loads of eight runs are in flight.
+template <typename E>
+__global__ __launch_bounds__(256) void attn_scan_kernel(AttnArgs<E> p) {
+  const int n = p.da * p.dc, per = (n + 255) / 256;
+  const int bh = blockIdx.x / per, e = (blockIdx.x - bh * per) * 256 + threadIdx.x;
+  if (e >= n) return;
+  const int b = bh / p.H, h = bh - b * p.H;
+  const float g = p.log_decay[h];
+  const int L = attn_length(p, b);
+  float v = 0.0f;
+  if (p.s_in) {
+    const int row = e / p.dc, col = e - row * p.dc;
+    v = p.s_in[(int64_t)bh * n + (p.s_in_t ? col * p.da + row : e)];
+  }
+  float* x = p.seg_state + (int64_t)bh * p.segs * n + e;
+  constexpr int AHEAD = 8;
+  for (int i0 = 0; i0 < p.segs; i0 += AHEAD) {
+    float u[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) u[i] = i0 + i < p.segs ? x[(int64_t)(i0 + i) * n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int seg = i0 + i;
+      if (seg < p.segs) {
+        x[(int64_t)seg * n] = v;
+        const int len = min(max(L - seg * p.seg_len, 0), p.seg_len);
+        v = v * decay_pow(g, len) + u[i];
+      }
+    }
   }
 }
 

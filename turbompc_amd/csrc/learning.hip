@@ -96,13 +96,43 @@ bool attn_shape_ok(const tmpc_decay_attention* a) {
          a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 0x7fffffff;
 }
 
+// One long history of few heads does not fill the chip, its chunks following one another:
+// it is cut into runs of whole chunks.  A first pass sums each run on its own (keys and
+// values alone), a scan carries the states through, and the outputs start from those.
+struct AttnSplit {
+  int segs, len;
+};
 template <typename E>
-void launch_attn(hipStream_t st, const AttnArgs<E>& p) {
+AttnSplit attn_split(int64_t bh, int T) {
+  constexpr int C = AttnTile<E>::C;
+  const int64_t chunks = std::max<int64_t>(1, ceil_div(T, C));
+  // a run of fewer than 8 chunks costs more in its state's traffic than it gains
+  const int64_t want = bh >= kCUs ? 1 : std::min(ceil_div(2 * kCUs, bh), std::max<int64_t>(1, chunks / 8));
+  const int64_t len = ceil_div(chunks, want);
+  return {(int)ceil_div(chunks, len), (int)(len * C)};
+}
+template <typename E>
+size_t attn_split_bytes(const tmpc_decay_attention* x) {
+  const int64_t bh = (int64_t)x->B * x->H;
+  const int segs = bh > 0 ? attn_split<E>(bh, x->T).segs : 1;
+  return segs > 1 ? align_up((size_t)bh * segs * x->dk * x->dv * sizeof(float)) : 0;
+}
+
+template <typename E>
+void launch_attn(hipStream_t st, AttnArgs<E> p, float* seg_state) {
+  const AttnSplit split = attn_split<E>((int64_t)p.B * p.H, p.T);
+  p.segs = split.segs, p.seg_len = split.len, p.seg_state = seg_state;
   auto go = [&](auto da, auto dc) {
     using S = AttnShape<E, da(), dc()>;
-    auto k = attn_chunk_kernel<E, da(), dc()>;
+    const dim3 grid((unsigned)(p.B * p.H * p.segs));
+    if (p.segs > 1) {
+      hipLaunchKernelGGL((attn_chunk_kernel<E, da(), dc(), false>), grid, dim3(S::THREADS), S::LDS_STATE, st, p);
+      hipLaunchKernelGGL((attn_scan_kernel<E>), dim3((unsigned)(p.B * p.H * ceil_div(p.da * p.dc, 256))), dim3(256), 0,
+                         st, p);
+    }
+    auto k = attn_chunk_kernel<E, da(), dc(), true>;
     lds_optin(k, S::LDS);
-    hipLaunchKernelGGL(k, dim3((unsigned)(p.B * p.H)), dim3(S::THREADS), S::LDS, st, p);
+    hipLaunchKernelGGL(k, grid, dim3(S::THREADS), S::LDS, st, p);
   };
   using std::integral_constant;
   auto with_c = [&](auto da) {
@@ -126,9 +156,10 @@ AttnArgs<E> attn_args(const tmpc_decay_attention* x) {
 
 template <typename E>
 size_t attn_ws_bytes(const tmpc_decay_attention* x, bool backward) {
-  if (!backward || x->H == x->Hk) return 0;
+  const size_t split = attn_split_bytes<E>(x);
+  if (!backward || x->H == x->Hk) return split;
   const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
-  return align_up(tok * x->dk) + align_up(tok * x->dv);
+  return split + align_up(tok * x->dk) + align_up(tok * x->dv);
 }
 
 template <typename E>
@@ -136,14 +167,16 @@ int attn_forward_impl(hipStream_t st, const tmpc_decay_attention* x, void* o, fl
   if (!attn_shape_ok(x)) return TMPC_EBADSHAPE;
   if (x->B == 0) return TMPC_OK;
   if (!x->log_decay || (x->T > 0 && (!x->q || !x->k || !x->v || !o))) return TMPC_EBADARG;
-  if (wsb < attn_ws_bytes<E>(x, false)) return TMPC_EWORKSPACE;
+  const size_t need = attn_ws_bytes<E>(x, false);
+  if (wsb < need) return TMPC_EWORKSPACE;
+  if (need > 0 && !ws) return TMPC_EBADARG;
   AttnArgs<E> p = attn_args<E>(x);
   p.a = (const E*)x->q, p.b = (const E*)x->k, p.c = (const E*)x->v;
   std::copy_n(x->q_stride, 3, p.as), std::copy_n(x->k_stride, 3, p.bs), std::copy_n(x->v_stride, 3, p.cs);
   p.gb = p.gc = x->H / x->Hk;
   p.ss = p.si = (float)x->scale, p.su = 1.0f;
   p.s_in = x->state_in, p.s_out = state_out, p.o = o;
-  launch_attn(st, p);
+  launch_attn(st, p, (float*)ws);
   return launch_status();
 }
 
@@ -157,6 +190,8 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
     return TMPC_EBADARG;
   if (wsb < attn_ws_bytes<E>(x, true)) return TMPC_EWORKSPACE;
   if (attn_ws_bytes<E>(x, true) > 0 && !ws) return TMPC_EBADARG;
+  float* seg_state = (float*)ws;
+  char* rest = (char*)ws + attn_split_bytes<E>(x);
   const int G = x->H / x->Hk;
   const float scale = (float)x->scale;
   {  // dq: (do, v, k) from the transposed state
@@ -167,11 +202,11 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
     p.gb = p.gc = G;
     p.ss = p.si = scale, p.su = 1.0f;
     p.s_in = x->state_in, p.s_in_t = 1, p.o = dq;
-    launch_attn(st, p);
+    launch_attn(st, p, seg_state);
   }
   const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
-  float* gk = G > 1 ? (float*)ws : nullptr;
-  float* gv = G > 1 ? (float*)((char*)ws + align_up(tok * x->dk)) : nullptr;
+  float* gk = G > 1 ? (float*)rest : nullptr;
+  float* gv = G > 1 ? (float*)(rest + align_up(tok * x->dk)) : nullptr;
   {  // dk: backwards, (v, do, q) from the transposed gradient of the state
     AttnArgs<E> p = attn_args<E>(x);
     p.da = x->dv, p.dc = x->dk, p.rev = 1;
@@ -181,7 +216,7 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
     p.ss = p.su = scale, p.si = 1.0f;
     p.s_in = d_state_out, p.s_in_t = 1;
     p.o = gk ? (void*)gk : dk, p.o_f32 = gk != nullptr;
-    launch_attn(st, p);
+    launch_attn(st, p, seg_state);
   }
   {  // dv: backwards, (k, q, do)
     AttnArgs<E> p = attn_args<E>(x);
@@ -192,7 +227,7 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
     p.ss = p.su = scale, p.si = 1.0f;
     p.s_in = d_state_out, p.s_out = d_state_in;
     p.o = gv ? (void*)gv : dv, p.o_f32 = gv != nullptr;
-    launch_attn(st, p);
+    launch_attn(st, p, seg_state);
   }
   if (G > 1 && x->T > 0) {
     auto sum = [&](const float* in, int d, void* out) {
