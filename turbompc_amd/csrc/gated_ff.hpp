@@ -41,6 +41,7 @@ template <typename E>
 struct GemmArgs {
   int64_t M;
   int N, nseg;
+  int pair;          // 1: two products A_0^T B_0 -> o0 and A_1^T B_0 -> o1, the grid's x twice as long
   int64_t K;
   const E *A[2], *B[2];
   int64_t lda, ldb;
@@ -48,7 +49,7 @@ struct GemmArgs {
   E *o0, *o1, *o2;
   float *g, *u;      // the saved projections: fp32, for rounding them would double the gradients' error
   int64_t ldo, ldg;  // pitches of o* and of g, u
-  float* part;       // split over K: (splits, M, N) partial sums
+  float* part;       // split over K: (splits, 1 + pair, M, N) partial sums
   int64_t k_split;   // contracted entries of a split (a multiple of the K tile)
 };
 
@@ -119,95 +120,39 @@ struct Stage {
       *reinterpret_cast<piece_t<E>*>(t + row * LD + c) = r[i];
     }
   }
-  // the quad of outer rows 16 o .., contracted entries 16 k ..
-  __device__ static quad_t<E> quad(const E* t, int row0, int k0, int lane) {
-    if constexpr (TR)
-      return lds_quad_t(t, LD, k0, row0, lane);
-    else
-      return lds_quad(t, LD, row0, k0, lane);
+  // The quads of outer rows row0 + 0..15 over 32 contracted entries from k0.  WHOLE: a lane
+  // takes 8 consecutive entries (one 16-byte read), which both operands have to do.
+  template <bool WHOLE>
+  __device__ static void quads(const E* t, int row0, int k0, int lane, quad_t<E>& q0, quad_t<E>& q1) {
+    if constexpr (TR) {
+      q0 = lds_quad_t(t, LD, k0, row0, lane);
+      q1 = lds_quad_t(t, LD, k0 + 16, row0, lane);
+    } else if constexpr (WHOLE && sizeof(E) == 2) {
+      const piece_t<E> v = *reinterpret_cast<const piece_t<E>*>(t + (row0 + (lane & 15)) * LD + k0 + 8 * (lane >> 4));
+      q0 = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+      q1 = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    } else {
+      q0 = lds_quad(t, LD, row0, k0, lane);
+      q1 = lds_quad(t, LD, row0, k0 + 16, lane);
+    }
   }
 };
 
-// BM x BN tile by WM x WN waves; BN counts both projections' columns with DUAL.
-template <typename E, int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI, int ACT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs<E> p) {
+// A wave's results: TM x TN tiles from row m0 and column tile j0 of the block's n0; a lane
+// has row i * 16 + lo, 4 consecutive columns.
+template <typename E, int EPI, int ACT, int TM, int TN>
+__device__ inline void gemm_epilogue(const GemmArgs<E>& p, const f32x4 (&acc)[TM][TN], int which, int64_t m0, int64_t n0,
+                                     int j0, int lo, int hi) {
   constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
-  constexpr int THREADS = 64 * WM * WN, BK = GemmTile<E>::BK;
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int BF = DUAL ? BN / 2 : BN;  // output columns of the tile
-  using SA = Stage<E, BM, THREADS, AT, false>;
-  using SB = Stage<E, BN, THREADS, BT, DUAL>;
-  extern __shared__ __align__(16) char smem[];
-  E* ta = reinterpret_cast<E*>(smem);
-  E* tb = ta + 2 * SA::ELEMS;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
-  const int wm = wave / WN, wn = wave - wm * WN;
-  const int64_t m0 = (int64_t)blockIdx.x * BM;
-  const int64_t n0 = (int64_t)blockIdx.y * BF;
-  const int64_t kb = (int64_t)blockIdx.z * p.k_split;
-  const int64_t ke = EPI == EPI_PART ? (kb + p.k_split < p.K ? kb + p.k_split : p.K) : p.K;
-  const int tiles = (int)((ke - kb + BK - 1) / BK), total = tiles * (DUAL ? 1 : p.nseg);
-
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-
-  SA sa;
-  SB sb;
-  int seg = 0;
-  int64_t k = kb;
-  if (total > 0) {
-    sa.load(p.A, 0, p.lda, m0, p.M, k, ke, tid);
-    sb.load(p.B, 0, p.ldb, n0, p.N, k, ke, tid);
-    sa.store(ta, tid);
-    sb.store(tb, tid);
-  }
-  __syncthreads();
-  for (int it = 0; it < total; ++it) {
-    const E* ca = ta + (it & 1) * SA::ELEMS;
-    const E* cb = tb + (it & 1) * SB::ELEMS;
-    const bool more = it + 1 < total;
-    if (more) {
-      k += BK;
-      if (k >= ke) k = kb, ++seg;
-      sa.load(p.A, seg, p.lda, m0, p.M, k, ke, tid);
-      sb.load(p.B, seg, p.ldb, n0, p.N, k, ke, tid);
-    }
-#pragma unroll
-    for (int kk = 0; kk < BK; kk += 32) {
-      quad_t<E> a0[TM], a1[TM];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        a0[i] = SA::quad(ca, (wm * TM + i) * 16, kk, lane);
-        a1[i] = SA::quad(ca, (wm * TM + i) * 16, kk + 16, lane);
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const quad_t<E> b0 = SB::quad(cb, (wn * TN + j) * 16, kk, lane);
-        const quad_t<E> b1 = SB::quad(cb, (wn * TN + j) * 16, kk + 16, lane);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][j] = mma2(b0, b1, a0[i], a1[i], acc[i][j]);
-      }
-    }
-    if (more) {  // the other buffer was last read before the previous barrier
-      sa.store(ta + ((it + 1) & 1) * SA::ELEMS, tid);
-      sb.store(tb + ((it + 1) & 1) * SB::ELEMS, tid);
-    }
-    __syncthreads();
-  }
-
-  // lane: row m, 4 consecutive columns
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int64_t m = m0 + (wm * TM + i) * 16 + lo;
+    const int64_t m = m0 + i * 16 + lo;
     if (m >= p.M) continue;
     if constexpr (DUAL) {
       static_assert(TN % 2 == 0, "a wave holds both projections of its features");
 #pragma unroll
       for (int j = 0; j < TN; j += 2) {
-        const int64_t c = n0 + (wn * TN + j) * 8 + 4 * hi;
+        const int64_t c = n0 + (j0 + j) * 8 + 4 * hi;
         f32x4 hv;
 #pragma unroll
         for (int r = 0; r < 4; ++r) hv[r] = act_only<ACT>(acc[i][j][r]) * acc[i][j + 1][r];
@@ -221,12 +166,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs<E> p) {
     } else {
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int64_t c = n0 + (wn * TN + j) * 16 + 4 * hi;
+        const int64_t c = n0 + (j0 + j) * 16 + 4 * hi;
         if (c >= p.N) continue;
         if constexpr (EPI == EPI_STORE) {
-          store_quad(p.o0 + m * p.ldo, (int)c, p.N, acc[i][j]);
+          store_quad((which ? p.o1 : p.o0) + m * p.ldo, (int)c, p.N, acc[i][j]);
         } else if constexpr (EPI == EPI_PART) {
-          store_quad(p.part + ((int64_t)blockIdx.z * p.M + m) * p.N, (int)c, p.N, acc[i][j]);
+          store_quad(p.part + ((int64_t)(blockIdx.z * (1 + p.pair) + which) * p.M + m) * p.N, (int)c, p.N, acc[i][j]);
         } else {
           const f32x4 gv = load_quad_f32(p.g + m * p.ldg, (int)c, p.N), uv = load_quad_f32(p.u + m * p.ldg, (int)c, p.N);
           f32x4 dg, du, hv;
@@ -245,15 +190,179 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs<E> p) {
   }
 }
 
-// out = sum of the partial sums over the splits, in order
-template <typename E>
-__global__ __launch_bounds__(256) void gemm_reduce_kernel(const float* __restrict__ part, int64_t n, int splits,
-                                                          E* __restrict__ out) {
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v += part[(int64_t)s * n + e];
-    out[e] = (E)v;
+// BM x BN tile by WM x WN waves; BN counts both projections' columns with DUAL.
+template <typename E, int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI, int ACT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs<E> p) {
+  constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
+  constexpr int THREADS = 64 * WM * WN, BK = GemmTile<E>::BK;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr bool WHOLE = !AT && !BT;
+  constexpr int BF = DUAL ? BN / 2 : BN;  // output columns of the tile
+  using SA = Stage<E, BM, THREADS, AT, false>;
+  using SB = Stage<E, BN, THREADS, BT, DUAL>;
+  extern __shared__ __align__(16) char smem[];
+  E* ta = reinterpret_cast<E*>(smem);
+  E* tb = ta + 2 * SA::ELEMS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int wm = wave / WN, wn = wave - wm * WN;
+  const int which = p.pair && blockIdx.x >= gridDim.x / 2;
+  const int64_t m0 = (int64_t)(blockIdx.x - which * (gridDim.x / 2)) * BM;
+  const int64_t n0 = (int64_t)blockIdx.y * BF;
+  const int64_t kb = (int64_t)blockIdx.z * p.k_split;
+  const int64_t ke = EPI == EPI_PART ? (kb + p.k_split < p.K ? kb + p.k_split : p.K) : p.K;
+  const int tiles = (int)((ke - kb + BK - 1) / BK), total = tiles * (DUAL ? 1 : p.nseg);
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  SA sa;
+  SB sb;
+  int seg = 0;
+  int64_t k = kb;
+  if (total > 0) {
+    sa.load(p.A, which, p.lda, m0, p.M, k, ke, tid);
+    sb.load(p.B, 0, p.ldb, n0, p.N, k, ke, tid);
+    sa.store(ta, tid);
+    sb.store(tb, tid);
   }
+  __syncthreads();
+  for (int it = 0; it < total; ++it) {
+    const E* ca = ta + (it & 1) * SA::ELEMS;
+    const E* cb = tb + (it & 1) * SB::ELEMS;
+    const bool more = it + 1 < total;
+    if (more) {
+      k += BK;
+      if (k >= ke) k = kb, ++seg;
+      sa.load(p.A, seg + which, p.lda, m0, p.M, k, ke, tid);
+      sb.load(p.B, seg, p.ldb, n0, p.N, k, ke, tid);
+    }
+#pragma unroll
+    for (int kk = 0; kk < BK; kk += 32) {
+      quad_t<E> a0[TM], a1[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) SA::template quads<WHOLE>(ca, (wm * TM + i) * 16, kk, lane, a0[i], a1[i]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        quad_t<E> b0, b1;
+        SB::template quads<WHOLE>(cb, (wn * TN + j) * 16, kk, lane, b0, b1);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = mma2(b0, b1, a0[i], a1[i], acc[i][j]);
+      }
+    }
+    if (more) {  // the other buffer was last read before the previous barrier
+      sa.store(ta + ((it + 1) & 1) * SA::ELEMS, tid);
+      sb.store(tb + ((it + 1) & 1) * SB::ELEMS, tid);
+    }
+    __syncthreads();
+  }
+
+  gemm_epilogue<E, EPI, ACT, TM, TN>(p, acc, which, m0 + wm * TM * 16, n0, wn * TN, lo, hi);
+}
+
+// The partial sums over the splits, in order: (splits, outputs, n) -> o0 and, of two
+// outputs, o1.  A thread 4 entries.
+template <typename E>
+__global__ __launch_bounds__(256) void gemm_reduce_kernel(const float* __restrict__ part, int64_t n, int outputs,
+                                                          int splits, E* __restrict__ o0, E* __restrict__ o1) {
+  const int64_t all = n * outputs;
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < all; e += (int64_t)gridDim.x * 1024) {
+    f32x4 v = {0, 0, 0, 0};
+    if (e + 4 <= all) {
+      for (int s = 0; s < splits; ++s) v += load_quad_f32(part + (int64_t)s * all + e, 0, 4);
+    } else {
+      for (int s = 0; s < splits; ++s) v += load_quad_f32(part + (int64_t)s * all + e, 0, (int)(all - e));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t i = e + r;
+      if (i < n) o0[i] = (E)v[r];
+      else if (i < all) o1[i - n] = (E)v[r];
+    }
+  }
+}
+
+// Few rows (M <= 16 MT): bound by reading the weights, and below that by latency.  A
+// workgroup has one tile of 16 output columns; its eight waves share the contracted
+// index, each reading its own 32-entry steps straight into operands, and meet in LDS.
+template <typename E, int MT, int EPI, int ACT>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs<E> p) {
+  constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
+  constexpr int NB = DUAL ? 2 : 1, P = Elem<E>::PIECE, STEP = 4 * P;  // contracted entries of a step
+  __shared__ f32x4 red[8][MT * NB][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n = n0 + lo < p.N ? n0 + lo : p.N - 1;  // past the edge: results not stored
+  const E* b[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) b[i] = p.B[i] + n * p.ldb;
+  const E* a[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = 16 * i + lo < p.M ? 16 * i + lo : p.M - 1;
+    a[i] = p.A[0] + m * p.lda;
+  }
+  f32x4 acc[MT][NB];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  auto mul = [&](const piece_t<E>(&pa)[MT], const piece_t<E>(&pb)[NB]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        if constexpr (sizeof(E) == 2) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pb[j], pa[i], acc[i][j], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(pb[j][e], pa[i][e], acc[i][j], 0, 0, 0);
+        }
+      }
+  };
+  // whole steps, U at a time so that their loads are in flight together
+  constexpr int U = 4;
+  const int64_t steps = p.K / STEP;
+  int64_t s = wave;
+  for (; s + 8 * (U - 1) < steps; s += 8 * U) {
+    piece_t<E> pa[U][MT], pb[U][NB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = (s + 8 * u) * STEP + P * hi;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) pb[u][j] = *reinterpret_cast<const typename Elem<E>::piece_u*>(b[j] + k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) pa[u][i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(a[i] + k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) mul(pa[u], pb[u]);
+  }
+  for (; s * STEP < p.K; s += 8) {
+    const int64_t k = s * STEP;
+    piece_t<E> pa[MT], pb[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) pb[j] = load_piece(b[j] + k, P * hi, (int)(p.K - k < STEP ? p.K - k : STEP), true);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) pa[i] = load_piece(a[i] + k, P * hi, (int)(p.K - k < STEP ? p.K - k : STEP), true);
+    mul(pa, pb);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) red[wave][i * NB + j][lane] = acc[i][j];
+  __syncthreads();
+  if (wave >= MT) return;
+  f32x4 sum[1][NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    sum[0][j] = red[0][wave * NB + j][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum[0][j] += red[w][wave * NB + j][lane];
+  }
+  gemm_epilogue<E, EPI, ACT, 1, NB>(p, sum, 0, 16 * wave, n0, 0, lo, hi);
 }
 
 template <typename E, int BM, int BN, bool AT, bool BT, int THREADS, bool DUAL>

@@ -5,6 +5,7 @@
 #include "../../include/tmpc.h"
 #include "decay_attention.hpp"
 #include "gated_ff.hpp"
+#include "gemm_wide.hpp"
 #include "rms_norm.hpp"
 
 namespace tmpc {
@@ -265,64 +266,133 @@ int64_t ff_pitch(const tmpc_gated_ff* a) {
   return ceil_div(a->F, Elem<E>::PIECE) * Elem<E>::PIECE;
 }
 
+// How a product runs: few rows (gemm_rows_kernel), the wide kernel, or tiles of 128, 64
+// or 32 rows; splits of the contracted index.
+enum GemmForm { FORM_ROWS, FORM_WIDE, FORM_128, FORM_64, FORM_32 };
+struct GemmPlan {
+  GemmForm form;
+  int splits;
+};
+
+inline int64_t tiles_of(int64_t rows, int64_t cols, int bm, int bf) { return ceil_div(rows, bm) * ceil_div(cols, bf); }
+
+// The wide kernel moves 16-byte pieces between memory and LDS: rows of whole pieces.
+template <typename E>
+bool wide_ok(const GemmArgs<E>& p, bool at, bool bt, bool own_a, bool own_b) {
+  if (sizeof(E) != 2) return false;
+  auto aligned = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
+  for (int i = 0; i < 2; ++i)
+    if (!aligned(p.A[i]) || !aligned(p.B[i])) return false;
+  // a transposed operand's last piece reaches past its columns, within the pitch of the
+  // block's own arrays alone
+  return p.lda % 8 == 0 && p.ldb % 8 == 0 && (!at || own_a || p.M % 8 == 0) && (!bt || own_b || p.N % 8 == 0);
+}
+
 template <typename E, bool AT, bool BT, int EPI, int ACT = 0>
-void launch_gemm(hipStream_t st, GemmArgs<E> p, int splits = 1) {
+void launch_gemm(hipStream_t st, GemmArgs<E> p, GemmPlan plan) {
   constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
-  auto go = [&](auto bm, auto bn, auto wm, auto wn) {
-    constexpr int BM = bm(), BN = bn(), THREADS = 64 * wm() * wn();
-    constexpr size_t lds = gemm_lds<E, BM, BN, AT, BT, THREADS, DUAL>();
-    auto k = gemm_kernel<E, BM, BN, wm(), wn(), AT, BT, EPI, ACT>;
+  if (plan.splits == 1) p.k_split = std::max<int64_t>(p.K, 1);
+  auto grid = [&](int bm, int bf) {
+    return dim3((unsigned)(ceil_div(p.M, bm) * (1 + p.pair)), (unsigned)ceil_div(p.N, bf), (unsigned)plan.splits);
+  };
+  auto go = [&](auto bm, auto bn) {
+    constexpr int BM = bm(), BN = bn();
+    constexpr size_t lds = gemm_lds<E, BM, BN, AT, BT, 256, DUAL>();
+    auto k = gemm_kernel<E, BM, BN, 2, 2, AT, BT, EPI, ACT>;
     lds_optin(k, lds);
-    const dim3 grid((unsigned)ceil_div(p.M, BM), (unsigned)ceil_div(p.N, DUAL ? BN / 2 : BN), (unsigned)splits);
-    hipLaunchKernelGGL(k, grid, dim3(THREADS), lds, st, p);
+    hipLaunchKernelGGL(k, grid(BM, DUAL ? BN / 2 : BN), dim3(256), lds, st, p);
   };
   using std::integral_constant;
-  if (splits == 1) p.k_split = std::max<int64_t>(p.K, 1);
-  go(integral_constant<int, 128>(), integral_constant<int, 128>(), integral_constant<int, 2>(),
-     integral_constant<int, 2>());
+  switch (plan.form) {
+    case FORM_ROWS:
+      if constexpr (!AT && !BT && EPI != EPI_PART) {
+        auto rows = [&](auto mt) {
+          hipLaunchKernelGGL((gemm_rows_kernel<E, mt(), EPI, ACT>), dim3((unsigned)ceil_div(p.N, 16)), dim3(512), 0, st, p);
+        };
+        if (p.M <= 16) rows(integral_constant<int, 1>());
+        else if (p.M <= 32) rows(integral_constant<int, 2>());
+        else rows(integral_constant<int, 4>());
+      }
+      break;
+    case FORM_WIDE:
+      if constexpr (sizeof(E) == 2) {
+        auto k = gemm_wide_kernel<AT, BT, EPI, ACT>;
+        lds_optin(k, kWideLds);
+        hipLaunchKernelGGL(k, grid(256, DUAL ? 128 : 256), dim3(512), kWideLds, st, p);
+      }
+      break;
+    case FORM_128: go(integral_constant<int, 128>(), integral_constant<int, 128>()); break;
+    case FORM_64: go(integral_constant<int, 64>(), integral_constant<int, 64>()); break;
+    case FORM_32: go(integral_constant<int, 32>(), integral_constant<int, 64>()); break;
+  }
 }
 
-// the weight gradients' rows are few and their contracted index is every row of the
-// batch: it is split until the tiles fill the chip
-template <typename E>
-int ff_splits(int64_t rows, int64_t cols, int64_t K) {
-  const int64_t tiles = ceil_div(rows, 128) * ceil_div(cols, 128);
-  const int64_t want = std::max<int64_t>(1, 2 * kCUs / tiles);
-  return (int)std::min<int64_t>(want, std::max<int64_t>(1, K / (8 * GemmTile<E>::BK)));
+// The form for a product that is not split: the largest tile that still gives most of the
+// chip work.
+template <typename E, bool AT, bool BT, int EPI>
+GemmPlan gemm_plan(const GemmArgs<E>& p, bool own_a, bool own_b) {
+  constexpr int D = EPI == EPI_GATE || EPI == EPI_GATE_SAVE ? 2 : 1;
+  if (!AT && !BT && p.nseg == 1 && p.M <= 64) return {FORM_ROWS, 1};
+  if (wide_ok(p, AT, BT, own_a, own_b) && tiles_of(p.M, p.N, 256, 256 / D) >= 96) return {FORM_WIDE, 1};
+  if (tiles_of(p.M, p.N, 128, 128 / D) >= 192) return {FORM_128, 1};
+  if (tiles_of(p.M, p.N, 64, 64 / D) >= 192) return {FORM_64, 1};
+  return {FORM_32, 1};
 }
 
+// The weight gradients' rows are few and their contracted index is every row of the batch:
+// it is split until the tiles fill the chip (of the `pair` products together), with at
+// least 8 K steps a split.  The same for every alignment, since it sizes the workspace.
 template <typename E>
-size_t ff_part_bytes(int64_t rows, int64_t cols, int64_t K) {
-  const int s = ff_splits<E>(rows, cols, K);
-  return s > 1 ? align_up((size_t)s * rows * cols * sizeof(float)) : 0;
+int grad_splits(int64_t rows, int64_t cols, int64_t K, int pair, int tile) {
+  const int64_t tiles = tiles_of(rows, cols, tile, tile) * (1 + pair);
+  return (int)std::max<int64_t>(1, std::min((tile == 256 ? 1 : 2) * kCUs / tiles, K / (8 * GemmTile<E>::BK)));
+}
+// the tile of a weight gradient: 256 where it wastes little of its edges, else 128, and 64
+// where those are few even when split
+template <typename E>
+int grad_tile(int64_t rows, int64_t cols, int64_t K, int pair) {
+  if (sizeof(E) == 2 && rows >= 192 && cols >= 192 && tiles_of(rows, cols, 256, 256) * 256 * 256 <= rows * cols * 3 / 2)
+    return 256;
+  const int64_t t = tiles_of(rows, cols, 128, 128) * (1 + pair);
+  return t * grad_splits<E>(rows, cols, K, pair, 128) >= kCUs / 2 ? 128 : 64;
+}
+template <typename E>
+size_t grad_part_bytes(int64_t rows, int64_t cols, int64_t K, int pair) {
+  // the wide kernel's tile and the one that stands in for it where the operands are not aligned
+  int most = 1;
+  for (int tile : {grad_tile<E>(rows, cols, K, pair), 128})
+    most = std::max(most, grad_splits<E>(rows, cols, K, pair, tile));
+  return most > 1 ? align_up((size_t)most * (1 + pair) * rows * cols * sizeof(float)) : 0;
 }
 
 template <typename E>
 size_t ff_ws_bytes(const tmpc_gated_ff* a, bool backward) {
   const size_t act = align_up((size_t)a->M * ff_pitch<E>(a) * sizeof(E));
   if (!backward) return act;
-  return 3 * act + std::max(ff_part_bytes<E>(a->F, a->D, a->M), ff_part_bytes<E>(a->Dout, a->F, a->M));
+  return 3 * act + std::max(grad_part_bytes<E>(a->F, a->D, a->M, 1), grad_part_bytes<E>(a->Dout, a->F, a->M, 0));
 }
 
-// dW (rows, cols) = P^T X over the batch's M rows
+// dW (rows, cols) = P^T X over the batch's M rows, and with P1 a second one beside it
 template <typename E>
-void launch_weight_grad(hipStream_t st, int64_t M, int rows, int cols, const E* P, int64_t ldp, const E* X, int64_t ldx,
-                        E* out, float* part) {
+void launch_weight_grad(hipStream_t st, int64_t M, int rows, int cols, const E* P, const E* P1, int64_t ldp, bool own_p,
+                        const E* X, int64_t ldx, bool own_x, E* out, E* out1, float* part) {
   GemmArgs<E> p{};
-  p.M = rows, p.N = cols, p.nseg = 1, p.K = M;
-  p.A[0] = P, p.lda = ldp, p.B[0] = X, p.ldb = ldx;
-  p.o0 = out, p.ldo = cols;
-  const int splits = ff_splits<E>(rows, cols, M);
-  if (splits == 1) {
-    launch_gemm<E, true, true, EPI_STORE>(st, p);
+  p.M = rows, p.N = cols, p.nseg = 1, p.K = M, p.pair = P1 != nullptr;
+  p.A[0] = P, p.A[1] = P1, p.lda = ldp, p.B[0] = X, p.ldb = ldx;
+  p.o0 = out, p.o1 = out1, p.ldo = cols, p.part = part;
+  int tile = grad_tile<E>(rows, cols, M, p.pair);
+  if (tile == 256 && !wide_ok(p, true, true, own_p, own_x)) tile = 128;
+  const GemmPlan plan{tile == 256 ? FORM_WIDE : tile == 128 ? FORM_128 : FORM_64,
+                      grad_splits<E>(rows, cols, M, p.pair, tile)};
+  if (plan.splits == 1) {
+    launch_gemm<E, true, true, EPI_STORE>(st, p, plan);
     return;
   }
-  p.part = part;
-  p.k_split = ceil_div(ceil_div(M, GemmTile<E>::BK), splits) * GemmTile<E>::BK;
-  launch_gemm<E, true, true, EPI_PART>(st, p, splits);
+  p.k_split = ceil_div(ceil_div(M, GemmTile<E>::BK), plan.splits) * GemmTile<E>::BK;
+  launch_gemm<E, true, true, EPI_PART>(st, p, plan);
   const int64_t n = (int64_t)rows * cols;
-  hipLaunchKernelGGL((gemm_reduce_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 16 * kCUs)), dim3(256),
-                     0, st, part, n, splits, out);
+  hipLaunchKernelGGL((gemm_reduce_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n * (1 + p.pair), 1024), 8 * kCUs)),
+                     dim3(256), 0, st, part, n, 1 + p.pair, plan.splits, out, out1);
 }
 
 template <typename E>
@@ -341,17 +411,18 @@ int ff_forward_impl(hipStream_t st, const tmpc_gated_ff* a, void* y, float* gate
   p.A[0] = (const E*)a->x, p.lda = a->ldx;
   p.B[0] = (const E*)a->w_gate, p.B[1] = (const E*)a->w_up, p.ldb = a->D;
   p.o0 = h, p.ldo = ldh, p.g = gate, p.u = up, p.ldg = a->F;
+  const GemmPlan plan = gemm_plan<E, false, false, EPI_GATE>(p, false, false);
   if (a->activation == ACT_SILU) {
-    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_SILU>(st, p);
-    else launch_gemm<E, false, false, EPI_GATE, ACT_SILU>(st, p);
+    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_SILU>(st, p, plan);
+    else launch_gemm<E, false, false, EPI_GATE, ACT_SILU>(st, p, plan);
   } else {
-    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_GELU>(st, p);
-    else launch_gemm<E, false, false, EPI_GATE, ACT_GELU>(st, p);
+    if (gate) launch_gemm<E, false, false, EPI_GATE_SAVE, ACT_GELU>(st, p, plan);
+    else launch_gemm<E, false, false, EPI_GATE, ACT_GELU>(st, p, plan);
   }
   GemmArgs<E> d{};
   d.M = a->M, d.N = a->Dout, d.nseg = 1, d.K = a->F;
   d.A[0] = h, d.lda = ldh, d.B[0] = (const E*)a->w_down, d.ldb = a->F, d.o0 = (E*)y, d.ldo = a->Dout;
-  launch_gemm<E, false, false, EPI_STORE>(st, d);
+  launch_gemm<E, false, false, EPI_STORE>(st, d, gemm_plan<E, false, false, EPI_STORE>(d, true, false));
   return launch_status();
 }
 
@@ -377,18 +448,18 @@ int ff_backward_impl(hipStream_t st, const tmpc_gated_ff* a, const float* gate, 
     p.M = a->M, p.N = a->F, p.nseg = 1, p.K = a->Dout;
     p.A[0] = (const E*)dy, p.lda = lddy, p.B[0] = (const E*)a->w_down, p.ldb = a->F;
     p.o0 = dg, p.o1 = du, p.o2 = h, p.ldo = ldh, p.g = const_cast<float*>(gate), p.u = const_cast<float*>(up), p.ldg = a->F;
-    if (a->activation == ACT_SILU) launch_gemm<E, false, true, EPI_DGATE, ACT_SILU>(st, p);
-    else launch_gemm<E, false, true, EPI_DGATE, ACT_GELU>(st, p);
+    const GemmPlan plan = gemm_plan<E, false, true, EPI_DGATE>(p, false, false);
+    if (a->activation == ACT_SILU) launch_gemm<E, false, true, EPI_DGATE, ACT_SILU>(st, p, plan);
+    else launch_gemm<E, false, true, EPI_DGATE, ACT_GELU>(st, p, plan);
     GemmArgs<E> d{};
     d.M = a->M, d.N = a->D, d.nseg = 2, d.K = a->F;
     d.A[0] = dg, d.A[1] = du, d.lda = ldh;
     d.B[0] = (const E*)a->w_gate, d.B[1] = (const E*)a->w_up, d.ldb = a->D;
     d.o0 = (E*)dx, d.ldo = a->D;
-    launch_gemm<E, false, true, EPI_STORE>(st, d);
+    launch_gemm<E, false, true, EPI_STORE>(st, d, gemm_plan<E, false, true, EPI_STORE>(d, true, false));
   }
-  launch_weight_grad<E>(st, a->M, a->F, a->D, dg, ldh, (const E*)a->x, a->ldx, (E*)dwg, part);
-  launch_weight_grad<E>(st, a->M, a->F, a->D, du, ldh, (const E*)a->x, a->ldx, (E*)dwu, part);
-  launch_weight_grad<E>(st, a->M, a->Dout, a->F, (const E*)dy, lddy, h, ldh, (E*)dwd, part);
+  launch_weight_grad<E>(st, a->M, a->F, a->D, dg, du, ldh, true, (const E*)a->x, a->ldx, false, (E*)dwg, (E*)dwu, part);
+  launch_weight_grad<E>(st, a->M, a->Dout, a->F, (const E*)dy, nullptr, lddy, false, h, ldh, true, (E*)dwd, nullptr, part);
   return launch_status();
 }
 
