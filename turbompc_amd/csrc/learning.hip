@@ -372,12 +372,12 @@ size_t ff_ws_bytes(const tmpc_gated_ff* a, bool backward) {
   return 3 * act + std::max(grad_part_bytes<E>(a->F, a->D, a->M, 1), grad_part_bytes<E>(a->Dout, a->F, a->M, 0));
 }
 
-// dW (rows, cols) = P^T X over the batch's M rows, and with P1 a second one beside it
+// dW (rows, cols) = P^T X over the batch's M rows, and with out1 a second one, P1^T X, beside it
 template <typename E>
 void launch_weight_grad(hipStream_t st, int64_t M, int rows, int cols, const E* P, const E* P1, int64_t ldp, bool own_p,
                         const E* X, int64_t ldx, bool own_x, E* out, E* out1, float* part) {
   GemmArgs<E> p{};
-  p.M = rows, p.N = cols, p.nseg = 1, p.K = M, p.pair = P1 != nullptr;
+  p.M = rows, p.N = cols, p.nseg = 1, p.K = M, p.pair = out1 != nullptr;
   p.A[0] = P, p.A[1] = P1, p.lda = ldp, p.B[0] = X, p.ldb = ldx;
   p.o0 = out, p.o1 = out1, p.ldo = cols, p.part = part;
   int tile = grad_tile<E>(rows, cols, M, p.pair);

@@ -11,6 +11,7 @@ raises TmpcError.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -24,32 +25,26 @@ MAX_HEAD_WIDTH = 128
 MAX_NORM_WIDTH = 8192
 
 
-def _suffix(dtype: torch.dtype) -> str:
-    if dtype not in _SUFFIX:
-        raise TypeError(f"unsupported dtype {dtype}; use float32 or bfloat16")
-    return _SUFFIX[dtype]
-
-
 def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape=None, dtype=None):
-    """t as given, with like's device and `dtype` (like's) and `shape`."""
-    if not torch.is_tensor(t):
+    """t has like's device and `dtype` (like's where None) and `shape`."""
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    dtype = like.dtype if dtype is None else dtype
-    if t.dtype != dtype:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.dtype is not (like.dtype if dtype is None else dtype):
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {like.dtype if dtype is None else dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t
 
 
 def _first(name: str, t: torch.Tensor, dims) -> str:
     """The suffix of the call whose first argument is t."""
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    sfx = _suffix(t.dtype)
-    if t.device.type != "cuda":
+    sfx = _SUFFIX.get(t.dtype)
+    if sfx is None:
+        raise TypeError(f"unsupported dtype {t.dtype}; use float32 or bfloat16")
+    if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}; the operators run on a HIP device")
     if t.dim() not in dims:
         raise ValueError(f"{name} has {t.dim()} dimensions, expected {' or '.join(map(str, dims))}")
@@ -58,38 +53,65 @@ def _first(name: str, t: torch.Tensor, dims) -> str:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous rows: itself where it has them."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
     """t as (rows, last axis) with contiguous rows: a view where one exists."""
-    return _rows(t.reshape(-1, t.shape[-1]))
+    return _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return t.data_ptr() if t is not None and t.numel() else None
+    return (t.data_ptr() or None) if t is not None else None  # an empty tensor's is null
+
+
+def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+_FUNCTIONS = {}
 
 
 def _call(fn: str, device: torch.device, *args):
-    with torch.cuda.device(device):
-        _lib.check(fn, getattr(_lib.load(), fn)(_lib.stream_handle(device), *args))
+    f = _FUNCTIONS.get(fn)
+    if f is None:
+        f = _FUNCTIONS[fn] = getattr(_lib.load(), fn)
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn, f(torch._C._cuda_getCurrentRawStream(device.index), *args))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn, f(_lib.stream_handle(device), *args))
+
+
+def _workspace(query: str, device: torch.device, *args):
+    """(bytes, tensor or None) of a call's workspace."""
+    nbytes = getattr(_lib.load(), query)(*args)
+    return nbytes, torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 # ------------------------------------------------------------------ norm --
+def _rms_forward(x, residual, weight, eps, sfx, rstd):
+    """(y, s); rstd: a (rows,) tensor to fill, or None."""
+    xm = _matrix(x)
+    rm = _matrix(residual) if residual is not None else None
+    M, D = xm.shape
+    y, s = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), xm.stride(0), _ptr(rm),
+          rm.stride(0) if rm is not None else 0, _ptr(weight), eps, _ptr(y), _ptr(s), _ptr(rstd))
+    return y, s
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, eps, sfx, train):
-        xm = _matrix(x)
-        rm = _matrix(residual) if residual is not None else None
-        w = weight.contiguous()
-        M, D = xm.shape
-        y, s = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        rstd = torch.empty(M, dtype=torch.float32, device=x.device) if train else None
-        _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), xm.stride(0), _ptr(rm),
-              rm.stride(0) if rm is not None else 0, _ptr(w), eps, _ptr(y), _ptr(s), _ptr(rstd))
+    def forward(ctx, x, residual, weight, eps, sfx):
+        rstd = torch.empty(x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        y, s = _rms_forward(x, residual, weight, eps, sfx, rstd)
         ctx.sfx, ctx.has_residual = sfx, residual is not None
-        if train:
-            ctx.save_for_backward(s, w, rstd)
+        ctx.save_for_backward(s, weight, rstd)
         ctx.set_materialize_grads(False)
         return y, s
 
@@ -102,12 +124,11 @@ class _RmsNorm(torch.autograd.Function):
         dym = _matrix(dy) if dy is not None else torch.zeros((M, D), dtype=s.dtype, device=s.device)
         dsm = _matrix(ds) if ds is not None else None
         dx, dw = torch.empty_like(s), torch.empty_like(w)
-        nbytes = _lib.load().tmpc_rms_norm_backward_workspace_bytes(s.element_size(), M, D)
-        ws = _lib.workspace(nbytes, s.device)
+        nbytes, ws = _workspace("tmpc_rms_norm_backward_workspace_bytes", s.device, s.element_size(), M, D)
         _call(f"tmpc_rms_norm_backward_{ctx.sfx}", s.device, M, D, _ptr(dym), dym.stride(0), _ptr(dsm),
               dsm.stride(0) if dsm is not None else 0, _ptr(s), D, _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws),
               nbytes)
-        return dx, dx if ctx.has_residual else None, dw, None, None, None
+        return dx, dx if ctx.has_residual else None, dw, None, None
 
 
 def rms_norm_residual(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
@@ -124,36 +145,41 @@ def rms_norm_residual(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
     _check("weight", weight, x, (D,))
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight))
-    return _RmsNorm.apply(x, residual, weight, float(eps), sfx, train)
+    weight, eps = weight.contiguous(), float(eps)
+    if _wants_grad(x, residual, weight):
+        return _RmsNorm.apply(x, residual, weight, eps, sfx)
+    return _rms_forward(x, residual, weight, eps, sfx, None)
 
 
 # ------------------------------------------------------------- attention --
-def _attention_args(q, k, v, log_decay, lengths, state, scale, step=False):
-    B, H, dk = q.shape[0], q.shape[-2], q.shape[-1]
-    T = 1 if step else q.shape[1]
-    a = _lib.DecayAttention(B=B, T=T, H=H, Hk=k.shape[-2], dk=dk, dv=v.shape[-1], q=_ptr(q), k=_ptr(k), v=_ptr(v),
-                            log_decay=_ptr(log_decay), lengths=_ptr(lengths), state_in=_ptr(state), scale=scale)
-    for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
-        st = t.stride()
-        setattr(a, name, (ctypes.c_int64 * 3)(st[0], 0 if step else st[1], st[-2]))
-    return a
+# tmpc_decay_attention, packed (its fields are naturally aligned)
+_ATTENTION = struct.Struct("@6i3P9q3Pd")
+assert _ATTENTION.size == ctypes.sizeof(_lib.DecayAttention)
+
+
+def _attention_args(q, k, v, log_decay, lengths, state, scale):
+    B, T, H, dk = q.shape if q.dim() == 4 else (q.shape[0], 1) + q.shape[1:]
+    p = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
+    st = [t.stride()[:3] if t.dim() == 4 else (t.stride(0), 0, t.stride(1)) for t in (q, k, v)]
+    return _lib.DecayAttention.from_buffer_copy(_ATTENTION.pack(
+        B, T, H, k.shape[-2], dk, v.shape[-1], p(q), p(k), p(v), *st[0], *st[1], *st[2], p(log_decay), p(lengths),
+        p(state), scale))
 
 
 def _check_attention(q, k, v, log_decay, scale, step):
     sfx = _first("q", q, (3,) if step else (4,))
-    lead = tuple(q.shape[:-2])
-    H, dk = q.shape[-2:]
     _check("k", k, q)
     _check("v", v, q)
-    if k.dim() != q.dim() or tuple(k.shape[:-2]) != lead or k.shape[-1] != dk:
-        raise ValueError(f"k has shape {tuple(k.shape)}, expected {lead + ('Hk', dk)}")
-    Hk = k.shape[-2]
-    if v.dim() != q.dim() or tuple(v.shape[:-1]) != lead + (Hk,):
-        raise ValueError(f"v has shape {tuple(v.shape)}, expected {lead + (Hk, 'dv')}")
+    qs, ks, vs = q.shape, k.shape, v.shape
+    lead, (H, dk) = qs[:-2], qs[-2:]
+    if len(ks) != len(qs) or ks[:-2] != lead or ks[-1] != dk:
+        raise ValueError(f"k has shape {tuple(ks)}, expected {tuple(lead) + ('Hk', dk)}")
+    Hk = ks[-2]
+    if len(vs) != len(qs) or vs[:-1] != ks[:-1]:
+        raise ValueError(f"v has shape {tuple(vs)}, expected {tuple(lead) + (Hk, 'dv')}")
     if H < 1 or Hk < 1 or H % Hk:
         raise ValueError(f"the {H} heads of q are not a multiple of the {Hk} heads of k and v")
-    for name, d in (("q and k", dk), ("v", v.shape[-1])):
+    for name, d in (("q and k", dk), ("v", vs[-1])):
         if not 1 <= d <= MAX_HEAD_WIDTH:
             raise ValueError(f"{name} have heads of {d} elements, expected 1 to {MAX_HEAD_WIDTH}")
     _check("log_decay", log_decay, q, (H,), torch.float32)
@@ -162,26 +188,24 @@ def _check_attention(q, k, v, log_decay, scale, step):
     return sfx, float(dk ** -0.5 if scale is None else scale)
 
 
+def _attention_forward(q, k, v, log_decay, state, lengths, scale, sfx):
+    B, T, H, dk = q.shape
+    dv = v.shape[-1]
+    o = torch.empty((B, T, H, dv), dtype=q.dtype, device=q.device)
+    out = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device)
+    a = _attention_args(q, k, v, log_decay, lengths, state, scale)
+    nbytes, ws = _workspace("tmpc_decay_attention_workspace_bytes", q.device, q.element_size(), a, 0)
+    _call(f"tmpc_decay_attention_forward_{sfx}", q.device, a, _ptr(o), _ptr(out), _ptr(ws), nbytes)
+    return o, out
+
+
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, state, lengths, scale, sfx, train):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        log_decay = log_decay.contiguous()
-        state = state.contiguous() if state is not None else None
-        lengths = lengths.contiguous() if lengths is not None else None
-        B, T, H, dk = q.shape
-        dv = v.shape[-1]
-        o = torch.empty((B, T, H, dv), dtype=q.dtype, device=q.device)
-        out = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device)
-        a = _attention_args(q, k, v, log_decay, lengths, state, scale)
-        nbytes = _lib.load().tmpc_decay_attention_workspace_bytes(q.element_size(), ctypes.byref(a), 0)
-        ws = _lib.workspace(nbytes, q.device)
-        _call(f"tmpc_decay_attention_forward_{sfx}", q.device, ctypes.byref(a), _ptr(o), _ptr(out), _ptr(ws), nbytes)
-        if train:
-            ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale, sfx):
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
         ctx.scale, ctx.sfx = scale, sfx
         ctx.set_materialize_grads(False)
-        return o, out
+        return _attention_forward(q, k, v, log_decay, state, lengths, scale, sfx)
 
     @staticmethod
     @once_differentiable
@@ -194,12 +218,11 @@ class _DecayAttention(torch.autograd.Function):
         dq, dk, dv = empty(q), empty(k), empty(v)
         d_state = empty(state) if state is not None and ctx.needs_input_grad[4] else None
         a = _attention_args(q, k, v, log_decay, lengths, state, ctx.scale)
-        nbytes = _lib.load().tmpc_decay_attention_workspace_bytes(q.element_size(), ctypes.byref(a), 1)
-        ws = _lib.workspace(nbytes, dev)
+        nbytes, ws = _workspace("tmpc_decay_attention_workspace_bytes", dev, q.element_size(), a, 1)
         st = (ctypes.c_int64 * 3)(*d_o.stride()[:3])
-        _call(f"tmpc_decay_attention_backward_{ctx.sfx}", dev, ctypes.byref(a), _ptr(d_o), st, _ptr(d_out), _ptr(dq),
-              _ptr(dk), _ptr(dv), _ptr(d_state), _ptr(ws), nbytes)
-        return dq, dk, dv, None, d_state, None, None, None, None
+        _call(f"tmpc_decay_attention_backward_{ctx.sfx}", dev, a, _ptr(d_o), st, _ptr(d_out), _ptr(dq), _ptr(dk),
+              _ptr(dv), _ptr(d_state), _ptr(ws), nbytes)
+        return dq, dk, dv, None, d_state, None, None, None
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -220,8 +243,10 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         _check("state", state, q, (B, H, dk, v.shape[-1]), torch.float32)
     if lengths is not None:
         _check("lengths", lengths, q, (B,), torch.int32)
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state))
-    return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale, sfx, train)
+    state = state.contiguous() if state is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    args = (_rows(q), _rows(k), _rows(v), log_decay.contiguous(), state, lengths, scale, sfx)
+    return _DecayAttention.apply(*args) if _wants_grad(q, k, v, state) else _attention_forward(*args)
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -240,52 +265,57 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if active is not None:
         _check("active", active, q, (B,), torch.bool)
         active = active.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if _wants_grad(q, k, v, state):
         raise ValueError("decay_attention_step has no gradient; use decay_attention, or torch.no_grad()")
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
-    a = _attention_args(q, k, v, log_decay, None, None, scale, step=True)
-    _call(f"tmpc_decay_attention_step_{sfx}", q.device, ctypes.byref(a), _ptr(active), _ptr(state), _ptr(o))
+    a = _attention_args(q, k, v, log_decay, None, None, scale)
+    _call(f"tmpc_decay_attention_step_{sfx}", q.device, a, _ptr(active), _ptr(state), _ptr(o))
     return o
 
 
 # ---------------------------------------------------------- feed-forward --
+_GATED_FF = struct.Struct("@q4iPq3P")  # tmpc_gated_ff, packed
+assert _GATED_FF.size == ctypes.sizeof(_lib.GatedFF)
+
+
+def _ff_args(xm, w_gate, w_up, w_down, act):
+    F, D = w_gate.shape
+    return _lib.GatedFF.from_buffer_copy(_GATED_FF.pack(xm.shape[0], D, F, w_down.shape[0], act, xm.data_ptr(),
+                                                        xm.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
+                                                        w_down.data_ptr()))
+
+
+def _ff_forward(x, xm, w_gate, w_up, w_down, act, sfx, gate, up):
+    """y; gate, up: fp32 tensors to fill, or None."""
+    a = _ff_args(xm, w_gate, w_up, w_down, act)
+    y = torch.empty(x.shape[:-1] + (w_down.shape[0],), dtype=x.dtype, device=x.device)
+    nbytes, ws = _workspace("tmpc_gated_ff_workspace_bytes", x.device, x.element_size(), a, 0)
+    _call(f"tmpc_gated_ff_forward_{sfx}", x.device, a, _ptr(y), _ptr(gate), _ptr(up), _ptr(ws), nbytes)
+    return y
+
+
 class _GatedFF(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, act, sfx, train):
+    def forward(ctx, x, w_gate, w_up, w_down, act, sfx):
         xm = _matrix(x)
-        w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
-        a = _GatedFF.args(xm, w_gate, w_up, w_down, act)
-        M, F = a.M, a.F
-        y = torch.empty(x.shape[:-1] + (a.Dout,), dtype=x.dtype, device=x.device)
-        gate = torch.empty((M, F), dtype=torch.float32, device=x.device) if train else None
-        up = torch.empty((M, F), dtype=torch.float32, device=x.device) if train else None
-        nbytes = _lib.load().tmpc_gated_ff_workspace_bytes(x.element_size(), ctypes.byref(a), 0)
-        ws = _lib.workspace(nbytes, x.device)
-        _call(f"tmpc_gated_ff_forward_{sfx}", x.device, ctypes.byref(a), _ptr(y), _ptr(gate), _ptr(up), _ptr(ws), nbytes)
-        if train:
-            ctx.save_for_backward(xm, w_gate, w_up, w_down, gate, up)
+        gate, up = (torch.empty((xm.shape[0], w_gate.shape[0]), dtype=torch.float32, device=x.device) for _ in range(2))
+        ctx.save_for_backward(xm, w_gate, w_up, w_down, gate, up)
         ctx.shape, ctx.act, ctx.sfx = x.shape, act, sfx
-        return y
-
-    @staticmethod
-    def args(xm, w_gate, w_up, w_down, act):
-        return _lib.GatedFF(M=xm.shape[0], D=xm.shape[1], F=w_gate.shape[0], Dout=w_down.shape[0], activation=act,
-                            x=_ptr(xm), ldx=xm.stride(0), w_gate=_ptr(w_gate), w_up=_ptr(w_up), w_down=_ptr(w_down))
+        return _ff_forward(x, xm, w_gate, w_up, w_down, act, sfx, gate, up)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xm, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
-        a = _GatedFF.args(xm, w_gate, w_up, w_down, ctx.act)
+        a = _ff_args(xm, w_gate, w_up, w_down, ctx.act)
         dym = _matrix(dy)
         dx = torch.empty(ctx.shape, dtype=xm.dtype, device=xm.device)
         dg, du, dd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
-        nbytes = _lib.load().tmpc_gated_ff_workspace_bytes(xm.element_size(), ctypes.byref(a), 1)
-        ws = _lib.workspace(nbytes, xm.device)
-        _call(f"tmpc_gated_ff_backward_{ctx.sfx}", xm.device, ctypes.byref(a), _ptr(gate), _ptr(up), _ptr(dym),
+        nbytes, ws = _workspace("tmpc_gated_ff_workspace_bytes", xm.device, xm.element_size(), a, 1)
+        _call(f"tmpc_gated_ff_backward_{ctx.sfx}", xm.device, a, _ptr(gate), _ptr(up), _ptr(dym),
               dym.stride(0), _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), _ptr(ws), nbytes)
-        return dx, dg, du, dd, None, None, None
+        return dx, dg, du, dd, None, None
 
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -304,5 +334,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     _check("w_down", w_down, x)
     if w_down.dim() != 2 or w_down.shape[1] != F or w_down.shape[0] < 1:
         raise ValueError(f"w_down has shape {tuple(w_down.shape)}, expected ('Dout', {F}), not empty")
-    train = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))
-    return _GatedFF.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation], sfx, train)
+    act = _ACTIVATIONS[activation]
+    w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
+    if _wants_grad(x, w_gate, w_up, w_down):
+        return _GatedFF.apply(x, w_gate, w_up, w_down, act, sfx)
+    return _ff_forward(x, _matrix(x), w_gate, w_up, w_down, act, sfx, None, None)
