@@ -70,25 +70,61 @@ struct AttnShape {
 };
 
 // A chunk's rows of one operand on their way from memory through registers to LDS: the
-// next chunk's are in flight while this one's are multiplied.
+// next chunk's are in flight while this one's are multiplied.  A thread moves N pieces
+// of one column, RS rows apart.
 template <typename E, int C, int D, int THREADS>
 struct AttnRows {
-  static constexpr int P = Elem<E>::PIECE, W = D / P, N = (C * W + THREADS - 1) / THREADS, LD = D + AttnTile<E>::PAD;
-  static_assert(C * W % THREADS == 0, "a whole number of pieces a thread");
+  static constexpr int P = Elem<E>::PIECE, W = D / P, RS = THREADS / W, N = C / RS, LD = D + AttnTile<E>::PAD;
+  static_assert(THREADS % W == 0 && C % RS == 0, "whole rows a pass");
   piece_t<E> r[N];
-  // rows t0 .. of `base`, which points at the first live step; n live ones
-  __device__ void load(const E* base, int64_t stride, int t0, int n, int width, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = tid + i * THREADS, row = e / W, c = (e - row * W) * P;
-      r[i] = load_piece(base + (t0 + row) * stride, c, width, row < n);
-    }
+  const E* at;      // this thread's first piece of the next chunk
+  int64_t step;     // elements between steps
+  int row, c;
+
+  __device__ void init(const E* base, int64_t stride, int t0, int tid) {
+    row = tid / W, c = (tid - row * W) * P, step = stride;
+    at = base + (t0 + row) * stride + c;
   }
-  __device__ void store(E* tile, int tid) const {
+  // the next chunk's rows, n of them live
+  __device__ void load(int n, int width) {
+    if (n >= C && width == D) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = tid + i * THREADS, row = e / W, c = (e - row * W) * P;
-      *reinterpret_cast<piece_t<E>*>(tile + row * LD + c) = r[i];
+      for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(at + i * RS * step);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = load_piece(at + i * RS * step - c, c, width, row + i * RS < n);
+    }
+    at += C * step;
+  }
+  __device__ void store(E* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<piece_t<E>*>(tile + (row + i * RS) * LD + c) = r[i];
+  }
+};
+
+__device__ inline float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
+// Powers of a head's decay that every whole chunk needs, of exponents >= 0 alone:
+// lag 16 d + lo - 4 hi - r of a score as tile[d] * near[r] (d >= 1; near has 16 more and tile
+// 16 fewer), diag[r] on the diagonal tile (0 above it), row i = 16 it + lo of the
+// carried state's part as tile[it] * rowf, step j = 16 jt + 4 hi + r of the update as
+// tile[CT - 1 - jt] * tail[r].
+template <int CT>
+struct AttnPowers {
+  float tile[CT], near[4], diag[4], rowf, tail[4], chunk;
+  __device__ void init(float g, int rev, float ss, float si, float su, int lo, int hi) {
+#pragma unroll
+    for (int d = 0; d < CT; ++d) tile[d] = uniform(decay_pow(g, 16 * d));
+    chunk = uniform(decay_pow(g, 16 * CT));
+    rowf = si * decay_pow(g, lo + 1 - rev);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int lag = lo - 4 * hi - r;
+      near[r] = ss * decay_pow(g, 16 + lag);
+      diag[r] = lag >= 0 ? ss * decay_pow(g, max(lag, 0)) : 0.0f;
+      tail[r] = su * decay_pow(g, 15 - 4 * hi - r + rev);
     }
   }
 };
@@ -139,22 +175,27 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
         s[m][n][r] = v;
       }
 
+  AttnPowers<CT> pw;
+  pw.init(g, p.rev, p.ss, p.si, p.su, lo, hi);
   AttnRows<E, C, DA, S::THREADS> ra, rb;
   AttnRows<E, C, DC, S::THREADS> rc;
-  auto fetch = [&](int t0) {
-    const int n = end - t0;
-    rb.load(pb, dir * p.bs[1], t0, n, p.da, tid);
-    rc.load(pc, dir * p.cs[1], t0, n, p.dc, tid);
-    if constexpr (FULL) ra.load(pa, dir * p.as[1], t0, n, p.da, tid);
+  rb.init(pb, dir * p.bs[1], begin, tid);
+  rc.init(pc, dir * p.cs[1], begin, tid);
+  if constexpr (FULL) ra.init(pa, dir * p.as[1], begin, tid);
+  auto fetch = [&](int n) {
+    rb.load(n, p.da);
+    rc.load(n, p.dc);
+    if constexpr (FULL) ra.load(n, p.da);
   };
-  if (begin < end) fetch(begin);
+  if (begin < end) fetch(end - begin);
+  int64_t orow0 = obase + (first + dir * (begin + lo)) * orow;  // the output row of tile 0
   for (int t0 = begin; t0 < end; t0 += C) {
     const int n = min(C, end - t0);  // live steps
-    rb.store(tb, tid);
-    rc.store(tc, tid);
-    if constexpr (FULL) ra.store(ta, tid);
+    rb.store(tb);
+    rc.store(tc);
+    if constexpr (FULL) ra.store(ta);
     __syncthreads();
-    if (t0 + C < end) fetch(t0 + C);
+    if (t0 + C < end) fetch(end - t0 - C);
 
     if constexpr (FULL) {
     // scores: tile (it, jt <= it) as its transpose, so that a lane holds 4 consecutive j of
@@ -162,16 +203,16 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
     for (int q = wave; q < CT * (CT + 1) / 2; q += W) {
       int it = 0, jt = q;
       while (jt > it) jt -= ++it;
+      float far = pw.tile[0];  // e^{16 g (it - jt - 1)}
+#pragma unroll
+      for (int d = 1; d < CT - 1; ++d) far = it - jt - 1 == d ? pw.tile[d] : far;
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < KA; k += 2)
         acc = mma2(lds_quad(tb, LDA, 16 * jt, 16 * k, lane), lds_quad(tb, LDA, 16 * jt, 16 * k + 16, lane),
                    lds_quad(ta, LDA, 16 * it, 16 * k, lane), lds_quad(ta, LDA, 16 * it, 16 * k + 16, lane), acc);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int lag = 16 * it + lo - (16 * jt + 4 * hi + r);
-        acc[r] = lag >= 0 ? acc[r] * (p.ss * decay_pow(g, lag)) : 0.0f;
-      }
+      for (int r = 0; r < 4; ++r) acc[r] = it == jt ? acc[r] * pw.diag[r] : acc[r] * (far * pw.near[r]);
       *reinterpret_cast<quad_t<E>*>(tp + (16 * it + lo) * LDP + 16 * jt + 4 * hi) = to_quad<E>(acc);
     }
     __syncthreads();
@@ -200,7 +241,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
         for (int x = 0; x < NV; ++x)  // the state rounds to E as this product's operand only
           acc[x] = mma2(to_quad<E>(s[k][x]), to_quad<E>(s[k + 1][x]), a0, a1, acc[x]);
       }
-      const float f = p.si * decay_pow(g, i + 1 - p.rev);
+      const float f = pw.rowf * pw.tile[it];
 #pragma unroll
       for (int x = 0; x < NV; ++x) acc[x] *= f;
 #pragma unroll
@@ -212,7 +253,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
           for (int x = 0; x < NV; ++x) acc[x] = mma2(v[j][x], v[j + 1][x], p0, p1, acc[x]);
         }
       if (i < n) {
-        const int64_t row = obase + (first + dir * (t0 + i)) * orow;
+        const int64_t row = orow0 + dir * 16 * it * orow;
 #pragma unroll
         for (int x = 0; x < NV; ++x) {
           const int c = col0 + 16 * x + 4 * hi;
@@ -227,7 +268,8 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
 
     // S update.  The decayed values are not exact in bf16: they enter as a sum of three bf16
     // terms (24 bits), for the state is an fp32 result
-    const float fl = decay_pow(g, n);
+    const bool whole = n == C;
+    const float fl = whole ? pw.chunk : decay_pow(g, n);
 #pragma unroll
     for (int m = 0; m < KA; ++m)
 #pragma unroll
@@ -237,6 +279,10 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
       f32x4 d0, d1;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        if (whole) {
+          d0[r] = pw.tile[CT - 1 - j] * pw.tail[r], d1[r] = pw.tile[CT - 2 - j] * pw.tail[r];
+          continue;
+        }
         const int j0 = 16 * j + 4 * hi + r;
         d0[r] = p.su * decay_pow(g, max(n - 1 - j0, 0) + p.rev);
         d1[r] = p.su * decay_pow(g, max(n - 17 - j0, 0) + p.rev);
@@ -262,6 +308,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
           for (int t = 0; t < TERMS; ++t) s[m][x] = mma2(b0, b1, w0[t][x], w1[t][x], s[m][x]);
       }
     }
+    orow0 += dir * C * orow;
     __syncthreads();  // the tiles are free
   }
 
