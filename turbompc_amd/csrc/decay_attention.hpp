@@ -55,48 +55,84 @@ struct AttnTile {
 __device__ inline float decay_pow(float g, int n) { return n == 0 ? 1.0f : __expf(g * (float)n); }
 
 // A workgroup carries one (problem, head) through its chunks.  Wave w owns NV
-// 16-column tiles of the values: S and O need no exchange between waves, only the
-// chunk's scores do (LDS).  S stays in registers, in the accumulator's layout, which
-// is the operand layout of the product with Q.
+// 16-column tiles of the values and all of the scores: S, the scores and O stay in
+// its registers (each product's accumulator is the next one's operand) and waves meet
+// only where a chunk's rows change in LDS.  Every wave forms the scores again, 10 of
+// its products of 16 x 16 for C = 64: cheaper than an exchange through LDS and the
+// barrier that it needs.
 template <typename E, int DA, int DC>
 struct AttnShape {
   static constexpr int W = DC / 16 < 4 ? DC / 16 : 4;  // waves
   static constexpr int NV = DC / 16 / W;               // value tiles of a wave
   static constexpr int THREADS = 64 * W;
   static constexpr int C = AttnTile<E>::C;
-  static constexpr int LDA = DA + AttnTile<E>::PAD, LDC = DC + AttnTile<E>::PAD, LDP = C + AttnTile<E>::PAD;
-  static constexpr size_t LDS_STATE = sizeof(E) * (size_t)(C * LDA + C * LDC);
-  static constexpr size_t LDS = LDS_STATE + sizeof(E) * (size_t)(C * LDA + C * LDP);
+  static constexpr int LDA = DA + AttnTile<E>::PAD, LDC = DC + AttnTile<E>::PAD;
+  // elements of a chunk's rows in LDS: b and c, and a with outputs
+  static constexpr int TILE_STATE = C * LDA + C * LDC, TILE = TILE_STATE + C * LDA;
+  // workgroups of a CU, by their registers; the tiles twice (one barrier a chunk instead of
+  // two) where they still fit
+  static constexpr int PER_CU = 2;
+  static constexpr int BUFS = 2 * sizeof(E) * TILE <= 160 * 1024 / PER_CU ? 2 : 1;
+  static constexpr size_t LDS_STATE = sizeof(E) * (size_t)BUFS * TILE_STATE;
+  static constexpr size_t LDS = sizeof(E) * (size_t)BUFS * TILE;
 };
+
+// Buffer descriptors let a load or store name a place past the end: the load gives zero,
+// the store is dropped, and no branch stands between the memory operations of a chunk.
+constexpr unsigned kBufferEnd = 0x80000000u, kNowhere = 0xfffffff0u;  // bytes from a descriptor's base
+__device__ inline __amdgpu_buffer_rsrc_t buffer_at(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, kBufferEnd, 0x00027000);
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // A chunk's rows of one operand on their way from memory through registers to LDS: the
 // next chunk's are in flight while this one's are multiplied.  A thread moves N pieces
-// of one column, RS rows apart.
-template <typename E, int C, int D, int THREADS>
+// of one column, RS rows apart.  VEC: rows of whole pieces at 4-byte addresses; else any
+// width and alignment, element by element.
+template <typename E, int C, int D, int THREADS, bool VEC>
 struct AttnRows {
-  static constexpr int P = Elem<E>::PIECE, W = D / P, RS = THREADS / W, N = C / RS, LD = D + AttnTile<E>::PAD;
+  static constexpr int P = Elem<E>::PIECE, W = D / P, RS = THREADS / W < C ? THREADS / W : C, N = C / RS;
+  static constexpr int LD = D + AttnTile<E>::PAD;
   static_assert(THREADS % W == 0 && C % RS == 0, "whole rows a pass");
   piece_t<E> r[N];
-  const E* at;      // this thread's first piece of the next chunk
-  int64_t step;     // elements between steps
+  const E* base;    // the first step of the next chunk
+  int64_t step;     // elements between steps, negative where they are walked backwards
+  unsigned off[N];  // bytes from the chunk's lowest address
   int row, c;
 
-  __device__ void init(const E* base, int64_t stride, int t0, int tid) {
+  __device__ void init(const E* b, int64_t stride, int t0, int width, int tid) {
     row = tid / W, c = (tid - row * W) * P, step = stride;
-    at = base + (t0 + row) * stride + c;
+    base = b + t0 * stride;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t s = stride < 0 ? -stride * (C - 1 - row - i * RS) : stride * (row + i * RS);
+      off[i] = c < width && row < RS ? (unsigned)((s + c) * (int64_t)sizeof(E)) : kNowhere;
+    }
   }
   // the next chunk's rows, n of them live
   __device__ void load(int n, int width) {
-    if (n >= C && width == D) {
+    const __amdgpu_buffer_rsrc_t rs = buffer_at(step < 0 ? base + (C - 1) * step : base);
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(at + i * RS * step);
-    } else {
+    for (int i = 0; i < N; ++i) {
+      const unsigned at = row + i * RS < n ? off[i] : kNowhere;
+      if constexpr (VEC) {
+        r[i] = __builtin_bit_cast(piece_t<E>, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = load_piece(at + i * RS * step - c, c, width, row + i * RS < n);
+        for (int e = 0; e < P; ++e) {
+          const unsigned ae = c + e < width && at != kNowhere ? at + e * (unsigned)sizeof(E) : kNowhere;
+          if constexpr (sizeof(E) == 4)
+            r[i][e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, ae, 0, 0));
+          else
+            r[i][e] = __builtin_bit_cast(bf16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, ae, 0, 0));
+        }
+      }
     }
-    at += C * step;
+    base += C * step;
   }
   __device__ void store(E* tile) const {
+    if (RS * W < THREADS && row >= RS) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) *reinterpret_cast<piece_t<E>*>(tile + (row + i * RS) * LD + c) = r[i];
   }
@@ -129,17 +165,168 @@ struct AttnPowers {
   }
 };
 
+// One chunk of one recurrence for a wave's NV value tiles (columns col0 ..): the outputs
+// through store(tile it, x, values of row 16 it + lo, columns 4 hi ..), and the state.
+// n live steps; ta, tb (C x DA, pitch LDA) and tc (pitch LDC) hold zeros after them.
+template <typename E, int KA, int NV, int CT, bool FULL, int LDA, int LDC, typename Store>
+__device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, int col0, f32x4 (&s)[KA][NV],
+                                  const AttnPowers<CT>& pw, float g, float su, int rev, int n, int lane, Store store) {
+  constexpr int C = 16 * CT;
+  const int hi = lane >> 4;
+  // the wave's values, contracted over the steps
+  quad_t<E> v[CT][NV];
+#pragma unroll
+  for (int j = 0; j < CT; ++j)
+#pragma unroll
+    for (int x = 0; x < NV; ++x) v[j][x] = lds_quad_t(tc, LDC, 16 * j, col0 + 16 * x, lane);
+
+  if constexpr (FULL) {
+    quad_t<E> sq[KA][NV];  // the state rounds to E as this product's operand only
+#pragma unroll
+    for (int k = 0; k < KA; ++k)
+#pragma unroll
+      for (int x = 0; x < NV; ++x) sq[k][x] = to_quad<E>(s[k][x]);
+#pragma unroll
+    for (int it = 0; it < CT; ++it) {
+      asm volatile("" ::: "memory");  // the keys are read again for each tile: kept, they would cost the registers
+      quad_t<E> a[KA];
+#pragma unroll
+      for (int k = 0; k < KA; ++k) a[k] = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
+      // O^T tiles: columns i, rows the values
+      f32x4 acc[NV];
+#pragma unroll
+      for (int x = 0; x < NV; ++x) acc[x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < KA; k += 2)
+#pragma unroll
+        for (int x = 0; x < NV; ++x) acc[x] = mma2(sq[k][x], sq[k + 1][x], a[k], a[k + 1], acc[x]);
+      const float f = pw.rowf * pw.tile[it];
+#pragma unroll
+      for (int x = 0; x < NV; ++x) acc[x] *= f;
+#pragma unroll
+      for (int j = 0; j <= it; j += 2) {
+        // score tiles as their transposes: a lane holds 4 consecutive j of one i, the operand
+        // of the product with V; rounded to E, as the output is
+        quad_t<E> p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int jt = j + e;
+          f32x4 t = {0, 0, 0, 0};
+          if (jt <= it) {
+#pragma unroll
+            for (int k = 0; k < KA; k += 2)
+              t = mma2(lds_quad(tb, LDA, 16 * jt, 16 * k, lane), lds_quad(tb, LDA, 16 * jt, 16 * k + 16, lane), a[k],
+                       a[k + 1], t);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] *= jt == it ? pw.diag[r] : pw.tile[it > jt ? it - jt - 1 : 0] * pw.near[r];
+          }
+          p[e] = to_quad<E>(t);
+        }
+#pragma unroll
+        for (int x = 0; x < NV; ++x) acc[x] = mma2(v[j][x], v[j + 1][x], p[0], p[1], acc[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < NV; ++x) store(it, x, acc[x]);
+    }
+  }
+
+  // S update.  The decayed values are not exact in bf16: they enter as a sum of three bf16
+  // terms (24 bits), for the state is an fp32 result
+  const bool whole = n == C;
+  const float fl = whole ? pw.chunk : decay_pow(g, n);
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+#pragma unroll
+    for (int x = 0; x < NV; ++x) s[m][x] *= fl;
+#pragma unroll
+  for (int j = 0; j < CT; j += 2) {
+    f32x4 d0, d1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (whole) {
+        d0[r] = pw.tile[CT - 1 - j] * pw.tail[r], d1[r] = pw.tile[CT - 2 - j] * pw.tail[r];
+      } else {
+        const int j0 = 16 * j + 4 * hi + r;
+        d0[r] = su * decay_pow(g, max(n - 1 - j0, 0) + rev);
+        d1[r] = su * decay_pow(g, max(n - 17 - j0, 0) + rev);
+      }
+    }
+    constexpr int TERMS = sizeof(E) == 2 ? 3 : 1;
+    quad_t<E> w0[TERMS][NV], w1[TERMS][NV];
+#pragma unroll
+    for (int x = 0; x < NV; ++x) {
+      f32x4 r0 = to_f32(v[j][x]) * d0, r1 = to_f32(v[j + 1][x]) * d1;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) {
+        w0[t][x] = to_quad<E>(r0), w1[t][x] = to_quad<E>(r1);
+        r0 -= to_f32(w0[t][x]), r1 -= to_f32(w1[t][x]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < KA; ++m) {
+      const quad_t<E> b0 = lds_quad_t(tb, LDA, 16 * j, 16 * m, lane);
+      const quad_t<E> b1 = lds_quad_t(tb, LDA, 16 * j + 16, 16 * m, lane);
+#pragma unroll
+      for (int x = 0; x < NV; ++x)
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) s[m][x] = mma2(b0, b1, w0[t][x], w1[t][x], s[m][x]);
+    }
+  }
+}
+
+// The state's rows 16 m + 4 hi + r, columns col0 + 16 x + lo of a (da, dc) matrix, or of
+// the transpose of a (dc, da) one; zeros where src is NULL and outside.
+template <int KA, int NV>
+__device__ inline void load_state(f32x4 (&s)[KA][NV], const float* src, bool transposed, int da, int dc, int col0, int lo,
+                                  int hi) {
+  const __amdgpu_buffer_rsrc_t rs = buffer_at(src);
+  const int rp = transposed ? 1 : dc, cp = transposed ? da : 1;
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+#pragma unroll
+    for (int x = 0; x < NV; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * m + 4 * hi + r, col = col0 + 16 * x + lo;
+        const unsigned at = src && row < da && col < dc ? (row * rp + col * cp) * 4u : kNowhere;
+        s[m][x][r] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0));
+      }
+}
+template <int KA, int NV>
+__device__ inline void store_state(const f32x4 (&s)[KA][NV], float* dst, int da, int dc, int col0, int lo, int hi) {
+  const __amdgpu_buffer_rsrc_t rs = buffer_at(dst);
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+#pragma unroll
+    for (int x = 0; x < NV; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * m + 4 * hi + r, col = col0 + 16 * x + lo;
+        const float v = s[m][x][r];
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rs,
+                                              row < da && col < dc ? (row * dc + col) * 4u : kNowhere, 0, 0);
+      }
+}
+
+// Zero rows [z0, z1) of an output (T, H, d) of one head from `base`.
+__device__ inline void zero_rows(void* o, bool f32, int elem, int64_t base, int64_t pitch, int d, int64_t z0, int64_t z1,
+                                 int tid, int threads) {
+  for (int64_t e = z0 * d + tid; e < z1 * d; e += threads) {
+    const int64_t t = e / d, at = base + t * pitch + (e - t * d);
+    if (f32 || elem == 4)
+      reinterpret_cast<float*>(o)[at] = 0.0f;
+    else
+      reinterpret_cast<uint16_t*>(o)[at] = 0;
+  }
+}
+
 // FULL: outputs and the carried state; else the run's own sum alone, into seg_state.
-template <typename E, int DA, int DC, bool FULL>
+template <typename E, int DA, int DC, bool FULL, bool VEC>
 __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk_kernel(AttnArgs<E> p) {
   using S = AttnShape<E, DA, DC>;
-  constexpr int C = S::C, W = S::W, NV = S::NV, LDA = S::LDA, LDC = S::LDC, LDP = S::LDP;
-  constexpr int CT = C / 16, KA = DA / 16;
+  constexpr int C = S::C, NV = S::NV, LDA = S::LDA, LDC = S::LDC, CT = C / 16, KA = DA / 16;
+  constexpr int TILE = FULL ? S::TILE : S::TILE_STATE;
   extern __shared__ __align__(16) char smem[];
-  E* tb = reinterpret_cast<E*>(smem);
-  E* tc = tb + C * LDA;
-  E* ta = tc + C * LDC;
-  E* tp = ta + C * LDA;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
   const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs;
   const int b = bh / p.H, h = bh - b * p.H;
@@ -156,185 +343,80 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
   const int64_t sbase = (int64_t)bh * p.da * p.dc;
   float* seg_state = p.segs > 1 ? p.seg_state + (int64_t)blockIdx.x * p.da * p.dc : nullptr;
 
-  // S[m][n]: rows 16 m + 4 hi + r, column col0 + 16 n + lo
-  f32x4 s[KA][NV];
-#pragma unroll
-  for (int m = 0; m < KA; ++m)
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * m + 4 * hi + r, col = col0 + 16 * n + lo;
-        float v = 0.0f;
-        if (FULL && row < p.da && col < p.dc) {
-          if (seg_state)
-            v = seg_state[(int64_t)row * p.dc + col];
-          else if (p.s_in)
-            v = p.s_in_t ? p.s_in[sbase + (int64_t)col * p.da + row] : p.s_in[sbase + (int64_t)row * p.dc + col];
-        }
-        s[m][n][r] = v;
-      }
-
-  AttnPowers<CT> pw;
-  pw.init(g, p.rev, p.ss, p.si, p.su, lo, hi);
-  AttnRows<E, C, DA, S::THREADS> ra, rb;
-  AttnRows<E, C, DC, S::THREADS> rc;
-  rb.init(pb, dir * p.bs[1], begin, tid);
-  rc.init(pc, dir * p.cs[1], begin, tid);
-  if constexpr (FULL) ra.init(pa, dir * p.as[1], begin, tid);
+  AttnRows<E, C, DA, S::THREADS, VEC> ra, rb;
+  AttnRows<E, C, DC, S::THREADS, VEC> rc;
+  rb.init(pb, dir * p.bs[1], begin, p.da, tid);
+  rc.init(pc, dir * p.cs[1], begin, p.dc, tid);
+  if constexpr (FULL) ra.init(pa, dir * p.as[1], begin, p.da, tid);
   auto fetch = [&](int n) {
     rb.load(n, p.da);
     rc.load(n, p.dc);
     if constexpr (FULL) ra.load(n, p.da);
   };
   if (begin < end) fetch(end - begin);
-  int64_t orow0 = obase + (first + dir * (begin + lo)) * orow;  // the output row of tile 0
+  f32x4 s[KA][NV];
+  if constexpr (FULL)
+    load_state(s, seg_state ? seg_state : p.s_in ? p.s_in + sbase : nullptr, !seg_state && p.s_in_t, p.da, p.dc, col0, lo, hi);
+  else
+    load_state(s, nullptr, false, p.da, p.dc, col0, lo, hi);
+  AttnPowers<CT> pw;
+  pw.init(g, p.rev, p.ss, p.si, p.su, lo, hi);
+  const int osize = p.o_f32 ? 4 : (int)sizeof(E);
+  // the output chunk's lowest row, and this lane's place in it
+  char* obuf = reinterpret_cast<char*>(p.o) + (obase + (first + dir * begin - (p.rev ? C - 1 : 0)) * orow) * osize;
+  unsigned ooff[NV];
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int c = col0 + 16 * x + 4 * hi;
+    ooff[x] = c < p.dc ? (unsigned)(((p.rev ? C - 1 - lo : lo) * orow + c) * osize) : kNowhere;
+  }
+  const int otile = (int)(dir * 16 * orow * osize);
+  int buf = 0;
   for (int t0 = begin; t0 < end; t0 += C) {
     const int n = min(C, end - t0);  // live steps
+    E* tb = reinterpret_cast<E*>(smem) + buf * TILE;
+    E* tc = tb + C * LDA;
+    E* ta = tc + C * LDC;
     rb.store(tb);
     rc.store(tc);
     if constexpr (FULL) ra.store(ta);
     __syncthreads();
     if (t0 + C < end) fetch(end - t0 - C);
-
-    if constexpr (FULL) {
-    // scores: tile (it, jt <= it) as its transpose, so that a lane holds 4 consecutive j of
-    // one i; rounded to E for the product with V (the output is E as well)
-    for (int q = wave; q < CT * (CT + 1) / 2; q += W) {
-      int it = 0, jt = q;
-      while (jt > it) jt -= ++it;
-      float far = pw.tile[0];  // e^{16 g (it - jt - 1)}
+    attn_chunk<E, KA, NV, CT, FULL, LDA, LDC>(ta, tb, tc, col0, s, pw, g, p.su, p.rev, n, lane,
+                                              [&](int it, int x, f32x4 v) {
+      const __amdgpu_buffer_rsrc_t rs = buffer_at(obuf);
+      const unsigned at = 16 * it + lo < n && ooff[x] != kNowhere ? ooff[x] + it * otile : kNowhere;
+      if constexpr (VEC) {
+        if (sizeof(E) == 4 || p.o_f32)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, to_bf16(v)), rs, at, 0, 0);
+      } else {
 #pragma unroll
-      for (int d = 1; d < CT - 1; ++d) far = it - jt - 1 == d ? pw.tile[d] : far;
-      f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < KA; k += 2)
-        acc = mma2(lds_quad(tb, LDA, 16 * jt, 16 * k, lane), lds_quad(tb, LDA, 16 * jt, 16 * k + 16, lane),
-                   lds_quad(ta, LDA, 16 * it, 16 * k, lane), lds_quad(ta, LDA, 16 * it, 16 * k + 16, lane), acc);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[r] = it == jt ? acc[r] * pw.diag[r] : acc[r] * (far * pw.near[r]);
-      *reinterpret_cast<quad_t<E>*>(tp + (16 * it + lo) * LDP + 16 * jt + 4 * hi) = to_quad<E>(acc);
-    }
-    __syncthreads();
-    }
-
-    // the wave's values, contracted over the steps
-    quad_t<E> v[CT][NV];
-#pragma unroll
-    for (int j = 0; j < CT; ++j)
-#pragma unroll
-      for (int x = 0; x < NV; ++x) v[j][x] = lds_quad_t(tc, LDC, 16 * j, col0 + 16 * x, lane);
-
-    // O^T tiles: columns i, rows the values
-    if constexpr (FULL) {
-#pragma unroll
-    for (int it = 0; it < CT; ++it) {
-      const int i = 16 * it + lo;
-      f32x4 acc[NV];
-#pragma unroll
-      for (int x = 0; x < NV; ++x) acc[x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < KA; k += 2) {
-        const quad_t<E> a0 = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
-        const quad_t<E> a1 = lds_quad(ta, LDA, 16 * it, 16 * k + 16, lane);
-#pragma unroll
-        for (int x = 0; x < NV; ++x)  // the state rounds to E as this product's operand only
-          acc[x] = mma2(to_quad<E>(s[k][x]), to_quad<E>(s[k + 1][x]), a0, a1, acc[x]);
-      }
-      const float f = pw.rowf * pw.tile[it];
-#pragma unroll
-      for (int x = 0; x < NV; ++x) acc[x] *= f;
-#pragma unroll
-      for (int j = 0; j < CT; j += 2)
-        if (j <= it) {  // the odd tile past the diagonal was not written: zero
-          const quad_t<E> p0 = lds_quad(tp, LDP, 16 * it, 16 * j, lane);
-          const quad_t<E> p1 = j + 1 <= it ? lds_quad(tp, LDP, 16 * it, 16 * j + 16, lane) : to_quad<E>(f32x4{0, 0, 0, 0});
-#pragma unroll
-          for (int x = 0; x < NV; ++x) acc[x] = mma2(v[j][x], v[j + 1][x], p0, p1, acc[x]);
-        }
-      if (i < n) {
-        const int64_t row = orow0 + dir * 16 * it * orow;
-#pragma unroll
-        for (int x = 0; x < NV; ++x) {
-          const int c = col0 + 16 * x + 4 * hi;
-          if (p.o_f32)
-            store_quad(reinterpret_cast<float*>(p.o) + row, c, p.dc, acc[x]);
+        for (int e = 0; e < 4; ++e) {
+          const unsigned ae = col0 + 16 * x + 4 * hi + e < p.dc && at != kNowhere ? at + e * osize : kNowhere;
+          const float f = v[e];
+          if (sizeof(E) == 4 || p.o_f32)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f), rs, ae, 0, 0);
           else
-            store_quad(reinterpret_cast<E*>(p.o) + row, c, p.dc, acc[x]);
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (bf16)f), rs, ae, 0, 0);
         }
       }
-    }
-    }
-
-    // S update.  The decayed values are not exact in bf16: they enter as a sum of three bf16
-    // terms (24 bits), for the state is an fp32 result
-    const bool whole = n == C;
-    const float fl = whole ? pw.chunk : decay_pow(g, n);
-#pragma unroll
-    for (int m = 0; m < KA; ++m)
-#pragma unroll
-      for (int x = 0; x < NV; ++x) s[m][x] *= fl;
-#pragma unroll
-    for (int j = 0; j < CT; j += 2) {
-      f32x4 d0, d1;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (whole) {
-          d0[r] = pw.tile[CT - 1 - j] * pw.tail[r], d1[r] = pw.tile[CT - 2 - j] * pw.tail[r];
-          continue;
-        }
-        const int j0 = 16 * j + 4 * hi + r;
-        d0[r] = p.su * decay_pow(g, max(n - 1 - j0, 0) + p.rev);
-        d1[r] = p.su * decay_pow(g, max(n - 17 - j0, 0) + p.rev);
-      }
-      constexpr int TERMS = sizeof(E) == 2 ? 3 : 1;
-      quad_t<E> w0[TERMS][NV], w1[TERMS][NV];
-#pragma unroll
-      for (int x = 0; x < NV; ++x) {
-        f32x4 r0 = to_f32(v[j][x]) * d0, r1 = to_f32(v[j + 1][x]) * d1;
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
-          w0[t][x] = to_quad<E>(r0), w1[t][x] = to_quad<E>(r1);
-          r0 -= to_f32(w0[t][x]), r1 -= to_f32(w1[t][x]);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        const quad_t<E> b0 = lds_quad_t(tb, LDA, 16 * j, 16 * m, lane);
-        const quad_t<E> b1 = lds_quad_t(tb, LDA, 16 * j + 16, 16 * m, lane);
-#pragma unroll
-        for (int x = 0; x < NV; ++x)
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t) s[m][x] = mma2(b0, b1, w0[t][x], w1[t][x], s[m][x]);
-      }
-    }
-    orow0 += dir * C * orow;
-    __syncthreads();  // the tiles are free
+    });
+    obuf += dir * C * orow * osize;
+    if constexpr (S::BUFS == 2)
+      buf ^= 1;  // the other tiles' readers passed this chunk's barrier
+    else
+      __syncthreads();
   }
 
-  if constexpr (FULL) {
-    // this run's steps past the end
-    const int64_t z0 = max(L, begin), z1 = min(p.T, begin + p.seg_len);
-    for (int64_t e = z0 * p.dc + tid; e < z1 * p.dc; e += S::THREADS) {
-      const int64_t t = e / p.dc, c = e - t * p.dc;
-      if (p.o_f32)
-        reinterpret_cast<float*>(p.o)[obase + t * orow + c] = 0.0f;
-      else
-        reinterpret_cast<E*>(p.o)[obase + t * orow + c] = E(0.0f);
-    }
-  }
-  // the run that holds the last live step has the final state
-  float* out = FULL ? (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0) ? p.s_out + sbase : nullptr) : seg_state;
-  if (out) {
-#pragma unroll
-    for (int m = 0; m < KA; ++m)
-#pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * m + 4 * hi + r, col = col0 + 16 * n + lo;
-          if (row < p.da && col < p.dc) out[(int64_t)row * p.dc + col] = s[m][n][r];
-        }
+  if constexpr (FULL) {  // this run's steps past the end
+    zero_rows(p.o, p.o_f32, sizeof(E), obase, orow, p.dc, max(L, begin), min((int64_t)p.T, (int64_t)begin + p.seg_len), tid,
+              S::THREADS);
+    // the run that holds the last live step has the final state
+    if (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0)) store_state(s, p.s_out + sbase, p.da, p.dc, col0, lo, hi);
+  } else {
+    store_state(s, seg_state, p.da, p.dc, col0, lo, hi);
   }
 }
 

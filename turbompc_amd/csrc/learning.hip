@@ -92,10 +92,15 @@ int rms_backward_impl(hipStream_t st, int64_t rows, int32_t width, const void* d
 }
 
 // --------------------------------------------------------- decay attention --
+constexpr int kMaxHeads = 32768;            // a chunk of contiguous output rows, 64 x H x 128 fp32, within 31 bits
+constexpr int64_t kMaxStep = (1 << 23) - 1; // elements between steps: 64 fp32 steps within 31 bits
+
 bool attn_shape_ok(const tmpc_decay_attention* a) {
   return a && a->B >= 0 && a->T >= 0 && a->H >= 1 && a->Hk >= 1 && a->H % a->Hk == 0 && a->dk >= 1 && a->dk <= 128 &&
-         a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 0x7fffffff;
+         a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 0x7fffffff && a->H <= kMaxHeads;
 }
+// a chunk's steps lie within the 31 bits of a descriptor
+bool step_ok(const int64_t* stride) { return stride[1] >= 0 && stride[1] <= kMaxStep; }
 
 // One long history of few heads does not fill the chip, its chunks following one another:
 // it is cut into runs of whole chunks.  A first pass sums each run on its own (keys and
@@ -119,21 +124,42 @@ size_t attn_split_bytes(const tmpc_decay_attention* x) {
   return segs > 1 ? align_up((size_t)bh * segs * x->dk * x->dv * sizeof(float)) : 0;
 }
 
+// Rows of whole 16-byte pieces at 4-byte addresses: moved a piece at a time.
+template <typename E>
+bool attn_vec_ok(const AttnArgs<E>& p) {
+  constexpr int P = Elem<E>::PIECE;
+  bool ok = p.da % P == 0 && p.dc % P == 0 && ((uintptr_t)p.o & 3) == 0;
+  auto operand = [&](const E* x, const int64_t* s) {
+    if (((uintptr_t)x & 3) != 0) ok = false;
+    for (int i = 0; i < 3; ++i)
+      if (s[i] * (int64_t)sizeof(E) % 4 != 0) ok = false;
+  };
+  operand(p.a, p.as), operand(p.b, p.bs), operand(p.c, p.cs);
+  return ok;
+}
+
 template <typename E>
 void launch_attn(hipStream_t st, AttnArgs<E> p, float* seg_state) {
   const AttnSplit split = attn_split<E>((int64_t)p.B * p.H, p.T);
   p.segs = split.segs, p.seg_len = split.len, p.seg_state = seg_state;
-  auto go = [&](auto da, auto dc) {
+  const bool vec = attn_vec_ok(p);
+  auto run = [&](auto da, auto dc, auto v) {
     using S = AttnShape<E, da(), dc()>;
     const dim3 grid((unsigned)(p.B * p.H * p.segs));
     if (p.segs > 1) {
-      hipLaunchKernelGGL((attn_chunk_kernel<E, da(), dc(), false>), grid, dim3(S::THREADS), S::LDS_STATE, st, p);
+      auto k = attn_chunk_kernel<E, da(), dc(), false, v()>;
+      lds_optin(k, S::LDS_STATE);
+      hipLaunchKernelGGL(k, grid, dim3(S::THREADS), S::LDS_STATE, st, p);
       hipLaunchKernelGGL((attn_scan_kernel<E>), dim3((unsigned)(p.B * p.H * ceil_div(p.da * p.dc, 256))), dim3(256), 0,
                          st, p);
     }
-    auto k = attn_chunk_kernel<E, da(), dc(), true>;
+    auto k = attn_chunk_kernel<E, da(), dc(), true, v()>;
     lds_optin(k, S::LDS);
     hipLaunchKernelGGL(k, grid, dim3(S::THREADS), S::LDS, st, p);
+  };
+  auto go = [&](auto da, auto dc) {
+    if (vec) run(da, dc, std::true_type());
+    else run(da, dc, std::false_type());
   };
   using std::integral_constant;
   auto with_c = [&](auto da) {
@@ -167,6 +193,7 @@ template <typename E>
 int attn_forward_impl(hipStream_t st, const tmpc_decay_attention* x, void* o, float* state_out, void* ws, size_t wsb) {
   if (!attn_shape_ok(x)) return TMPC_EBADSHAPE;
   if (x->B == 0) return TMPC_OK;
+  if (!step_ok(x->q_stride) || !step_ok(x->k_stride) || !step_ok(x->v_stride)) return TMPC_EBADSHAPE;
   if (!x->log_decay || (x->T > 0 && (!x->q || !x->k || !x->v || !o))) return TMPC_EBADARG;
   const size_t need = attn_ws_bytes<E>(x, false);
   if (wsb < need) return TMPC_EWORKSPACE;
@@ -187,6 +214,8 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
                        size_t wsb) {
   if (!attn_shape_ok(x)) return TMPC_EBADSHAPE;
   if (x->B == 0) return TMPC_OK;
+  if (!step_ok(x->q_stride) || !step_ok(x->k_stride) || !step_ok(x->v_stride) || (dos && !step_ok(dos)))
+    return TMPC_EBADSHAPE;
   if (!x->log_decay || !dos || (x->T > 0 && (!x->q || !x->k || !x->v || !d_o || !dq || !dk || !dv)))
     return TMPC_EBADARG;
   if (wsb < attn_ws_bytes<E>(x, true)) return TMPC_EWORKSPACE;

@@ -22,6 +22,7 @@ from .. import _lib
 _SUFFIX = {torch.float32: "f32", torch.bfloat16: "bf16"}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 MAX_HEAD_WIDTH = 128
+MAX_HEADS = 32768
 MAX_NORM_WIDTH = 8192
 
 
@@ -54,6 +55,12 @@ def _first(name: str, t: torch.Tensor, dims) -> str:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with contiguous rows: itself where it has them."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _steps(t: torch.Tensor) -> torch.Tensor:
+    """A history (B, T, H, d) as the kernels read it: contiguous rows, steps less than 2^23
+    elements apart."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(1) < 1 << 23 else t.contiguous()
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
@@ -179,6 +186,8 @@ def _check_attention(q, k, v, log_decay, scale, step):
         raise ValueError(f"v has shape {tuple(vs)}, expected {tuple(lead) + (Hk, 'dv')}")
     if H < 1 or Hk < 1 or H % Hk:
         raise ValueError(f"the {H} heads of q are not a multiple of the {Hk} heads of k and v")
+    if H > MAX_HEADS:
+        raise ValueError(f"q has {H} heads, expected at most {MAX_HEADS}")
     for name, d in (("q and k", dk), ("v", vs[-1])):
         if not 1 <= d <= MAX_HEAD_WIDTH:
             raise ValueError(f"{name} have heads of {d} elements, expected 1 to {MAX_HEAD_WIDTH}")
@@ -212,7 +221,7 @@ class _DecayAttention(torch.autograd.Function):
     def backward(ctx, d_o, d_out):
         q, k, v, log_decay, state, lengths = ctx.saved_tensors
         dev = q.device
-        d_o = _rows(d_o) if d_o is not None else torch.zeros(q.shape[:-1] + v.shape[-1:], dtype=q.dtype, device=dev)
+        d_o = _steps(d_o) if d_o is not None else torch.zeros(q.shape[:-1] + v.shape[-1:], dtype=q.dtype, device=dev)
         d_out = d_out.contiguous() if d_out is not None else None
         empty = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
         dq, dk, dv = empty(q), empty(k), empty(v)
@@ -245,7 +254,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         _check("lengths", lengths, q, (B,), torch.int32)
     state = state.contiguous() if state is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    args = (_rows(q), _rows(k), _rows(v), log_decay.contiguous(), state, lengths, scale, sfx)
+    args = (_steps(q), _steps(k), _steps(v), log_decay.contiguous(), state, lengths, scale, sfx)
     return _DecayAttention.apply(*args) if _wants_grad(q, k, v, state) else _attention_forward(*args)
 
 
