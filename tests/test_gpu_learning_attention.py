@@ -282,3 +282,12 @@ def test_refusals():
                     (ValueError, dict(q=q.clone().requires_grad_(True))), (ValueError, dict(q=x["q"]))]:
         with pytest.raises(err):
             learning.decay_attention_step(**{**dict(q=q, k=k, v=v, log_decay=x["g"], state=x["state"]), **kw})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B", [6, 130])
+def test_shared_heads_of_small_and_large_batches(B, dtype):
+    """Key/value heads shared by four: the gradients are sums over a group's heads."""
+    x = inputs(B, 70, 8, 2, 16, 24, dtype, seed=18)
+    lengths = torch.arange(B, dtype=torch.int32, device=DEV) % 72
+    check(x, run(x, lengths), dtype, lengths)

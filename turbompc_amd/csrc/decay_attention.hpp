@@ -57,9 +57,8 @@ __device__ inline float decay_pow(float g, int n) { return n == 0 ? 1.0f : __exp
 // A workgroup carries one (problem, head) through its chunks.  Wave w owns NV
 // 16-column tiles of the values and all of the scores: S, the scores and O stay in
 // its registers (each product's accumulator is the next one's operand) and waves meet
-// only where a chunk's rows change in LDS.  Every wave forms the scores again, 10 of
-// its products of 16 x 16 for C = 64: cheaper than an exchange through LDS and the
-// barrier that it needs.
+// only where a chunk's rows change in LDS.  Every wave forms the scores again: cheaper than
+// an exchange through LDS and the barrier that it needs, up to 128 x 128.
 template <typename E, int DA, int DC>
 struct AttnShape {
   static constexpr int W = DC / 16 < 4 ? DC / 16 : 4;  // waves
@@ -67,8 +66,12 @@ struct AttnShape {
   static constexpr int THREADS = 64 * W;
   static constexpr int C = AttnTile<E>::C;
   static constexpr int LDA = DA + AttnTile<E>::PAD, LDC = DC + AttnTile<E>::PAD;
-  // elements of a chunk's rows in LDS: b and c, and a with outputs
-  static constexpr int TILE_STATE = C * LDA + C * LDC, TILE = TILE_STATE + C * LDA;
+  // 128 x 128: the registers do not hold the operands of all scores beside S, so the waves
+  // share the scores out and exchange them in LDS
+  static constexpr bool SHARE = DA == 128 && DC == 128;
+  static constexpr int LDP = C + AttnTile<E>::PAD;
+  // elements of a chunk's rows in LDS: b and c, and a (and the scores) with outputs
+  static constexpr int TILE_STATE = C * LDA + C * LDC, TILE = TILE_STATE + C * LDA + (SHARE ? C * LDP : 0);
   // workgroups of a CU, by their registers; the tiles twice (one barrier a chunk instead of
   // two) where they still fit
   static constexpr int PER_CU = 2;
@@ -168,11 +171,37 @@ struct AttnPowers {
 // One chunk of one recurrence for a wave's NV value tiles (columns col0 ..): the outputs
 // through store(tile it, x, values of row 16 it + lo, columns 4 hi ..), and the state.
 // n live steps; ta, tb (C x DA, pitch LDA) and tc (pitch LDC) hold zeros after them.
-template <typename E, int KA, int NV, int CT, bool FULL, int LDA, int LDC, typename Store>
-__device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, int col0, f32x4 (&s)[KA][NV],
+template <typename E, typename S, int KA, int NV, int CT, bool FULL, typename Store>
+__device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, int col0, f32x4 (&s)[KA][NV],
                                   const AttnPowers<CT>& pw, float g, float su, int rev, int n, int lane, Store store) {
-  constexpr int C = 16 * CT;
-  const int hi = lane >> 4;
+  constexpr int C = S::C, LDA = S::LDA, LDC = S::LDC, LDP = S::LDP;
+  const int lo = lane & 15, hi = lane >> 4;
+  // A tile (it, jt <= it) of the scores as its transpose: a lane holds 4 consecutive j of one
+  // i, the operand of the product with V; rounded to E, as the output is.  a: row tile it's quads.
+  auto score = [&](int jt, const quad_t<E>(&a)[KA]) {
+    f32x4 t = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < KA; k += 2)
+      t = mma2(lds_quad(tb, LDA, 16 * jt, 16 * k, lane), lds_quad(tb, LDA, 16 * jt, 16 * k + 16, lane), a[k], a[k + 1], t);
+    return t;
+  };
+  if constexpr (FULL && S::SHARE) {
+    for (int q = S::W - 1 - (col0 / (16 * NV)); q < CT * (CT + 1) / 2; q += S::W) {
+      int it = 0, jt = q;
+      while (jt > it) jt -= ++it;
+      float far = 1.0f;
+#pragma unroll
+      for (int d = 1; d < CT - 1; ++d) far *= it - jt - 1 >= d ? pw.tile[1] : 1.0f;
+      quad_t<E> a[KA];
+#pragma unroll
+      for (int k = 0; k < KA; ++k) a[k] = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
+      f32x4 t = score(jt, a);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[r] *= it == jt ? pw.diag[r] : far * pw.near[r];
+      *reinterpret_cast<quad_t<E>*>(tp + (16 * it + lo) * LDP + 16 * jt + 4 * hi) = to_quad<E>(t);
+    }
+    __syncthreads();
+  }
   // the wave's values, contracted over the steps
   quad_t<E> v[CT][NV];
 #pragma unroll
@@ -188,7 +217,7 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, int col
       for (int x = 0; x < NV; ++x) sq[k][x] = to_quad<E>(s[k][x]);
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
-      asm volatile("" ::: "memory");  // the keys are read again for each tile: kept, they would cost the registers
+      if constexpr ((KA == 4 && NV == 2) || S::SHARE) asm volatile("" ::: "memory");  // no operand is kept from tile to tile: too many
       quad_t<E> a[KA];
 #pragma unroll
       for (int k = 0; k < KA; ++k) a[k] = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
@@ -205,22 +234,20 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, int col
       for (int x = 0; x < NV; ++x) acc[x] *= f;
 #pragma unroll
       for (int j = 0; j <= it; j += 2) {
-        // score tiles as their transposes: a lane holds 4 consecutive j of one i, the operand
-        // of the product with V; rounded to E, as the output is
         quad_t<E> p[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int jt = j + e;
-          f32x4 t = {0, 0, 0, 0};
-          if (jt <= it) {
-#pragma unroll
-            for (int k = 0; k < KA; k += 2)
-              t = mma2(lds_quad(tb, LDA, 16 * jt, 16 * k, lane), lds_quad(tb, LDA, 16 * jt, 16 * k + 16, lane), a[k],
-                       a[k + 1], t);
+          if (jt > it) {
+            p[e] = to_quad<E>(f32x4{0, 0, 0, 0});
+          } else if constexpr (S::SHARE) {
+            p[e] = lds_quad(tp, LDP, 16 * it, 16 * jt, lane);
+          } else {
+            f32x4 t = score(jt, a);
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] *= jt == it ? pw.diag[r] : pw.tile[it > jt ? it - jt - 1 : 0] * pw.near[r];
+            p[e] = to_quad<E>(t);
           }
-          p[e] = to_quad<E>(t);
         }
 #pragma unroll
         for (int x = 0; x < NV; ++x) acc[x] = mma2(v[j][x], v[j + 1][x], p[0], p[1], acc[x]);
@@ -382,7 +409,7 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
     if constexpr (FULL) ra.store(ta);
     __syncthreads();
     if (t0 + C < end) fetch(end - t0 - C);
-    attn_chunk<E, KA, NV, CT, FULL, LDA, LDC>(ta, tb, tc, col0, s, pw, g, p.su, p.rev, n, lane,
+    attn_chunk<E, S, KA, NV, CT, FULL>(ta, tb, tc, ta + C * LDA, col0, s, pw, g, p.su, p.rev, n, lane,
                                               [&](int it, int x, f32x4 v) {
       const __amdgpu_buffer_rsrc_t rs = buffer_at(obuf);
       const unsigned at = 16 * it + lo < n && ooff[x] != kNowhere ? ooff[x] + it * otile : kNowhere;
@@ -454,15 +481,18 @@ __global__ __launch_bounds__(256) void attn_scan_kernel(AttnArgs<E> p) {
 }
 
 // Sums the shared heads' gradients: (tokens, Hk, G, d) fp32 -> (tokens, Hk, d), in order.
+// A thread 4 columns of a row; q = ceil(d / 4).
 template <typename E>
-__global__ __launch_bounds__(256) void attn_head_sum_kernel(const float* __restrict__ in, int64_t n, int G, int d,
+__global__ __launch_bounds__(256) void attn_head_sum_kernel(const float* __restrict__ in, int64_t rows, int G, int d, int q,
                                                             E* __restrict__ out) {
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    const int64_t row = e / d;
-    const float* src = in + row * G * d + (e - row * d);
-    float v = 0.0f;
-    for (int i = 0; i < G; ++i) v += src[(int64_t)i * d];
-    out[e] = (E)v;
+  const int per = 256 / q;  // rows a block at a time
+  const int r = threadIdx.x / q, c = (threadIdx.x - r * q) * 4;
+  if (r >= per) return;
+  for (int64_t row = (int64_t)blockIdx.x * per + r; row < rows; row += (int64_t)gridDim.x * per) {
+    const float* src = in + row * G * d;
+    f32x4 v = {0, 0, 0, 0};
+    for (int i = 0; i < G; ++i) v += load_quad_f32(src + (int64_t)i * d, c, d);
+    store_quad(out + row * d, c, d, v);
   }
 }
 

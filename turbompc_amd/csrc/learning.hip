@@ -234,6 +234,8 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
     p.s_in = x->state_in, p.s_in_t = 1, p.o = dq;
     launch_attn(st, p, seg_state);
   }
+  // shared heads' gradients: every head's part in fp32, then their sum.  (Taking a group's heads
+  // in turn in one workgroup needs no such parts, but its registers spill: 1755 us against 1088.)
   const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
   float* gk = G > 1 ? (float*)rest : nullptr;
   float* gv = G > 1 ? (float*)(rest + align_up(tok * x->dk)) : nullptr;
@@ -261,9 +263,10 @@ int attn_backward_impl(hipStream_t st, const tmpc_decay_attention* x, const void
   }
   if (G > 1 && x->T > 0) {
     auto sum = [&](const float* in, int d, void* out) {
-      const int64_t n = (int64_t)x->B * x->T * x->Hk * d;
-      hipLaunchKernelGGL((attn_head_sum_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 16 * kCUs)),
-                         dim3(256), 0, st, in, n, G, d, (E*)out);
+      const int64_t rows = (int64_t)x->B * x->T * x->Hk;
+      const int q = (d + 3) / 4;
+      hipLaunchKernelGGL((attn_head_sum_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(rows, 256 / q), 16 * kCUs)),
+                         dim3(256), 0, st, in, rows, G, d, q, (E*)out);
     };
     sum(gk, x->dk, dk);
     sum(gv, x->dv, dv);
