@@ -658,7 +658,7 @@ int tmpc_decay_attention_step_bf16(hipStream_t stream, const tmpc_decay_attentio
 
 /* Gated feed-forward block: y = (act(x w_gate^T) o (x w_up^T)) w_down^T for
  * rows x (M, D) of pitch ldx, w_gate, w_up (F, D), w_down (Dout, F) contiguous;
- * activation 0: silu, 1: gelu (exact). */
+ * activation 0: silu, 1: gelu (exact).  Widths and pitches at most 2^21. */
 typedef struct tmpc_gated_ff {
   int64_t M;
   int32_t D, F, Dout, activation;

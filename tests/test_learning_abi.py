@@ -66,6 +66,8 @@ def test_feed_forward_refusals(lib, sfx):
     assert fwd(None, make(), X, None, None, X, need - 1) == 3
     assert bwd(None, make(), X, X, X, 8, X, X, X, X, X, need - 1) == 3
     assert fwd(None, make(M=0), None, None, None, None, 0) == 0
+    for backward in (0, 1):  # an empty batch has a workspace query too
+        assert lib.tmpc_gated_ff_workspace_bytes(eb, make(M=0), backward) == 0
 
 
 @pytest.mark.parametrize("sfx", SFX)

@@ -62,60 +62,70 @@ enum GemmEpi {
 };
 
 template <typename E>
-struct GemmTile {
-  static constexpr int BK = sizeof(E) == 2 ? 64 : 32;
-  static constexpr int PAD = 16 / sizeof(E);
-};
+constexpr int kGemmBK = 128 / sizeof(E);  // contracted entries of a step
 
 // The operand tile of one K step: global memory -> registers -> LDS.
-template <typename E, int BR, int THREADS, bool TR, bool DUAL>
+template <typename E, int BR, int BK, int THREADS, bool TR, bool DUAL>
 struct Stage {
-  static constexpr int BK = GemmTile<E>::BK, P = Elem<E>::PIECE, PAD = GemmTile<E>::PAD;
+  static constexpr int P = Elem<E>::PIECE, PAD = 16 / sizeof(E);
   static constexpr int LD = TR ? BR + PAD : BK + PAD;
   static constexpr int ELEMS = TR ? BK * LD : BR * LD;
-  static constexpr int PIECES = BR * BK / P, NP = (PIECES + THREADS - 1) / THREADS;
+  static constexpr int NP = BR * BK / P / THREADS;
+  static_assert(NP * THREADS * P == BR * BK, "a whole number of pieces a thread");
   piece_t<E> r[NP];
 
-  // rows r0 .. of an operand with `rows` rows (outer index) and K contracted entries
+  // Rows r0 .. of an operand with `rows` rows (outer index) and K contracted entries, zeros
+  // past K.  Which of the three ways is the same for the whole tile, and none branches
+  // between its loads, so that all of them are in flight together.
   __device__ void load(const E* const* src, int seg, int64_t ld, int64_t r0, int64_t rows, int64_t k0, int64_t K, int tid) {
-    const bool k_in = k0 + BK <= K, r_in = r0 + BR <= rows;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int e = tid + i * THREADS;
-      if (PIECES % THREADS != 0 && e >= PIECES) break;
-      if constexpr (!TR) {
-        const int row = e / (BK / P), c = (e - row * (BK / P)) * P;
-        int64_t gr;
-        const E* base;
-        if constexpr (DUAL) {  // 16 rows of the one, 16 of the other
-          gr = r0 + (row >> 5) * 16 + (row & 15);
-          base = src[(row >> 4) & 1];
-        } else {
-          gr = r0 + row;
-          base = src[seg];
-        }
-        gr = gr < rows ? gr : rows - 1;  // past the edge: any row, its results are not stored
-        const E* rp = base + gr * ld;
-        if (k_in)
-          r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(rp + k0 + c);
-        else
-          r[i] = load_piece(rp + k0, c, (int)(K - k0), true);
+    const int rl = (int)(rows - r0 < BR ? rows - r0 : BR), kl = (int)(K - k0 < BK ? K - k0 : BK);  // live ones, >= 1
+    const int width = TR ? rl : kl, deep = TR ? kl : rl;  // of a stored row; stored rows
+    // piece i's place in the tile, and its row of the operand (past the edge: the last one)
+    auto piece = [&](int i, int& row, int& c) -> const E* {
+      const int e = tid + i * THREADS, w = (TR ? BR : BK) / P;
+      row = e / w, c = (e - row * w) * P;
+      if constexpr (DUAL) {  // 16 rows of the one, 16 of the other
+        const int f = (row >> 5) * 16 + (row & 15);
+        return src[(row >> 4) & 1] + (r0 + min(f, deep - 1)) * ld + k0;
       } else {
-        const int kr = e / (BR / P), c = (e - kr * (BR / P)) * P;
-        const E* rp = src[seg] + (k0 + kr) * ld + r0;
-        if (k_in && r_in)
-          r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(rp + c);
-        else
-          r[i] = load_piece(rp, c, (int)(rows - r0 < BR ? rows - r0 : BR), k0 + kr < K);
+        const int64_t f = min(row, deep - 1);
+        return src[seg] + (TR ? (k0 + f) * ld + r0 : (r0 + f) * ld + k0);
+      }
+    };
+    if (width == (TR ? BR : BK) && (!TR || deep == BK)) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        int row, c;
+        const E* at = piece(i, row, c);
+        r[i] = *reinterpret_cast<const typename Elem<E>::piece_u*>(at + c);
+      }
+    } else if (width % P == 0) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        int row, c;
+        const E* at = piece(i, row, c);
+        const piece_t<E> v = *reinterpret_cast<const typename Elem<E>::piece_u*>(at + min(c, width - P));
+        const bool live = c < width && (!TR || row < deep);
+#pragma unroll
+        for (int e = 0; e < P; ++e) r[i][e] = live ? v[e] : E(0.0f);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        int row, c;
+        const E* at = piece(i, row, c);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const E v = at[min(c + e, width - 1)];
+          r[i][e] = c + e < width && (!TR || row < deep) ? v : E(0.0f);
+        }
       }
     }
   }
   __device__ void store(E* t, int tid) const {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int e = tid + i * THREADS;
-      if (PIECES % THREADS != 0 && e >= PIECES) break;
-      const int w = TR ? BR / P : BK / P;
+      const int e = tid + i * THREADS, w = (TR ? BR : BK) / P;
       const int row = e / w, c = (e - row * w) * P;
       *reinterpret_cast<piece_t<E>*>(t + row * LD + c) = r[i];
     }
@@ -194,12 +204,12 @@ __device__ inline void gemm_epilogue(const GemmArgs<E>& p, const f32x4 (&acc)[TM
 template <typename E, int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI, int ACT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs<E> p) {
   constexpr bool DUAL = EPI == EPI_GATE || EPI == EPI_GATE_SAVE;
-  constexpr int THREADS = 64 * WM * WN, BK = GemmTile<E>::BK;
+  constexpr int THREADS = 64 * WM * WN, BK = kGemmBK<E>;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr bool WHOLE = !AT && !BT;
   constexpr int BF = DUAL ? BN / 2 : BN;  // output columns of the tile
-  using SA = Stage<E, BM, THREADS, AT, false>;
-  using SB = Stage<E, BN, THREADS, BT, DUAL>;
+  using SA = Stage<E, BM, BK, THREADS, AT, false>;
+  using SB = Stage<E, BN, BK, THREADS, BT, DUAL>;
   extern __shared__ __align__(16) char smem[];
   E* ta = reinterpret_cast<E*>(smem);
   E* tb = ta + 2 * SA::ELEMS;
@@ -367,7 +377,8 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs<E> p) {
 
 template <typename E, int BM, int BN, bool AT, bool BT, int THREADS, bool DUAL>
 constexpr size_t gemm_lds() {
-  return 2 * sizeof(E) * (size_t)(Stage<E, BM, THREADS, AT, false>::ELEMS + Stage<E, BN, THREADS, BT, DUAL>::ELEMS);
+  constexpr int BK = kGemmBK<E>;
+  return 2 * sizeof(E) * (size_t)(Stage<E, BM, BK, THREADS, AT, false>::ELEMS + Stage<E, BN, BK, THREADS, BT, DUAL>::ELEMS);
 }
 
 }  // namespace tmpc

@@ -289,8 +289,11 @@ int attn_step_impl(hipStream_t st, const tmpc_decay_attention* x, const uint8_t*
 }
 
 // ------------------------------------------------------ gated feed-forward --
+constexpr int64_t kMaxPitch = 1 << 21;  // elements: 256 rows of a tile lie within 31 bits
+
 bool ff_shape_ok(const tmpc_gated_ff* a) {
-  return a && a->M >= 0 && a->D >= 1 && a->F >= 1 && a->Dout >= 1 && a->M <= 0x7fffffff;
+  return a && a->M >= 0 && a->M <= 0x7fffffff && a->D >= 1 && a->D <= kMaxPitch && a->F >= 1 && a->F <= kMaxPitch &&
+         a->Dout >= 1 && a->Dout <= kMaxPitch && a->ldx <= kMaxPitch;
 }
 // pitch of the block's own (M, F) arrays: rows of whole 16-byte pieces
 template <typename E>
@@ -349,8 +352,8 @@ void launch_gemm(hipStream_t st, GemmArgs<E> p, GemmPlan plan) {
     case FORM_WIDE:
       if constexpr (sizeof(E) == 2) {
         auto k = gemm_wide_kernel<AT, BT, EPI, ACT>;
-        lds_optin(k, kWideLds);
-        hipLaunchKernelGGL(k, grid(256, DUAL ? 128 : 256), dim3(512), kWideLds, st, p);
+        lds_optin(k, wide_lds(EPI));
+        hipLaunchKernelGGL(k, grid(256, DUAL ? 128 : 256), dim3(512), wide_lds(EPI), st, p);
       }
       break;
     case FORM_128: go(integral_constant<int, 128>(), integral_constant<int, 128>()); break;
@@ -359,16 +362,47 @@ void launch_gemm(hipStream_t st, GemmArgs<E> p, GemmPlan plan) {
   }
 }
 
-// The form for a product that is not split: the largest tile that still gives most of the
-// chip work.
+// Small products have few tiles, each a chain of K steps whose loads' latency (about 1.3 us a
+// step) nothing hides: the contracted index is split until four workgroups a CU hide it
+// (fp32, 2091 x 200 from 2 x 520: 44 us in one, 29 in three with their sum).
+template <typename E>
+int store_splits(int64_t M, int64_t N, int64_t K, GemmForm form) {
+  if (M == 0 || (form != FORM_64 && form != FORM_32)) return 1;
+  const int64_t tiles = tiles_of(M, N, form == FORM_64 ? 64 : 32, 64);
+  return (int)std::max<int64_t>(1, std::min(4 * kCUs / tiles, ceil_div(K, kGemmBK<E>) / 4));
+}
+// workspace for it: no form makes more splits of more rows than this
+template <typename E>
+size_t store_part_bytes(int64_t M, int64_t N, int64_t K) {
+  int most = 1;
+  for (GemmForm f : {FORM_64, FORM_32}) most = std::max(most, store_splits<E>(M, N, K, f));
+  return most > 1 ? align_up((size_t)most * M * N * sizeof(float)) : 0;
+}
+
+// The form of a product: the largest tile that still gives most of the chip work.
 template <typename E, bool AT, bool BT, int EPI>
 GemmPlan gemm_plan(const GemmArgs<E>& p, bool own_a, bool own_b) {
   constexpr int D = EPI == EPI_GATE || EPI == EPI_GATE_SAVE ? 2 : 1;
   if (!AT && !BT && p.nseg == 1 && p.M <= 64) return {FORM_ROWS, 1};
   if (wide_ok(p, AT, BT, own_a, own_b) && tiles_of(p.M, p.N, 256, 256 / D) >= 96) return {FORM_WIDE, 1};
   if (tiles_of(p.M, p.N, 128, 128 / D) >= 192) return {FORM_128, 1};
-  if (tiles_of(p.M, p.N, 64, 64 / D) >= 192) return {FORM_64, 1};
-  return {FORM_32, 1};
+  const GemmForm form = tiles_of(p.M, p.N, 64, 64 / D) >= 192 ? FORM_64 : FORM_32;
+  return {form, EPI == EPI_STORE ? store_splits<E>(p.M, p.N, p.K, form) : 1};
+}
+
+// launch_gemm, with the sum over the plan's splits through `part`
+template <typename E, bool AT, bool BT>
+void launch_store(hipStream_t st, GemmArgs<E> p, GemmPlan plan, float* part) {
+  if (plan.splits == 1) {
+    launch_gemm<E, AT, BT, EPI_STORE>(st, p, plan);
+    return;
+  }
+  p.part = part;
+  p.k_split = ceil_div(ceil_div(p.K, kGemmBK<E>), plan.splits) * kGemmBK<E>;
+  launch_gemm<E, AT, BT, EPI_PART>(st, p, plan);
+  const int64_t n = p.M * p.N;
+  hipLaunchKernelGGL((gemm_reduce_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n * (1 + p.pair), 1024), 8 * kCUs)),
+                     dim3(256), 0, st, part, n, 1 + p.pair, plan.splits, p.o0, p.o1);
 }
 
 // The weight gradients' rows are few and their contracted index is every row of the batch:
@@ -377,22 +411,21 @@ GemmPlan gemm_plan(const GemmArgs<E>& p, bool own_a, bool own_b) {
 template <typename E>
 int grad_splits(int64_t rows, int64_t cols, int64_t K, int pair, int tile) {
   const int64_t tiles = tiles_of(rows, cols, tile, tile) * (1 + pair);
-  return (int)std::max<int64_t>(1, std::min((tile == 256 ? 1 : 2) * kCUs / tiles, K / (8 * GemmTile<E>::BK)));
+  return (int)std::max<int64_t>(1, std::min((tile == 256 ? 1 : 2) * kCUs / tiles, K / (8 * kGemmBK<E>)));
 }
-// the tile of a weight gradient: 256 where it wastes little of its edges, else 128, and 64
-// where those are few even when split
+// the tile of a weight gradient: 256 where it wastes little of its edges, 128 where those are
+// many (fp32, 520 x 200 over 2091 rows: 42 us in 128s, 25 splits of 20 tiles, 20 us in 64s)
 template <typename E>
-int grad_tile(int64_t rows, int64_t cols, int64_t K, int pair) {
+int grad_tile(int64_t rows, int64_t cols, int pair) {
   if (sizeof(E) == 2 && rows >= 192 && cols >= 192 && tiles_of(rows, cols, 256, 256) * 256 * 256 <= rows * cols * 3 / 2)
     return 256;
-  const int64_t t = tiles_of(rows, cols, 128, 128) * (1 + pair);
-  return t * grad_splits<E>(rows, cols, K, pair, 128) >= kCUs / 2 ? 128 : 64;
+  return tiles_of(rows, cols, 128, 128) * (1 + pair) >= kCUs / 4 ? 128 : 64;
 }
 template <typename E>
 size_t grad_part_bytes(int64_t rows, int64_t cols, int64_t K, int pair) {
   // the wide kernel's tile and the one that stands in for it where the operands are not aligned
   int most = 1;
-  for (int tile : {grad_tile<E>(rows, cols, K, pair), 128})
+  for (int tile : {grad_tile<E>(rows, cols, pair), 128})
     most = std::max(most, grad_splits<E>(rows, cols, K, pair, tile));
   return most > 1 ? align_up((size_t)most * (1 + pair) * rows * cols * sizeof(float)) : 0;
 }
@@ -400,8 +433,8 @@ size_t grad_part_bytes(int64_t rows, int64_t cols, int64_t K, int pair) {
 template <typename E>
 size_t ff_ws_bytes(const tmpc_gated_ff* a, bool backward) {
   const size_t act = align_up((size_t)a->M * ff_pitch<E>(a) * sizeof(E));
-  if (!backward) return act;
-  return 3 * act + std::max(grad_part_bytes<E>(a->F, a->D, a->M, 1), grad_part_bytes<E>(a->Dout, a->F, a->M, 0));
+  if (!backward) return act + store_part_bytes<E>(a->M, a->Dout, a->F);
+  return 3 * act + std::max(store_part_bytes<E>(a->M, a->D, a->F), std::max(grad_part_bytes<E>(a->F, a->D, a->M, 1), grad_part_bytes<E>(a->Dout, a->F, a->M, 0)));
 }
 
 // dW (rows, cols) = P^T X over the batch's M rows, and with out1 a second one, P1^T X, beside it
@@ -411,20 +444,11 @@ void launch_weight_grad(hipStream_t st, int64_t M, int rows, int cols, const E* 
   GemmArgs<E> p{};
   p.M = rows, p.N = cols, p.nseg = 1, p.K = M, p.pair = out1 != nullptr;
   p.A[0] = P, p.A[1] = P1, p.lda = ldp, p.B[0] = X, p.ldb = ldx;
-  p.o0 = out, p.o1 = out1, p.ldo = cols, p.part = part;
-  int tile = grad_tile<E>(rows, cols, M, p.pair);
+  p.o0 = out, p.o1 = out1, p.ldo = cols;
+  int tile = grad_tile<E>(rows, cols, p.pair);
   if (tile == 256 && !wide_ok(p, true, true, own_p, own_x)) tile = 128;
-  const GemmPlan plan{tile == 256 ? FORM_WIDE : tile == 128 ? FORM_128 : FORM_64,
-                      grad_splits<E>(rows, cols, M, p.pair, tile)};
-  if (plan.splits == 1) {
-    launch_gemm<E, true, true, EPI_STORE>(st, p, plan);
-    return;
-  }
-  p.k_split = ceil_div(ceil_div(M, GemmTile<E>::BK), plan.splits) * GemmTile<E>::BK;
-  launch_gemm<E, true, true, EPI_PART>(st, p, plan);
-  const int64_t n = (int64_t)rows * cols;
-  hipLaunchKernelGGL((gemm_reduce_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(n * (1 + p.pair), 1024), 8 * kCUs)),
-                     dim3(256), 0, st, part, n, 1 + p.pair, plan.splits, out, out1);
+  launch_store<E, true, true>(st, p, {tile == 256 ? FORM_WIDE : tile == 128 ? FORM_128 : FORM_64,
+                                      grad_splits<E>(rows, cols, M, p.pair, tile)}, part);
 }
 
 template <typename E>
@@ -454,14 +478,15 @@ int ff_forward_impl(hipStream_t st, const tmpc_gated_ff* a, void* y, float* gate
   GemmArgs<E> d{};
   d.M = a->M, d.N = a->Dout, d.nseg = 1, d.K = a->F;
   d.A[0] = h, d.lda = ldh, d.B[0] = (const E*)a->w_down, d.ldb = a->F, d.o0 = (E*)y, d.ldo = a->Dout;
-  launch_gemm<E, false, false, EPI_STORE>(st, d, gemm_plan<E, false, false, EPI_STORE>(d, true, false));
+  launch_store<E, false, false>(st, d, gemm_plan<E, false, false, EPI_STORE>(d, true, false),
+                                 (float*)((char*)ws + align_up((size_t)a->M * ldh * sizeof(E))));
   return launch_status();
 }
 
 template <typename E>
 int ff_backward_impl(hipStream_t st, const tmpc_gated_ff* a, const float* gate, const float* up, const void* dy,
                      int64_t lddy, void* dx, void* dwg, void* dwu, void* dwd, void* ws, size_t wsb) {
-  if (!ff_shape_ok(a)) return TMPC_EBADSHAPE;
+  if (!ff_shape_ok(a) || lddy > kMaxPitch) return TMPC_EBADSHAPE;
   if (!a->w_gate || !a->w_up || !a->w_down || !dwg || !dwu || !dwd || a->ldx < 0 || lddy < 0 ||
       (a->M > 0 && (!a->x || !gate || !up || !dy || !dx)) ||
       (a->activation != ACT_SILU && a->activation != ACT_GELU))
@@ -488,7 +513,7 @@ int ff_backward_impl(hipStream_t st, const tmpc_gated_ff* a, const float* gate, 
     d.A[0] = dg, d.A[1] = du, d.lda = ldh;
     d.B[0] = (const E*)a->w_gate, d.B[1] = (const E*)a->w_up, d.ldb = a->D;
     d.o0 = (E*)dx, d.ldo = a->D;
-    launch_gemm<E, false, true, EPI_STORE>(st, d, gemm_plan<E, false, true, EPI_STORE>(d, true, false));
+    launch_store<E, false, true>(st, d, gemm_plan<E, false, true, EPI_STORE>(d, true, false), part);
   }
   launch_weight_grad<E>(st, a->M, a->F, a->D, dg, du, ldh, true, (const E*)a->x, a->ldx, false, (E*)dwg, (E*)dwu, part);
   launch_weight_grad<E>(st, a->M, a->Dout, a->F, (const E*)dy, nullptr, lddy, false, h, ldh, true, (E*)dwd, nullptr, part);

@@ -24,6 +24,7 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 MAX_HEAD_WIDTH = 128
 MAX_HEADS = 32768
 MAX_NORM_WIDTH = 8192
+MAX_FF_WIDTH = 1 << 21
 
 
 def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape=None, dtype=None):
@@ -64,8 +65,9 @@ def _steps(t: torch.Tensor) -> torch.Tensor:
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
-    """t as (rows, last axis) with contiguous rows: a view where one exists."""
-    return _rows(t if t.dim() == 2 else t.reshape(-1, t.shape[-1]))
+    """t as (rows, last axis) with contiguous rows, at most 2^21 elements apart: a view where one exists."""
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(0) <= MAX_FF_WIDTH else t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -339,6 +341,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if w_gate.dim() != 2 or w_gate.shape[1] != D or D < 1 or w_gate.shape[0] < 1:
         raise ValueError(f"w_gate has shape {tuple(w_gate.shape)}, expected ('F', {D}), neither empty")
     F = w_gate.shape[0]
+    if max(D, F, w_down.shape[0] if w_down.dim() else 0) > MAX_FF_WIDTH:
+        raise ValueError(f"the widths of x, w_gate and w_down must be at most {MAX_FF_WIDTH}")
     _check("w_up", w_up, x, (F, D))
     _check("w_down", w_down, x)
     if w_down.dim() != 2 or w_down.shape[1] != F or w_down.shape[0] < 1:
