@@ -622,7 +622,7 @@ int tmpc_rms_norm_backward_bf16(hipStream_t stream, int64_t rows, int32_t width,
  * Hk; head h reads key/value head h / (H / Hk).  1 <= dk, dv <= 128.  q (B, T,
  * H, dk), k (B, T, Hk, dk), v (B, T, Hk, dv) have contiguous rows and the given
  * strides (elements) of problem, step and head, that of a step at most 2^23 - 1;
- * H <= 32768. */
+ * H <= 32768 and B H <= 2^23. */
 typedef struct tmpc_decay_attention {
   int32_t B, T, H, Hk, dk, dv;
   const void *q, *k, *v;
@@ -658,7 +658,8 @@ int tmpc_decay_attention_step_bf16(hipStream_t stream, const tmpc_decay_attentio
 
 /* Gated feed-forward block: y = (act(x w_gate^T) o (x w_up^T)) w_down^T for
  * rows x (M, D) of pitch ldx, w_gate, w_up (F, D), w_down (Dout, F) contiguous;
- * activation 0: silu, 1: gelu (exact).  Widths and pitches at most 2^21. */
+ * activation 0: silu, 1: gelu (exact).  Widths and pitches at most 2^20,
+ * M at most 2^30. */
 typedef struct tmpc_gated_ff {
   int64_t M;
   int32_t D, F, Dout, activation;

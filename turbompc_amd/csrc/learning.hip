@@ -97,7 +97,7 @@ constexpr int64_t kMaxStep = (1 << 23) - 1; // elements between steps: 64 fp32 s
 
 bool attn_shape_ok(const tmpc_decay_attention* a) {
   return a && a->B >= 0 && a->T >= 0 && a->H >= 1 && a->Hk >= 1 && a->H % a->Hk == 0 && a->dk >= 1 && a->dk <= 128 &&
-         a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 0x7fffffff && a->H <= kMaxHeads;
+         a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 1 << 23 && a->H <= kMaxHeads;  // threads of a launch within 32 bits
 }
 // a chunk's steps lie within the 31 bits of a descriptor
 bool step_ok(const int64_t* stride) { return stride[1] >= 0 && stride[1] <= kMaxStep; }
@@ -289,10 +289,10 @@ int attn_step_impl(hipStream_t st, const tmpc_decay_attention* x, const uint8_t*
 }
 
 // ------------------------------------------------------ gated feed-forward --
-constexpr int64_t kMaxPitch = 1 << 21;  // elements: 256 rows of a tile lie within 31 bits
+constexpr int64_t kMaxPitch = 1 << 20;  // elements: 256 rows of a tile within 31 bits, 65535 tiles of 32 columns
 
 bool ff_shape_ok(const tmpc_gated_ff* a) {
-  return a && a->M >= 0 && a->M <= 0x7fffffff && a->D >= 1 && a->D <= kMaxPitch && a->F >= 1 && a->F <= kMaxPitch &&
+  return a && a->M >= 0 && a->M <= 1 << 30 && a->D >= 1 && a->D <= kMaxPitch && a->F >= 1 && a->F <= kMaxPitch &&
          a->Dout >= 1 && a->Dout <= kMaxPitch && a->ldx <= kMaxPitch;
 }
 // pitch of the block's own (M, F) arrays: rows of whole 16-byte pieces

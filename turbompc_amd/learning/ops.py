@@ -24,7 +24,7 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 MAX_HEAD_WIDTH = 128
 MAX_HEADS = 32768
 MAX_NORM_WIDTH = 8192
-MAX_FF_WIDTH = 1 << 21
+MAX_FF_WIDTH = 1 << 20
 
 
 def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape=None, dtype=None):
@@ -65,7 +65,7 @@ def _steps(t: torch.Tensor) -> torch.Tensor:
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
-    """t as (rows, last axis) with contiguous rows, at most 2^21 elements apart: a view where one exists."""
+    """t as (rows, last axis) with contiguous rows, at most 2^20 elements apart: a view where one exists."""
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(0) <= MAX_FF_WIDTH else t.contiguous()
 
