@@ -225,6 +225,9 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
       for (int x = 0; x < NV; ++x) sq[k][x] = to_quad<E>(s[k][x]);
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
+      // past the last live step.  (128 x 128 heads run long histories of whole chunks: there the
+      // branch cost 5% and saves nothing.)
+      if (!S::SHARE && 16 * it >= n) break;
       if constexpr ((KA == 4 && NV == 2) || S::SHARE) asm volatile("" ::: "memory");  // no operand is kept from tile to tile: too many
       quad_t<E> a[KA];
 #pragma unroll
@@ -275,6 +278,7 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
     for (int x = 0; x < NV; ++x) s[m][x] *= fl;
 #pragma unroll
   for (int j = 0; j < CT; j += 2) {
+    if (!S::SHARE && 16 * j >= n) break;
     f32x4 d0, d1;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
