@@ -1,5 +1,5 @@
-// What the history model's kernels (learning.hip) share: the element types, the
-// matrix-instruction operands ("quads") and wave reductions.
+// What the history model's kernels (learning.hip) share: the element types and the
+// matrix-instruction operands ("quads").
 //
 // Operand convention of the 16x16 matrix instructions here: lane l holds index
 // l % 16 of the operand's outer dimension and 4 consecutive entries of the
@@ -155,12 +155,6 @@ __device__ inline f32x4 mma2(f32x4 a0, f32x4 a1, f32x4 b0, f32x4 b1, f32x4 acc) 
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[e], b1[e], acc, 0, 0, 0);
   return acc;
-}
-
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
 }
 
 }  // namespace tmpc
