@@ -72,11 +72,16 @@ class HistoryWeights(nn.Module):
         return dict(zip(self.sizes, w.split(list(self.sizes.values()), dim=-1)))
 
     def forward(self, history: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
-        """Weights (B, size) from histories (B, T, features); lengths (B,) int32 of ragged ones
-        (a problem without history is read from its first row's stream alone)."""
+        """Weights (B, size) from histories (B, T >= 1, features); lengths (B,) int32 of ragged
+        ones, clamped to 0..T (a problem without history is read from its first row's stream
+        alone)."""
         B, T = history.shape[:2]
+        if T < 1:
+            raise ValueError("the histories have no rows")
         x = history.to(self.w_in.dtype)
-        if lengths is not None:  # rows past a history's end may hold anything, which w_in's gradient would read
+        if lengths is not None:
+            lengths = lengths.clamp(0, T)
+            # rows past a history's end may hold anything, which w_in's gradient would read
             live = torch.arange(T, device=x.device) < lengths[:, None]
             x = torch.where(live[..., None], x, torch.zeros((), dtype=x.dtype, device=x.device))
         a, s = nn.functional.linear(x, self.w_in), None
