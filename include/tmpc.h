@@ -622,7 +622,7 @@ int tmpc_rms_norm_backward_bf16(hipStream_t stream, int64_t rows, int32_t width,
  * Hk; head h reads key/value head h / (H / Hk).  1 <= dk, dv <= 128.  q (B, T,
  * H, dk), k (B, T, Hk, dk), v (B, T, Hk, dv) have contiguous rows and the given
  * strides (elements) of problem, step and head, that of a step at most 2^23 - 1;
- * H <= 32768 and B H <= 2^23. */
+ * T <= 2^30, H <= 32768 and B H <= 2^23. */
 typedef struct tmpc_decay_attention {
   int32_t B, T, H, Hk, dk, dv;
   const void *q, *k, *v;

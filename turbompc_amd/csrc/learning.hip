@@ -94,9 +94,10 @@ int rms_backward_impl(hipStream_t st, int64_t rows, int32_t width, const void* d
 // --------------------------------------------------------- decay attention --
 constexpr int kMaxHeads = 32768;            // a chunk of contiguous output rows, 64 x H x 128 fp32, within 31 bits
 constexpr int64_t kMaxStep = (1 << 23) - 1; // elements between steps: 64 fp32 steps within 31 bits
+constexpr int kMaxSteps = 1 << 30;          // the last run's end, less than T + a run, and t0 + C within 31 bits
 
 bool attn_shape_ok(const tmpc_decay_attention* a) {
-  return a && a->B >= 0 && a->T >= 0 && a->H >= 1 && a->Hk >= 1 && a->H % a->Hk == 0 && a->dk >= 1 && a->dk <= 128 &&
+  return a && a->B >= 0 && a->T >= 0 && a->T <= kMaxSteps && a->H >= 1 && a->Hk >= 1 && a->H % a->Hk == 0 && a->dk >= 1 && a->dk <= 128 &&
          a->dv >= 1 && a->dv <= 128 && (int64_t)a->B * a->H <= 1 << 23 && a->H <= kMaxHeads;  // threads of a launch within 32 bits
 }
 // a chunk's steps lie within the 31 bits of a descriptor

@@ -23,6 +23,7 @@ _SUFFIX = {torch.float32: "f32", torch.bfloat16: "bf16"}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 MAX_HEAD_WIDTH = 128
 MAX_HEADS = 32768
+MAX_STEPS = 1 << 30
 MAX_NORM_WIDTH = 8192
 MAX_FF_WIDTH = 1 << 20
 
@@ -190,6 +191,8 @@ def _check_attention(q, k, v, log_decay, scale, step):
         raise ValueError(f"the {H} heads of q are not a multiple of the {Hk} heads of k and v")
     if H > MAX_HEADS:
         raise ValueError(f"q has {H} heads, expected at most {MAX_HEADS}")
+    if not step and qs[1] > MAX_STEPS:
+        raise ValueError(f"q has {qs[1]} steps, expected at most {MAX_STEPS}")
     for name, d in (("q and k", dk), ("v", vs[-1])):
         if not 1 <= d <= MAX_HEAD_WIDTH:
             raise ValueError(f"{name} have heads of {d} elements, expected 1 to {MAX_HEAD_WIDTH}")
@@ -242,7 +245,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     """Linear attention with a decay for each head over whole histories.
 
     q (B, T, H, dk), k (B, T, Hk, dk), v (B, T, Hk, dv), H a multiple of Hk,
-    widths 1 to 128; log_decay (H,) float32, <= 0, a constant.  Per problem and head
+    T at most 2^30, widths 1 to 128; log_decay (H,) float32, <= 0, a constant.  Per problem and head
       S_t = exp(log_decay) S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,
     from state (B, H, dk, dv) float32 (zero where None), for t < lengths[b]
     (int32, clamped to 0..T; None: T); later steps give zero rows, and what
