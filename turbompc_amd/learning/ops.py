@@ -16,6 +16,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 
@@ -285,6 +286,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
     a = _attention_args(q, k, v, log_decay, None, None, scale)
     _call(f"tmpc_decay_attention_step_{sfx}", q.device, a, _ptr(active), _ptr(state), _ptr(o))
+    increment_version(state)  # a backward pass that saved it has to see the change
     return o
 
 
