@@ -2,6 +2,7 @@
 views, torch's autograd rules."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from turbompc_amd import learning
 
@@ -54,3 +55,25 @@ def test_a_step_in_inference_mode():
         for s in (state, inside):
             assert torch.equal(learning.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s), o)
             assert torch.equal(s, want)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is never dropped: there is no forward-mode rule, so a dual input is an error."""
+    q, k, v, g, state = attention_inputs(2, 3, 2, 1, 8, 8, torch.float32)
+    x, w, wd, n = torch.randn(4, 8, device=DEV), torch.randn(6, 8, device=DEV), torch.randn(8, 6, device=DEV), torch.ones(8, device=DEV)
+    calls = {
+        "attention": (learning.decay_attention, [q, k, v, g, state], (0, 1, 2, 3, 4)),
+        "step": (learning.decay_attention_step, [q[:, 0], k[:, 0], v[:, 0], g, state], (0, 1, 2, 3, 4)),
+        "feed_forward": (learning.gated_feed_forward, [x, w, w, wd], (0, 1, 2, 3)),
+        "norm": (learning.rms_norm_residual, [x, x, n], (0, 1, 2)),
+    }
+    for name, (fn, args, places) in calls.items():
+        for i in places:
+            for mode in (torch.enable_grad, torch.no_grad):
+                with forward_ad.dual_level(), mode():
+                    dual = list(args)
+                    dual[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises(NotImplementedError):
+                        fn(*dual)
+        with forward_ad.dual_level():
+            fn(*args)  # no tangent among them: as anywhere else

@@ -6,7 +6,8 @@ in the same type); states and statistics are float32.  Every call is enqueued on
 last axis) are read in place when contiguous, whatever the other strides, and
 copied otherwise.  Shapes, types and devices that a kernel does not take raise
 ValueError or TypeError before anything is enqueued; a failure in the library
-raises TmpcError.  There is no CPU path.
+raises TmpcError.  There is no CPU path.  Forward-mode derivatives are refused
+(NotImplementedError).
 """
 from __future__ import annotations
 
@@ -15,6 +16,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -77,6 +79,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
+    # a tangent is no matter of requires_grad or grad mode; outside a level there are none
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the history model's operators have no forward-mode derivatives")
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
@@ -261,7 +268,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     state = state.contiguous() if state is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
     args = (_steps(q), _steps(k), _steps(v), log_decay.contiguous(), state, lengths, scale, sfx)
-    return _DecayAttention.apply(*args) if _wants_grad(q, k, v, state) else _attention_forward(*args)
+    return _DecayAttention.apply(*args) if _wants_grad(q, k, v, state, log_decay) else _attention_forward(*args)
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -280,7 +287,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if active is not None:
         _check("active", active, q, (B,), torch.bool)
         active = active.contiguous()
-    if _wants_grad(q, k, v, state):
+    if _wants_grad(q, k, v, state, log_decay):
         raise ValueError("decay_attention_step has no gradient; use decay_attention, or torch.no_grad()")
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
