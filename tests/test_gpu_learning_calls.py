@@ -77,3 +77,47 @@ def test_forward_mode_derivatives_are_refused():
                         fn(*dual)
         with forward_ad.dual_level():
             fn(*args)  # no tangent among them: as anywhere else
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_of_a_long_history(dtype):
+    """The stride of an axis of one entry is never used, however wide it is: the last step
+    of one vehicle's log, with its rows 2^21 elements and more apart."""
+    gen = torch.Generator().manual_seed(20)
+    log = torch.randn((1, 9000, 256), generator=gen).to(dtype).to(DEV)
+    wg, wu = (torch.randn((40, 256), generator=gen).to(dtype).to(DEV) / 16 for _ in range(2))
+    wd, n = torch.randn((256, 40), generator=gen).to(dtype).to(DEV) / 8, torch.ones(256, dtype=dtype, device=DEV)
+    ops = {"ff": lambda x: learning.gated_feed_forward(x, wg, wu, wd),
+           "norm": lambda x: learning.rms_norm_residual(x, None, n)[0],
+           "residual": lambda x: learning.rms_norm_residual(x * 2, x, n)[0]}
+    row = log[:, -1]
+    dy = log.flip(1)[:, 17]
+    wide_dy = torch.randn((1, 9000, 256), generator=gen).to(dtype).to(DEV)[:, 3]
+    assert row.stride(0) > 1 << 20 and wide_dy.stride(0) > 1 << 20
+    for name, op in ops.items():
+        for g in (dy, wide_dy):
+            a = row.detach().requires_grad_(True)
+            b = torch.empty(1, 256, dtype=dtype, device=DEV).copy_(row).requires_grad_(True)
+            ya, yb = op(a), op(b)
+            assert torch.equal(ya, yb), name
+            ga, = torch.autograd.grad(ya, a, g)
+            gb, = torch.autograd.grad(yb, b, torch.empty(1, 256, dtype=dtype, device=DEV).copy_(g))
+            assert torch.equal(ga, gb), name
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_step_of_time_major_histories(dtype):
+    B, H, d = 1100, 64, 128
+    x = [torch.randn((1, B, H, d), generator=torch.Generator().manual_seed(s)).to(dtype).to(DEV) for s in range(4)]
+    assert x[0].transpose(0, 1).stride(1) >= 1 << 23
+    g = torch.full((H,), -0.5, device=DEV)
+
+    def run(q, k, v, do):
+        leaf = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o, s = learning.decay_attention(*leaf, g)
+        return (o.detach(), s.detach(), *torch.autograd.grad(o, leaf, do))
+
+    views = run(*(t.transpose(0, 1) for t in x))
+    plain = run(*(torch.empty((B, 1, H, d), dtype=dtype, device=DEV).copy_(t.transpose(0, 1)) for t in x))
+    for a, b in zip(views, plain):
+        assert torch.equal(a, b)

@@ -62,16 +62,30 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+# An axis of one entry may have any stride, which a copy keeps: the calls get one of their own.
 def _steps(t: torch.Tensor) -> torch.Tensor:
     """A history (B, T, H, d) as the kernels read it: contiguous rows, steps less than 2^23
     elements apart."""
-    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(1) < 1 << 23 else t.contiguous()
+    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and _step_strides(t)[1] < 1 << 23 else t.contiguous()
+
+
+def _step_strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides of problem, step and head of a history (B, T, H, d), or of one step of each (B, H, d)."""
+    s = t.stride()
+    if t.dim() == 3:
+        return s[0], 0, s[1]
+    return s[0], s[1] if t.shape[1] > 1 else 0, s[2]
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
     """t as (rows, last axis) with contiguous rows, at most 2^20 elements apart: a view where one exists."""
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and t.stride(0) <= MAX_FF_WIDTH else t.contiguous()
+    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and _pitch(t) <= MAX_FF_WIDTH else t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements between the rows of a matrix."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -118,8 +132,8 @@ def _rms_forward(x, residual, weight, eps, sfx, rstd):
     rm = _matrix(residual) if residual is not None else None
     M, D = xm.shape
     y, s = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
-    _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), xm.stride(0), _ptr(rm),
-          rm.stride(0) if rm is not None else 0, _ptr(weight), eps, _ptr(y), _ptr(s), _ptr(rstd))
+    _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), _pitch(xm), _ptr(rm),
+          _pitch(rm) if rm is not None else 0, _ptr(weight), eps, _ptr(y), _ptr(s), _ptr(rstd))
     return y, s
 
 
@@ -143,8 +157,8 @@ class _RmsNorm(torch.autograd.Function):
         dsm = _matrix(ds) if ds is not None else None
         dx, dw = torch.empty_like(s), torch.empty_like(w)
         nbytes, ws = _workspace("tmpc_rms_norm_backward_workspace_bytes", s.device, s.element_size(), M, D)
-        _call(f"tmpc_rms_norm_backward_{ctx.sfx}", s.device, M, D, _ptr(dym), dym.stride(0), _ptr(dsm),
-              dsm.stride(0) if dsm is not None else 0, _ptr(s), D, _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws),
+        _call(f"tmpc_rms_norm_backward_{ctx.sfx}", s.device, M, D, _ptr(dym), _pitch(dym), _ptr(dsm),
+              _pitch(dsm) if dsm is not None else 0, _ptr(s), D, _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws),
               nbytes)
         return dx, dx if ctx.has_residual else None, dw, None, None
 
@@ -178,10 +192,9 @@ assert _ATTENTION.size == ctypes.sizeof(_lib.DecayAttention)
 def _attention_args(q, k, v, log_decay, lengths, state, scale):
     B, T, H, dk = q.shape if q.dim() == 4 else (q.shape[0], 1) + q.shape[1:]
     p = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
-    st = [t.stride()[:3] if t.dim() == 4 else (t.stride(0), 0, t.stride(1)) for t in (q, k, v)]
     return _lib.DecayAttention.from_buffer_copy(_ATTENTION.pack(
-        B, T, H, k.shape[-2], dk, v.shape[-1], p(q), p(k), p(v), *st[0], *st[1], *st[2], p(log_decay), p(lengths),
-        p(state), scale))
+        B, T, H, k.shape[-2], dk, v.shape[-1], p(q), p(k), p(v), *_step_strides(q), *_step_strides(k),
+        *_step_strides(v), p(log_decay), p(lengths), p(state), scale))
 
 
 def _check_attention(q, k, v, log_decay, scale, step):
@@ -241,7 +254,7 @@ class _DecayAttention(torch.autograd.Function):
         d_state = empty(state) if state is not None and ctx.needs_input_grad[4] else None
         a = _attention_args(q, k, v, log_decay, lengths, state, ctx.scale)
         nbytes, ws = _workspace("tmpc_decay_attention_workspace_bytes", dev, q.element_size(), a, 1)
-        st = (ctypes.c_int64 * 3)(*d_o.stride()[:3])
+        st = (ctypes.c_int64 * 3)(*_step_strides(d_o))
         _call(f"tmpc_decay_attention_backward_{ctx.sfx}", dev, a, _ptr(d_o), st, _ptr(d_out), _ptr(dq), _ptr(dk),
               _ptr(dv), _ptr(d_state), _ptr(ws), nbytes)
         return dq, dk, dv, None, d_state, None, None, None
@@ -305,7 +318,7 @@ assert _GATED_FF.size == ctypes.sizeof(_lib.GatedFF)
 def _ff_args(xm, w_gate, w_up, w_down, act):
     F, D = w_gate.shape
     return _lib.GatedFF.from_buffer_copy(_GATED_FF.pack(xm.shape[0], D, F, w_down.shape[0], act, xm.data_ptr(),
-                                                        xm.stride(0), w_gate.data_ptr(), w_up.data_ptr(),
+                                                        _pitch(xm), w_gate.data_ptr(), w_up.data_ptr(),
                                                         w_down.data_ptr()))
 
 
@@ -337,7 +350,7 @@ class _GatedFF(torch.autograd.Function):
         dg, du, dd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
         nbytes, ws = _workspace("tmpc_gated_ff_workspace_bytes", xm.device, xm.element_size(), a, 1)
         _call(f"tmpc_gated_ff_backward_{ctx.sfx}", xm.device, a, _ptr(gate), _ptr(up), _ptr(dym),
-              dym.stride(0), _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), _ptr(ws), nbytes)
+              _pitch(dym), _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), _ptr(ws), nbytes)
         return dx, dg, du, dd, None, None
 
 
