@@ -121,3 +121,32 @@ def test_one_step_of_time_major_histories(dtype):
     plain = run(*(torch.empty((B, 1, H, d), dtype=dtype, device=DEV).copy_(t.transpose(0, 1)) for t in x))
     for a, b in zip(views, plain):
         assert torch.equal(a, b)
+
+
+def test_sizes_past_the_limits_are_value_errors():
+    """Limits of the library are refused with the shape's name before anything is enqueued."""
+    one = torch.zeros((1, 1, 1), device=DEV)
+    heads = torch.zeros(32, device=DEV)
+    B = (1 << 18) + 1  # 2^23 + 32 problems' heads
+    q, state = one.expand(B, 32, 1), torch.zeros((B, 32, 1, 1), device=DEV)
+    with pytest.raises(ValueError):
+        learning.decay_attention_step(q, q, q, heads, state)
+    with pytest.raises(ValueError):
+        learning.decay_attention(*(t[:, None] for t in (q, q, q)), heads)
+    w = torch.zeros((1, 1), device=DEV)
+    with pytest.raises(ValueError):
+        learning.gated_feed_forward(one[0].expand((1 << 30) + 1, 1), w, w, w)
+
+
+def test_arguments_that_are_no_tensors_are_type_errors():
+    x, w, wd = torch.zeros((2, 8), device=DEV), torch.zeros((4, 8), device=DEV), torch.zeros((8, 4), device=DEV)
+    for args in ((None, w, w, wd), (x, None, w, wd), (x, w, None, wd), (x, w, w, None)):
+        with pytest.raises(TypeError):
+            learning.gated_feed_forward(*args)
+    for args in ((None, None, wd[:, 0]), (x, 1.0, wd[:, 0]), (x, None, None)):
+        with pytest.raises(TypeError):
+            learning.rms_norm_residual(*args)
+    q, g = torch.zeros((1, 2, 2, 8), device=DEV), torch.zeros(2, device=DEV)
+    for args in ((None, q, q, g), (q, None, q, g), (q, q, None, g), (q, q, q, None), (q, q, q, g, 0.0)):
+        with pytest.raises(TypeError):
+            learning.decay_attention(*args)

@@ -27,8 +27,10 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 MAX_HEAD_WIDTH = 128
 MAX_HEADS = 32768
 MAX_STEPS = 1 << 30
+MAX_BATCH_HEADS = 1 << 23
 MAX_NORM_WIDTH = 8192
 MAX_FF_WIDTH = 1 << 20
+MAX_FF_ROWS = 1 << 30
 
 
 def _check(name: str, t: torch.Tensor, like: torch.Tensor, shape=None, dtype=None):
@@ -212,6 +214,8 @@ def _check_attention(q, k, v, log_decay, scale, step):
         raise ValueError(f"the {H} heads of q are not a multiple of the {Hk} heads of k and v")
     if H > MAX_HEADS:
         raise ValueError(f"q has {H} heads, expected at most {MAX_HEADS}")
+    if qs[0] * H > MAX_BATCH_HEADS:
+        raise ValueError(f"q has {qs[0]} problems of {H} heads, expected at most {MAX_BATCH_HEADS} together")
     if not step and qs[1] > MAX_STEPS:
         raise ValueError(f"q has {qs[1]} steps, expected at most {MAX_STEPS}")
     for name, d in (("q and k", dk), ("v", vs[-1])):
@@ -366,12 +370,14 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if w_gate.dim() != 2 or w_gate.shape[1] != D or D < 1 or w_gate.shape[0] < 1:
         raise ValueError(f"w_gate has shape {tuple(w_gate.shape)}, expected ('F', {D}), neither empty")
     F = w_gate.shape[0]
-    if max(D, F, w_down.shape[0] if w_down.dim() else 0) > MAX_FF_WIDTH:
-        raise ValueError(f"the widths of x, w_gate and w_down must be at most {MAX_FF_WIDTH}")
     _check("w_up", w_up, x, (F, D))
     _check("w_down", w_down, x)
     if w_down.dim() != 2 or w_down.shape[1] != F or w_down.shape[0] < 1:
         raise ValueError(f"w_down has shape {tuple(w_down.shape)}, expected ('Dout', {F}), not empty")
+    if max(D, F, w_down.shape[0]) > MAX_FF_WIDTH:
+        raise ValueError(f"the widths of x, w_gate and w_down must be at most {MAX_FF_WIDTH}")
+    if x.numel() // D > MAX_FF_ROWS:
+        raise ValueError(f"x has {x.numel() // D} rows, expected at most {MAX_FF_ROWS}")
     act = _ACTIVATIONS[activation]
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     if _wants_grad(x, w_gate, w_up, w_down):
