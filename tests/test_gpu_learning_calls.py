@@ -150,3 +150,24 @@ def test_arguments_that_are_no_tensors_are_type_errors():
     for args in ((None, q, q, g), (q, None, q, g), (q, q, None, g), (q, q, q, None), (q, q, q, g, 0.0)):
         with pytest.raises(TypeError):
             learning.decay_attention(*args)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_model_cast_after_it_was_made(dtype):
+    """`to`, `bfloat16` and `float` cast the parameters; the decays stay float32, with their values."""
+    model = learning.HistoryWeights(5, {"a": 2}, width=32, layers=2, heads=2, hidden=48,
+                           dtype=torch.float32 if dtype == torch.bfloat16 else torch.bfloat16)
+    decays = [b.log_decay.clone() for b in model.blocks]
+    model = model.bfloat16() if dtype == torch.bfloat16 else model.to(dtype)
+    assert all(p.dtype == dtype for p in model.parameters())
+    assert all(b.log_decay.dtype == torch.float32 and torch.equal(b.log_decay, d) for b, d in zip(model.blocks, decays))
+    history = torch.randn(3, 7, 5, device="cuda")
+    w = model(history)["a"]
+    w.sum().backward()
+    assert bool(torch.isfinite(w).all()) and all(p.grad is not None for p in model.parameters())
+    state = model.initial_state(3)
+    model.step(history[:, 0], state)
+    saved = model.state_dict()
+    other = learning.HistoryWeights(5, {"a": 2}, width=32, layers=2, heads=2, hidden=48, dtype=dtype)
+    other.load_state_dict(saved)
+    assert torch.equal(other(history)["a"], model(history)["a"])

@@ -54,3 +54,13 @@ def test_lengths_outside_the_history_are_clamped(model):
 def test_histories_without_a_row_are_refused(model, lengths):
     with pytest.raises(ValueError):
         model(torch.zeros(3, 0, 5), lengths)
+
+
+def test_a_cast_leaves_the_decays():
+    m = HistoryWeights(5, {"a": 2}, width=16, layers=2, heads=2, device="cpu")
+    decays = [b.log_decay.clone() for b in m.blocks]
+    for cast in (lambda: m.bfloat16(), lambda: m.to(torch.float64), lambda: m.to("cpu", torch.float32)):
+        assert cast() is m
+        for b, d in zip(m.blocks, decays):
+            assert b.log_decay.dtype == torch.float32 and torch.equal(b.log_decay, d)
+            assert "log_decay" in dict(b.named_buffers())

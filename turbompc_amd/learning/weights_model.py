@@ -39,6 +39,14 @@ class _Block(nn.Module):
         # a head's memory halves after 1 to 128 steps
         self.register_buffer("log_decay", -0.6931472 * torch.exp2(-torch.linspace(0.0, 7.0, heads, device=kw.get("device"))))
 
+    def _apply(self, fn, *args, **kwargs):
+        # a cast of the model is one of its parameters: the operator takes float32 decays
+        decay = self.log_decay
+        super()._apply(fn, *args, **kwargs)
+        if self.log_decay.dtype != decay.dtype:
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
+
     def qkv(self, y):
         x = nn.functional.linear(y, self.w_qkv).unflatten(-1, (-1, self.d))
         return x.split([self.heads, self.kv_heads, self.kv_heads], dim=-2)
