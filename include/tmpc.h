@@ -618,7 +618,9 @@ int tmpc_rms_norm_backward_bf16(hipStream_t stream, int64_t rows, int32_t width,
 /* Linear attention with a decay for each head: for problem b and head h, with
  * g = log_decay[h] <= 0 and t < lengths[b] (clamped to 0..T; NULL: T)
  *   S_t = e^g S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,  S_{-1} = state_in (or zero);
- * steps past the length give o = 0 and leave the state.  H is a multiple of
+ * steps past the length give o = 0 and leave the state.  An infinite or NaN value at
+ * a live step reaches what it has a part in: no earlier step's output, no other
+ * head or problem.  H is a multiple of
  * Hk; head h reads key/value head h / (H / Hk).  1 <= dk, dv <= 128.  q (B, T,
  * H, dk), k (B, T, Hk, dk), v (B, T, Hk, dv) have contiguous rows and the given
  * strides (elements) of problem, step and head, that of a step at most 2^23 - 1;

@@ -5,7 +5,8 @@
 //   O = (Q K^T o Gamma) V + diag(e^{g (i+1)}) Q S_in,  Gamma_ij = e^{g (i-j)} for i >= j, else 0
 //   S_out = e^{g L} S_in + K^T diag(e^{g (L-1-j)}) V,  L the chunk's live steps;
 // every exponent's factor of g is >= 0, so a strong decay underflows to zero and
-// nothing overflows.
+// nothing overflows.  Gamma's zeros hold for finite values alone: runs with others are made
+// again step by step (attn_by_step).
 //
 // Backward.  With D_t = dL/dS_t = e^g D_{t+1} + scale q_t^T do_t,
 //   dq_t = scale do_t S_t^T,  dk_t = v_t D_t^T,  dv_t = k_t D_t :
@@ -153,6 +154,10 @@ __device__ inline float uniform(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
+// a b, and 0 where either is zero, an infinity's factor or not: what overflows above the
+// diagonal has no part in a score
+extern "C" __device__ float mul_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
 // Powers of a head's decay that every whole chunk needs, of exponents >= 0 alone:
 // lag 16 d + lo - 4 hi - r of a score as tile[d] * near[r] (d >= 1; near has 16 more and tile
 // 16 fewer), diag[r] on the diagonal tile (0 above it), row i = 16 it + lo of the
@@ -205,7 +210,7 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
       for (int k = 0; k < KA; ++k) a[k] = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
       f32x4 t = score(jt, a);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[r] *= it == jt ? pw.diag[r] : far * pw.near[r];
+      for (int r = 0; r < 4; ++r) t[r] = mul_zero(t[r], it == jt ? pw.diag[r] : far * pw.near[r]);
       *reinterpret_cast<quad_t<E>*>(tp + (16 * it + lo) * LDP + 16 * jt + 4 * hi) = to_quad<E>(t);
     }
     __syncthreads();
@@ -256,7 +261,8 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
           } else {
             f32x4 t = score(jt, a);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[r] *= jt == it ? pw.diag[r] : pw.tile[it > jt ? it - jt - 1 : 0] * pw.near[r];
+            for (int r = 0; r < 4; ++r)
+              t[r] = mul_zero(t[r], jt == it ? pw.diag[r] : pw.tile[it > jt ? it - jt - 1 : 0] * pw.near[r]);
             p[e] = to_quad<E>(t);
           }
         }
@@ -359,6 +365,61 @@ __device__ inline void zero_rows(void* o, bool f32, int elem, int64_t base, int6
   }
 }
 
+// A wave's columns of a run whose keys or values are not all finite, by the definition, a step
+// at a time: in a chunk they meet the earlier steps' outputs with a factor of zero, which
+// makes those NaN.  Rare, so simple and in few registers.
+template <typename E, int KA, int NV>
+__device__ __attribute__((always_inline)) inline void attn_by_step(const AttnArgs<E>& p, int block, int tid) {
+  const int lo = tid & 15, hi = (tid & 63) >> 4, col0 = (tid >> 6) * NV * 16;
+  const int bh = block / p.segs, seg = block - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const float g = p.log_decay[h];
+  const int L = attn_length(p, b), begin = seg * p.seg_len, end = min(L, begin + p.seg_len);
+  const int64_t first = p.rev ? L - 1 : 0, dir = p.rev ? -1 : 1;
+  const E* pa = p.a + b * p.as[0] + (h / p.ga) * p.as[2] + first * p.as[1];
+  const E* pb = p.b + b * p.bs[0] + (h / p.gb) * p.bs[2] + first * p.bs[1];
+  const E* pc = p.c + b * p.cs[0] + (h / p.gc) * p.cs[2] + first * p.cs[1];
+  const int64_t orow = (int64_t)p.H * p.dc, o = ((int64_t)b * p.T * p.H + h) * p.dc + first * orow;
+  const int64_t size = (int64_t)p.da * p.dc, sbase = bh * size;
+  f32x4 s[KA][NV];
+  if (p.segs > 1) load_state(s, p.seg_state + block * size, false, p.da, p.dc, col0, lo, hi);
+  else load_state(s, p.s_in ? p.s_in + sbase : nullptr, p.s_in_t, p.da, p.dc, col0, lo, hi);
+  const float gamma = decay_pow(g, 1), before = p.rev ? 1.0f : gamma, after = p.rev ? gamma : 1.0f;
+  for (int t = begin; t < end; ++t) {
+    const E *at = pa + dir * t * p.as[1], *bt = pb + dir * t * p.bs[1], *ct = pc + dir * t * p.cs[1];
+    float cv[NV], sum[NV];
+#pragma unroll
+    for (int x = 0; x < NV; ++x) {
+      const int col = col0 + 16 * x + lo;
+      cv[x] = col < p.dc ? p.su * (float)ct[col] : 0.0f, sum[x] = 0.0f;
+    }
+#pragma unroll
+    for (int m = 0; m < KA; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * m + 4 * hi + r;
+        if (row >= p.da) continue;
+        const float av = (float)at[row], bv = (float)bt[row];
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+          s[m][x][r] = s[m][x][r] * before + bv * cv[x];
+          sum[x] += av * s[m][x][r];
+          s[m][x][r] *= after;
+        }
+      }
+#pragma unroll
+    for (int x = 0; x < NV; ++x) {
+      const int col = col0 + 16 * x + lo;
+      sum[x] += __shfl_xor(sum[x], 16, 64);
+      sum[x] += __shfl_xor(sum[x], 32, 64);
+      if (hi == 0 && col < p.dc) {
+        if (p.o_f32) reinterpret_cast<float*>(p.o)[o + dir * t * orow + col] = p.si * sum[x];
+        else reinterpret_cast<E*>(p.o)[o + dir * t * orow + col] = (E)(p.si * sum[x]);
+      }
+    }
+  }
+  if (p.s_out && seg == (L - 1) / p.seg_len) store_state(s, p.s_out + sbase, p.da, p.dc, col0, lo, hi);
+}
+
 // FULL: outputs and the carried state; else the run's own sum alone, into seg_state.
 template <typename E, int DA, int DC, bool FULL, bool VEC>
 __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk_kernel(AttnArgs<E> p) {
@@ -454,6 +515,25 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
               S::THREADS);
     // the run that holds the last live step has the final state
     if (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0)) store_state(s, p.s_out + sbase, p.da, p.dc, col0, lo, hi);
+    // An infinite or NaN key or value leaves the state so, to the end: in all columns, or in its own.
+    f32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < KA; ++m)
+#pragma unroll
+      for (int x = 0; x < NV; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][x][r], 0.0f, zero[r]);
+    if (begin < end && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
+      __threadfence_block();  // the rows written above are written again
+      // The arguments are read again and the indexes made again, behind an assignment that the
+      // compiler does not see through: kept from the ones above they cost registers in every
+      // chunk (64 x 128 heads, 101 steps: 5%).  (In a function that is called the arguments' address
+      // is null: it is taken in the kernel.)
+      auto* args = __builtin_amdgcn_kernarg_segment_ptr();
+      int block = blockIdx.x, thread = threadIdx.x;
+      asm volatile("" : "+s"(args), "+s"(block), "+v"(thread));
+      attn_by_step<E, KA, NV>(*(const AttnArgs<E>*)args, block, thread);
+    }
   } else {
     store_state(s, seg_state, p.da, p.dc, col0, lo, hi);
   }

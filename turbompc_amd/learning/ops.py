@@ -274,7 +274,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
       S_t = exp(log_decay) S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,
     from state (B, H, dk, dv) float32 (zero where None), for t < lengths[b]
     (int32, clamped to 0..T; None: T); later steps give zero rows, and what
-    their inputs hold is not read.  scale is dk^-1/2 where None.  Returns o
+    their inputs hold is not read.  An infinite or NaN value at a live step spoils
+    what it has a part in: no earlier step, other head or problem.  scale is dk^-1/2 where None.  Returns o
     (B, T, H, dv) and the state after each history's last step (float32)."""
     sfx, scale = _check_attention(q, k, v, log_decay, scale, False)
     B, _, H, dk = q.shape
