@@ -79,6 +79,16 @@ struct AttnShape {
   // share the scores out and exchange them in LDS
   static constexpr bool SHARE = DA == 128 && DC == 128;
   static constexpr int LDP = C + AttnTile<E>::PAD;
+  // Registers that a lane holds through a whole chunk: S and the next chunk's rows on their way (a
+  // row of `d` elements takes d / P threads).  Where they are many, no operand is kept from one row
+  // tile to the next, or they spill: 64 x 512 x 8 heads, bf16, 128 x 32 (104 held) 75 us against
+  // 120, 128 x 128 (112) 86 both, 128 x 64 (72) 66 against 63, 64 x 128 and 64 x 64 (64, 40) no difference.
+  static constexpr int rows_held(int d) {
+    constexpr int P = Elem<E>::PIECE;
+    return 4 * C / (THREADS / (d / P) < C ? THREADS / (d / P) : C);
+  }
+  static constexpr int HELD = DA / 16 * NV * 4 + 2 * rows_held(DA) + rows_held(DC);
+  static constexpr bool FENCE = HELD > 96;
   // elements of a chunk's rows in LDS: b and c, and a (and the scores) with outputs
   static constexpr int TILE_STATE = C * LDA + C * LDC, TILE = TILE_STATE + C * LDA + (SHARE ? C * LDP : 0);
   // workgroups of a CU, by their registers; the tiles twice (one barrier a chunk instead of
@@ -230,10 +240,11 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
       for (int x = 0; x < NV; ++x) sq[k][x] = to_quad<E>(s[k][x]);
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
-      // past the last live step.  (128 x 128 heads run long histories of whole chunks: there the
-      // branch cost 5% and saves nothing.)
+      // Past the last live step.  With the scores shared the loop is the shorter part, and the
+      // branch keeps its tiles apart: 64 x 512 x 8 heads 99.8 us against 85.5; ragged batches of
+      // 512 x 4 heads of up to 512, 200 and 70 steps 302, 148 and 82 against 281, 144 and 86.
       if (!S::SHARE && 16 * it >= n) break;
-      if constexpr ((KA == 4 && NV == 2) || S::SHARE) asm volatile("" ::: "memory");  // no operand is kept from tile to tile: too many
+      if constexpr (S::FENCE) asm volatile("" ::: "memory");
       quad_t<E> a[KA];
 #pragma unroll
       for (int k = 0; k < KA; ++k) a[k] = lds_quad(ta, LDA, 16 * it, 16 * k, lane);
