@@ -106,6 +106,12 @@ bool step_ok(const int64_t* stride) { return stride[1] >= 0 && stride[1] <= kMax
 // One long history of few heads does not fill the chip, its chunks following one another:
 // it is cut into runs of whole chunks.  A first pass sums each run on its own (keys and
 // values alone), a scan carries the states through, and the outputs start from those.
+// As many runs as are resident together, two workgroups a CU (one more round of them costs more:
+// 96 heads of 2048 steps, 64 wide, bf16, 48 us in 5 runs a head, 58 in 6); two runs a head do not pay
+// for reading keys and values twice (192 heads, 1024 steps: 53 us against 44 whole; 160 heads in
+// three: 45 against 43, and 71 against 91 with 2048 steps).  A run has four chunks at least (16
+// heads, 1024 steps: 25 us against 35 with eight), a history that is cut 16 (512 steps whole 22
+// us, in two runs 25).
 struct AttnSplit {
   int segs, len;
 };
@@ -113,8 +119,8 @@ template <typename E>
 AttnSplit attn_split(int64_t bh, int T) {
   constexpr int C = AttnTile<E>::C;
   const int64_t chunks = std::max<int64_t>(1, ceil_div(T, C));
-  // a run of fewer than 8 chunks costs more in its state's traffic than it gains
-  const int64_t want = bh >= kCUs ? 1 : std::min(ceil_div(2 * kCUs, bh), std::max<int64_t>(1, chunks / 8));
+  const int64_t runs = 2 * kCUs / std::max<int64_t>(bh, 1);
+  const int64_t want = runs < 3 || chunks < 16 ? 1 : std::min(runs, chunks / 4);
   const int64_t len = ceil_div(chunks, want);
   return {(int)ceil_div(chunks, len), (int)(len * C)};
 }
