@@ -386,14 +386,23 @@ size_t store_part_bytes(int64_t M, int64_t N, int64_t K) {
   return most > 1 ? align_up((size_t)most * M * N * sizeof(float)) : 0;
 }
 
-// The form of a product: the largest tile that still gives most of the chip work.
+// The form of a product, where both were measured (us of one product; bf16 unless it says fp32):
+//   up to 64 rows, as many as gemm_rows_kernel's registers hold: 64 rows of 512 x 1408 14.2
+//     against 15.2 in tiles, 16 rows 9.0 against 15.1; 64 of 2048 x 5504 51 and 55, fp32 108 and 100;
+//   wide tiles once the 128s, four for each, take more than the one round of two workgroups a CU
+//     that 128 wide tiles make: K = 512, 128 tiles 4.5 slower, 144 to 160 5.3 to 5.9 faster; K =
+//     1408, 128 tiles 3.8 slower, 144 22 faster;
+//   tiles of 128 once they are more than the CUs: K = 512, 256 tiles 2.6 slower than in 64s, 264 2.3
+//     faster; K = 1408, 188 11 slower; fp32, 192 10 slower, 440 5.7 faster;
+//   tiles of 64 from three for four CUs on: under it 32s are up to 1.6 faster (fp32 3.4), from 700
+//     on up to 5 slower, in between the two are within 1.4 (fp32 4.3).
 template <typename E, bool AT, bool BT, int EPI>
 GemmPlan gemm_plan(const GemmArgs<E>& p, bool own_a, bool own_b) {
   constexpr int D = EPI == EPI_GATE || EPI == EPI_GATE_SAVE ? 2 : 1;
   if (!AT && !BT && p.nseg == 1 && p.M <= 64) return {FORM_ROWS, 1};
-  if (wide_ok(p, AT, BT, own_a, own_b) && tiles_of(p.M, p.N, 256, 256 / D) >= 96) return {FORM_WIDE, 1};
-  if (tiles_of(p.M, p.N, 128, 128 / D) >= 192) return {FORM_128, 1};
-  const GemmForm form = tiles_of(p.M, p.N, 64, 64 / D) >= 192 ? FORM_64 : FORM_32;
+  if (wide_ok(p, AT, BT, own_a, own_b) && tiles_of(p.M, p.N, 256, 256 / D) > kCUs / 2) return {FORM_WIDE, 1};
+  if (tiles_of(p.M, p.N, 128, 128 / D) > kCUs) return {FORM_128, 1};
+  const GemmForm form = tiles_of(p.M, p.N, 64, 64 / D) >= 3 * kCUs / 4 ? FORM_64 : FORM_32;
   return {form, EPI == EPI_STORE ? store_splits<E>(p.M, p.N, p.K, form) : 1};
 }
 
