@@ -28,7 +28,9 @@ void lds_optin(K kernel, size_t bytes) {
 
 // ---------------------------------------------------------------- rms norm --
 constexpr int kMaxWidth = 8192;
-constexpr int kRmsBlocks = 1024;  // of the backward pass: rows meet in its blocks' partial sums
+// Blocks of the backward pass, whose rows meet in the blocks' partial sums.  bf16, forward and backward,
+// with 512, 1024 and 2048: 206848 rows of 512 349, 330 and 373 us; 4096 of 8192 130, 148 and 187.
+constexpr int kRmsBlocks = 1024;
 
 // f(threads per row, pieces per thread) of the smallest form that holds `width`
 template <typename E, typename F>
@@ -424,13 +426,21 @@ void launch_store(hipStream_t st, GemmArgs<E> p, GemmPlan plan, float* part) {
 // The weight gradients' rows are few and their contracted index is every row of the batch:
 // it is split until the tiles fill the chip (of the `pair` products together), with at
 // least 8 K steps a split.  The same for every alignment, since it sizes the workspace.
+// A training step's us, bf16: with 4, 8 and 16 steps a split 160, 156 and 170 (8000 rows of 512 x
+// 512), 65, 84 and 83 (1000 of 200 x 520), 125, 112 and 114 (20000 of 64 x 256); with one, two and
+// four tiles a CU (of 128 and 64) 361, 273 and 254 (20000 of 200 x 520), 152, 122 and 119 (3000 of 264
+// x 1040), fp32 180, 188 and 194 (20000 of 64 x 256).
 template <typename E>
 int grad_splits(int64_t rows, int64_t cols, int64_t K, int pair, int tile) {
   const int64_t tiles = tiles_of(rows, cols, tile, tile) * (1 + pair);
   return (int)std::max<int64_t>(1, std::min((tile == 256 ? 1 : 2) * kCUs / tiles, K / (8 * kGemmBK<E>)));
 }
 // the tile of a weight gradient: 256 where it wastes little of its edges, 128 where those are
-// many (fp32, 520 x 200 over 2091 rows: 42 us in 128s, 25 splits of 20 tiles, 20 us in 64s)
+// many (fp32, 520 x 200 over 2091 rows: 42 us in 128s, 25 splits of 20 tiles, 20 us in 64s).
+// Without the 256s a bf16 training step of 20705 rows of 512 x 1408 takes 730 us, not 542 (500 rows 77,
+// not 95); with up to twice the work in them, not 3/2, 20000 rows of 200 x 520 223, not 273, and 2091
+// 94, not 83.  128s from half as many and twice as many tiles on: within 2% but for fp32, 500 rows
+// of 512 x 1408 (164 us, 190 and 143) and 8000 of 512 x 512 (432, 415 and 432).
 template <typename E>
 int grad_tile(int64_t rows, int64_t cols, int pair) {
   if (sizeof(E) == 2 && rows >= 192 && cols >= 192 && tiles_of(rows, cols, 256, 256) * 256 * 256 <= rows * cols * 3 / 2)
