@@ -171,3 +171,24 @@ def test_model_cast_after_it_was_made(dtype):
     other = learning.HistoryWeights(5, {"a": 2}, width=32, layers=2, heads=2, hidden=48, dtype=dtype)
     other.load_state_dict(saved)
     assert torch.equal(other(history)["a"], model(history)["a"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_saved_tensors_may_come_back_with_other_strides(dtype):
+    """Saved on the host between the passes, the views of a wider tensor return contiguous."""
+    q, k, v, g, state = attention_inputs(2, 9, 2, 1, 16, 24, dtype)
+    wide = torch.randn((30, 50), generator=torch.Generator().manual_seed(24)).to(dtype).to(DEV)
+    w, wd = wide[:24, :16].contiguous() / 4, wide[:16, :24].contiguous() / 5
+
+    def grads():
+        x = wide[:, 3:19].detach().requires_grad_(True)
+        p = torch.cat([q, k], 2).requires_grad_(True)
+        y, s = learning.rms_norm_residual(learning.gated_feed_forward(x, w, w, wd), x, wd[:, 0])
+        o, e = learning.decay_attention(p[:, :, :2], p[:, :, 2:], v, g, state)
+        return torch.autograd.grad(y.sum() + s.sum() + o.sum() + e.sum(), [x, p])
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

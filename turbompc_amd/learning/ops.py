@@ -79,15 +79,15 @@ def _step_strides(t: torch.Tensor) -> Tuple[int, int, int]:
     return s[0], s[1] if t.shape[1] > 1 else 0, s[2]
 
 
-def _matrix(t: torch.Tensor) -> torch.Tensor:
-    """t as (rows, last axis) with contiguous rows, at most 2^20 elements apart: a view where one exists."""
+def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """t as (rows, last axis) with contiguous rows, at most 2^20 elements apart (a view where one
+    exists), and the elements between its rows."""
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t if (t.stride(-1) == 1 or t.shape[-1] <= 1) and _pitch(t) <= MAX_FF_WIDTH else t.contiguous()
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Elements between the rows of a matrix."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, width = t.shape
+    pitch = t.stride(0) if rows > 1 else width
+    if (width <= 1 or t.stride(1) == 1) and pitch <= MAX_FF_WIDTH:
+        return t, pitch
+    return t.contiguous(), width
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -130,12 +130,12 @@ def _workspace(query: str, device: torch.device, *args):
 # ------------------------------------------------------------------ norm --
 def _rms_forward(x, residual, weight, eps, sfx, rstd):
     """(y, s); rstd: a (rows,) tensor to fill, or None."""
-    xm = _matrix(x)
-    rm = _matrix(residual) if residual is not None else None
+    xm, ldx = _matrix(x)
+    rm, ldr = _matrix(residual) if residual is not None else (None, 0)
     M, D = xm.shape
     y, s = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
-    _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), _pitch(xm), _ptr(rm),
-          _pitch(rm) if rm is not None else 0, _ptr(weight), eps, _ptr(y), _ptr(s), _ptr(rstd))
+    _call(f"tmpc_rms_norm_forward_{sfx}", x.device, M, D, _ptr(xm), ldx, _ptr(rm), ldr,
+          _ptr(weight), eps, _ptr(y), _ptr(s), _ptr(rstd))
     return y, s
 
 
@@ -155,13 +155,12 @@ class _RmsNorm(torch.autograd.Function):
         s, w, rstd = ctx.saved_tensors
         D = s.shape[-1]
         M = s.numel() // D
-        dym = _matrix(dy) if dy is not None else torch.zeros((M, D), dtype=s.dtype, device=s.device)
-        dsm = _matrix(ds) if ds is not None else None
+        dym, lddy = _matrix(dy) if dy is not None else (torch.zeros((M, D), dtype=s.dtype, device=s.device), D)
+        dsm, ldds = _matrix(ds) if ds is not None else (None, 0)
         dx, dw = torch.empty_like(s), torch.empty_like(w)
         nbytes, ws = _workspace("tmpc_rms_norm_backward_workspace_bytes", s.device, s.element_size(), M, D)
-        _call(f"tmpc_rms_norm_backward_{ctx.sfx}", s.device, M, D, _ptr(dym), _pitch(dym), _ptr(dsm),
-              _pitch(dsm) if dsm is not None else 0, _ptr(s), D, _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws),
-              nbytes)
+        _call(f"tmpc_rms_norm_backward_{ctx.sfx}", s.device, M, D, _ptr(dym), lddy, _ptr(dsm), ldds,
+              _ptr(s), D, _ptr(w), _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(ws), nbytes)
         return dx, dx if ctx.has_residual else None, dw, None, None
 
 
@@ -320,16 +319,16 @@ _GATED_FF = struct.Struct("@q4iPq3P")  # tmpc_gated_ff, packed
 assert _GATED_FF.size == ctypes.sizeof(_lib.GatedFF)
 
 
-def _ff_args(xm, w_gate, w_up, w_down, act):
+def _ff_args(xm, ldx, w_gate, w_up, w_down, act):
     F, D = w_gate.shape
     return _lib.GatedFF.from_buffer_copy(_GATED_FF.pack(xm.shape[0], D, F, w_down.shape[0], act, xm.data_ptr(),
-                                                        _pitch(xm), w_gate.data_ptr(), w_up.data_ptr(),
+                                                        ldx, w_gate.data_ptr(), w_up.data_ptr(),
                                                         w_down.data_ptr()))
 
 
-def _ff_forward(x, xm, w_gate, w_up, w_down, act, sfx, gate, up):
+def _ff_forward(x, xm, ldx, w_gate, w_up, w_down, act, sfx, gate, up):
     """y; gate, up: fp32 tensors to fill, or None."""
-    a = _ff_args(xm, w_gate, w_up, w_down, act)
+    a = _ff_args(xm, ldx, w_gate, w_up, w_down, act)
     y = torch.empty(x.shape[:-1] + (w_down.shape[0],), dtype=x.dtype, device=x.device)
     nbytes, ws = _workspace("tmpc_gated_ff_workspace_bytes", x.device, x.element_size(), a, 0)
     _call(f"tmpc_gated_ff_forward_{sfx}", x.device, a, _ptr(y), _ptr(gate), _ptr(up), _ptr(ws), nbytes)
@@ -339,23 +338,24 @@ def _ff_forward(x, xm, w_gate, w_up, w_down, act, sfx, gate, up):
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, sfx):
-        xm = _matrix(x)
+        xm, ldx = _matrix(x)
         gate, up = (torch.empty((xm.shape[0], w_gate.shape[0]), dtype=torch.float32, device=x.device) for _ in range(2))
         ctx.save_for_backward(xm, w_gate, w_up, w_down, gate, up)
         ctx.shape, ctx.act, ctx.sfx = x.shape, act, sfx
-        return _ff_forward(x, xm, w_gate, w_up, w_down, act, sfx, gate, up)
+        return _ff_forward(x, xm, ldx, w_gate, w_up, w_down, act, sfx, gate, up)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xm, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
-        a = _ff_args(xm, w_gate, w_up, w_down, ctx.act)
-        dym = _matrix(dy)
+        xm, ldx = _matrix(xm)
+        a = _ff_args(xm, ldx, w_gate, w_up, w_down, ctx.act)
+        dym, lddy = _matrix(dy)
         dx = torch.empty(ctx.shape, dtype=xm.dtype, device=xm.device)
         dg, du, dd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
         nbytes, ws = _workspace("tmpc_gated_ff_workspace_bytes", xm.device, xm.element_size(), a, 1)
         _call(f"tmpc_gated_ff_backward_{ctx.sfx}", xm.device, a, _ptr(gate), _ptr(up), _ptr(dym),
-              _pitch(dym), _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), _ptr(ws), nbytes)
+              lddy, _ptr(dx), _ptr(dg), _ptr(du), _ptr(dd), _ptr(ws), nbytes)
         return dx, dg, du, dd, None, None
 
 
@@ -383,4 +383,4 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     w_gate, w_up, w_down = w_gate.contiguous(), w_up.contiguous(), w_down.contiguous()
     if _wants_grad(x, w_gate, w_up, w_down):
         return _GatedFF.apply(x, w_gate, w_up, w_down, act, sfx)
-    return _ff_forward(x, _matrix(x), w_gate, w_up, w_down, act, sfx, None, None)
+    return _ff_forward(x, *_matrix(x), w_gate, w_up, w_down, act, sfx, None, None)
