@@ -59,3 +59,22 @@ def test_the_steps_after_a_spoiled_chunk_are_whole_again():
     got = run(x, lengths)
     for k, (v, tol) in bounds(x, reference(x, lengths), torch.float32).items():
         ref.assert_within(k, got[k], v, tol)
+
+
+@pytest.mark.parametrize("value", [0.5, float("inf")])
+def test_a_state_given_and_returned_in_one_buffer(value):
+    """A C caller may let state_out be state_in, whether or not a run has to be made again."""
+    from turbompc_amd import _lib
+    from turbompc_amd.learning import ops
+
+    x = inputs(2, 100, 2, 1, 32, 48, torch.float32, seed=25)
+    x["v"][1, 60, 0, 7] = value
+    with torch.no_grad():
+        want_o, want_s = learning.decay_attention(x["q"], x["k"], x["v"], x["g"], x["state"])
+    state, o = x["state"].clone(), torch.empty_like(want_o)
+    a = ops._attention_args(x["q"], x["k"], x["v"], x["g"], None, state, 32 ** -0.5)
+    _lib.check("forward", _lib.load().tmpc_decay_attention_forward_f32(
+        torch.cuda.current_stream().cuda_stream, a, o.data_ptr(), state.data_ptr(), None, 0))
+    for got, want in ((o, want_o), (state, want_s)):
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+        assert torch.equal(torch.isnan(got), torch.isnan(want))

@@ -521,11 +521,15 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
       __syncthreads();
   }
 
+  // What follows makes its indexes again from one that the compiler does not see through: its
+  // addresses and load_state's would be kept through every chunk (64 x 1024 x 8 heads, 64 x 64, with
+  // gradients 267 us against 271, 2048 x 101 x 4, 64 x 128, 918 against 975).
+  int end_tid = tid;
+  asm volatile("" : "+v"(end_tid));
+  const int end_lo = end_tid & 15, end_hi = (end_tid & 63) >> 4, end_col = (end_tid >> 6) * NV * 16;
   if constexpr (FULL) {  // this run's steps past the end
     zero_rows(p.o, p.o_f32, sizeof(E), obase, orow, p.dc, max(L, begin), min((int64_t)p.T, (int64_t)begin + p.seg_len), tid,
               S::THREADS);
-    // the run that holds the last live step has the final state
-    if (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0)) store_state(s, p.s_out + sbase, p.da, p.dc, col0, lo, hi);
     // An infinite or NaN key or value leaves the state so, to the end: in all columns, or in its own.
     f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
@@ -535,18 +539,18 @@ __global__ __launch_bounds__((AttnShape<E, DA, DC>::THREADS), 2) void attn_chunk
 #pragma unroll
         for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][x][r], 0.0f, zero[r]);
     if (begin < end && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
-      __threadfence_block();  // the rows written above are written again
-      // The arguments are read again and the indexes made again, behind an assignment that the
-      // compiler does not see through: kept from the ones above they cost registers in every
-      // chunk (64 x 128 heads, 101 steps: 5%).  (In a function that is called the arguments' address
-      // is null: it is taken in the kernel.)
+      __threadfence_block();  // the rows written above are written again; the state is not written yet
+      // The arguments are read again too, for the same reason.  (In a function that is called their
+      // address is null: it is taken in the kernel.)
       auto* args = __builtin_amdgcn_kernarg_segment_ptr();
-      int block = blockIdx.x, thread = threadIdx.x;
-      asm volatile("" : "+s"(args), "+s"(block), "+v"(thread));
-      attn_by_step<E, KA, NV>(*(const AttnArgs<E>*)args, block, thread);
+      int block = blockIdx.x;
+      asm volatile("" : "+s"(args), "+s"(block));
+      attn_by_step<E, KA, NV>(*(const AttnArgs<E>*)args, block, end_tid);
+    } else if (p.s_out && seg == (L > 0 ? (L - 1) / p.seg_len : 0)) {  // the run that holds the last live step
+      store_state(s, p.s_out + sbase, p.da, p.dc, end_col, end_lo, end_hi);
     }
   } else {
-    store_state(s, seg_state, p.da, p.dc, col0, lo, hi);
+    store_state(s, seg_state, p.da, p.dc, end_col, end_lo, end_hi);
   }
 }
 
