@@ -81,8 +81,8 @@ struct AttnShape {
   static constexpr int LDP = C + AttnTile<E>::PAD;
   // Registers that a lane holds through a whole chunk: S and the next chunk's rows on their way (a
   // row of `d` elements takes d / P threads).  Where they are many, no operand is kept from one row
-  // tile to the next, or they spill: 64 x 512 x 8 heads, bf16, 128 x 32 (104 held) 75 us against
-  // 120, 128 x 128 (112) 86 both, 128 x 64 (72) 66 against 63, 64 x 128 and 64 x 64 (64, 40) no difference.
+  // tile to the next, or they spill: 64 x 512 x 8 heads, bf16, 128 x 32 (104 held) 78 us against
+  // 116, 128 x 128 (112) no difference, 128 x 64 (72) 66 against 62, 64 x 128 and 64 x 64 (64, 40) none.
   static constexpr int rows_held(int d) {
     constexpr int P = Elem<E>::PIECE;
     return 4 * C / (THREADS / (d / P) < C ? THREADS / (d / P) : C);
@@ -240,9 +240,9 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
       for (int x = 0; x < NV; ++x) sq[k][x] = to_quad<E>(s[k][x]);
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
-      // Past the last live step.  With the scores shared the loop is the shorter part, and the
-      // branch keeps its tiles apart: 64 x 512 x 8 heads 99.8 us against 85.5; ragged batches of
-      // 512 x 4 heads of up to 512, 200 and 70 steps 302, 148 and 82 against 281, 144 and 86.
+      // Past the last live step.  With the scores shared the branch costs registers, which spill: 64 x
+      // 512 x 8 heads 97.5 us against 87.9; ragged batches of 512 x 4 heads of up to 512, 200 and 70
+      // steps 286, 142 and 80 against 268, 138 and 82.
       if (!S::SHARE && 16 * it >= n) break;
       if constexpr (S::FENCE) asm volatile("" ::: "memory");
       quad_t<E> a[KA];
@@ -295,7 +295,7 @@ __device__ inline void attn_chunk(const E* ta, const E* tb, const E* tc, E* tp, 
     for (int x = 0; x < NV; ++x) s[m][x] *= fl;
 #pragma unroll
   for (int j = 0; j < CT; j += 2) {
-    if (!S::SHARE && 16 * j >= n) break;
+    if (16 * j >= n) break;  // (128 x 128, the same cases: 88, 268, 138 and 82 us against 99, 335, 168 and 98 without)
     f32x4 d0, d1;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
