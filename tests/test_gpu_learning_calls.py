@@ -192,3 +192,12 @@ def test_saved_tensors_may_come_back_with_other_strides(dtype):
         got = grads()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_model_with_lengths_past_the_history():
+    model = learning.HistoryWeights(5, {"a": 2}, width=32, layers=2, heads=2, hidden=48)
+    history = torch.randn(4, 11, 5, device=DEV)
+    with torch.no_grad():
+        got = model(history, torch.tensor([11, 12, 500, -3], dtype=torch.int32, device=DEV))["a"]
+        want = model(history, torch.tensor([11, 11, 11, 0], dtype=torch.int32, device=DEV))["a"]
+    assert torch.equal(got, want)
