@@ -59,9 +59,9 @@ __device__ inline float decay_pow(float g, int n) { return n == 0 ? 1.0f : __exp
 // By its bytes (q, k, v read and o written once) the operator is bound by memory; what the
 // kernels meet first is the latency of the chain inside a chunk, two waves a SIMD, with
 // vector and matrix instructions each issuing about a third of the time (64 x 64 heads:
-// 410 and 58 a wave and chunk).  One launch over 512 heads of 1024 steps, 64 wide, bf16: 72
-// us, 3.7 TB/s of the 4.9 that a copy reaches; 50001 steps of 16 heads, 128 wide, in 32 runs
-// a head: 299 us, and 118 and 15 us for the runs' sums and their scan.
+// 413 and 58 a wave and chunk).  One launch over 512 heads of 1024 steps, 64 wide, bf16: 74
+// us, 3.6 TB/s of the 4.9 that a copy reaches; 50001 steps of 16 heads, 128 wide, in 32 runs
+// a head: 254 us, and 121 and 16 us for the runs' sums and their scan.
 //
 // A workgroup carries one (problem, head) through its chunks.  Wave w owns NV
 // 16-column tiles of the values and all of the scores: S, the scores and O stay in
