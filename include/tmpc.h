@@ -615,6 +615,49 @@ int tmpc_rms_norm_backward_bf16(hipStream_t stream, int64_t rows, int32_t width,
                                 const void* ds, int64_t ldds, const void* s, int64_t lds, const void* weight,
                                 const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes);
 
+/* Dropout of rows x (rows, width) of pitch ldx into y (contiguous; it may be x where ldx is
+ * the width): elements are kept where their 16 random bits are at least least = p 65536, rounded
+ * to a whole number, and multiplied by 65536 / (65536 - least); the others are zero, whatever
+ * they hold.  The bits of element (row, column) are half word column % 8 (low half first) of
+ * Philox-4x32-10 at the counter (column / 8, row, call, low word of key[1]) under the key key[0] (64
+ * bits).  key (2 int64, on the device) is a seed and a step; call tells the calls of a step
+ * apart.  The same call on a gradient is the backward pass.  0 <= p, least < 65536, rows <
+ * 2^31, 1 <= width <= 2^24. */
+int tmpc_dropout_f32(hipStream_t stream, int64_t rows, int32_t width, const void* x, int64_t ldx, double p,
+                     const int64_t* key, uint32_t call, void* y);
+int tmpc_dropout_bf16(hipStream_t stream, int64_t rows, int32_t width, const void* x, int64_t ldx, double p,
+                      const int64_t* key, uint32_t call, void* y);
+
+/* Layer norm with the residual's addition, over rows of 1 <= width <= 8192: s = d(x) +
+ * residual, y = (s - mean s) rstd weight + bias, rstd = (mean (s - mean s)^2 + eps)^-1/2, d being
+ * the dropout above with p, key and call (p 0: d(x) = x and key is not read).  residual and
+ * bias may be NULL: zero. */
+typedef struct tmpc_layer_norm {
+  int64_t rows;
+  int32_t width;
+  uint32_t call;
+  const void *x, *residual, *weight, *bias;
+  int64_t ldx, ldr; /* row pitches of x and residual */
+  double eps, p;
+  const int64_t* key;
+} tmpc_layer_norm;
+/* y and s (rows, width), contiguous; stats (rows, 2), or NULL: mean and rstd, which the backward
+ * pass reads. */
+int tmpc_layer_norm_forward_f32(hipStream_t stream, const tmpc_layer_norm* args, void* y, void* s, float* stats);
+int tmpc_layer_norm_forward_bf16(hipStream_t stream, const tmpc_layer_norm* args, void* y, void* s, float* stats);
+/* Its gradients from dy (pitch lddy), ds (pitch ldds, or NULL: zero), s (pitch lds) and stats:
+ * dx and dresidual (rows, width; dresidual NULL: not wanted; equal to dx where p is 0), dweight and
+ * dbias (width; dbias NULL: not wanted).  x, residual and bias are not read. */
+size_t tmpc_layer_norm_backward_workspace_bytes(int elem_bytes, int64_t rows, int32_t width);
+int tmpc_layer_norm_backward_f32(hipStream_t stream, const tmpc_layer_norm* args, const void* dy, int64_t lddy,
+                                 const void* ds, int64_t ldds, const void* s, int64_t lds, const float* stats,
+                                 void* dx, void* dresidual, void* dweight, void* dbias, void* workspace,
+                                 size_t workspace_bytes);
+int tmpc_layer_norm_backward_bf16(hipStream_t stream, const tmpc_layer_norm* args, const void* dy, int64_t lddy,
+                                  const void* ds, int64_t ldds, const void* s, int64_t lds, const float* stats,
+                                  void* dx, void* dresidual, void* dweight, void* dbias, void* workspace,
+                                  size_t workspace_bytes);
+
 /* Linear attention with a decay for each head: for problem b and head h, with
  * g = log_decay[h] <= 0 and t < lengths[b] (clamped to 0..T; NULL: T)
  *   S_t = e^g S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,  S_{-1} = state_in (or zero);

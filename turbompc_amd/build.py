@@ -1,7 +1,7 @@
 """Builds libtmpc_hip.so for gfx950 in-tree (turbompc_amd/lib/).
 
-Three translation units, compiled side by side: csrc/resident.hip (the on-chip ADMM
-path), csrc/learning.hip (the history model's operators) and csrc/capi.hip (every
+Translation units, compiled side by side: csrc/resident.hip (the on-chip ADMM
+path), csrc/learning*.hip (the history model's operators) and csrc/capi.hip (every
 other kernel and the solver's C ABI).  All HIP code is
 compiled with packed-FP32 instructions disabled.
 """
@@ -15,7 +15,7 @@ import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
-SOURCES = [PKG / "csrc" / n for n in ("capi.hip", "resident.hip", "learning.hip")]
+SOURCES = [PKG / "csrc" / n for n in ("capi.hip", "resident.hip", "learning.hip", "learning_norm.hip")]
 OUT = PKG / "lib" / "libtmpc_hip.so"
 ARCH = os.environ.get("TMPC_OFFLOAD_ARCH", "gfx950")
 

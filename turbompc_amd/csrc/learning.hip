@@ -2,64 +2,28 @@
 // choice of tile and workspace, launches.
 #include <algorithm>
 
-#include "../../include/tmpc.h"
 #include "decay_attention.hpp"
 #include "gated_ff.hpp"
 #include "gemm_wide.hpp"
+#include "learn_host.hpp"
 #include "rms_norm.hpp"
 
 namespace tmpc {
 namespace {
 
-constexpr int kCUs = 256;
-
-inline size_t align_up(size_t n) { return (n + 255) & ~size_t(255); }
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-int launch_status() { return hipGetLastError() == hipSuccess ? TMPC_OK : TMPC_ELAUNCH; }
-
-// Dynamic LDS above the 64 KiB default needs an explicit opt-in per kernel.
-template <typename K>
-void lds_optin(K kernel, size_t bytes) {
-  if (bytes > 65536)
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)bytes);
-}
-
 // ---------------------------------------------------------------- rms norm --
-constexpr int kMaxWidth = 8192;
 // Blocks of the backward pass, whose rows meet in the blocks' partial sums.  bf16, forward and backward,
 // with 512, 1024 and 2048: 206848 rows of 512 349, 330 and 373 us; 4096 of 8192 130, 148 and 187.
 constexpr int kRmsBlocks = 1024;
 
-// f(threads per row, pieces per thread) of the smallest form that holds `width`
-template <typename E, typename F>
-void with_row(int width, F f) {
-  const int pieces = (width + Elem<E>::PIECE - 1) / Elem<E>::PIECE;
-  using std::integral_constant;
-  if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
-  else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else if (pieces <= 128) f(integral_constant<int, 64>(), integral_constant<int, 2>());
-  else if (pieces <= 256) f(integral_constant<int, 256>(), integral_constant<int, 1>());
-  else if (pieces <= 512) f(integral_constant<int, 256>(), integral_constant<int, 2>());
-  else if (pieces <= 1024) f(integral_constant<int, 256>(), integral_constant<int, 4>());
-  else f(integral_constant<int, 256>(), integral_constant<int, 8>());
-}
-
-inline int64_t rms_rows_per_block(int width, int elem_bytes) {
-  const int pieces = (width * elem_bytes + 15) / 16;
-  return pieces <= 16 ? 16 : pieces <= 128 ? 4 : 1;
-}
 inline int64_t rms_backward_blocks(int64_t rows, int width, int elem_bytes) {
-  return std::min<int64_t>(ceil_div(rows, rms_rows_per_block(width, elem_bytes)), kRmsBlocks);
+  return std::min<int64_t>(ceil_div(rows, rows_per_block(width, elem_bytes)), kRmsBlocks);
 }
-
-bool rms_shape_ok(int64_t rows, int width) { return rows >= 0 && width >= 1 && width <= kMaxWidth; }
 
 template <typename E>
 int rms_forward_impl(hipStream_t st, int64_t rows, int32_t width, const void* x, int64_t ldx, const void* r,
                      int64_t ldr, const void* w, double eps, void* y, void* s, float* rstd) {
-  if (!rms_shape_ok(rows, width)) return TMPC_EBADSHAPE;
+  if (!norm_shape_ok(rows, width)) return TMPC_EBADSHAPE;
   if (rows == 0) return TMPC_OK;
   if (!x || !w || !y || !(eps >= 0.0) || ldx < 0 || ldr < 0) return TMPC_EBADARG;
   const RmsArgs<E> a{rows, width, (const E*)x, (const E*)r, (const E*)w, ldx, ldr, (float)eps, (E*)y, (E*)s, rstd};
@@ -75,7 +39,7 @@ template <typename E>
 int rms_backward_impl(hipStream_t st, int64_t rows, int32_t width, const void* dy, int64_t lddy, const void* ds,
                       int64_t ldds, const void* s, int64_t lds, const void* w, const float* rstd, void* dx, void* dw,
                       void* ws, size_t wsb) {
-  if (!rms_shape_ok(rows, width)) return TMPC_EBADSHAPE;
+  if (!norm_shape_ok(rows, width)) return TMPC_EBADSHAPE;
   if (!dw || (rows > 0 && (!dy || !s || !w || !rstd || !dx)) || lddy < 0 || ldds < 0 || lds < 0) return TMPC_EBADARG;
   const int64_t blocks = rms_backward_blocks(rows, width, sizeof(E));
   const size_t need = (size_t)blocks * width * sizeof(float);
@@ -554,7 +518,7 @@ using namespace tmpc;
 extern "C" {
 
 size_t tmpc_rms_norm_backward_workspace_bytes(int elem_bytes, int64_t rows, int32_t width) {
-  if (!rms_shape_ok(rows, width) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  if (!norm_shape_ok(rows, width) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
   return align_up((size_t)rms_backward_blocks(rows, width, elem_bytes) * width * sizeof(float));
 }
 size_t tmpc_decay_attention_workspace_bytes(int elem_bytes, const tmpc_decay_attention* a, int backward) {
