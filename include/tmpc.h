@@ -701,6 +701,37 @@ int tmpc_decay_attention_step_f32(hipStream_t stream, const tmpc_decay_attention
 int tmpc_decay_attention_step_bf16(hipStream_t stream, const tmpc_decay_attention* args, const uint8_t* active,
                                    float* state, void* o);
 
+/* Gated delta rule: for problem b and head h, with a_t = exp(log_decay), log_decay <= 0 (-inf: 0),
+ * and t < lengths[b] (clamped to 0..T; NULL: T)
+ *   u_t = beta_t (v_t - a_t k_t S_{t-1}),  S_t = a_t S_{t-1} + k_t^T u_t,  o_t = scale q_t S_t,
+ * S_{-1} = state_in (or zero); steps past the length give o = 0 and leave the state.  An infinite or
+ * NaN value at a live step reaches what it has a part in: no earlier step's output, no other
+ * head or problem.  H is a multiple of each of Hq, Hk, Hv; head h reads head h / (H / Hq) of q, and so
+ * on.  1 <= dk, dv <= 128.  q (B, T, Hq, dk), k (B, T, Hk, dk), v (B, T, Hv, dv) have contiguous rows;
+ * beta (B, T, H) is of their type, log_decay (B, T, H) fp32.  Strides (elements) are those of
+ * problem, step and head, that of a step at most 2^23 - 1; T <= 2^30, H <= 32768 and B H <= 2^23. */
+typedef struct tmpc_delta_attention {
+  int32_t B, T, H, Hq, Hk, Hv, dk, dv;
+  const void *q, *k, *v, *beta;
+  const float* log_decay;
+  int64_t q_stride[3], k_stride[3], v_stride[3], beta_stride[3], log_decay_stride[3];
+  const int32_t* lengths; /* (B) or NULL */
+  const float* state_in;  /* (B, H, dk, dv) or NULL */
+  double scale;
+} tmpc_delta_attention;
+size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_attention* args, int backward);
+/* o (B, T, H, dv) and state_out (B, H, dk, dv, or NULL), contiguous. */
+int tmpc_delta_attention_forward_f32(hipStream_t stream, const tmpc_delta_attention* args, void* o, float* state_out,
+                                     void* workspace, size_t workspace_bytes);
+int tmpc_delta_attention_forward_bf16(hipStream_t stream, const tmpc_delta_attention* args, void* o, float* state_out,
+                                      void* workspace, size_t workspace_bytes);
+/* One step (T = 1; lengths, state_in and the strides of a step are not read): state (B, H, dk, dv) is
+ * updated in place, o (B, H, dv).  Where active (B bytes, or NULL: all) is 0, o is 0 and the state stays. */
+int tmpc_delta_attention_step_f32(hipStream_t stream, const tmpc_delta_attention* args, const uint8_t* active,
+                                  float* state, void* o);
+int tmpc_delta_attention_step_bf16(hipStream_t stream, const tmpc_delta_attention* args, const uint8_t* active,
+                                   float* state, void* o);
+
 /* Gated feed-forward block: y = (act(x w_gate^T) o (x w_up^T)) w_down^T for
  * rows x (M, D) of pitch ldx, w_gate, w_up (F, D), w_down (Dout, F) contiguous;
  * activation 0: silu, 1: gelu (exact).  Widths and pitches at most 2^20,

@@ -161,6 +161,14 @@ class GatedFF(ctypes.Structure):
     ] + [(k, ctypes.c_void_p) for k in ("w_gate", "w_up", "w_down")]
 
 
+class DeltaAttention(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int32) for k in ("B", "T", "H", "Hq", "Hk", "Hv", "dk", "dv")] + [
+        (k, ctypes.c_void_p) for k in ("q", "k", "v", "beta", "log_decay")
+    ] + [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride", "beta_stride", "log_decay_stride")] + [
+        (k, ctypes.c_void_p) for k in ("lengths", "state_in")
+    ] + [("scale", ctypes.c_double)]
+
+
 class LayerNorm(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("width", ctypes.c_int32), ("call", ctypes.c_uint32)] + [
         (k, ctypes.c_void_p) for k in ("x", "residual", "weight", "bias")
@@ -173,6 +181,7 @@ class LayerNorm(ctypes.Structure):
 _VP, _I32, _U32, _F64, _SZ = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_double, ctypes.c_size_t
 _I64 = ctypes.c_int64
 _PDA, _PFF, _PLN = ctypes.POINTER(DecayAttention), ctypes.POINTER(GatedFF), ctypes.POINTER(LayerNorm)
+_PDL = ctypes.POINTER(DeltaAttention)
 _PD, _PQ, _PS, _PC, _PSQ = (ctypes.POINTER(t) for t in (Dims, QP, State, AdmmCfg, SqpStep))
 SIGNATURES = {
     "tmpc_version": [],
@@ -235,6 +244,7 @@ SIGNATURES = {
     "tmpc_decay_attention_workspace_bytes": [ctypes.c_int, _PDA, ctypes.c_int],
     "tmpc_gated_ff_workspace_bytes": [ctypes.c_int, _PFF, ctypes.c_int],
     "tmpc_layer_norm_backward_workspace_bytes": [ctypes.c_int, _I64, _I32],
+    "tmpc_delta_attention_workspace_bytes": [ctypes.c_int, _PDL, ctypes.c_int],
 }
 for _sfx in ("f32", "bf16"):
     SIGNATURES.update({
@@ -246,6 +256,8 @@ for _sfx in ("f32", "bf16"):
         f"tmpc_decay_attention_step_{_sfx}": [_VP, _PDA, _VP, _VP, _VP],
         f"tmpc_gated_ff_forward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _VP, _SZ],
         f"tmpc_gated_ff_backward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _I64] + [_VP] * 5 + [_SZ],
+        f"tmpc_delta_attention_forward_{_sfx}": [_VP, _PDL, _VP, _VP, _VP, _SZ],
+        f"tmpc_delta_attention_step_{_sfx}": [_VP, _PDL, _VP, _VP, _VP],
         f"tmpc_dropout_{_sfx}": [_VP, _I64, _I32, _VP, _I64, _F64, _VP, _U32, _VP],
         f"tmpc_layer_norm_forward_{_sfx}": [_VP, _PLN, _VP, _VP, _VP],
         f"tmpc_layer_norm_backward_{_sfx}": [_VP, _PLN] + [_VP, _I64] * 3 + [_VP] * 6 + [_SZ],
@@ -260,6 +272,7 @@ _SIZE_FNS = {
     "tmpc_decay_attention_workspace_bytes",
     "tmpc_gated_ff_workspace_bytes",
     "tmpc_layer_norm_backward_workspace_bytes",
+    "tmpc_delta_attention_workspace_bytes",
 }
 
 _LIB: Optional[ctypes.CDLL] = None
