@@ -725,6 +725,19 @@ int tmpc_delta_attention_forward_f32(hipStream_t stream, const tmpc_delta_attent
                                      void* workspace, size_t workspace_bytes);
 int tmpc_delta_attention_forward_bf16(hipStream_t stream, const tmpc_delta_attention* args, void* o, float* state_out,
                                       void* workspace, size_t workspace_bytes);
+/* Gradients from those of o (d_o, strides d_o_stride) and of the final state (d_state_out, or NULL:
+ * zero): dq (B, T, Hq, dk), dk (B, T, Hk, dk), dv (B, T, Hv, dv), dlog_decay (B, T, H, fp32; zero where the decay
+ * is), dbeta (B, T, H) and d_state_in (B, H, dk, dv, or NULL), contiguous; zero past a length.  The state is
+ * formed again; nothing of the forward call is kept.  Values that are not finite may spoil the
+ * gradients of their whole history and head. */
+int tmpc_delta_attention_backward_f32(hipStream_t stream, const tmpc_delta_attention* args, const void* d_o,
+                                       const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,
+                                       void* dv, float* dlog_decay, void* dbeta, float* d_state_in, void* workspace,
+                                       size_t workspace_bytes);
+int tmpc_delta_attention_backward_bf16(hipStream_t stream, const tmpc_delta_attention* args, const void* d_o,
+                                        const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,
+                                        void* dv, float* dlog_decay, void* dbeta, float* d_state_in, void* workspace,
+                                        size_t workspace_bytes);
 /* One step (T = 1; lengths, state_in and the strides of a step are not read): state (B, H, dk, dv) is
  * updated in place, o (B, H, dv).  Where active (B bytes, or NULL: all) is 0, o is 0 and the state stays. */
 int tmpc_delta_attention_step_f32(hipStream_t stream, const tmpc_delta_attention* args, const uint8_t* active,

@@ -257,6 +257,7 @@ for _sfx in ("f32", "bf16"):
         f"tmpc_gated_ff_forward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _VP, _SZ],
         f"tmpc_gated_ff_backward_{_sfx}": [_VP, _PFF, _VP, _VP, _VP, _I64] + [_VP] * 5 + [_SZ],
         f"tmpc_delta_attention_forward_{_sfx}": [_VP, _PDL, _VP, _VP, _VP, _SZ],
+        f"tmpc_delta_attention_backward_{_sfx}": [_VP, _PDL, _VP, ctypes.POINTER(_I64)] + [_VP] * 8 + [_SZ],
         f"tmpc_delta_attention_step_{_sfx}": [_VP, _PDL, _VP, _VP, _VP],
         f"tmpc_dropout_{_sfx}": [_VP, _I64, _I32, _VP, _I64, _F64, _VP, _U32, _VP],
         f"tmpc_layer_norm_forward_{_sfx}": [_VP, _PLN, _VP, _VP, _VP],

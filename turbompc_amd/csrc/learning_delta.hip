@@ -86,6 +86,95 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
   return launch_status();
 }
 
+// The backward pass' arrays in the workspace, one after another.
+struct BackwardPlan {
+  int chunks, segs, DK, DV;
+  size_t e, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, bytes;
+};
+inline int tile_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+template <typename E>
+BackwardPlan backward_plan(const tmpc_delta_attention* x) {
+  constexpr int C = AttnTile<E>::C;
+  BackwardPlan p{};
+  p.chunks = (int)ceil_div(x->T, C), p.segs = (int)ceil_div(x->T, kDeltaSeg);
+  p.DK = tile_width(x->dk), p.DV = tile_width(x->dv);
+  const size_t bh = (size_t)x->B * x->H, state = (size_t)p.DK * p.DV, rows = bh * p.chunks * C;
+  const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
+  auto take = [&](size_t bytes) {
+    const size_t at = p.bytes;
+    p.bytes += align_up(bytes);
+    return at;
+  };
+  p.e = take(rows * p.DV * sizeof(E));
+  p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
+  p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
+  p.s_seg = take(bh * p.segs * state * sizeof(float)), p.dot = take(bh * p.segs * sizeof(float));
+  if (x->Hv != x->H) p.y = take(rows * p.DV * sizeof(E)), p.y_part = take(tok * x->dv);
+  if (x->Hq != x->H) p.q_part = take(tok * x->dk);
+  if (x->Hk != x->H) p.k_part = take(tok * x->dk);
+  return p;
+}
+
+template <typename E>
+int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o, const int64_t* dos,
+                  const float* d_out, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* d_in, void* ws,
+                  size_t wsb) {
+  if (!shape_ok(x)) return TMPC_EBADSHAPE;
+  if (x->B == 0) return TMPC_OK;
+  if (!steps_ok(x) || (dos && (dos[1] < 0 || dos[1] > kMaxStep))) return TMPC_EBADSHAPE;
+  if (!dos || !data_ok(x) || (x->T > 0 && (!d_o || !dq || !dk || !dv || !dg || !dbeta))) return TMPC_EBADARG;
+  const BackwardPlan w = backward_plan<E>(x);
+  if (wsb < w.bytes) return TMPC_EWORKSPACE;
+  if (w.bytes > 0 && !ws) return TMPC_EBADARG;
+  char* base = (char*)ws;
+  DeltaBwdArgs<E> a{};
+  a.f = delta_args<E>(x);
+  a.d_o = (const E*)d_o, a.d_out = d_out;
+  std::copy_n(dos, 3, a.dos);
+  a.chunks = w.chunks, a.segs = w.segs;
+  a.e = (E*)(base + w.e), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
+  a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot);
+  if (x->Hv != x->H) {
+    a.y = (E*)(base + w.y), a.y_part = (float*)(base + w.y_part), a.y_width = w.DV;
+    a.ys[0] = (int64_t)w.chunks * AttnTile<E>::C * w.DV, a.ys[1] = w.DV;
+  } else {
+    a.y = (E*)dv, a.y_width = x->dv, a.ys[0] = (int64_t)x->T * x->H * x->dv, a.ys[1] = (int64_t)x->H * x->dv;
+  }
+  a.q_part = x->Hq != x->H, a.k_part = x->Hk != x->H;
+  a.dq = a.q_part ? base + w.q_part : dq, a.dk = a.k_part ? base + w.k_part : dk;
+  a.dbeta = (E*)dbeta, a.dg = dg, a.d_in = d_in;
+  const int64_t bh = (int64_t)x->B * x->H;
+  const bool vec = rows_ok(a.f.q, a.f.qs, x->dk) && rows_ok(a.f.k, a.f.ks, x->dk) && rows_ok(a.f.v, a.f.vs, x->dv) &&
+                   rows_ok(a.d_o, a.dos, x->dv) && ((uintptr_t)dv & 3) == 0;
+  with_widths(x->dk, x->dv, [&](auto dkw, auto dvw) {
+    auto go = [&](auto v) {
+      constexpr int THREADS = DeltaShape<E, dkw(), dvw()>::THREADS;
+      auto launch = [&](auto k, int64_t blocks, int threads, size_t lds) {
+        lds_optin(k, lds);
+        hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), lds, st, a);
+      };
+      if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw(), v()>, bh, THREADS, delta_states_lds<E, dkw(), dvw()>());
+      launch(delta_reverse_kernel<E, dkw(), dvw(), v()>, bh, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
+      if (x->T > 0) launch(delta_dqk_kernel<E, dkw(), dvw(), v()>, bh * w.chunks, 256, delta_dqk_lds<E, dkw(), dvw()>());
+    };
+    if (vec) go(std::true_type());
+    else go(std::false_type());
+  });
+  if (x->T > 0) {
+    hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.segs)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
+    auto sum = [&](const void* in, int heads, int d, void* out) {
+      const int64_t rows = (int64_t)x->B * x->T * heads;
+      const int q = (d + 3) / 4;
+      hipLaunchKernelGGL((attn_head_sum_kernel<E>), dim3((unsigned)std::min<int64_t>(ceil_div(rows, 256 / q), 16 * kCUs)),
+                         dim3(256), 0, st, (const float*)in, rows, x->H / heads, d, q, (E*)out);
+    };
+    if (x->Hq != x->H) sum(a.dq, x->Hq, x->dk, dq);
+    if (x->Hk != x->H) sum(a.dk, x->Hk, x->dk, dk);
+    if (x->Hv != x->H) sum(a.y_part, x->Hv, x->dv, dv);
+  }
+  return launch_status();
+}
+
 template <typename E>
 int step_impl(hipStream_t st, const tmpc_delta_attention* x, const uint8_t* active, float* state, void* o) {
   if (!shape_ok(x) || x->T != 1) return TMPC_EBADSHAPE;
@@ -118,14 +207,20 @@ extern "C" {
 
 size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_attention* a, int backward) {
   if (!a || !shape_ok(a) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
-  (void)backward;
-  return 0;
+  if (!backward) return 0;
+  return elem_bytes == 2 ? backward_plan<bf16>(a).bytes : backward_plan<float>(a).bytes;
 }
 
 #define TMPC_LEARNING_DELTA(SFX, E)                                                                                    \
   int tmpc_delta_attention_forward_##SFX(hipStream_t s, const tmpc_delta_attention* a, void* o, float* state_out,      \
                                          void* ws, size_t wsb) {                                                       \
     return forward_impl<E>(s, a, o, state_out, ws, wsb);                                                               \
+  }                                                                                                                    \
+  int tmpc_delta_attention_backward_##SFX(hipStream_t s, const tmpc_delta_attention* a, const void* d_o,               \
+                                          const int64_t* d_o_stride, const float* d_state_out, void* dq, void* dk,     \
+                                          void* dv, float* dlog_decay, void* dbeta, float* d_state_in, void* ws,       \
+                                          size_t wsb) {                                                                \
+    return backward_impl<E>(s, a, d_o, d_o_stride, d_state_out, dq, dk, dv, dlog_decay, dbeta, d_state_in, ws, wsb);   \
   }                                                                                                                    \
   int tmpc_delta_attention_step_##SFX(hipStream_t s, const tmpc_delta_attention* a, const uint8_t* active,             \
                                       float* state, void* o) {                                                         \

@@ -7,6 +7,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from .. import _lib
@@ -78,6 +79,32 @@ def _delta_forward(q, k, v, log_decay, beta, state, lengths, scale, sfx):
     return o, out
 
 
+class _DeltaAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, beta, state, lengths, scale, sfx):
+        ctx.save_for_backward(q, k, v, log_decay, beta, state, lengths)
+        ctx.scale, ctx.sfx = scale, sfx
+        ctx.set_materialize_grads(False)
+        return _delta_forward(q, k, v, log_decay, beta, state, lengths, scale, sfx)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_o, d_out):
+        q, k, v, log_decay, beta, state, lengths = ctx.saved_tensors
+        dev = q.device
+        d_o = _steps(d_o) if d_o is not None else torch.zeros(log_decay.shape + v.shape[-1:], dtype=q.dtype, device=dev)
+        d_out = d_out.contiguous() if d_out is not None else None
+        empty = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+        dq, dk, dv, dg, dbeta = (empty(t) for t in (q, k, v, log_decay, beta))
+        d_state = empty(state) if state is not None and ctx.needs_input_grad[5] else None
+        a = _delta_args(q, k, v, log_decay, beta, lengths, state, ctx.scale)
+        nbytes, ws = _workspace("tmpc_delta_attention_workspace_bytes", dev, q.element_size(), a, 1)
+        st = (ctypes.c_int64 * 3)(*_step_strides(d_o))
+        _call(f"tmpc_delta_attention_backward_{ctx.sfx}", dev, a, _ptr(d_o), st, _ptr(d_out), _ptr(dq), _ptr(dk),
+              _ptr(dv), _ptr(dg), _ptr(dbeta), _ptr(d_state), _ptr(ws), nbytes)
+        return dq, dk, dv, dg, dbeta, d_state, None, None, None
+
+
 def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, beta: torch.Tensor,
                     state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                     scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -103,7 +130,7 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     state = state.contiguous() if state is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
     args = (_steps(q), _steps(k), _steps(v), _gate(log_decay), _gate(beta), state, lengths, scale, sfx)
-    return _delta_forward(*args)
+    return _DeltaAttention.apply(*args) if _wants_grad(q, k, v, log_decay, beta, state) else _delta_forward(*args)
 
 
 def delta_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
