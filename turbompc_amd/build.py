@@ -15,7 +15,7 @@ import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
-SOURCES = [PKG / "csrc" / n for n in ("capi.hip", "resident.hip", "learning.hip", "learning_delta.hip", "learning_norm.hip")]
+SOURCES = [PKG / "csrc" / n for n in ("capi.hip", "resident.hip", "learning.hip", "learning_delta_f32.hip", "learning_delta_bf16.hip", "learning_norm.hip")]
 OUT = PKG / "lib" / "libtmpc_hip.so"
 ARCH = os.environ.get("TMPC_OFFLOAD_ARCH", "gfx950")
 

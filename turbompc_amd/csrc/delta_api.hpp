@@ -1,4 +1,7 @@
-// C ABI of the gated delta rule (include/tmpc.h): argument checks, workspace, launches.
+// The gated delta rule's C entry points (include/tmpc.h) for an element type: argument checks,
+// workspace, launches.  Each type is a translation unit of its own (learning_delta_*.hip): they are
+// the library's longest to compile.
+#pragma once
 #include <algorithm>
 
 #include "delta_attention.hpp"
@@ -73,15 +76,12 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
   if (!data_ok(x) || (x->T > 0 && !o)) return TMPC_EBADARG;
   DeltaArgs<E> p = delta_args<E>(x);
   p.s_out = state_out, p.o = (E*)o;
+  p.vec = vec_ok(p);
   with_widths(x->dk, x->dv, [&](auto dk, auto dv) {
-    auto go = [&](auto vec) {
-      constexpr size_t lds = delta_forward_lds<E, dk(), dv()>();
-      auto k = delta_forward_kernel<E, dk(), dv(), vec()>;
-      lds_optin(k, lds);
-      hipLaunchKernelGGL(k, dim3((unsigned)(x->B * x->H)), dim3(DeltaShape<E, dk(), dv()>::THREADS), lds, st, p);
-    };
-    if (vec_ok(p)) go(std::true_type());
-    else go(std::false_type());
+    constexpr size_t lds = delta_forward_lds<E, dk(), dv()>();
+    auto k = delta_forward_kernel<E, dk(), dv()>;
+    lds_optin(k, lds);
+    hipLaunchKernelGGL(k, dim3((unsigned)(x->B * x->H)), dim3(DeltaShape<E, dk(), dv()>::THREADS), lds, st, p);
   });
   return launch_status();
 }
@@ -144,21 +144,17 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   a.dq = a.q_part ? base + w.q_part : dq, a.dk = a.k_part ? base + w.k_part : dk;
   a.dbeta = (E*)dbeta, a.dg = dg, a.d_in = d_in;
   const int64_t bh = (int64_t)x->B * x->H;
-  const bool vec = rows_ok(a.f.q, a.f.qs, x->dk) && rows_ok(a.f.k, a.f.ks, x->dk) && rows_ok(a.f.v, a.f.vs, x->dv) &&
-                   rows_ok(a.d_o, a.dos, x->dv) && ((uintptr_t)dv & 3) == 0;
+  a.f.vec = rows_ok(a.f.q, a.f.qs, x->dk) && rows_ok(a.f.k, a.f.ks, x->dk) && rows_ok(a.f.v, a.f.vs, x->dv) &&
+            rows_ok(a.d_o, a.dos, x->dv) && ((uintptr_t)dv & 3) == 0;
   with_widths(x->dk, x->dv, [&](auto dkw, auto dvw) {
-    auto go = [&](auto v) {
-      constexpr int THREADS = DeltaShape<E, dkw(), dvw()>::THREADS;
-      auto launch = [&](auto k, int64_t blocks, int threads, size_t lds) {
-        lds_optin(k, lds);
-        hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), lds, st, a);
-      };
-      if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw(), v()>, bh, THREADS, delta_states_lds<E, dkw(), dvw()>());
-      launch(delta_reverse_kernel<E, dkw(), dvw(), v()>, bh, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
-      if (x->T > 0) launch(delta_dqk_kernel<E, dkw(), dvw(), v()>, bh * w.chunks, 256, delta_dqk_lds<E, dkw(), dvw()>());
+    constexpr int THREADS = DeltaShape<E, dkw(), dvw()>::THREADS;
+    auto launch = [&](auto k, int64_t blocks, int threads, size_t lds) {
+      lds_optin(k, lds);
+      hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), lds, st, a);
     };
-    if (vec) go(std::true_type());
-    else go(std::false_type());
+    if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw()>, bh, THREADS, delta_states_lds<E, dkw(), dvw()>());
+    launch(delta_reverse_kernel<E, dkw(), dvw()>, bh, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
+    if (x->T > 0) launch(delta_dqk_kernel<E, dkw(), dvw()>, bh * w.chunks, 256, delta_dqk_lds<E, dkw(), dvw()>());
   });
   if (x->T > 0) {
     hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.segs)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
@@ -201,16 +197,6 @@ int step_impl(hipStream_t st, const tmpc_delta_attention* x, const uint8_t* acti
 }  // namespace
 }  // namespace tmpc
 
-using namespace tmpc;
-
-extern "C" {
-
-size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_attention* a, int backward) {
-  if (!a || !shape_ok(a) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
-  if (!backward) return 0;
-  return elem_bytes == 2 ? backward_plan<bf16>(a).bytes : backward_plan<float>(a).bytes;
-}
-
 #define TMPC_LEARNING_DELTA(SFX, E)                                                                                    \
   int tmpc_delta_attention_forward_##SFX(hipStream_t s, const tmpc_delta_attention* a, void* o, float* state_out,      \
                                          void* ws, size_t wsb) {                                                       \
@@ -226,7 +212,3 @@ size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_att
                                       float* state, void* o) {                                                         \
     return step_impl<E>(s, a, active, state, o);                                                                       \
   }
-TMPC_LEARNING_DELTA(f32, float)
-TMPC_LEARNING_DELTA(bf16, bf16)
-
-}  // extern "C"

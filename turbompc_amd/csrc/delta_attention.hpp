@@ -1,20 +1,23 @@
 // Gated delta rule.  Problem b, head h, a_t = exp(g_t) (S fp32, dk x dv):
 //   e_t = v_t - a_t k_t S_{t-1},  u_t = beta_t e_t,  S_t = a_t S_{t-1} + k_t^T u_t,  o_t = scale q_t S_t.
 //
-// Blocks of 16 steps, G_i the sum of g up to step i of the block, Gamma_ij = exp(G_i - G_j) for
+// Blocks of 16 NB steps, G_i the sum of g up to step i of the block, Gamma_ij = exp(G_i - G_j) for
 // j <= i, else 0.  With A_ij = Gamma_ij (k_i . k_j) beta_j for j < i, the block's steps are
 //   E = (I + A)^-1 (V - diag(exp G) K S),  U = diag(beta) E,
-//   O = scale (diag(exp G) Q S + (Q K^T o Gamma) U),  S := exp(G_15) S + K^T diag(exp(G_15 - G)) U.
-// The inverse is formed by substitution, row by row: its entries stay as small as the recurrence's
-// products of (I - beta k^T k), where a product of powers of A would cancel large terms for keys
-// that repeat themselves.  Sums of g are held in 64 bits, so that their differences are exact to 32
-// also behind a decay of zero (g = -inf, taken as -1e5, whose exponential is zero).
+//   O = scale (diag(exp G) Q S + (Q K^T o Gamma) U),  S := exp(G_end) S + K^T diag(exp(G_end - G)) U.
+// The inverses of the 16 x 16 tiles on the diagonal are formed by substitution, row by row: their
+// entries stay as small as the recurrence's products of (I - beta k^T k), where a product of powers of A
+// would cancel large terms for keys that repeat themselves.  Sums of g are held in 64 bits, so that
+// their differences are exact to 32 also behind a decay of zero (g = -inf, taken as -1e5, whose
+// exponential is zero).
 //
-// A block is as long as a matrix instruction's tile, so that the chain from state to state stays in a
-// wave's registers: S is the operand of K S, whose result is the operand of the product with the
-// inverse, whose result is the operand of the state's update.  A wave owns 16 columns of the values and
-// walks its head's blocks without meeting the other waves; what depends on the block alone (the
-// inverse, Q K^T o Gamma, the powers) is made once a chunk of several blocks, a wave a block, in LDS.
+// Blocks are short, so that the chain from state to state stays in a wave's registers: S is the
+// operand of K S, whose result is the operand of the product with the inverse, whose result is the operand
+// of the state's update.  A wave owns 16 columns of the values and walks its head's blocks without
+// meeting the other waves; what depends on the block alone (the inverse, Q K^T o Gamma, the powers) is
+// made once a chunk of several blocks, the waves sharing it out, in LDS.  In bf16 the state, an fp32
+// result, enters products as three bf16 terms (24 bits); a block has two tiles there, so that they are
+// formed half as often.
 //
 // Backward.  With R_t = dL/dS_t from later steps, D_t = R_t + scale q_t^T do_t:
 //   du_t = k_t D_t,  y_t = dv_t = beta_t du_t,  R_{t-1} = a_t (D_t - k_t^T y_t),  dbeta_t = du_t . e_t,
@@ -35,6 +38,7 @@ struct DeltaArgs {
   int64_t qs[3], ks[3], vs[3], bs[3], gs[3];  // strides of problem, step, head
   const int32_t* lengths;                     // (B) or NULL
   float scale;
+  int vec;            // rows of whole pieces at 4-byte addresses, all operands'
   const float* s_in;  // (B, H, dk, dv) or NULL
   float* s_out;       // (B, H, dk, dv) or NULL
   E* o;               // (B, T, H, dv)
@@ -43,13 +47,17 @@ struct DeltaArgs {
 template <typename E, int DK, int DV>
 struct DeltaShape {
   static constexpr int W = DV / 16, THREADS = 64 * W;  // a wave 16 value columns
-  static constexpr int C = AttnTile<E>::C, SUB = C / 16, PAD = AttnTile<E>::PAD;
+  static constexpr int C = AttnTile<E>::C, PAD = AttnTile<E>::PAD;
+  static constexpr int NB = sizeof(E) == 2 ? 2 : 1, BS = 16 * NB, NBLK = C / BS, TRI = NB * (NB + 1) / 2;
   static constexpr int LDK = DK + PAD, LDV = DV + PAD;
-  static constexpr int LDT = 20;  // pitch of a 16 x 16 fp32 tile: its quads spread over the banks
-  static constexpr int LDP = sizeof(E) == 2 ? 24 : 20;
-  // floats: the chunk's gates, powers and inverses
-  static constexpr int GATES = 4 * C + 4, INV = SUB * 16 * LDT;
+  static constexpr int LDT = 20, TILE = 16 * LDT;  // a 16 x 16 fp32 tile, its quads spread over the banks
+  static constexpr int LDP = sizeof(E) == 2 ? 24 : 20, TILE_P = 16 * LDP;  // one of E
+  static constexpr int GATES = 2 * C + 3 * C + 4;  // floats
+  static constexpr int INV = NBLK * TRI * TILE, SCORES = NBLK * TRI * TILE_P;
+  static constexpr int WAVES_PER_SIMD = 2;
 };
+// tile (i, j <= i) of a block
+constexpr int tri(int i, int j) { return i * (i + 1) / 2 + j; }
 
 __device__ inline f32x4 lds_f4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 
@@ -60,23 +68,42 @@ __device__ inline f32x4 mma16(f32x4 a, f32x4 b, f32x4 acc) {
   return acc;
 }
 
-// What a block's products are made of, per chunk in LDS.
+// The same value, which the compiler takes for another: what is computed from it is computed where it is
+// used, and not before the loop around, to be kept in (or spilled from) registers through all of it.
+__device__ inline int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// A chunk's gates in LDS: the sums of g from each block's start, beta (zeros past the last live
+// step), exp(G), exp(G_end - G), exp(G_end).
 struct DeltaGates {
-  float *g, *beta;      // the chunk's, zeros past its last live step
-  float *from, *to;     // exp(G_i) and exp(G_15 - G_i) of each block
-  float* total;         // exp(G_15)
-  float* inv;           // tiles of the inverses, pitch LDT
+  double* G;
+  float *beta, *from, *to, *total;
 };
 template <typename S>
-__device__ inline DeltaGates delta_gates(float* base) {
+__device__ inline DeltaGates delta_gates(char* base) {
   DeltaGates d;
-  d.g = base, d.beta = base + S::C, d.from = base + 2 * S::C, d.to = base + 3 * S::C, d.total = base + 4 * S::C;
-  d.inv = base + S::GATES;
+  d.G = reinterpret_cast<double*>(base), d.beta = reinterpret_cast<float*>(d.G + S::C);
+  d.from = d.beta + S::C, d.to = d.from + S::C, d.total = d.to + S::C;
   return d;
 }
 
-// The chunk's gates on their way from memory to LDS: a thread a step.
-template <typename E, int C>
+template <int CTRL>
+__device__ inline double dpp_f64(double v) {  // zero where there is no such lane
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t l = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, 0xf, 0xf, true);
+  const uint32_t h = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
+}
+__device__ inline double lane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t l = __builtin_amdgcn_readlane((uint32_t)u, lane), h = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
+}
+
+// The chunk's gates on their way from memory to LDS: the first wave's lanes a step each.
+template <typename E, typename S>
 struct DeltaGateRows {
   const float* g;
   const E* beta;
@@ -84,72 +111,158 @@ struct DeltaGateRows {
   float vg, vb;
   __device__ void load(int t0, int n, int tid) {
     vg = vb = 0.0f;
-    if (tid < n && tid < C) {
-      vg = g[(t0 + tid) * gs];
-      vb = (float)beta[(t0 + tid) * bs];
-    }
+    if (tid < n && tid < S::C) vg = g[(t0 + tid) * gs], vb = (float)beta[(t0 + tid) * bs];
   }
   __device__ void store(const DeltaGates& d, int tid) const {
-    if (tid < C) d.g[tid] = vg < kNoDecay ? kNoDecay : vg, d.beta[tid] = vb;
+    if (tid >= 64) return;
+    double x = vg < kNoDecay ? kNoDecay : vg;
+    x += dpp_f64<0x111>(x);  // within 16 lanes
+    x += dpp_f64<0x112>(x);
+    x += dpp_f64<0x114>(x);
+    x += dpp_f64<0x118>(x);
+    double end;
+    const double e0 = lane_f64(x, 15), e1 = lane_f64(x, 31), e2 = lane_f64(x, 47), e3 = lane_f64(x, 63);
+    if constexpr (S::NB == 2) {
+      if (tid & 16) x += tid & 32 ? e2 : e0;
+      end = tid & 32 ? e2 + e3 : e0 + e1;
+    } else {
+      end = tid & 32 ? (tid & 16 ? e3 : e2) : (tid & 16 ? e1 : e0);
+    }
+    if (tid < S::C) {
+      d.G[tid] = x, d.beta[tid] = vb, d.from[tid] = __expf((float)x), d.to[tid] = __expf((float)(end - x));
+      if (tid % S::BS == 0) d.total[tid / S::BS] = __expf((float)end);
+    }
   }
 };
 
-// Block `sub` of a chunk, by one wave: the powers, and G_i - G_j of a lane's i = lo and j = 4 hi + r.
-template <typename S>
-__device__ inline f32x4 delta_powers(const DeltaGates& d, int sub, int lane) {
-  const int lo = lane & 15, hi = lane >> 4;
-  double sum = 0.0, mine = 0.0, at[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16; j += 4) {
-    const f32x4 g = lds_f4(d.g + 16 * sub + j);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sum += (double)g[r];
-      if (j + r == lo) mine = sum;
-      if (j == 4 * hi) at[r] = sum;
-    }
-  }
-  if (hi == 0) d.from[16 * sub + lo] = __expf((float)mine), d.to[16 * sub + lo] = __expf((float)(sum - mine));
-  if (lane == 0) d.total[sub] = __expf((float)sum);
+// G_i - G_j for a lane's i = i0 + lo and j = j0 + 4 hi + r
+__device__ inline f32x4 delta_lag(const DeltaGates& d, int i0, int j0, int lane) {
+  const double mine = d.G[i0 + (lane & 15)];
+  const double* at = d.G + j0 + 4 * (lane >> 4);
   f32x4 lag;
 #pragma unroll
   for (int r = 0; r < 4; ++r) lag[r] = (float)(mine - at[r]);
   return lag;
 }
 
-// (I + A)^-1 of a block from A's rows: lane lo has A[lo][4 hi + r] in `a`, zeros from the diagonal on.
-// The rows of the inverse (or, with TRANSPOSED, its columns) go to the block's tile.
-template <typename S, bool TRANSPOSED>
-__device__ inline void delta_inverse(const DeltaGates& d, int sub, f32x4 a, int lane) {
-  const int lo = lane & 15, hi = lane >> 4;
-  float* tile = d.inv + sub * 16 * S::LDT;
-  *reinterpret_cast<f32x4*>(tile + lo * S::LDT + 4 * hi) = a;
+// (X Y^T)^T of 16 rows of each: lane lo has row y0 + lo of Y, and of X rows x0 + 4 hi + r
+template <typename E, int D>
+__device__ inline f32x4 row_products(const E* x, int x0, const E* y, int y0, int ld, int lane) {
+  f32x4 t = {0, 0, 0, 0};
+#pragma unroll
+  for (int m = 0; m < D; m += 32)
+    t = mma2(lds_quad(x, ld, x0, m, lane), lds_quad(x, ld, x0, m + 16, lane), lds_quad(y, ld, y0, m, lane),
+             lds_quad(y, ld, y0, m + 16, lane), t);
+  return t;
+}
+
+// The inverse of I + A for block `blk` of a chunk, by one wave, into its tiles at `inv`.  A_ij has
+// beta_j, or with REVERSE beta_i, and the inverse's transpose is left.
+template <typename E, typename S, int DK, bool REVERSE>
+__device__ inline void delta_inverse(const DeltaGates& d, float* inv, const E* tk, int blk, int lane) {
+  constexpr int NB = S::NB, LDT = S::LDT;
+  const int lo = lane & 15, hi = lane >> 4, r0 = blk * S::BS;
+  float* tiles = inv + blk * S::TRI * S::TILE;
+  auto a_tile = [&](int i, int j) {
+    f32x4 a = row_products<E, DK>(tk, r0 + 16 * j, tk, r0 + 16 * i, S::LDK, lane);
+    const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
+    const float bi = d.beta[r0 + 16 * i + lo];
+    const f32x4 bj = lds_f4(d.beta + r0 + 16 * j + 4 * hi);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] = i > j || 4 * hi + r < lo ? a[r] * __expf(lag[r]) * (REVERSE ? bi : bj[r]) : 0.0f;
+    return a;
+  };
+#pragma unroll
+  for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4*>(tiles + tri(i, i) * S::TILE + lo * LDT + 4 * hi) = a_tile(i, i);
+  f32x4 a10;
+  if constexpr (NB == 2) a10 = a_tile(1, 0);
   __builtin_amdgcn_wave_barrier();
-  float t[16];  // column lo of the inverse
+  float* tile = tiles + (NB == 2 && (hi & 1) ? tri(1, 1) * S::TILE : 0);  // lanes of odd hi: the other tile
+  float t[16];                                                            // column lo of its inverse
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float v = i == lo ? 1.0f : 0.0f;
 #pragma unroll
     for (int j = 0; j < i; j += 4) {
-      const f32x4 row = lds_f4(tile + i * S::LDT + j);
+      const f32x4 row = lds_f4(tile + i * LDT + j);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (j + r < i) v = fmaf(-row[r], t[j + r], v);
     }
     t[i] = v;
+    if (i % 2 == 1) asm volatile("" ::: "memory");  // not all rows' reads at once: their registers
   }
   __builtin_amdgcn_wave_barrier();
-  if constexpr (TRANSPOSED) {
-    if (hi == 0)
+  if (hi < NB) {
+    if constexpr (REVERSE) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<f32x4*>(tile + lo * S::LDT + j) = f32x4{t[j], t[j + 1], t[j + 2], t[j + 3]};
-  } else {
-    if (hi == 0)
+      for (int j = 0; j < 16; j += 4) *reinterpret_cast<f32x4*>(tile + lo * LDT + j) = f32x4{t[j], t[j + 1], t[j + 2], t[j + 3]};
+    } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) tile[j * S::LDT + lo] = t[j];
+      for (int j = 0; j < 16; ++j) tile[j * LDT + lo] = t[j];
+    }
+  }
+  if constexpr (NB == 2) {  // the corner: -T11 A10 T00
+    __builtin_amdgcn_wave_barrier();
+    const float *t00 = tiles, *t11 = tiles + tri(1, 1) * S::TILE;
+    auto rows = [&](const float* x) { return lds_f4(x + lo * LDT + 4 * hi); };
+    auto columns = [&](const float* x) { return lds_quad_t(x, LDT, 0, 0, lane); };
+    const f32x4 y = mma16(a10, REVERSE ? rows(t00) : columns(t00), f32x4{0, 0, 0, 0});
+    const f32x4 c = -mma16(REVERSE ? columns(t11) : rows(t11), y, f32x4{0, 0, 0, 0});
+    float* out = tiles + tri(1, 0) * S::TILE;
+    if constexpr (REVERSE) {
+      *reinterpret_cast<f32x4*>(out + lo * LDT + 4 * hi) = c;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) out[(4 * hi + r) * LDT + lo] = c[r];
+    }
   }
 }
+
+// A chunk's rows of one operand on their way from memory through registers to LDS, as AttnRows moves
+// them; whether they are whole pieces at 4-byte addresses is asked at run time (a variant of every kernel for
+// it would double what there is to compile).
+template <typename E, int C, int D, int THREADS>
+struct DeltaRows {
+  static constexpr int P = Elem<E>::PIECE, W = D / P, RS = THREADS / W < C ? THREADS / W : C, N = C / RS;
+  static constexpr int LD = D + AttnTile<E>::PAD;
+  static_assert(THREADS % W == 0 && C % RS == 0, "whole rows a pass");
+  piece_t<E> r[N];
+  const E* base;  // step 0
+  int64_t step;   // elements between steps
+  int width, row, c;
+  bool vec;
+
+  __device__ void init(const E* b, int64_t stride, int d, bool whole, int tid) {
+    row = tid / W, c = (tid - row * W) * P, step = stride, base = b, width = d, vec = whole;
+  }
+  // rows t0 ..., n of them live (zeros behind them)
+  __device__ void load(int t0, int n) {
+    const __amdgpu_buffer_rsrc_t rs = buffer_at(base + t0 * step);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int t = row + i * RS;
+      const unsigned at = t < n && c < width && row < RS ? (unsigned)((t * step + c) * (int64_t)sizeof(E)) : kNowhere;
+      if (vec) {
+        r[i] = __builtin_bit_cast(piece_t<E>, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+      } else {
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const unsigned ae = c + e < width && at != kNowhere ? at + e * (unsigned)sizeof(E) : kNowhere;
+          if constexpr (sizeof(E) == 4)
+            r[i][e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, ae, 0, 0));
+          else
+            r[i][e] = __builtin_bit_cast(bf16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, ae, 0, 0));
+        }
+      }
+    }
+  }
+  __device__ void store(E* tile) const {
+    if (RS * W < THREADS && row >= RS) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<piece_t<E>*>(tile + (row + i * RS) * LD + c) = r[i];
+  }
+};
 
 // x (fp32) as an operand of products whose other operand is exact in E: three bf16 terms (24
 // bits), or itself.
@@ -157,6 +270,7 @@ template <typename E>
 struct Terms {
   static constexpr int N = sizeof(E) == 2 ? 3 : 1;
   quad_t<E> t[N];
+  __device__ Terms() {}
   __device__ Terms(f32x4 x) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -165,33 +279,58 @@ struct Terms {
     }
   }
 };
-// acc += A x over 16 contracted entries, x by its terms
-__device__ inline f32x4 mma_terms(bf16x4 a, const Terms<bf16>& x, f32x4 acc) {
-  const bf16x4 zero = to_bf16(f32x4{0, 0, 0, 0});
-  acc = mma2(a, a, x.t[0], x.t[1], acc);
-  return mma2(a, zero, x.t[2], zero, acc);
-}
-__device__ inline f32x4 mma_terms(f32x4 a, const Terms<float>& x, f32x4 acc) { return mma16(a, x.t[0], acc); }
 
-// K s (rows i of the block at k: 16 x dk, the wave's 16 columns) exact to fp32, and with OT > 0
-// (Q s)^T by s's first OT terms.
-template <typename E, int KA, int OT>
-__device__ inline f32x4 delta_state_products(const E* k, const E* q, int ld, int row0, const f32x4 (&s)[KA][1], f32x4& qs,
-                                             int lane) {
-  f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+// acc += sum over NB tiles of A_i x_i, 16 contracted entries each, x by its terms
+template <int NB>
+__device__ inline f32x4 mma_terms(const bf16x4 (&a)[NB], const Terms<bf16> (&x)[NB], f32x4 acc) {
+  static_assert(NB == 2, "pairs");
+#pragma unroll
+  for (int t = 0; t < 3; ++t) acc = mma2(a[0], a[1], x[0].t[t], x[1].t[t], acc);
+  return acc;
+}
+template <int NB>
+__device__ inline f32x4 mma_terms(const f32x4 (&a)[NB], const Terms<float> (&x)[NB], f32x4 acc) {
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc = mma16(a[i], x[i].t[0], acc);
+  return acc;
+}
+
+// For the block's tiles i: K_i s (16 rows, the wave's 16 columns) exact to fp32, and with OT > 0
+// (Q_i s)^T by s's first OT terms.
+template <typename E, typename S, int KA, int OT>
+__device__ inline void delta_state_products(const E* k, const E* q, int row0, const f32x4 (&s)[KA][1], f32x4 (&ks)[S::NB],
+                                            f32x4 (&qs)[S::NB], int lane) {
+#pragma unroll
+  for (int i = 0; i < S::NB; ++i) ks[i] = qs[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
   for (int m = 0; m < KA; m += 2) {
-    const quad_t<E> k0 = lds_quad(k, ld, row0, 16 * m, lane), k1 = lds_quad(k, ld, row0, 16 * m + 16, lane);
-    quad_t<E> q0, q1;
-    if constexpr (OT > 0) q0 = lds_quad(q, ld, row0, 16 * m, lane), q1 = lds_quad(q, ld, row0, 16 * m + 16, lane);
     const Terms<E> a(s[m][0]), b(s[m + 1][0]);
 #pragma unroll
-    for (int t = 0; t < Terms<E>::N; ++t) {
-      x[t & 1] = mma2(k0, k1, a.t[t], b.t[t], x[t & 1]);
-      if (t < OT) qs = mma2(a.t[t], b.t[t], q0, q1, qs);
+    for (int i = 0; i < S::NB; ++i) {
+      const int r0 = row0 + 16 * i;
+      const quad_t<E> k0 = lds_quad(k, S::LDK, r0, 16 * m, lane), k1 = lds_quad(k, S::LDK, r0, 16 * m + 16, lane);
+#pragma unroll
+      for (int t = 0; t < Terms<E>::N; ++t) ks[i] = mma2(k0, k1, a.t[t], b.t[t], ks[i]);
+      if constexpr (OT > 0) {
+        const quad_t<E> q0 = lds_quad(q, S::LDK, r0, 16 * m, lane), q1 = lds_quad(q, S::LDK, r0, 16 * m + 16, lane);
+#pragma unroll
+        for (int t = 0; t < OT; ++t) qs[i] = mma2(a.t[t], b.t[t], q0, q1, qs[i]);
+      }
     }
   }
-  return x[0] + x[1];
+}
+
+// e = (I + A)^-1 x over the block's tiles, from the inverse's tiles or with REVERSE its transpose's
+template <typename S, bool REVERSE>
+__device__ inline void delta_solve(const float* tiles, const f32x4 (&x)[S::NB], f32x4 (&e)[S::NB], int lane) {
+  const float* at = tiles + (lane & 15) * S::LDT + 4 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < S::NB; ++i) {
+    e[i] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j)
+      if (REVERSE ? j >= i : j <= i) e[i] = mma16(lds_f4(at + (REVERSE ? tri(j, i) : tri(i, j)) * S::TILE), x[j], e[i]);
+  }
 }
 
 // A wave's columns of a history whose state is not finite in the end, by the definition, a step at
@@ -239,109 +378,141 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
 template <typename E, int DK, int DV>
 constexpr size_t delta_forward_lds() {
   using S = DeltaShape<E, DK, DV>;
-  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (2 * S::C * S::LDK + S::C * S::LDV + S::SUB * 16 * S::LDP);
+  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::SCORES + 2 * S::C * S::LDK + S::C * S::LDV);
 }
 
 // A workgroup a (problem, head).
-template <typename E, int DK, int DV, bool VEC>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_forward_kernel(DeltaArgs<E> p) {
+template <typename E, int DK, int DV>
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_forward_kernel(
+    DeltaArgs<E> p) {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, SUB = S::SUB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, LDP = S::LDP;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP;
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
   const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
   const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const DeltaGates d = delta_gates<S>(reinterpret_cast<float*>(smem));
-  E* tk = reinterpret_cast<E*>(d.inv + S::INV);
+  const DeltaGates d = delta_gates<S>(smem);
+  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
+  E* tp = reinterpret_cast<E*>(inv + S::INV);  // the blocks' scores
+  E* tk = tp + S::SCORES;
   E* tq = tk + C * LDK;
   E* tv = tq + C * LDK;
-  E* tp = tv + C * LDV;  // the blocks' scores, pitch LDP
 
-  AttnRows<E, C, DK, S::THREADS, VEC> rk, rq;
-  AttnRows<E, C, DV, S::THREADS, VEC> rv;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], 0, p.dk, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], 0, p.dk, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], 0, p.dv, tid);
-  DeltaGateRows<E, C> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+  DeltaRows<E, C, DK, S::THREADS> rk, rq;
+  DeltaRows<E, C, DV, S::THREADS> rv;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
+  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
   auto fetch = [&](int t0) {
-    rk.load(L - t0, p.dk), rq.load(L - t0, p.dk), rv.load(L - t0, p.dv), rg.load(t0, L - t0, tid);
+    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rg.load(t0, L - t0, tid);
   };
   if (L > 0) fetch(0);
-  const int64_t size = (int64_t)p.dk * p.dv;
   f32x4 s[KA][1];
-  load_state(s, p.s_in ? p.s_in + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
+  load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
   const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
   const int oc = col0 + 4 * hi;
+  const unsigned ooff = oc < p.dv ? (unsigned)((lo * orow + oc) * sizeof(E)) : kNowhere;
+  const unsigned otile = (unsigned)(16 * orow * sizeof(E));
 
   for (int t0 = 0; t0 < L; t0 += C) {
     const int n = min(C, L - t0);
     rk.store(tk), rq.store(tq), rv.store(tv), rg.store(d, tid);
     __syncthreads();
-    if (t0 + C < L) fetch(t0 + C);
-    for (int sub = wave; 16 * sub < n; sub += S::W) {
-      const f32x4 lag = delta_powers<S>(d, sub, lane);
-      f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
-#pragma unroll
-      for (int m = 0; m < KA; m += 2) {
-        const quad_t<E> k0 = lds_quad(tk, LDK, 16 * sub, 16 * m, lane), k1 = lds_quad(tk, LDK, 16 * sub, 16 * m + 16, lane);
-        kk = mma2(k0, k1, k0, k1, kk);
-        qk = mma2(k0, k1, lds_quad(tq, LDK, 16 * sub, 16 * m, lane), lds_quad(tq, LDK, 16 * sub, 16 * m + 16, lane), qk);
+    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
+      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+      if (r0 >= n) continue;
+      if (task < S::NBLK) {
+        delta_inverse<E, S, DK, false>(d, inv, tk, blk, lane);
+        continue;
       }
-      const f32x4 beta = lds_f4(d.beta + 16 * sub + 4 * hi);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = 4 * hi + r;
-        kk[r] = j < lo ? kk[r] * __expf(lag[r]) * beta[r] : 0.0f;
-        qk[r] = j <= lo ? p.scale * (qk[r] * __expf(lag[r])) : 0.0f;
-      }
-      *reinterpret_cast<quad_t<E>*>(tp + (16 * sub + lo) * LDP + 4 * hi) = to_quad<E>(qk);
-      delta_inverse<S, false>(d, sub, kk, lane);
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j) {
+          f32x4 x = row_products<E, DK>(tk, r0 + 16 * j, tq, r0 + 16 * i, LDK, lane);
+          const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r <= lo ? p.scale * (x[r] * __expf(lag[r])) : 0.0f;
+          *reinterpret_cast<quad_t<E>*>(tp + (blk * S::TRI + tri(i, j)) * S::TILE_P + lo * LDP + 4 * hi) = to_quad<E>(x);
+        }
     }
     __syncthreads();
-    for (int sub = 0; 16 * sub < n; ++sub) {
-      f32x4 o = {0, 0, 0, 0};
-      const f32x4 ks = delta_state_products<E, KA, 1>(tk, tq, LDK, 16 * sub, s, o, lane);
-      const f32x4 v = to_f32(lds_quad_t(tv, LDV, 16 * sub, col0, lane));
-      const f32x4 x = v - lds_f4(d.from + 16 * sub + 4 * hi) * ks;
-      const f32x4 u = lds_f4(d.beta + 16 * sub + 4 * hi) * mma16(lds_f4(d.inv + (16 * sub + lo) * LDT + 4 * hi), x, f32x4{0, 0, 0, 0});
-      o *= p.scale * d.from[16 * sub + lo];
-      const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(tp + (16 * sub + lo) * LDP + 4 * hi);
-      if constexpr (sizeof(E) == 2) {
-        const bf16x4 uh = to_bf16(u);
-        o = mma2(uh, to_bf16(u - to_f32(uh)), pq, pq, o);
-      } else {
-        o = mma16(u, pq, o);
+    if (t0 + C < L) fetch(t0 + C);
+    const __amdgpu_buffer_rsrc_t rs = buffer_at(p.o + obase + t0 * orow);
+#pragma unroll 1
+    for (int blk = 0; blk * S::BS < n; ++blk) {
+      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
+      f32x4 o[NB], x[NB], u[NB];
+      delta_state_products<E, S, KA, 1>(tk, tq, r0, s, x, o, lane);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        x[i] = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane)) - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
+      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
+      Terms<E> w[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        u[i] *= lds_f4(d.beta + r0 + 16 * i + 4 * hi);
+        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * u[i]);
       }
-      const int t = t0 + 16 * sub + lo;
-      if (t < L) {
-        E* row = p.o + obase + t * orow;
-        if (VEC) {
-          if (oc < p.dv) *reinterpret_cast<quad_t<E>*>(row + oc) = to_quad<E>(o);
+      const float total = d.total[blk];
+#pragma unroll
+      for (int m = 0; m < KA; ++m) {
+        quad_t<E> kt[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
+        s[m][0] = mma_terms(kt, w, s[m][0] * total);
+      }
+      // outputs; the scores are rounded to E, u is by two terms
+      quad_t<E> uh[NB], ul[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) uh[i] = to_quad<E>(u[i]), ul[i] = to_quad<E>(u[i] - to_f32(uh[i]));
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        o[i] *= p.scale * d.from[r0 + 16 * i + lo];
+        const E* pt = tp + (blk * S::TRI + tri(i, 0)) * S::TILE_P + lo * LDP + 4 * hi;
+#pragma unroll
+        for (int j = 0; j <= i; ++j) {
+          const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(pt + j * S::TILE_P);
+          if constexpr (sizeof(E) == 2) o[i] = mma2(uh[j], ul[j], pq, pq, o[i]);
+          else o[i] = mma16(u[j], pq, o[i]);
+        }
+        const unsigned at = r0 + 16 * i + lo < n && ooff != kNowhere ? ooff + (blk * NB + i) * otile : kNowhere;
+        if (p.vec) {
+          if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i]), rs, at, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, to_bf16(o[i])), rs, at, 0, 0);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (oc + e < p.dv) row[oc + e] = (E)o[e];
+          for (int e = 0; e < 4; ++e) {
+            const unsigned ae = oc + e < p.dv && at != kNowhere ? at + e * (unsigned)sizeof(E) : kNowhere;
+            const float f = o[i][e];
+            if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f), rs, ae, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (bf16)f), rs, ae, 0, 0);
+          }
         }
       }
-      const Terms<E> w(lds_f4(d.to + 16 * sub + 4 * hi) * u);
-      const float total = d.total[sub];
-#pragma unroll
-      for (int m = 0; m < KA; ++m) s[m][0] = mma_terms(lds_quad_t(tk, LDK, 16 * sub, 16 * m, lane), w, s[m][0] * total);
     }
     __syncthreads();
   }
-  zero_rows(p.o, false, sizeof(E), obase, orow, p.dv, L, p.T, tid, S::THREADS);
+  // What follows makes its indexes and reads its arguments again: they would be kept through every chunk.
+  auto* args = __builtin_amdgcn_kernarg_segment_ptr();
+  int etid = tid, ebh = bh;
+  asm volatile("" : "+v"(etid), "+s"(args), "+s"(ebh));
+  const DeltaArgs<E>& a = *(const DeltaArgs<E>*)args;
+  const int eb = ebh / a.H, eL = a.lengths ? min(max(a.lengths[eb], 0), a.T) : a.T;
+  zero_rows(a.o, false, sizeof(E), ((int64_t)eb * a.T * a.H + (ebh - eb * a.H)) * a.dv, (int64_t)a.H * a.dv, a.dv, eL, a.T, etid,
+            S::THREADS);
   // An infinite or NaN value leaves the state so, to the end.
   f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
   for (int m = 0; m < KA; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][0][r], 0.0f, zero[r]);
-  if (L > 0 && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
+  if (eL > 0 && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
     __threadfence_block();  // rows written above are written again
-    delta_by_step<E, KA>(p, bh, tid);
-  } else if (p.s_out) {
-    store_state(s, p.s_out + bh * size, p.dk, p.dv, col0, lo, hi);
+    delta_by_step<E, KA>(a, ebh, etid);
+  } else if (a.s_out) {
+    store_state(s, a.s_out + ebh * ((int64_t)a.dk * a.dv), a.dk, a.dv, (etid >> 6) * 16, etid & 15, (etid & 63) >> 4);
   }
 }
 
@@ -422,32 +593,34 @@ constexpr size_t delta_states_lds() {
   return sizeof(float) * (S::GATES + 2 * S::INV + S::W * S::C) + sizeof(E) * (2 * S::C * S::LDK + 2 * S::C * S::LDV);
 }
 
-template <typename E, int DK, int DV, bool VEC>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_states_kernel(DeltaBwdArgs<E> a) {
+template <typename E, int DK, int DV>
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_states_kernel(
+    DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, SEG = kDeltaSeg / C;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, SEG = kDeltaSeg / C;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
   const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
   const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const DeltaGates d = delta_gates<S>(reinterpret_cast<float*>(smem));
-  float* tp = d.inv + S::INV;  // the blocks' scores
-  float* sums = tp + S::INV;   // (waves, steps)
+  const DeltaGates d = delta_gates<S>(smem);
+  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
+  float* tp = inv + S::INV;   // the blocks' scores
+  float* sums = tp + S::INV;  // (waves, steps)
   E* tk = reinterpret_cast<E*>(sums + S::W * C);
   E* tq = tk + C * LDK;
   E* tv = tq + C * LDK;
   E* tdo = tv + C * LDV;
 
-  AttnRows<E, C, DK, S::THREADS, VEC> rk, rq;
-  AttnRows<E, C, DV, S::THREADS, VEC> rv, rdo;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], 0, p.dk, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], 0, p.dk, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], 0, p.dv, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], 0, p.dv, tid);
-  DeltaGateRows<E, C> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+  DeltaRows<E, C, DK, S::THREADS> rk, rq;
+  DeltaRows<E, C, DV, S::THREADS> rv, rdo;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
+  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
+  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
   auto fetch = [&](int t0) {
-    rk.load(L - t0, p.dk), rq.load(L - t0, p.dk), rv.load(L - t0, p.dv), rdo.load(L - t0, p.dv), rg.load(t0, L - t0, tid);
+    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), rg.load(t0, L - t0, tid);
   };
   if (L > 0) fetch(0);
   f32x4 s[KA][1];
@@ -458,47 +631,63 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_states
     rk.store(tk), rq.store(tq), rv.store(tv), rdo.store(tdo), rg.store(d, tid);
     store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + chunk) * DK * DV, s, col0, lo, hi);
     __syncthreads();
-    if (t0 + C < L) fetch(t0 + C);
-    for (int sub = wave; 16 * sub < n; sub += S::W) {
-      const f32x4 lag = delta_powers<S>(d, sub, lane);
-      f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
-#pragma unroll
-      for (int m = 0; m < KA; m += 2) {
-        const quad_t<E> k0 = lds_quad(tk, LDK, 16 * sub, 16 * m, lane), k1 = lds_quad(tk, LDK, 16 * sub, 16 * m + 16, lane);
-        kk = mma2(k0, k1, k0, k1, kk);
-        qk = mma2(k0, k1, lds_quad(tq, LDK, 16 * sub, 16 * m, lane), lds_quad(tq, LDK, 16 * sub, 16 * m + 16, lane), qk);
+    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
+      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+      if (r0 >= n) continue;
+      if (task < S::NBLK) {
+        delta_inverse<E, S, DK, false>(d, inv, tk, blk, lane);
+        continue;
       }
-      const f32x4 beta = lds_f4(d.beta + 16 * sub + 4 * hi);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = 4 * hi + r;
-        kk[r] = j < lo ? kk[r] * __expf(lag[r]) * beta[r] : 0.0f;
-        qk[r] = j <= lo ? p.scale * (qk[r] * __expf(lag[r])) : 0.0f;
-      }
-      *reinterpret_cast<f32x4*>(tp + (16 * sub + lo) * LDT + 4 * hi) = qk;
-      delta_inverse<S, false>(d, sub, kk, lane);
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j) {
+          f32x4 x = row_products<E, DK>(tk, r0 + 16 * j, tq, r0 + 16 * i, LDK, lane);
+          const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r <= lo ? p.scale * (x[r] * __expf(lag[r])) : 0.0f;
+          *reinterpret_cast<f32x4*>(tp + (blk * S::TRI + tri(i, j)) * S::TILE + lo * LDT + 4 * hi) = x;
+        }
     }
     __syncthreads();
-    for (int sub = 0; 16 * sub < n; ++sub) {
-      f32x4 o = {0, 0, 0, 0};
-      const f32x4 ks = delta_state_products<E, KA, Terms<E>::N>(tk, tq, LDK, 16 * sub, s, o, lane);
-      const f32x4 v = to_f32(lds_quad_t(tv, LDV, 16 * sub, col0, lane));
-      const f32x4 x = v - lds_f4(d.from + 16 * sub + 4 * hi) * ks;
-      const f32x4 e = mma16(lds_f4(d.inv + (16 * sub + lo) * LDT + 4 * hi), x, f32x4{0, 0, 0, 0});
-      const f32x4 u = lds_f4(d.beta + 16 * sub + 4 * hi) * e;
-      // these columns of V are this wave's alone and have been read
+    if (t0 + C < L) fetch(t0 + C);
+#pragma unroll 1
+    for (int blk = 0; blk * S::BS < n; ++blk) {
+      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
+      f32x4 o[NB], x[NB], u[NB];
+      delta_state_products<E, S, KA, Terms<E>::N>(tk, tq, r0, s, x, o, lane);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tv[(16 * sub + 4 * hi + r) * LDV + col0 + lo] = (E)e[r];
-      o *= p.scale * d.from[16 * sub + lo];
-      o = mma16(u, lds_f4(tp + (16 * sub + lo) * LDT + 4 * hi), o);
-      o *= to_f32(lds_quad(tdo, LDV, 16 * sub, col0, lane));
-      float w = o[0] + o[1] + o[2] + o[3];
-      w += __shfl_xor(w, 16, 64), w += __shfl_xor(w, 32, 64);
-      if (hi == 0) sums[wave * C + 16 * sub + lo] = w;
-      const Terms<E> du(lds_f4(d.to + 16 * sub + 4 * hi) * u);
-      const float total = d.total[sub];
+      for (int i = 0; i < NB; ++i)
+        x[i] = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane)) - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
+      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
+      Terms<E> w[NB];
 #pragma unroll
-      for (int m = 0; m < KA; ++m) s[m][0] = mma_terms(lds_quad_t(tk, LDK, 16 * sub, 16 * m, lane), du, s[m][0] * total);
+      for (int i = 0; i < NB; ++i) {
+        // these columns of V are this wave's alone and have been read: e takes their place
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tv[(r0 + 16 * i + 4 * hi + r) * LDV + col0 + lo] = (E)u[i][r];
+        u[i] *= lds_f4(d.beta + r0 + 16 * i + 4 * hi);
+        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * u[i]);
+      }
+      const float total = d.total[blk];
+#pragma unroll
+      for (int m = 0; m < KA; ++m) {
+        quad_t<E> kt[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
+        s[m][0] = mma_terms(kt, w, s[m][0] * total);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        o[i] *= p.scale * d.from[r0 + 16 * i + lo];
+#pragma unroll
+        for (int j = 0; j <= i; ++j)
+          o[i] = mma16(u[j], lds_f4(tp + (blk * S::TRI + tri(i, j)) * S::TILE + lo * LDT + 4 * hi), o[i]);
+        o[i] *= to_f32(lds_quad(tdo, LDV, r0 + 16 * i, col0, lane));
+        float w1 = o[i][0] + o[i][1] + o[i][2] + o[i][3];
+        w1 += __shfl_xor(w1, 16, 64), w1 += __shfl_xor(w1, 32, 64);
+        if (hi == 0) sums[wave * C + r0 + 16 * i + lo] = w1;
+      }
     }
     if ((chunk + 1) % SEG == 0 || t0 + C >= L) {
       f32x4* dst = reinterpret_cast<f32x4*>(a.s_seg + ((int64_t)bh * a.segs + chunk / SEG) * DK * DV) + wave * KA * 64 + lane;
@@ -519,43 +708,44 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_states
 template <typename E, int DK, int DV>
 constexpr size_t delta_reverse_lds() {
   using S = DeltaShape<E, DK, DV>;
-  return sizeof(float) * (S::GATES + 2 * S::INV + 2 * S::W * S::C + 8) + sizeof(E) * (2 * S::C * S::LDK + 3 * S::C * S::LDV);
+  return sizeof(float) * (S::GATES + S::INV + 2 * S::W * S::C + 8) +
+         sizeof(E) * (Terms<E>::N * S::SCORES + 2 * S::C * S::LDK + 3 * S::C * S::LDV);
 }
 
-template <typename E, int DK, int DV, bool VEC>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_reverse_kernel(DeltaBwdArgs<E> a) {
+template <typename E, int DK, int DV>
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
+    DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, SEG = kDeltaSeg / C;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP, SEG = kDeltaSeg / C;
+  constexpr int TERMS = Terms<E>::N;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
   const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
   const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-  const DeltaGates d = delta_gates<S>(reinterpret_cast<float*>(smem));
-  float* tp = d.inv + S::INV;         // the blocks' scores, transposed
-  float* sum_beta = tp + S::INV;      // (waves, steps)
+  const DeltaGates d = delta_gates<S>(smem);
+  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
+  float* sum_beta = inv + S::INV;     // (waves, steps)
   float* sum_z = sum_beta + S::W * C;
   float* sum_dot = sum_z + S::W * C;  // (waves)
-  E* tk = reinterpret_cast<E*>(sum_dot + 8);
+  E* tp = reinterpret_cast<E*>(sum_dot + 8);  // the blocks' scores, transposed, by their terms
+  E* tk = tp + TERMS * S::SCORES;
   E* tq = tk + C * LDK;
   E* tv = tq + C * LDK;
   E* tdo = tv + C * LDV;
   E* te = tdo + C * LDV;
 
-  AttnRows<E, C, DK, S::THREADS, VEC> rk, rq;
-  AttnRows<E, C, DV, S::THREADS, VEC> rv, rdo;
-  AttnRows<E, C, DV, S::THREADS, true> re;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], 0, p.dk, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], 0, p.dk, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], 0, p.dv, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], 0, p.dv, tid);
-  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, 0, DV, tid);
-  const E *bk = rk.base, *bq = rq.base, *bv = rv.base, *bdo = rdo.base, *be = re.base;
-  DeltaGateRows<E, C> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+  DeltaRows<E, C, DK, S::THREADS> rk, rq;
+  DeltaRows<E, C, DV, S::THREADS> rv, rdo;
+  DeltaRows<E, C, DV, S::THREADS> re;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
+  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
+  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid);
+  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
   auto fetch = [&](int t0) {
-    rk.base = bk + t0 * p.ks[1], rq.base = bq + t0 * p.qs[1], rv.base = bv + t0 * p.vs[1];
-    rdo.base = bdo + t0 * a.dos[1], re.base = be + (int64_t)t0 * DV;
-    rk.load(L - t0, p.dk), rq.load(L - t0, p.dk), rv.load(L - t0, p.dv), rdo.load(L - t0, p.dv), re.load(L - t0, DV);
+    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), re.load(t0, L - t0);
     rg.load(t0, L - t0, tid);
   };
   const int last = L > 0 ? (L - 1) / C : -1;
@@ -589,58 +779,80 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS)) void delta_revers
       for (int i = 0; i < S::W; ++i) dot += sum_dot[i];
       a.dot[(int64_t)bh * a.segs + chunk / SEG] = dot;
     }
-    if (chunk > 0) fetch(t0 - C);
-    for (int sub = wave; 16 * sub < n; sub += S::W) {
-      const f32x4 lag = delta_powers<S>(d, sub, lane);
-      f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
-#pragma unroll
-      for (int m = 0; m < KA; m += 2) {
-        const quad_t<E> k0 = lds_quad(tk, LDK, 16 * sub, 16 * m, lane), k1 = lds_quad(tk, LDK, 16 * sub, 16 * m + 16, lane);
-        kk = mma2(k0, k1, k0, k1, kk);
-        qk = mma2(lds_quad(tq, LDK, 16 * sub, 16 * m, lane), lds_quad(tq, LDK, 16 * sub, 16 * m + 16, lane), k0, k1, qk);
+    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
+      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+      if (r0 >= n) continue;
+      if (task < S::NBLK) {
+        delta_inverse<E, S, DK, true>(d, inv, tk, blk, lane);
+        continue;
       }
-      const float beta = d.beta[16 * sub + lo];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int x = 4 * hi + r;
-        kk[r] = x < lo ? kk[r] * __expf(lag[r]) * beta : 0.0f;
-        qk[r] = x >= lo ? p.scale * (qk[r] * __expf(-lag[r])) : 0.0f;  // row lo is the key's
-      }
-      *reinterpret_cast<f32x4*>(tp + (16 * sub + lo) * LDT + 4 * hi) = qk;
-      delta_inverse<S, true>(d, sub, kk, lane);
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j <= i; ++j) {  // lane lo has the key's row
+          f32x4 x = row_products<E, DK>(tq, r0 + 16 * i, tk, r0 + 16 * j, LDK, lane);
+          const f32x4 lag = delta_lag(d, r0 + 16 * j, r0 + 16 * i, lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r >= lo ? p.scale * (x[r] * __expf(-lag[r])) : 0.0f;
+          const Terms<E> terms(x);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+            *reinterpret_cast<quad_t<E>*>(tp + ((blk * S::TRI + tri(i, j)) * TERMS + t) * S::TILE_P + lo * LDP + 4 * hi) = terms.t[t];
+        }
     }
     __syncthreads();
-    for (int sub = (n - 1) / 16; sub >= 0; --sub) {
-      f32x4 none;
-      const f32x4 from = lds_f4(d.from + 16 * sub + 4 * hi);
-      const f32x4 g = to_f32(lds_quad_t(tdo, LDV, 16 * sub, col0, lane));
-      f32x4 x = lds_f4(d.to + 16 * sub + 4 * hi) * delta_state_products<E, KA, 0>(tk, tq, LDK, 16 * sub, s, none, lane);
-      x = mma16(lds_f4(tp + (16 * sub + lo) * LDT + 4 * hi), g, x);
-      const f32x4 du = mma16(lds_f4(d.inv + (16 * sub + lo) * LDT + 4 * hi), x, f32x4{0, 0, 0, 0});
-      const f32x4 y = lds_f4(d.beta + 16 * sub + 4 * hi) * du;
-      const f32x4 pe = du * to_f32(lds_quad_t(te, LDV, 16 * sub, col0, lane));
-      const f32x4 pv = y * to_f32(lds_quad_t(tv, LDV, 16 * sub, col0, lane));
+    if (chunk > 0) fetch(t0 - C);
+#pragma unroll 1
+    for (int blk = (n - 1) / S::BS; blk >= 0; --blk) {
+      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
+      f32x4 x[NB], du[NB], none[NB];
+      delta_state_products<E, S, KA, 0>(tk, tq, r0, s, x, none, lane);
+      quad_t<E> g[NB];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * sub + 4 * hi + r;
-        const float sb = row16_sum(pe[r]), sz = row16_sum(pv[r]);
-        if (lo == 0) sum_beta[wave * C + t] = sb, sum_z[wave * C + t] = sz;
-        tdo[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
-        if (a.y_part && t < n && col0 + lo < p.dv)
-          a.y_part[(((int64_t)b * p.T + t0 + t) * p.H + h) * p.dv + col0 + lo] = y[r];
+      for (int i = 0; i < NB; ++i) {
+        g[i] = lds_quad_t(tdo, LDV, r0 + 16 * i, col0, lane);
+        x[i] *= lds_f4(d.to + r0 + 16 * i + 4 * hi);
       }
-      const Terms<E> wq(p.scale * from * g), wk(-(from * y));
-      const float total = d.total[sub];
+      const E* pt = tp + blk * S::TRI * TERMS * S::TILE_P + lo * LDP + 4 * hi;
+      auto score = [&](int i, int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * TERMS + t) * S::TILE_P); };
+      if constexpr (NB == 2) {
+        const quad_t<E> zero = to_quad<E>(f32x4{0, 0, 0, 0});
+#pragma unroll
+        for (int t = 0; t < 3; ++t) x[0] = mma2(score(0, 0, t), score(1, 0, t), g[0], g[1], x[0]);
+        x[1] = mma2(score(1, 1, 0), score(1, 1, 1), g[1], g[1], x[1]);
+        x[1] = mma2(score(1, 1, 2), zero, g[1], zero, x[1]);
+      } else {
+        x[0] = mma16(score(0, 0, 0), g[0], x[0]);
+      }
+      delta_solve<S, true>(inv + blk * S::TRI * S::TILE, x, du, lane);
+      Terms<E> wq[NB], wk[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const f32x4 from = lds_f4(d.from + r0 + 16 * i + 4 * hi);
+        const f32x4 y = lds_f4(d.beta + r0 + 16 * i + 4 * hi) * du[i];
+        const f32x4 pe = du[i] * to_f32(lds_quad_t(te, LDV, r0 + 16 * i, col0, lane));
+        const f32x4 pv = y * to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane));
+        wq[i] = Terms<E>(p.scale * from * to_f32(g[i])), wk[i] = Terms<E>(-(from * y));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = r0 + 16 * i + 4 * hi + r;
+          const float sb = row16_sum(pe[r]), sz = row16_sum(pv[r]);
+          if (lo == 0) sum_beta[wave * C + t] = sb, sum_z[wave * C + t] = sz;
+          tdo[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
+          if (a.y_part && t < n && col0 + lo < p.dv)
+            a.y_part[(((int64_t)b * p.T + t0 + t) * p.H + h) * p.dv + col0 + lo] = y[r];
+        }
+      }
+      const float total = d.total[blk];
 #pragma unroll
       for (int m = 0; m < KA; ++m) {
-        const quad_t<E> qt = lds_quad_t(tq, LDK, 16 * sub, 16 * m, lane), kt = lds_quad_t(tk, LDK, 16 * sub, 16 * m, lane);
-        s[m][0] *= total;
-        if constexpr (sizeof(E) == 2) {
+        quad_t<E> qt[NB], kt[NB];
 #pragma unroll
-          for (int t = 0; t < 3; ++t) s[m][0] = mma2(qt, kt, wq.t[t], wk.t[t], s[m][0]);
-        } else {
-          s[m][0] = mma16(kt, wk.t[0], mma16(qt, wq.t[0], s[m][0]));
+        for (int i = 0; i < NB; ++i) {
+          qt[i] = lds_quad_t(tq, LDK, r0 + 16 * i, 16 * m, lane);
+          kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
         }
+        s[m][0] = mma_terms(kt, wk, mma_terms(qt, wq, s[m][0] * total));
       }
     }
     __syncthreads();
@@ -699,7 +911,7 @@ constexpr size_t delta_dqk_lds() {
 }
 
 // dq and dk of a chunk: a wave 16 rows (and with fp32 chunks of 32 steps half of the columns).
-template <typename E, int DK, int DV, bool VEC>
+template <typename E, int DK, int DV>
 __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
   constexpr int C = S::C, CT = C / 16, WC = 4 / CT, KT = DK / 16 / WC, VA = DV / 16, LDK = S::LDK, LDV = S::LDV;
@@ -725,20 +937,14 @@ __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   E* ty = tdo + C * LDV;
   E* ts = ty + C * LDV;  // a state or its gradient, (DV, DK)
 
-  AttnRows<E, C, DK, 256, VEC> rk, rq;
-  AttnRows<E, C, DV, 256, VEC> rdo;
-  AttnRows<E, C, DV, 256, true> re;
-  AttnRows<E, C, DV, 256, false> ry;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], t0, p.dk, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], t0, p.dk, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], t0, p.dv, tid);
-  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, t0, DV, tid);
-  const E* y = a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv);
-  rk.load(n, p.dk), rq.load(n, p.dk), rdo.load(n, p.dv), re.load(n, DV);
-  AttnRows<E, C, DV, 256, true> ryv;
-  const bool yv = a.y_part || (VEC && p.dv % Elem<E>::PIECE == 0);
-  if (yv) ryv.init(y, a.ys[1], t0, a.y_width, tid), ryv.load(n, a.y_width);
-  else ry.init(y, a.ys[1], t0, a.y_width, tid), ry.load(n, a.y_width);
+  DeltaRows<E, C, DK, 256> rk, rq;
+  DeltaRows<E, C, DV, 256> rdo, re, ry;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
+  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid);
+  ry.init(a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv), a.ys[1], a.y_width, a.y_part || p.vec, tid);
+  rk.load(t0, n), rq.load(t0, n), rdo.load(t0, n), re.load(t0, n), ry.load(t0, n);
   // rows of the state: DV of DK elements, whole pieces
   constexpr int P = Elem<E>::PIECE, SP = (DV * DK / P + 255) / 256;
   piece_t<E> sp[SP];
@@ -773,8 +979,7 @@ __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
     }
   }
   rk.store(tk), rq.store(tq), rdo.store(tdo);
-  if (yv) ryv.store(ty);
-  else ry.store(ty);
+  ry.store(ty);
   state_store();
   __syncthreads();
 #pragma unroll
