@@ -49,6 +49,37 @@ def test_gradients_over_several_stretches(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 1100, (1, 1, 1, 1), 32, 48), (1, 1300, (2, 1, 2, 2), 64, 40), (3, 1030, (1, 1, 1, 1), 20, 100)],
+                         ids=SHAPE_IDS)
+def test_long_histories_in_runs(shape, dtype):
+    """Few heads of many steps: cut into runs, forwards and backwards, ragged (a run that is not reached, one
+    that ends inside, lengths of zero and one)."""
+    B, T = shape[:2]
+    check(inputs(*shape, dtype, seed=109))
+    x = inputs(*shape, dtype, seed=110, lengths=[T - 300, 1, 0][:B] if B != 2 else [513, T])
+    want = check(x)
+    for b, L in enumerate(x["lengths"].tolist()):
+        for n in ("o", "dq", "dk", "dv", "dg", "dbeta"):
+            assert not bool(want[n][b, L:].any()), n
+
+
+def test_spoiled_values_in_runs():
+    """A value that is not finite in one run of several: earlier runs' outputs stay, later ones are spoiled."""
+    x = inputs(1, 1300, (2, 2, 2, 2), 32, 32, torch.float32, seed=111)
+    with torch.no_grad():
+        o, s = learning.delta_attention(*(x[n] for n in NAMES))
+        for n in ("k", "v"):
+            y = dict(x, **{n: x[n].clone()})
+            y[n][0, 700, 1, 3] = float("nan")
+            po, ps = learning.delta_attention(*(y[m] for m in NAMES))
+            assert torch.equal(po[:, :, 0], o[:, :, 0]) and torch.equal(ps[:, 0], s[:, 0])
+            want = ref.delta(*(x[m][:, :700] for m in NAMES[:5]), x["state"])["o"]
+            ref.assert_within(n, po[:, :700], want, 2)
+            cols = slice(3, 4) if n == "v" else slice(None)
+            assert bool(torch.isnan(po[0, 700:, 1, cols]).all()) and bool(torch.isnan(ps[0, 1, :, cols]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_ragged_gradients(dtype):
     x = inputs(len(LENGTHS), 90, (4, 4, 2, 2), 33, 40, dtype, seed=102, lengths=LENGTHS)
     want = check(x)

@@ -64,6 +64,38 @@ bool vec_ok(const DeltaArgs<E>& p) {
   return rows_ok(p.q, p.qs, p.dk) && rows_ok(p.k, p.ks, p.dk) && rows_ok(p.v, p.vs, p.dv) && ((uintptr_t)p.o & 15) == 0;
 }
 
+// How a history is cut into runs, and their arrays in the workspace.  (Both passes' runs: see below.)
+struct RunPlan {
+  int segs, len;
+  size_t state, map;  // bytes of a head's states and maps of all runs, of all heads
+};
+inline int tile_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+inline RunPlan run_plan(const tmpc_delta_attention* x) {
+  const int64_t bh = std::max<int64_t>(1, (int64_t)x->B * x->H), stretches = std::max<int64_t>(1, ceil_div(x->T, kDeltaSeg));
+  const int64_t fill = 2 * kCUs / bh;
+  int64_t want = std::min(fill, stretches);
+  while (want > 8 && want * want > 40 * stretches) --want;
+  if (want < 4) want = 1;
+  const int64_t len = ceil_div(stretches, want);
+  RunPlan p{(int)ceil_div(stretches, len), (int)(len * kDeltaSeg), 0, 0};
+  if (p.segs > 1) {
+    const size_t DK = tile_width(x->dk), DV = tile_width(x->dv), n = (size_t)x->B * x->H * p.segs * sizeof(float);
+    p.state = align_up(n * DK * DV), p.map = align_up(n * DK * DK);
+  }
+  return p;
+}
+// the runs' starts, from the pass before the outputs'
+template <typename E, int DK>
+void launch_runs(hipStream_t st, const DeltaArgs<E>& p, int DV) {
+  const int64_t bh = (int64_t)p.B * p.H;
+  constexpr size_t lds = delta_run_lds<E, DK>();
+  auto k = delta_run_kernel<E, DK>;
+  lds_optin(k, lds);
+  hipLaunchKernelGGL(k, dim3((unsigned)(bh * p.segs), (unsigned)ceil_div(DV + DK, 64)), dim3(256), lds, st, p, DV);
+  hipLaunchKernelGGL((delta_scan_kernel<DK, false>), dim3((unsigned)(bh * (DV / 16))), dim3(256), 0, st, p.seg_map, p.seg_state,
+                     p.segs, DV, p.s_in, p.dk, p.dv);
+}
+
 bool data_ok(const tmpc_delta_attention* x) {
   return x->T == 0 || (x->q && x->k && x->v && x->log_decay && x->beta);
 }
@@ -77,11 +109,16 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
   DeltaArgs<E> p = delta_args<E>(x);
   p.s_out = state_out, p.o = (E*)o;
   p.vec = vec_ok(p);
+  const RunPlan runs = run_plan(x);
+  if (wsb < runs.state + runs.map) return TMPC_EWORKSPACE;
+  if (runs.segs > 1 && !ws) return TMPC_EBADARG;
+  p.segs = runs.segs, p.seg_len = runs.len, p.seg_state = (float*)ws, p.seg_map = (float*)((char*)ws + runs.state);
   with_widths(x->dk, x->dv, [&](auto dk, auto dv) {
+    if (p.segs > 1) launch_runs<E, dk()>(st, p, dv());
     constexpr size_t lds = delta_forward_lds<E, dk(), dv()>();
     auto k = delta_forward_kernel<E, dk(), dv()>;
     lds_optin(k, lds);
-    hipLaunchKernelGGL(k, dim3((unsigned)(x->B * x->H)), dim3(DeltaShape<E, dk(), dv()>::THREADS), lds, st, p);
+    hipLaunchKernelGGL(k, dim3((unsigned)(x->B * x->H * p.segs)), dim3(DeltaShape<E, dk(), dv()>::THREADS), lds, st, p);
   });
   return launch_status();
 }
@@ -89,9 +126,9 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
 // The backward pass' arrays in the workspace, one after another.
 struct BackwardPlan {
   int chunks, segs, DK, DV;
-  size_t e, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, bytes;
+  size_t e, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
+  RunPlan runs;
 };
-inline int tile_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 template <typename E>
 BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   constexpr int C = AttnTile<E>::C;
@@ -112,6 +149,8 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   if (x->Hv != x->H) p.y = take(rows * p.DV * sizeof(E)), p.y_part = take(tok * x->dv);
   if (x->Hq != x->H) p.q_part = take(tok * x->dk);
   if (x->Hk != x->H) p.k_part = take(tok * x->dk);
+  p.runs = run_plan(x);
+  p.run_state = take(p.runs.state), p.run_map = take(p.runs.map), p.run_grad = take(p.runs.state);
   return p;
 }
 
@@ -143,7 +182,9 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   a.q_part = x->Hq != x->H, a.k_part = x->Hk != x->H;
   a.dq = a.q_part ? base + w.q_part : dq, a.dk = a.k_part ? base + w.k_part : dk;
   a.dbeta = (E*)dbeta, a.dg = dg, a.d_in = d_in;
-  const int64_t bh = (int64_t)x->B * x->H;
+  a.f.segs = w.runs.segs, a.f.seg_len = w.runs.len, a.f.seg_state = (float*)(base + w.run_state);
+  a.f.seg_map = (float*)(base + w.run_map), a.r_seg = (float*)(base + w.run_grad);
+  const int64_t bh = (int64_t)x->B * x->H, runs = bh * a.f.segs;
   a.f.vec = rows_ok(a.f.q, a.f.qs, x->dk) && rows_ok(a.f.k, a.f.ks, x->dk) && rows_ok(a.f.v, a.f.vs, x->dv) &&
             rows_ok(a.d_o, a.dos, x->dv) && ((uintptr_t)dv & 3) == 0;
   with_widths(x->dk, x->dv, [&](auto dkw, auto dvw) {
@@ -152,8 +193,17 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
       lds_optin(k, lds);
       hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), lds, st, a);
     };
-    if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw()>, bh, THREADS, delta_states_lds<E, dkw(), dvw()>());
-    launch(delta_reverse_kernel<E, dkw(), dvw()>, bh, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
+    if (a.f.segs > 1) {
+      launch_runs<E, dkw()>(st, a.f, dvw());
+      auto k = delta_reverse_run_kernel<E, dkw()>;
+      constexpr size_t lds = delta_reverse_run_lds<E, dkw()>();
+      lds_optin(k, lds);
+      hipLaunchKernelGGL(k, dim3((unsigned)runs, (unsigned)ceil_div(dvw(), 64)), dim3(256), lds, st, a, (int)dvw());
+      hipLaunchKernelGGL((delta_scan_kernel<dkw(), true>), dim3((unsigned)(bh * (dvw() / 16))), dim3(256), 0, st, a.f.seg_map,
+                         a.r_seg, a.f.segs, (int)dvw(), a.d_out, x->dk, x->dv);
+    }
+    if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw()>, runs, THREADS, delta_states_lds<E, dkw(), dvw()>());
+    launch(delta_reverse_kernel<E, dkw(), dvw()>, runs, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
     if (x->T > 0) launch(delta_dqk_kernel<E, dkw(), dvw()>, bh * w.chunks, 256, delta_dqk_lds<E, dkw(), dvw()>());
   });
   if (x->T > 0) {

@@ -42,7 +42,16 @@ struct DeltaArgs {
   const float* s_in;  // (B, H, dk, dv) or NULL
   float* s_out;       // (B, H, dk, dv) or NULL
   E* o;               // (B, T, H, dv)
+  int segs, seg_len;  // the steps in segs runs of seg_len (a multiple of kDeltaSeg)
+  float* seg_state;   // segs > 1: (B H, segs, DK, DV): each run's own sum, then the state it starts from
+  float* seg_map;     // segs > 1: (B H, segs, DK, DK): what a run does to the state it starts from
 };
+constexpr int kDeltaSeg = 256;  // steps
+
+template <typename E>
+__device__ inline int delta_length(const DeltaArgs<E>& p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+}
 
 template <typename E, int DK, int DV>
 struct DeltaShape {
@@ -335,11 +344,11 @@ __device__ inline void delta_solve(const float* tiles, const f32x4 (&x)[S::NB], 
 
 // A wave's columns of a history whose state is not finite in the end, by the definition, a step at
 // a time: in a block such a step meets the earlier ones with factors of zero, which makes those NaN.
-template <typename E, int KA>
-__device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaArgs<E>& p, int bh, int tid) {
+template <typename E, int KA, int DV>
+__device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaArgs<E>& p, int block, int tid) {
   const int lo = tid & 15, hi = (tid & 63) >> 4, col0 = (tid >> 6) * 16, c = col0 + lo;
-  const int b = bh / p.H, h = bh - b * p.H;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int bh = block / p.segs, seg = block - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int L = delta_length(p, b);
   const E* pq = p.q + b * p.qs[0] + (h / p.gq) * p.qs[2];
   const E* pk = p.k + b * p.ks[0] + (h / p.gk) * p.ks[2];
   const E* pv = p.v + b * p.vs[0] + (h / p.gv) * p.vs[2];
@@ -347,8 +356,9 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
   const float* pg = p.g + b * p.gs[0] + h * p.gs[2];
   const int64_t size = (int64_t)p.dk * p.dv;
   f32x4 s[KA][1];
-  load_state(s, p.s_in ? p.s_in + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
-  for (int t = 0; t < L; ++t) {
+  if (p.segs > 1) load_state(s, p.seg_state + block * (int64_t)(KA * 16 * DV), false, KA * 16, DV, col0, lo, hi);
+  else load_state(s, p.s_in ? p.s_in + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
+  for (int t = seg * p.seg_len; t < min(L, (seg + 1) * p.seg_len); ++t) {
     const E *qt = pq + t * p.qs[1], *kt = pk + t * p.ks[1];
     const float a = __expf(pg[t * p.gs[1]]), beta = (float)pb[t * p.bs[1]];
     float ks = 0.0f, qs = 0.0f;
@@ -372,7 +382,7 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
     qs += __shfl_xor(qs, 16, 64), qs += __shfl_xor(qs, 32, 64);
     if (hi == 0 && c < p.dv) p.o[(((int64_t)b * p.T + t) * p.H + h) * p.dv + c] = (E)(p.scale * qs);
   }
-  if (p.s_out) store_state(s, p.s_out + bh * size, p.dk, p.dv, col0, lo, hi);
+  if (p.s_out && seg == (L - 1) / p.seg_len) store_state(s, p.s_out + bh * size, p.dk, p.dv, col0, lo, hi);
 }
 
 template <typename E, int DK, int DV>
@@ -381,7 +391,7 @@ constexpr size_t delta_forward_lds() {
   return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::SCORES + 2 * S::C * S::LDK + S::C * S::LDV);
 }
 
-// A workgroup a (problem, head).
+// A workgroup a run of a (problem, head).
 template <typename E, int DK, int DV>
 __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_forward_kernel(
     DeltaArgs<E> p) {
@@ -389,8 +399,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP;
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
   const DeltaGates d = delta_gates<S>(smem);
   float* inv = reinterpret_cast<float*>(smem) + S::GATES;
   E* tp = reinterpret_cast<E*>(inv + S::INV);  // the blocks' scores
@@ -407,15 +417,16 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   auto fetch = [&](int t0) {
     rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rg.load(t0, L - t0, tid);
   };
-  if (L > 0) fetch(0);
+  if (begin < L) fetch(begin);
   f32x4 s[KA][1];
-  load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
+  if (p.segs > 1) load_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
+  else load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
   const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
   const int oc = col0 + 4 * hi;
   const unsigned ooff = oc < p.dv ? (unsigned)((lo * orow + oc) * sizeof(E)) : kNowhere;
   const unsigned otile = (unsigned)(16 * orow * sizeof(E));
 
-  for (int t0 = 0; t0 < L; t0 += C) {
+  for (int t0 = begin; t0 < L; t0 += C) {
     const int n = min(C, L - t0);
     rk.store(tk), rq.store(tq), rv.store(tv), rg.store(d, tid);
     __syncthreads();
@@ -496,23 +507,174 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   }
   // What follows makes its indexes and reads its arguments again: they would be kept through every chunk.
   auto* args = __builtin_amdgcn_kernarg_segment_ptr();
-  int etid = tid, ebh = bh;
-  asm volatile("" : "+v"(etid), "+s"(args), "+s"(ebh));
+  int etid = tid, block = blockIdx.x;
+  asm volatile("" : "+v"(etid), "+s"(args), "+s"(block));
   const DeltaArgs<E>& a = *(const DeltaArgs<E>*)args;
-  const int eb = ebh / a.H, eL = a.lengths ? min(max(a.lengths[eb], 0), a.T) : a.T;
-  zero_rows(a.o, false, sizeof(E), ((int64_t)eb * a.T * a.H + (ebh - eb * a.H)) * a.dv, (int64_t)a.H * a.dv, a.dv, eL, a.T, etid,
-            S::THREADS);
+  const int ebh = block / a.segs, eseg = block - ebh * a.segs, eb = ebh / a.H, eL = delta_length(a, eb);
+  const int ebegin = eseg * a.seg_len;
+  zero_rows(a.o, false, sizeof(E), ((int64_t)eb * a.T * a.H + (ebh - eb * a.H)) * a.dv, (int64_t)a.H * a.dv, a.dv, max(eL, ebegin),
+            min((int64_t)a.T, (int64_t)ebegin + a.seg_len), etid, S::THREADS);
   // An infinite or NaN value leaves the state so, to the end.
   f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
   for (int m = 0; m < KA; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][0][r], 0.0f, zero[r]);
-  if (eL > 0 && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
+  if (ebegin < eL && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
     __threadfence_block();  // rows written above are written again
-    delta_by_step<E, KA>(a, ebh, etid);
-  } else if (a.s_out) {
+    delta_by_step<E, KA, DV>(a, block, etid);
+  } else if (a.s_out && eseg == (eL > 0 ? (eL - 1) / a.seg_len : 0)) {  // the run that holds the last live step
     store_state(s, a.s_out + ebh * ((int64_t)a.dk * a.dv), a.dk, a.dv, (etid >> 6) * 16, etid & 15, (etid & 63) >> 4);
+  }
+}
+
+// A long history of few heads does not fill the chip: it is cut into runs.  A run is a linear map of the
+// state it starts from, S -> M S + N: a first pass makes each run's M (its columns start from the unit
+// matrix, with values of zero) and N (from zero), a scan carries the states through, and the outputs
+// start from those.  A wave 16 columns of [N | M].
+template <typename E, int DK>
+constexpr size_t delta_run_lds() {
+  using S = DeltaShape<E, DK, 64>;
+  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::C * S::LDK + S::C * S::LDV);
+}
+template <typename E, int DK>
+__global__ __launch_bounds__(256, 2) void delta_run_kernel(DeltaArgs<E> p, int DV) {
+  using S = DeltaShape<E, DK, 64>;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV;
+  extern __shared__ __align__(16) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);
+  const int tile = blockIdx.y * 4 + wave, unit = tile * 16 - DV;  // the first of its columns of the unit matrix
+  const DeltaGates d = delta_gates<S>(smem);
+  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
+  E* tk = reinterpret_cast<E*>(inv + S::INV);
+  E* tv = tk + C * LDK;
+  DeltaRows<E, C, DK, 256> rk;
+  DeltaRows<E, C, 64, 256> rv;
+  const int c0 = blockIdx.y * 64;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2] + min(c0, p.dv), p.vs[1], min(max(p.dv - c0, 0), 64), p.vec, tid);
+  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+  auto fetch = [&](int t0) { rk.load(t0, L - t0), rv.load(t0, L - t0), rg.load(t0, L - t0, tid); };
+  if (begin < L) fetch(begin);
+  f32x4 s[KA][1];
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[m][0][r] = 16 * m + 4 * hi + r == unit + lo ? 1.0f : 0.0f;
+  for (int t0 = begin; t0 < L; t0 += C) {
+    const int n = min(C, L - t0);
+    rk.store(tk), rv.store(tv), rg.store(d, tid);
+    __syncthreads();
+    if (wave < S::NBLK && wave * S::BS < n) delta_inverse<E, S, DK, false>(d, inv, tk, wave, here(lane));
+    __syncthreads();
+    if (t0 + C < L) fetch(t0 + C);
+#pragma unroll 1
+    for (int blk = 0; blk * S::BS < n; ++blk) {
+      const int r0 = blk * S::BS, lane = here(tid & 63), hi = lane >> 4, col0 = here(wave) * 16;
+      f32x4 none[NB], x[NB], u[NB];
+      delta_state_products<E, S, KA, 0>(tk, tk, r0, s, x, none, lane);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const f32x4 v = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane));  // zeros for the unit matrix' columns
+        x[i] = v - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
+      }
+      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
+      Terms<E> w[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * (lds_f4(d.beta + r0 + 16 * i + 4 * hi) * u[i]));
+      const float total = d.total[blk];
+#pragma unroll
+      for (int m = 0; m < KA; ++m) {
+        quad_t<E> kt[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
+        s[m][0] = mma_terms(kt, w, s[m][0] * total);
+      }
+    }
+    __syncthreads();
+  }
+  if (unit >= 0) {
+    if (unit < DK) store_state(s, p.seg_map + blockIdx.x * (int64_t)(DK * DK), DK, DK, unit, lo, hi);
+  } else {
+    store_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), DK, DV, tile * 16, lo, hi);
+  }
+}
+
+// The same backwards in time: what a run adds to the gradient of the state that it starts from.
+template <typename E, int DK>
+constexpr size_t delta_reverse_run_lds() {
+  using S = DeltaShape<E, DK, 64>;
+  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (Terms<E>::N * S::SCORES + 2 * S::C * S::LDK + S::C * S::LDV);
+}
+
+// Between the passes: each run's sum becomes the state it starts from (REVERSE: the state's gradient
+// that it ends with, through the maps' transposes), for 16 columns a workgroup; its waves share the rows out.
+template <int DK, bool REVERSE>
+__global__ __launch_bounds__(256) void delta_scan_kernel(const float* map, float* state, int segs, int DV, const float* start,
+                                                         int dk, int dv) {
+  constexpr int KA = DK / 16, MT = (KA + 3) / 4, LD = DK + 4;
+  __shared__ __align__(16) float ts[2][16 * LD];  // (column, row)
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int tiles = DV / 16, bh = blockIdx.x / tiles, col = (blockIdx.x - bh * tiles) * 16 + lo;
+  map += (int64_t)bh * segs * DK * DK, state += (int64_t)bh * segs * DK * DV;
+  const int first = REVERSE ? segs - 1 : 0, dir = REVERSE ? -1 : 1;
+  f32x4 a[MT][KA], n[MT], s[MT];
+  auto load = [&](int seg) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = wave + 4 * i;
+      if (m >= KA) continue;
+#pragma unroll
+      for (int k = 0; k < KA; ++k) {
+        const float* x = map + (int64_t)seg * DK * DK;
+        if constexpr (REVERSE) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a[i][k][r] = x[(16 * k + 4 * hi + r) * DK + 16 * m + lo];
+        } else {
+          a[i][k] = *reinterpret_cast<const f32x4*>(x + (16 * m + lo) * DK + 16 * k + 4 * hi);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) n[i][r] = state[(int64_t)seg * DK * DV + (16 * m + 4 * hi + r) * DV + col];
+    }
+  };
+  load(first);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * (wave + 4 * i) + 4 * hi + r;
+      s[i][r] = start && row < dk && col < dv ? start[((int64_t)bh * dk + row) * dv + col] : 0.0f;
+    }
+  for (int j = 0; j < segs; ++j) {
+    const int seg = first + dir * j;
+    float* t = ts[j & 1];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = wave + 4 * i;
+      if (m < KA) *reinterpret_cast<f32x4*>(t + lo * LD + 16 * m + 4 * hi) = s[i];
+    }
+    __syncthreads();
+    f32x4 all[KA];
+#pragma unroll
+    for (int k = 0; k < KA; ++k) all[k] = lds_f4(t + lo * LD + 16 * k + 4 * hi);
+    f32x4 next[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = wave + 4 * i;
+      if (m >= KA) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) state[(int64_t)seg * DK * DV + (16 * m + 4 * hi + r) * DV + col] = s[i][r];
+      next[i] = n[i];
+#pragma unroll
+      for (int k = 0; k < KA; ++k) next[i] = mma16(a[i][k], all[k], next[i]);
+    }
+    if (j + 1 < segs) load(seg + dir);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) s[i] = next[i];
   }
 }
 
@@ -549,11 +711,10 @@ struct DeltaBwdArgs {
   E* dbeta;            // (B, T, H)
   float* dg;           // (B, T, H)
   float* d_in;         // (B, H, dk, dv) or NULL
+  float* r_seg;        // f.segs > 1: as f.seg_state, of the state's gradient at the runs' ends
   void *dq, *dk;       // (B, T, H, dk) of E, or fp32 parts
   int q_part, k_part;
 };
-constexpr int kDeltaSeg = 256;  // steps
-
 // sum over the 16 lanes of a row
 __device__ inline float row16_sum(float v) {
 #define TMPC_ROR(n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + n, 0xf, 0xf, false))
@@ -601,8 +762,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
   const DeltaGates d = delta_gates<S>(smem);
   float* inv = reinterpret_cast<float*>(smem) + S::GATES;
   float* tp = inv + S::INV;   // the blocks' scores
@@ -622,11 +783,12 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   auto fetch = [&](int t0) {
     rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), rg.load(t0, L - t0, tid);
   };
-  if (L > 0) fetch(0);
+  if (begin < L) fetch(begin);
   f32x4 s[KA][1];
-  load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
+  if (p.segs > 1) load_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
+  else load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
 
-  for (int t0 = 0; t0 < L; t0 += C) {
+  for (int t0 = begin; t0 < L; t0 += C) {
     const int n = min(C, L - t0), chunk = t0 / C;
     rk.store(tk), rq.store(tq), rv.store(tv), rdo.store(tdo), rg.store(d, tid);
     store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + chunk) * DK * DV, s, col0, lo, hi);
@@ -705,6 +867,86 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   }
 }
 
+// The inverses' transposes and the scores, transposed and by their terms, of a chunk's blocks.
+template <typename E, typename S, int DK>
+__device__ inline void delta_reverse_setup(const DeltaGates& d, float* inv, E* tp, const E* tk, const E* tq, int n, float scale,
+                                           int wave, int tid) {
+  for (int task = wave; task < 2 * S::NBLK; task += S::W) {
+    const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+    if (r0 >= n) continue;
+    if (task < S::NBLK) {
+      delta_inverse<E, S, DK, true>(d, inv, tk, blk, lane);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < S::NB; ++i)
+#pragma unroll
+      for (int j = 0; j <= i; ++j) {  // lane lo has the key's row
+        f32x4 x = row_products<E, DK>(tq, r0 + 16 * i, tk, r0 + 16 * j, S::LDK, lane);
+        const f32x4 lag = delta_lag(d, r0 + 16 * j, r0 + 16 * i, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r >= lo ? scale * (x[r] * __expf(-lag[r])) : 0.0f;
+        const Terms<E> terms(x);
+#pragma unroll
+        for (int t = 0; t < Terms<E>::N; ++t)
+          *reinterpret_cast<quad_t<E>*>(tp + ((blk * S::TRI + tri(i, j)) * Terms<E>::N + t) * S::TILE_P + lo * S::LDP + 4 * hi) = terms.t[t];
+      }
+  }
+}
+
+// dU of a block, and dO's columns as operands
+template <typename E, typename S, int KA>
+__device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv, const E* tp, const E* tk, const E* tdo, int blk,
+                                           const f32x4 (&s)[KA][1], quad_t<E> (&g)[S::NB], f32x4 (&du)[S::NB], int col0, int lane) {
+  constexpr int NB = S::NB, TERMS = Terms<E>::N;
+  const int r0 = blk * S::BS, lo = lane & 15, hi = lane >> 4;
+  f32x4 x[NB], none[NB];
+  delta_state_products<E, S, KA, 0>(tk, tk, r0, s, x, none, lane);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    g[i] = lds_quad_t(tdo, S::LDV, r0 + 16 * i, col0, lane);
+    x[i] *= lds_f4(d.to + r0 + 16 * i + 4 * hi);
+  }
+  const E* pt = tp + blk * S::TRI * TERMS * S::TILE_P + lo * S::LDP + 4 * hi;
+  auto score = [&](int i, int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * TERMS + t) * S::TILE_P); };
+  if constexpr (NB == 2) {
+    const quad_t<E> zero = to_quad<E>(f32x4{0, 0, 0, 0});
+#pragma unroll
+    for (int t = 0; t < 3; ++t) x[0] = mma2(score(0, 0, t), score(1, 0, t), g[0], g[1], x[0]);
+    x[1] = mma2(score(1, 1, 0), score(1, 1, 1), g[1], g[1], x[1]);
+    x[1] = mma2(score(1, 1, 2), zero, g[1], zero, x[1]);
+  } else {
+    x[0] = mma16(score(0, 0, 0), g[0], x[0]);
+  }
+  delta_solve<S, true>(inv + blk * S::TRI * S::TILE, x, du, lane);
+}
+
+// R := exp(G_end) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y
+template <typename E, typename S, int KA>
+__device__ inline void delta_reverse_update(const DeltaGates& d, const E* tk, const E* tq, int blk, float scale,
+                                            const quad_t<E> (&g)[S::NB], const f32x4 (&du)[S::NB], f32x4 (&s)[KA][1], int lane) {
+  constexpr int NB = S::NB;
+  const int r0 = blk * S::BS, hi = lane >> 4;
+  Terms<E> wq[NB], wk[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const f32x4 from = lds_f4(d.from + r0 + 16 * i + 4 * hi);
+    wq[i] = Terms<E>(scale * from * to_f32(g[i]));
+    wk[i] = Terms<E>(-(from * (lds_f4(d.beta + r0 + 16 * i + 4 * hi) * du[i])));
+  }
+  const float total = d.total[blk];
+#pragma unroll
+  for (int m = 0; m < KA; ++m) {
+    quad_t<E> qt[NB], kt[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      qt[i] = lds_quad_t(tq, S::LDK, r0 + 16 * i, 16 * m, lane);
+      kt[i] = lds_quad_t(tk, S::LDK, r0 + 16 * i, 16 * m, lane);
+    }
+    s[m][0] = mma_terms(kt, wk, mma_terms(qt, wq, s[m][0] * total));
+  }
+}
+
 template <typename E, int DK, int DV>
 constexpr size_t delta_reverse_lds() {
   using S = DeltaShape<E, DK, DV>;
@@ -721,8 +963,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
   const DeltaGates d = delta_gates<S>(smem);
   float* inv = reinterpret_cast<float*>(smem) + S::GATES;
   float* sum_beta = inv + S::INV;     // (waves, steps)
@@ -748,14 +990,15 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), re.load(t0, L - t0);
     rg.load(t0, L - t0, tid);
   };
-  const int last = L > 0 ? (L - 1) / C : -1;
+  const int last = begin < L ? (L - 1) / C : -1;
   if (last >= 0) fetch(last * C);
   const int64_t size = (int64_t)p.dk * p.dv;
   f32x4 s[KA][1];
-  load_state(s, a.d_out ? a.d_out + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
+  if (p.segs > 1) load_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
+  else load_state(s, a.d_out ? a.d_out + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
   E* yrow = a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv);
 
-  for (int chunk = last; chunk >= 0; --chunk) {
+  for (int chunk = last; chunk * C >= begin; --chunk) {
     const int t0 = chunk * C, n = min(C, L - t0);
     rk.store(tk), rq.store(tq), rv.store(tv), rdo.store(tdo), re.store(te), rg.store(d, tid);
     store_columns<E, DK>(a.r + ((int64_t)bh * a.chunks + chunk) * DK * DV, s, col0, lo, hi);
@@ -779,60 +1022,20 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       for (int i = 0; i < S::W; ++i) dot += sum_dot[i];
       a.dot[(int64_t)bh * a.segs + chunk / SEG] = dot;
     }
-    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
-      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
-      if (r0 >= n) continue;
-      if (task < S::NBLK) {
-        delta_inverse<E, S, DK, true>(d, inv, tk, blk, lane);
-        continue;
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j <= i; ++j) {  // lane lo has the key's row
-          f32x4 x = row_products<E, DK>(tq, r0 + 16 * i, tk, r0 + 16 * j, LDK, lane);
-          const f32x4 lag = delta_lag(d, r0 + 16 * j, r0 + 16 * i, lane);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r >= lo ? p.scale * (x[r] * __expf(-lag[r])) : 0.0f;
-          const Terms<E> terms(x);
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-            *reinterpret_cast<quad_t<E>*>(tp + ((blk * S::TRI + tri(i, j)) * TERMS + t) * S::TILE_P + lo * LDP + 4 * hi) = terms.t[t];
-        }
-    }
+    delta_reverse_setup<E, S, DK>(d, inv, tp, tk, tq, n, p.scale, wave, tid);
     __syncthreads();
-    if (chunk > 0) fetch(t0 - C);
+    if (t0 > begin) fetch(t0 - C);
 #pragma unroll 1
     for (int blk = (n - 1) / S::BS; blk >= 0; --blk) {
       const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
-      f32x4 x[NB], du[NB], none[NB];
-      delta_state_products<E, S, KA, 0>(tk, tq, r0, s, x, none, lane);
+      f32x4 du[NB];
       quad_t<E> g[NB];
+      delta_reverse_solve<E, S, KA>(d, inv, tp, tk, tdo, blk, s, g, du, col0, lane);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        g[i] = lds_quad_t(tdo, LDV, r0 + 16 * i, col0, lane);
-        x[i] *= lds_f4(d.to + r0 + 16 * i + 4 * hi);
-      }
-      const E* pt = tp + blk * S::TRI * TERMS * S::TILE_P + lo * LDP + 4 * hi;
-      auto score = [&](int i, int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * TERMS + t) * S::TILE_P); };
-      if constexpr (NB == 2) {
-        const quad_t<E> zero = to_quad<E>(f32x4{0, 0, 0, 0});
-#pragma unroll
-        for (int t = 0; t < 3; ++t) x[0] = mma2(score(0, 0, t), score(1, 0, t), g[0], g[1], x[0]);
-        x[1] = mma2(score(1, 1, 0), score(1, 1, 1), g[1], g[1], x[1]);
-        x[1] = mma2(score(1, 1, 2), zero, g[1], zero, x[1]);
-      } else {
-        x[0] = mma16(score(0, 0, 0), g[0], x[0]);
-      }
-      delta_solve<S, true>(inv + blk * S::TRI * S::TILE, x, du, lane);
-      Terms<E> wq[NB], wk[NB];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const f32x4 from = lds_f4(d.from + r0 + 16 * i + 4 * hi);
         const f32x4 y = lds_f4(d.beta + r0 + 16 * i + 4 * hi) * du[i];
         const f32x4 pe = du[i] * to_f32(lds_quad_t(te, LDV, r0 + 16 * i, col0, lane));
         const f32x4 pv = y * to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane));
-        wq[i] = Terms<E>(p.scale * from * to_f32(g[i])), wk[i] = Terms<E>(-(from * y));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = r0 + 16 * i + 4 * hi + r;
@@ -843,17 +1046,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
             a.y_part[(((int64_t)b * p.T + t0 + t) * p.H + h) * p.dv + col0 + lo] = y[r];
         }
       }
-      const float total = d.total[blk];
-#pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        quad_t<E> qt[NB], kt[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          qt[i] = lds_quad_t(tq, LDK, r0 + 16 * i, 16 * m, lane);
-          kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
-        }
-        s[m][0] = mma_terms(kt, wk, mma_terms(qt, wq, s[m][0] * total));
-      }
+      delta_reverse_update<E, S, KA>(d, tk, tq, blk, p.scale, g, du, s, lane);
     }
     __syncthreads();
     copy_out(rdo, tdo, yrow + t0 * a.ys[1], a.ys[1], n, a.y_width);
@@ -865,11 +1058,61 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       a.z[(int64_t)bh * a.chunks * C + t0 + tid] = sz;
     }
   }
-  if (a.d_in) store_state(s, a.d_in + bh * size, p.dk, p.dv, col0, lo, hi);
-  for (int t = L + tid; t < p.T; t += S::THREADS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
+  if (a.d_in && seg == 0) store_state(s, a.d_in + bh * size, p.dk, p.dv, col0, lo, hi);
+  const int z0 = max(delta_length(p, b), begin), z1 = (int)min((int64_t)p.T, (int64_t)begin + p.seg_len);
+  for (int t = z0 + tid; t < z1; t += S::THREADS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
   const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
-  if (a.y_part) zero_rows(a.y_part, true, 4, obase, orow, p.dv, L, p.T, tid, S::THREADS);
-  else zero_rows(a.y, false, sizeof(E), obase, orow, p.dv, L, p.T, tid, S::THREADS);
+  if (a.y_part) zero_rows(a.y_part, true, 4, obase, orow, p.dv, z0, z1, tid, S::THREADS);
+  else zero_rows(a.y, false, sizeof(E), obase, orow, p.dv, z0, z1, tid, S::THREADS);
+}
+
+template <typename E, int DK>
+__global__ __launch_bounds__(256, 2) void delta_reverse_run_kernel(DeltaBwdArgs<E> a, int DV) {
+  using S = DeltaShape<E, DK, 64>;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, TERMS = Terms<E>::N;
+  extern __shared__ __align__(16) char smem[];
+  const DeltaArgs<E>& p = a.f;
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
+  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);
+  const DeltaGates d = delta_gates<S>(smem);
+  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
+  E* tp = reinterpret_cast<E*>(inv + S::INV);
+  E* tk = tp + TERMS * S::SCORES;
+  E* tq = tk + C * LDK;
+  E* tdo = tq + C * LDK;
+  DeltaRows<E, C, DK, 256> rk, rq;
+  DeltaRows<E, C, 64, 256> rdo;
+  const int c0 = blockIdx.y * 64;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + min(c0, p.dv), a.dos[1], min(max(p.dv - c0, 0), 64), p.vec, tid);
+  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+  auto fetch = [&](int t0) { rk.load(t0, L - t0), rq.load(t0, L - t0), rdo.load(t0, L - t0), rg.load(t0, L - t0, tid); };
+  const int last = begin < L ? (L - 1) / C : -1;
+  if (last >= 0) fetch(last * C);
+  f32x4 s[KA][1];
+#pragma unroll
+  for (int m = 0; m < KA; ++m) s[m][0] = f32x4{0, 0, 0, 0};
+  for (int chunk = last; chunk * C >= begin; --chunk) {
+    const int t0 = chunk * C, n = min(C, L - t0);
+    rk.store(tk), rq.store(tq), rdo.store(tdo), rg.store(d, tid);
+    __syncthreads();
+    delta_reverse_setup<E, S, DK>(d, inv, tp, tk, tq, n, p.scale, wave, tid);
+    __syncthreads();
+    if (t0 > begin) fetch(t0 - C);
+#pragma unroll 1
+    for (int blk = (n - 1) / S::BS; blk >= 0; --blk) {
+      f32x4 du[NB];
+      quad_t<E> g[NB];
+      const int lane = here(tid & 63), col0 = here(wave) * 16;
+      delta_reverse_solve<E, S, KA>(d, inv, tp, tk, tdo, blk, s, g, du, col0, lane);
+      delta_reverse_update<E, S, KA>(d, tk, tq, blk, p.scale, g, du, s, lane);
+    }
+    __syncthreads();
+  }
+  const int col0 = c0 + wave * 16;
+  if (col0 < DV) store_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * DV), DK, DV, col0, tid & 15, (tid & 63) >> 4);
 }
 
 // log_decay's gradient: a wave a stretch, four steps a lane; in 64 bits, for the terms are.
@@ -877,7 +1120,7 @@ template <typename E>
 __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows) {
   const DeltaArgs<E>& p = a.f;
   const int seg = blockIdx.x % a.segs, bh = blockIdx.x / a.segs, b = bh / p.H, h = bh - b * p.H, lane = threadIdx.x;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int L = delta_length(p, b);
   const int t0 = seg * kDeltaSeg + lane * 4;
   const int64_t at = (int64_t)bh * rows + t0;
   double x[4], sum = 0.0;
@@ -919,7 +1162,7 @@ __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
   const int chunk = blockIdx.x % a.chunks, bh = blockIdx.x / a.chunks, b = bh / p.H, h = bh - b * p.H;
-  const int L = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const int L = delta_length(p, b);
   const int t0 = chunk * C, n = min(C, L - t0);
   const int64_t orow = (int64_t)p.H * p.dk, obase = ((int64_t)b * p.T * p.H + h) * p.dk;
   const int64_t z0 = max(L, t0), z1 = min(p.T, t0 + C);

@@ -7,7 +7,10 @@ extern "C" {
 
 size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_attention* a, int backward) {
   if (!a || !shape_ok(a) || (elem_bytes != 2 && elem_bytes != 4)) return 0;
-  if (!backward) return 0;
+  if (!backward) {
+    const RunPlan runs = run_plan(a);
+    return runs.state + runs.map;
+  }
   return elem_bytes == 2 ? backward_plan<bf16>(a).bytes : backward_plan<float>(a).bytes;
 }
 
