@@ -23,6 +23,8 @@
 //   du_t = k_t D_t,  y_t = dv_t = beta_t du_t,  R_{t-1} = a_t (D_t - k_t^T y_t),  dbeta_t = du_t . e_t,
 //   dq_t = scale do_t S_t^T,  dk_t = u_t D_t^T - a_t y_t S_{t-1}^T,  dg_t = <R_{t-1}, S_{t-1}>.
 #pragma once
+#include <type_traits>
+
 #include "decay_attention.hpp"
 
 namespace tmpc {
@@ -63,7 +65,8 @@ struct DeltaShape {
   static constexpr int LDP = sizeof(E) == 2 ? 24 : 20, TILE_P = 16 * LDP;  // one of E
   static constexpr int GATES = 2 * C + 3 * C + 4;  // floats
   static constexpr int INV = NBLK * TRI * TILE, SCORES = NBLK * TRI * TILE_P;
-  static constexpr int WAVES_PER_SIMD = 2;
+  // waves of a SIMD that the registers hold
+  static constexpr int WAVES_FORWARD = DK <= 64 ? (W == 8 ? 4 : 3) : 2, WAVES_BACKWARD = DK <= 64 ? 3 : 2;
 };
 // tile (i, j <= i) of a block
 constexpr int tri(int i, int j) { return i * (i + 1) / 2 + j; }
@@ -165,6 +168,20 @@ __device__ inline f32x4 row_products(const E* x, int x0, const E* y, int y0, int
   return t;
 }
 
+// f(0) ... f(N - 1) with constants
+template <int N, typename F, int I = 0>
+__device__ inline void steps(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    steps<N, F, I + 1>(f);
+  }
+}
+// lane I's of each 16
+template <int I>
+__device__ inline float row_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + I, 0xf, 0xf, true));
+}
+
 // The inverse of I + A for block `blk` of a chunk, by one wave, into its tiles at `inv`.  A_ij has
 // beta_j, or with REVERSE beta_i, and the inverse's transpose is left.
 template <typename E, typename S, int DK, bool REVERSE>
@@ -181,50 +198,45 @@ __device__ inline void delta_inverse(const DeltaGates& d, float* inv, const E* t
     for (int r = 0; r < 4; ++r) a[r] = i > j || 4 * hi + r < lo ? a[r] * __expf(lag[r]) * (REVERSE ? bi : bj[r]) : 0.0f;
     return a;
   };
+  auto rows = [&](int k) { return reinterpret_cast<f32x4*>(tiles + k * S::TILE + lo * LDT + 4 * hi); };
+  auto columns = [&](int k) { return lds_quad_t(tiles + k * S::TILE, LDT, 0, 0, lane); };
+  f32x4 a10, a[NB][4], t[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4*>(tiles + tri(i, i) * S::TILE + lo * LDT + 4 * hi) = a_tile(i, i);
-  f32x4 a10;
+  for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = a_tile(i, i);
   if constexpr (NB == 2) a10 = a_tile(1, 0);
   __builtin_amdgcn_wave_barrier();
-  float* tile = tiles + (NB == 2 && (hi & 1) ? tri(1, 1) * S::TILE : 0);  // lanes of odd hi: the other tile
-  float t[16];                                                            // column lo of its inverse
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float v = i == lo ? 1.0f : 0.0f;
+  for (int i = 0; i < NB; ++i) {
 #pragma unroll
-    for (int j = 0; j < i; j += 4) {
-      const f32x4 row = lds_f4(tile + i * LDT + j);
+    for (int j = 0; j < 4; ++j) a[i][j] = lds_f4(tiles + tri(i, i) * S::TILE + lo * LDT + 4 * j);  // row lo
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (j + r < i) v = fmaf(-row[r], t[j + r], v);
-    }
-    t[i] = v;
-    if (i % 2 == 1) asm volatile("" ::: "memory");  // not all rows' reads at once: their registers
+    for (int r = 0; r < 4; ++r) t[i][r] = 4 * hi + r == lo ? 1.0f : 0.0f;
   }
+  // row lo of the inverse, columns 4 hi + r: takes off A[lo][j] times row j, which is final by then
+  steps<15>([&](auto j) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[i][r] = fmaf(-a[i][j() / 4][j() % 4], row_lane<j()>(t[i][r]), t[i][r]);
+  });
   __builtin_amdgcn_wave_barrier();
-  if (hi < NB) {
-    if constexpr (REVERSE) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) *reinterpret_cast<f32x4*>(tile + lo * LDT + j) = f32x4{t[j], t[j + 1], t[j + 2], t[j + 3]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) tile[j * LDT + lo] = t[j];
-    }
-  }
+  for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = t[i];
+  f32x4 corner;
   if constexpr (NB == 2) {  // the corner: -T11 A10 T00
     __builtin_amdgcn_wave_barrier();
-    const float *t00 = tiles, *t11 = tiles + tri(1, 1) * S::TILE;
-    auto rows = [&](const float* x) { return lds_f4(x + lo * LDT + 4 * hi); };
-    auto columns = [&](const float* x) { return lds_quad_t(x, LDT, 0, 0, lane); };
-    const f32x4 y = mma16(a10, REVERSE ? rows(t00) : columns(t00), f32x4{0, 0, 0, 0});
-    const f32x4 c = -mma16(REVERSE ? columns(t11) : rows(t11), y, f32x4{0, 0, 0, 0});
-    float* out = tiles + tri(1, 0) * S::TILE;
-    if constexpr (REVERSE) {
-      *reinterpret_cast<f32x4*>(out + lo * LDT + 4 * hi) = c;
-    } else {
+    const f32x4 zero = {0, 0, 0, 0}, y = mma16(a10, columns(tri(0, 0)), zero);
+    corner = REVERSE ? -mma16(t[1], y, zero) : -mma16(y, t[1], zero);
+    *rows(tri(1, 0)) = corner;
+  }
+  if constexpr (REVERSE) {
+    __builtin_amdgcn_wave_barrier();
+    f32x4 c[NB];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) out[(4 * hi + r) * LDT + lo] = c[r];
-    }
+    for (int i = 0; i < NB; ++i) c[i] = columns(tri(i, i));
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = c[i];
   }
 }
 
@@ -273,18 +285,31 @@ struct DeltaRows {
   }
 };
 
-// x (fp32) as an operand of products whose other operand is exact in E: three bf16 terms (24
-// bits), or itself.
+// x (fp32) as an operand of products whose other operand is exact in E: itself, or three bf16 terms, the
+// upper 8 bits of what is left each time (24 bits together; cut off, not rounded: the terms' sum is
+// exact all the same, and a pair of them is one byte permutation).
 template <typename E>
-struct Terms {
-  static constexpr int N = sizeof(E) == 2 ? 3 : 1;
-  quad_t<E> t[N];
+struct Terms;
+template <>
+struct Terms<float> {
+  static constexpr int N = 1;
+  f32x4 t[1];
+  __device__ Terms() {}
+  __device__ Terms(f32x4 x) : t{x} {}
+};
+template <>
+struct Terms<bf16> {
+  static constexpr int N = 3;
+  bf16x4 t[3];
   __device__ Terms() {}
   __device__ Terms(f32x4 x) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      t[i] = to_quad<E>(x);
-      if (i + 1 < N) x -= to_f32(t[i]);
+    for (int i = 0; i < 3; ++i) {
+      const u4 b = __builtin_bit_cast(u4, x);
+      const u32x2 p = {__builtin_amdgcn_perm(b[1], b[0], 0x07060302u), __builtin_amdgcn_perm(b[3], b[2], 0x07060302u)};
+      t[i] = __builtin_bit_cast(bf16x4, p);
+      if (i < 2) x -= __builtin_bit_cast(f32x4, b & 0xffff0000u);
     }
   }
 };
@@ -393,7 +418,7 @@ constexpr size_t delta_forward_lds() {
 
 // A workgroup a run of a (problem, head).
 template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_forward_kernel(
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_FORWARD)) void delta_forward_kernel(
     DeltaArgs<E> p) {
   using S = DeltaShape<E, DK, DV>;
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP;
@@ -455,7 +480,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     for (int blk = 0; blk * S::BS < n; ++blk) {
       const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
       f32x4 o[NB], x[NB], u[NB];
-      delta_state_products<E, S, KA, 1>(tk, tq, r0, s, x, o, lane);
+      delta_state_products<E, S, KA, Terms<E>::N == 3 ? 2 : 1>(tk, tq, r0, s, x, o, lane);
 #pragma unroll
       for (int i = 0; i < NB; ++i)
         x[i] = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane)) - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
@@ -474,10 +499,10 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
         s[m][0] = mma_terms(kt, w, s[m][0] * total);
       }
-      // outputs; the scores are rounded to E, u is by two terms
-      quad_t<E> uh[NB], ul[NB];
+      // outputs, bf16: the scores are rounded, the state and u enter by two terms (16 bits)
+      Terms<E> ut[NB];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) uh[i] = to_quad<E>(u[i]), ul[i] = to_quad<E>(u[i] - to_f32(uh[i]));
+      for (int i = 0; i < NB; ++i) ut[i] = Terms<E>(u[i]);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         o[i] *= p.scale * d.from[r0 + 16 * i + lo];
@@ -485,7 +510,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 #pragma unroll
         for (int j = 0; j <= i; ++j) {
           const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(pt + j * S::TILE_P);
-          if constexpr (sizeof(E) == 2) o[i] = mma2(uh[j], ul[j], pq, pq, o[i]);
+          if constexpr (sizeof(E) == 2) o[i] = mma2(ut[j].t[0], ut[j].t[1], pq, pq, o[i]);
           else o[i] = mma16(u[j], pq, o[i]);
         }
         const unsigned at = r0 + 16 * i + lo < n && ooff != kNowhere ? ooff + (blk * NB + i) * otile : kNowhere;
@@ -538,7 +563,7 @@ constexpr size_t delta_run_lds() {
   return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::C * S::LDK + S::C * S::LDV);
 }
 template <typename E, int DK>
-__global__ __launch_bounds__(256, 2) void delta_run_kernel(DeltaArgs<E> p, int DV) {
+__global__ __launch_bounds__(256, DK <= 64 ? 3 : 2) void delta_run_kernel(DeltaArgs<E> p, int DV) {
   using S = DeltaShape<E, DK, 64>;
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV;
   extern __shared__ __align__(16) char smem[];
@@ -755,7 +780,7 @@ constexpr size_t delta_states_lds() {
 }
 
 template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_states_kernel(
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_BACKWARD)) void delta_states_kernel(
     DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, SEG = kDeltaSeg / C;
@@ -955,7 +980,7 @@ constexpr size_t delta_reverse_lds() {
 }
 
 template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_BACKWARD)) void delta_reverse_kernel(
     DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP, SEG = kDeltaSeg / C;
@@ -1067,7 +1092,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 }
 
 template <typename E, int DK>
-__global__ __launch_bounds__(256, 2) void delta_reverse_run_kernel(DeltaBwdArgs<E> a, int DV) {
+__global__ __launch_bounds__(256, DK <= 64 ? 3 : 2) void delta_reverse_run_kernel(DeltaBwdArgs<E> a, int DV) {
   using S = DeltaShape<E, DK, 64>;
   constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, TERMS = Terms<E>::N;
   extern __shared__ __align__(16) char smem[];
