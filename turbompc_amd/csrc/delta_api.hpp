@@ -84,16 +84,28 @@ inline RunPlan run_plan(const tmpc_delta_attention* x) {
   }
   return p;
 }
+template <typename K, typename... A>
+void launch(hipStream_t st, K k, dim3 grid, int threads, size_t lds, A... args) {
+  lds_optin(k, lds);
+  hipLaunchKernelGGL(k, grid, dim3(threads), lds, st, args...);
+}
+template <typename E, int DK, int DV, int MODE>
+void launch_walk(hipStream_t st, const DeltaBwdArgs<E>& a, int columns, int run_width) {
+  const dim3 grid((unsigned)((int64_t)a.f.B * a.f.H * a.f.segs), (unsigned)ceil_div(columns, DV));
+  launch(st, delta_walk_kernel<E, DK, DV, MODE>, grid, DeltaShape<E, DK, DV>::THREADS, DeltaWalkLds<E, DK, DV, MODE>::all, a, run_width);
+}
+template <typename E, int DK, int DV, bool RUN>
+void launch_reverse(hipStream_t st, const DeltaBwdArgs<E>& a, int columns, int run_width) {
+  const dim3 grid((unsigned)((int64_t)a.f.B * a.f.H * a.f.segs), (unsigned)ceil_div(columns, DV));
+  launch(st, delta_reverse_kernel<E, DK, DV, RUN>, grid, DeltaShape<E, DK, DV>::THREADS, DeltaReverseLds<E, DK, DV, RUN>::all, a, run_width);
+}
 // the runs' starts, from the pass before the outputs'
 template <typename E, int DK>
-void launch_runs(hipStream_t st, const DeltaArgs<E>& p, int DV) {
-  const int64_t bh = (int64_t)p.B * p.H;
-  constexpr size_t lds = delta_run_lds<E, DK>();
-  auto k = delta_run_kernel<E, DK>;
-  lds_optin(k, lds);
-  hipLaunchKernelGGL(k, dim3((unsigned)(bh * p.segs), (unsigned)ceil_div(DV + DK, 64)), dim3(256), lds, st, p, DV);
-  hipLaunchKernelGGL((delta_scan_kernel<DK, false>), dim3((unsigned)(bh * (DV / 16))), dim3(256), 0, st, p.seg_map, p.seg_state,
-                     p.segs, DV, p.s_in, p.dk, p.dv);
+void launch_runs(hipStream_t st, const DeltaBwdArgs<E>& a, int DV) {
+  const DeltaArgs<E>& p = a.f;
+  launch_walk<E, DK, 64, WALK_RUN>(st, a, DV + DK, DV);
+  launch(st, delta_scan_kernel<DK, false>, dim3((unsigned)((int64_t)p.B * p.H * (DV / 16))), 256, 0, (const float*)p.seg_map, p.seg_state,
+         p.segs, DV, p.s_in, p.dk, p.dv);
 }
 
 bool data_ok(const tmpc_delta_attention* x) {
@@ -106,7 +118,9 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
   if (x->B == 0) return TMPC_OK;
   if (!steps_ok(x)) return TMPC_EBADSHAPE;
   if (!data_ok(x) || (x->T > 0 && !o)) return TMPC_EBADARG;
-  DeltaArgs<E> p = delta_args<E>(x);
+  DeltaBwdArgs<E> a{};
+  a.f = delta_args<E>(x);
+  DeltaArgs<E>& p = a.f;
   p.s_out = state_out, p.o = (E*)o;
   p.vec = vec_ok(p);
   const RunPlan runs = run_plan(x);
@@ -114,18 +128,15 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
   if (runs.segs > 1 && !ws) return TMPC_EBADARG;
   p.segs = runs.segs, p.seg_len = runs.len, p.seg_state = (float*)ws, p.seg_map = (float*)((char*)ws + runs.state);
   with_widths(x->dk, x->dv, [&](auto dk, auto dv) {
-    if (p.segs > 1) launch_runs<E, dk()>(st, p, dv());
-    constexpr size_t lds = delta_forward_lds<E, dk(), dv()>();
-    auto k = delta_forward_kernel<E, dk(), dv()>;
-    lds_optin(k, lds);
-    hipLaunchKernelGGL(k, dim3((unsigned)(x->B * x->H * p.segs)), dim3(DeltaShape<E, dk(), dv()>::THREADS), lds, st, p);
+    if (p.segs > 1) launch_runs<E, dk()>(st, a, dv());
+    launch_walk<E, dk(), dv(), WALK_OUT>(st, a, dv(), 0);
   });
   return launch_status();
 }
 
 // The backward pass' arrays in the workspace, one after another.
 struct BackwardPlan {
-  int chunks, segs, DK, DV;
+  int chunks, stretches, DK, DV;
   size_t e, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
   RunPlan runs;
 };
@@ -133,7 +144,7 @@ template <typename E>
 BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   constexpr int C = AttnTile<E>::C;
   BackwardPlan p{};
-  p.chunks = (int)ceil_div(x->T, C), p.segs = (int)ceil_div(x->T, kDeltaSeg);
+  p.chunks = (int)ceil_div(x->T, C), p.stretches = (int)ceil_div(x->T, kDeltaSeg);
   p.DK = tile_width(x->dk), p.DV = tile_width(x->dv);
   const size_t bh = (size_t)x->B * x->H, state = (size_t)p.DK * p.DV, rows = bh * p.chunks * C;
   const size_t tok = (size_t)x->B * x->T * x->H * sizeof(float);
@@ -145,7 +156,7 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   p.e = take(rows * p.DV * sizeof(E));
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
-  p.s_seg = take(bh * p.segs * state * sizeof(float)), p.dot = take(bh * p.segs * sizeof(float));
+  p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
   if (x->Hv != x->H) p.y = take(rows * p.DV * sizeof(E)), p.y_part = take(tok * x->dv);
   if (x->Hq != x->H) p.q_part = take(tok * x->dk);
   if (x->Hk != x->H) p.k_part = take(tok * x->dk);
@@ -170,7 +181,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   a.f = delta_args<E>(x);
   a.d_o = (const E*)d_o, a.d_out = d_out;
   std::copy_n(dos, 3, a.dos);
-  a.chunks = w.chunks, a.segs = w.segs;
+  a.chunks = w.chunks, a.stretches = w.stretches;
   a.e = (E*)(base + w.e), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
   a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot);
   if (x->Hv != x->H) {
@@ -184,30 +195,23 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   a.dbeta = (E*)dbeta, a.dg = dg, a.d_in = d_in;
   a.f.segs = w.runs.segs, a.f.seg_len = w.runs.len, a.f.seg_state = (float*)(base + w.run_state);
   a.f.seg_map = (float*)(base + w.run_map), a.r_seg = (float*)(base + w.run_grad);
-  const int64_t bh = (int64_t)x->B * x->H, runs = bh * a.f.segs;
+  const int64_t bh = (int64_t)x->B * x->H;
   a.f.vec = rows_ok(a.f.q, a.f.qs, x->dk) && rows_ok(a.f.k, a.f.ks, x->dk) && rows_ok(a.f.v, a.f.vs, x->dv) &&
             rows_ok(a.d_o, a.dos, x->dv) && ((uintptr_t)dv & 3) == 0;
   with_widths(x->dk, x->dv, [&](auto dkw, auto dvw) {
-    constexpr int THREADS = DeltaShape<E, dkw(), dvw()>::THREADS;
-    auto launch = [&](auto k, int64_t blocks, int threads, size_t lds) {
-      lds_optin(k, lds);
-      hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(threads), lds, st, a);
-    };
     if (a.f.segs > 1) {
-      launch_runs<E, dkw()>(st, a.f, dvw());
-      auto k = delta_reverse_run_kernel<E, dkw()>;
-      constexpr size_t lds = delta_reverse_run_lds<E, dkw()>();
-      lds_optin(k, lds);
-      hipLaunchKernelGGL(k, dim3((unsigned)runs, (unsigned)ceil_div(dvw(), 64)), dim3(256), lds, st, a, (int)dvw());
-      hipLaunchKernelGGL((delta_scan_kernel<dkw(), true>), dim3((unsigned)(bh * (dvw() / 16))), dim3(256), 0, st, a.f.seg_map,
-                         a.r_seg, a.f.segs, (int)dvw(), a.d_out, x->dk, x->dv);
+      launch_runs<E, dkw()>(st, a, dvw());
+      launch_reverse<E, dkw(), 64, true>(st, a, dvw(), dvw());
+      launch(st, delta_scan_kernel<dkw(), true>, dim3((unsigned)(bh * (dvw() / 16))), 256, 0, (const float*)a.f.seg_map, a.r_seg,
+             a.f.segs, (int)dvw(), d_out, x->dk, x->dv);
     }
-    if (x->T > 0) launch(delta_states_kernel<E, dkw(), dvw()>, runs, THREADS, delta_states_lds<E, dkw(), dvw()>());
-    launch(delta_reverse_kernel<E, dkw(), dvw()>, runs, THREADS, delta_reverse_lds<E, dkw(), dvw()>());
-    if (x->T > 0) launch(delta_dqk_kernel<E, dkw(), dvw()>, bh * w.chunks, 256, delta_dqk_lds<E, dkw(), dvw()>());
+    if (x->T > 0) launch_walk<E, dkw(), dvw(), WALK_STATES>(st, a, dvw(), 0);
+    launch_reverse<E, dkw(), dvw(), false>(st, a, dvw(), 0);
+    if (x->T > 0)
+      launch(st, delta_dqk_kernel<E, dkw(), dvw()>, dim3((unsigned)(bh * w.chunks)), 256, delta_dqk_lds<E, dkw(), dvw()>(), a);
   });
   if (x->T > 0) {
-    hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.segs)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
+    hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.stretches)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
     auto sum = [&](const void* in, int heads, int d, void* out) {
       const int64_t rows = (int64_t)x->B * x->T * heads;
       const int q = (d + 3) / 4;

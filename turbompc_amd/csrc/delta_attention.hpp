@@ -13,9 +13,10 @@
 //
 // Blocks are short, so that the chain from state to state stays in a wave's registers: S is the
 // operand of K S, whose result is the operand of the product with the inverse, whose result is the operand
-// of the state's update.  A wave owns 16 columns of the values and walks its head's blocks without
-// meeting the other waves; what depends on the block alone (the inverse, Q K^T o Gamma, the powers) is
-// made once a chunk of several blocks, the waves sharing it out, in LDS.  In bf16 the state, an fp32
+// of the state's update.  A wave owns 16 columns of the values and walks its head's blocks.  The chain
+// leaves each SIMD waiting, so it has nothing else to do: further waves, the helpers, bring the next
+// block's rows to LDS and make what depends on its blocks alone (the inverses, Q K^T o Gamma, the
+// powers) while the walkers work on this one.  In bf16 the state, an fp32
 // result, enters products as three bf16 terms (24 bits); a block has two tiles there, so that they are
 // formed half as often.
 //
@@ -57,16 +58,16 @@ __device__ inline int delta_length(const DeltaArgs<E>& p, int b) {
 
 template <typename E, int DK, int DV>
 struct DeltaShape {
-  static constexpr int W = DV / 16, THREADS = 64 * W;  // a wave 16 value columns
-  static constexpr int C = AttnTile<E>::C, PAD = AttnTile<E>::PAD;
-  static constexpr int NB = sizeof(E) == 2 ? 2 : 1, BS = 16 * NB, NBLK = C / BS, TRI = NB * (NB + 1) / 2;
+  static constexpr int W = DV / 16, HELPERS = 3;  // walkers, a wave 16 value columns, and helpers
+  static constexpr int WALKERS = 64 * W, THREADS = 64 * (W + HELPERS);
+  static constexpr int PAD = AttnTile<E>::PAD;
+  static constexpr int NB = sizeof(E) == 2 ? 2 : 1, C = 16 * NB, TRI = NB * (NB + 1) / 2;  // a block's tiles and steps
   static constexpr int LDK = DK + PAD, LDV = DV + PAD;
   static constexpr int LDT = 20, TILE = 16 * LDT;  // a 16 x 16 fp32 tile, its quads spread over the banks
-  static constexpr int LDP = sizeof(E) == 2 ? 24 : 20, TILE_P = 16 * LDP;  // one of E
-  static constexpr int GATES = 2 * C + 3 * C + 4;  // floats
-  static constexpr int INV = NBLK * TRI * TILE, SCORES = NBLK * TRI * TILE_P;
-  // waves of a SIMD that the registers hold
-  static constexpr int WAVES_FORWARD = DK <= 64 ? (W == 8 ? 4 : 3) : 2, WAVES_BACKWARD = DK <= 64 ? 3 : 2;
+  static constexpr int LDP = 20, TILE_P = 16 * LDP;  // one of E
+  // of a buffer, of which there are two: floats of the gates and the inverses; elements of E of the scores
+  static constexpr int GATES = 6 * C + 4, INV = TRI * TILE, SCORES = TRI * TILE_P;
+  static constexpr int WAVES_PER_SIMD = W == 2 ? 2 : 3;
 };
 // tile (i, j <= i) of a block
 constexpr int tri(int i, int j) { return i * (i + 1) / 2 + j; }
@@ -87,18 +88,25 @@ __device__ inline int here(int v) {
   return v;
 }
 
-// A chunk's gates in LDS: the sums of g from each block's start, beta (zeros past the last live
-// step), exp(G), exp(G_end - G), exp(G_end).
+// A block's gates in LDS: the sums of g from its start (as two floats), beta (zeros past the
+// last live step), exp(G), exp(G_end - G), exp(G_end).
 struct DeltaGates {
-  double* G;
+  float2* G;
   float *beta, *from, *to, *total;
 };
 template <typename S>
-__device__ inline DeltaGates delta_gates(char* base) {
+__device__ inline DeltaGates delta_gates(float* base) {
   DeltaGates d;
-  d.G = reinterpret_cast<double*>(base), d.beta = reinterpret_cast<float*>(d.G + S::C);
+  d.G = reinterpret_cast<float2*>(base), d.beta = base + 2 * S::C;
   d.from = d.beta + S::C, d.to = d.from + S::C, d.total = d.to + S::C;
   return d;
+}
+
+// Every wave of the workgroup, each from its own place in the code: the walkers and the helpers meet here.
+__device__ inline void meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 template <int CTRL>
@@ -114,58 +122,63 @@ __device__ inline double lane_f64(double v, int lane) {
   return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
 }
 
-// The chunk's gates on their way from memory to LDS: the first wave's lanes a step each.
+// A block's gates on their way from memory to LDS, a lane a step: by the first helper, which makes the
+// inverses too.  The second and third move the rows, and the second makes the scores.
 template <typename E, typename S>
 struct DeltaGateRows {
   const float* g;
   const E* beta;
   int64_t gs, bs;
   float vg, vb;
-  __device__ void load(int t0, int n, int tid) {
-    vg = vb = 0.0f;
-    if (tid < n && tid < S::C) vg = g[(t0 + tid) * gs], vb = (float)beta[(t0 + tid) * bs];
+  // from here on g and beta are the lane's own, and move from block to block
+  __device__ void start(int64_t t, bool back) {
+    g += t * gs, beta += t * bs;
+    gs *= back ? -S::C : S::C, bs *= back ? -S::C : S::C;
   }
-  __device__ void store(const DeltaGates& d, int tid) const {
-    if (tid >= 64) return;
+  __device__ void load(int n, int lane) {  // the next block's, n of its steps live
+    vg = vb = 0.0f;
+    if (lane < n && lane < S::C) vg = *g, vb = (float)*beta;
+    g += gs, beta += bs;
+  }
+  // the sums and the powers, in registers
+  float2 sum;
+  float from, to, total, vb_scanned;
+  __device__ void scan(int lane) {
     double x = vg < kNoDecay ? kNoDecay : vg;
     x += dpp_f64<0x111>(x);  // within 16 lanes
     x += dpp_f64<0x112>(x);
     x += dpp_f64<0x114>(x);
     x += dpp_f64<0x118>(x);
-    double end;
-    const double e0 = lane_f64(x, 15), e1 = lane_f64(x, 31), e2 = lane_f64(x, 47), e3 = lane_f64(x, 63);
+    double end = lane_f64(x, 15);
     if constexpr (S::NB == 2) {
-      if (tid & 16) x += tid & 32 ? e2 : e0;
-      end = tid & 32 ? e2 + e3 : e0 + e1;
-    } else {
-      end = tid & 32 ? (tid & 16 ? e3 : e2) : (tid & 16 ? e1 : e0);
+      const double second = lane_f64(x, 31);
+      if (lane >= 16) x += end;
+      end += second;
     }
-    if (tid < S::C) {
-      d.G[tid] = x, d.beta[tid] = vb, d.from[tid] = __expf((float)x), d.to[tid] = __expf((float)(end - x));
-      if (tid % S::BS == 0) d.total[tid / S::BS] = __expf((float)end);
-    }
+    const float top = (float)x;
+    sum = make_float2(top, (float)(x - top)), vb_scanned = vb;
+    from = __expf((float)x), to = __expf((float)(end - x)), total = __expf((float)end);
+  }
+  __device__ void store(const DeltaGates& d, int lane) const {
+    if (lane < S::C) d.G[lane] = sum, d.beta[lane] = vb_scanned, d.from[lane] = from, d.to[lane] = to;
+    if (lane == 0) *d.total = total;
   }
 };
 
-// G_i - G_j for a lane's i = i0 + lo and j = j0 + 4 hi + r
-__device__ inline f32x4 delta_lag(const DeltaGates& d, int i0, int j0, int lane) {
-  const double mine = d.G[i0 + (lane & 15)];
-  const double* at = d.G + j0 + 4 * (lane >> 4);
-  f32x4 lag;
+// Gamma_ij for a lane's i = i0 + lo and j = j0 + 4 hi + r, or with SWAP the other way round
+template <bool SWAP>
+__device__ inline f32x4 delta_ratio(const DeltaGates& d, int i0, int j0, int lane) {
+  const float2 mine = d.G[i0 + (lane & 15)];
+  const f32x4* at = reinterpret_cast<const f32x4*>(d.G + j0 + 4 * (lane >> 4));
+  const f32x4 a = at[0], b = at[1];
+  const f32x4 top = {a[0], a[2], b[0], b[2]}, rest = {a[1], a[3], b[1], b[3]};
+  f32x4 ratio;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) lag[r] = (float)(mine - at[r]);
-  return lag;
-}
-
-// (X Y^T)^T of 16 rows of each: lane lo has row y0 + lo of Y, and of X rows x0 + 4 hi + r
-template <typename E, int D>
-__device__ inline f32x4 row_products(const E* x, int x0, const E* y, int y0, int ld, int lane) {
-  f32x4 t = {0, 0, 0, 0};
-#pragma unroll
-  for (int m = 0; m < D; m += 32)
-    t = mma2(lds_quad(x, ld, x0, m, lane), lds_quad(x, ld, x0, m + 16, lane), lds_quad(y, ld, y0, m, lane),
-             lds_quad(y, ld, y0, m + 16, lane), t);
-  return t;
+  for (int r = 0; r < 4; ++r) {
+    const float lag = (mine.x - top[r]) + (mine.y - rest[r]);
+    ratio[r] = __expf(SWAP ? -lag : lag);
+  }
+  return ratio;
 }
 
 // f(0) ... f(N - 1) with constants
@@ -176,67 +189,90 @@ __device__ inline void steps(F f) {
     steps<N, F, I + 1>(f);
   }
 }
-// lane I's of each 16
+// x += a times x of lane I of each 16, y += b times y's.  (The wait is that of a lane permutation behind a
+// vector write of its operand; a value that one of these writes is read eight of them later.)
 template <int I>
-__device__ inline float row_lane(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + I, 0xf, 0xf, true));
+__device__ inline void subtract_row(f32x4& x, float a, f32x4& y, float b) {
+#define TMPC_ROW(v, f) "v_fmac_f32_dpp " v ", " v ", " f " row_newbcast:%10 row_mask:0xf bank_mask:0xf\n\t"
+  float x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3], y0 = y[0], y1 = y[1], y2 = y[2], y3 = y[3];
+  asm("s_nop 1\n\t" TMPC_ROW("%0", "%8") TMPC_ROW("%1", "%8") TMPC_ROW("%2", "%8") TMPC_ROW("%3", "%8") TMPC_ROW("%4", "%9")
+          TMPC_ROW("%5", "%9") TMPC_ROW("%6", "%9") TMPC_ROW("%7", "%9")
+      : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3), "+v"(y0), "+v"(y1), "+v"(y2), "+v"(y3)
+      : "v"(a), "v"(b), "n"(I));
+#undef TMPC_ROW
+  x = f32x4{x0, x1, x2, x3}, y = f32x4{y0, y1, y2, y3};
 }
 
-// The inverse of I + A for block `blk` of a chunk, by one wave, into its tiles at `inv`.  A_ij has
-// beta_j, or with REVERSE beta_i, and the inverse's transpose is left.
-template <typename E, typename S, int DK, bool REVERSE>
-__device__ inline void delta_inverse(const DeltaGates& d, float* inv, const E* tk, int blk, int lane) {
-  constexpr int NB = S::NB, LDT = S::LDT;
-  const int lo = lane & 15, hi = lane >> 4, r0 = blk * S::BS;
-  float* tiles = inv + blk * S::TRI * S::TILE;
-  auto a_tile = [&](int i, int j) {
-    f32x4 a = row_products<E, DK>(tk, r0 + 16 * j, tk, r0 + 16 * i, S::LDK, lane);
-    const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
-    const float bi = d.beta[r0 + 16 * i + lo];
-    const f32x4 bj = lds_f4(d.beta + r0 + 16 * j + 4 * hi);
+// (X Y^T)^T of 16 rows of each, from their quads: a lane has Y's row lo, and of X rows 4 hi + r
+template <typename E, int KA>
+__device__ inline f32x4 row_products(const quad_t<E> (&x)[KA], const quad_t<E> (&y)[KA]) {
+  f32x4 t = {0, 0, 0, 0};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) a[r] = i > j || 4 * hi + r < lo ? a[r] * __expf(lag[r]) * (REVERSE ? bi : bj[r]) : 0.0f;
-    return a;
-  };
-  auto rows = [&](int k) { return reinterpret_cast<f32x4*>(tiles + k * S::TILE + lo * LDT + 4 * hi); };
-  auto columns = [&](int k) { return lds_quad_t(tiles + k * S::TILE, LDT, 0, 0, lane); };
-  f32x4 a10, a[NB][4], t[NB];
+  for (int m = 0; m < KA; m += 2) t = mma2(x[m], x[m + 1], y[m], y[m + 1], t);
+  return t;
+}
+
+// What the walkers need of a block, by one wave.  INVERSE: the tiles on the diagonal of (I + A)^-1, or with
+// REVERSE of (I + A')^-T, and the other tile of -A, or of -A'^T; each has beta of the column.  SCORES: put(tile (i, j),
+// values) with scale (q_i . k_j) Gamma_ij, a lane having i = lo and j = 4 hi + r, or with REVERSE j = lo and
+// i = 4 hi + r.
+template <typename E, typename S, int DK, bool REVERSE, bool INVERSE, bool SCORES, typename Put>
+__device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk, const E* tq, float scale, int lane, Put put) {
+  constexpr int NB = S::NB, LDT = S::LDT, KA = DK / 16;
+  const int lo = lane & 15, hi = lane >> 4;
+  quad_t<E> k[NB][KA];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = a_tile(i, i);
-  if constexpr (NB == 2) a10 = a_tile(1, 0);
-  __builtin_amdgcn_wave_barrier();
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
+    for (int m = 0; m < KA; ++m) k[i][m] = lds_quad(tk, S::LDK, 16 * i, 16 * m, lane);
+  if constexpr (SCORES) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[i][j] = lds_f4(tiles + tri(i, i) * S::TILE + lo * LDT + 4 * j);  // row lo
+    for (int i = 0; i < NB; ++i) {
+      quad_t<E> q[KA];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t[i][r] = 4 * hi + r == lo ? 1.0f : 0.0f;
+      for (int m = 0; m < KA; ++m) q[m] = lds_quad(tq, S::LDK, 16 * i, 16 * m, lane);
+#pragma unroll
+      for (int j = 0; j <= i; ++j) {
+        f32x4 x = REVERSE ? row_products<E, KA>(q, k[j]) : row_products<E, KA>(k[j], q);
+        const f32x4 ratio = delta_ratio<REVERSE>(d, REVERSE ? 16 * j : 16 * i, REVERSE ? 16 * i : 16 * j, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[r] = i > j || (REVERSE ? 4 * hi + r >= lo : 4 * hi + r <= lo) ? scale * (x[r] * ratio[r]) : 0.0f;
+        put(tri(i, j), x);
+      }
+    }
   }
-  // row lo of the inverse, columns 4 hi + r: takes off A[lo][j] times row j, which is final by then
-  steps<15>([&](auto j) {
+  if constexpr (INVERSE) {
+    auto rows = [&](int k) { return reinterpret_cast<f32x4*>(inv + k * S::TILE + lo * LDT + 4 * hi); };
+    auto a_tile = [&](int i, int j) {  // lane: row 16 i + lo, columns 16 j + 4 hi + r
+      f32x4 a = row_products<E, KA>(k[j], k[i]);
+      const f32x4 ratio = delta_ratio<REVERSE>(d, 16 * i, 16 * j, lane), beta = lds_f4(d.beta + 16 * j + 4 * hi);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+      for (int r = 0; r < 4; ++r)
+        a[r] = i != j || (REVERSE ? 4 * hi + r > lo : 4 * hi + r < lo) ? -(a[r] * ratio[r] * beta[r]) : 0.0f;
+      return a;
+    };
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[i][r] = fmaf(-a[i][j() / 4][j() % 4], row_lane<j()>(t[i][r]), t[i][r]);
-  });
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll
-  for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = t[i];
-  f32x4 corner;
-  if constexpr (NB == 2) {  // the corner: -T11 A10 T00
-    __builtin_amdgcn_wave_barrier();
-    const f32x4 zero = {0, 0, 0, 0}, y = mma16(a10, columns(tri(0, 0)), zero);
-    corner = REVERSE ? -mma16(t[1], y, zero) : -mma16(y, t[1], zero);
-    *rows(tri(1, 0)) = corner;
-  }
-  if constexpr (REVERSE) {
-    __builtin_amdgcn_wave_barrier();
-    f32x4 c[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) c[i] = columns(tri(i, i));
+    for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = a_tile(i, i);
+    if constexpr (NB == 2) *rows(tri(1, 0)) = REVERSE ? a_tile(0, 1) : a_tile(1, 0);
+    f32x4 a[NB][4], t[2];
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = c[i];
+    for (int i = 0; i < 2; ++i) {
+      if (i < NB)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[i][j] = lds_f4(inv + tri(i, i) * S::TILE + lo * LDT + 4 * j);  // -A's row lo
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[i][r] = 4 * hi + r == lo ? 1.0f : 0.0f;
+    }
+    // row lo of the inverse, columns 4 hi + r: takes off A[lo][j] times row j, which is final by then
+    steps<15>([&](auto n) {
+      constexpr int j = REVERSE ? 15 - n() : n();
+      subtract_row<j>(t[0], a[0][j / 4][j % 4], t[1], a[NB - 1][j / 4][j % 4]);
+    });
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = t[i];
   }
 }
 
@@ -252,28 +288,29 @@ struct DeltaRows {
   const E* base;  // step 0
   int64_t step;   // elements between steps
   int width, row, c;
+  unsigned off;   // bytes of the thread's first piece
   bool vec;
 
   __device__ void init(const E* b, int64_t stride, int d, bool whole, int tid) {
     row = tid / W, c = (tid - row * W) * P, step = stride, base = b, width = d, vec = whole;
+    off = c < width && row < RS ? (unsigned)(row * (int)step + c) * (unsigned)sizeof(E) : kNowhere;
   }
   // rows t0 ..., n of them live (zeros behind them)
-  __device__ void load(int t0, int n) {
+  __device__ void load(int64_t t0, int n) {
     const __amdgpu_buffer_rsrc_t rs = buffer_at(base + t0 * step);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int t = row + i * RS;
-      const unsigned at = t < n && c < width && row < RS ? (unsigned)((t * step + c) * (int64_t)sizeof(E)) : kNowhere;
+      const unsigned at = row + i * RS < n ? off : kNowhere, past = (unsigned)(i * RS * (int)step) * (unsigned)sizeof(E);
       if (vec) {
-        r[i] = __builtin_bit_cast(piece_t<E>, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+        r[i] = __builtin_bit_cast(piece_t<E>, __builtin_amdgcn_raw_buffer_load_b128(rs, at, past, 0));
       } else {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
           const unsigned ae = c + e < width && at != kNowhere ? at + e * (unsigned)sizeof(E) : kNowhere;
           if constexpr (sizeof(E) == 4)
-            r[i][e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, ae, 0, 0));
+            r[i][e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, ae, past, 0));
           else
-            r[i][e] = __builtin_bit_cast(bf16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, ae, 0, 0));
+            r[i][e] = __builtin_bit_cast(bf16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, ae, past, 0));
         }
       }
     }
@@ -332,7 +369,7 @@ __device__ inline f32x4 mma_terms(const f32x4 (&a)[NB], const Terms<float> (&x)[
 // For the block's tiles i: K_i s (16 rows, the wave's 16 columns) exact to fp32, and with OT > 0
 // (Q_i s)^T by s's first OT terms.
 template <typename E, typename S, int KA, int OT>
-__device__ inline void delta_state_products(const E* k, const E* q, int row0, const f32x4 (&s)[KA][1], f32x4 (&ks)[S::NB],
+__device__ inline void delta_state_products(const E* k, const E* q, const f32x4 (&s)[KA][1], f32x4 (&ks)[S::NB],
                                             f32x4 (&qs)[S::NB], int lane) {
 #pragma unroll
   for (int i = 0; i < S::NB; ++i) ks[i] = qs[i] = f32x4{0, 0, 0, 0};
@@ -341,7 +378,7 @@ __device__ inline void delta_state_products(const E* k, const E* q, int row0, co
     const Terms<E> a(s[m][0]), b(s[m + 1][0]);
 #pragma unroll
     for (int i = 0; i < S::NB; ++i) {
-      const int r0 = row0 + 16 * i;
+      const int r0 = 16 * i;
       const quad_t<E> k0 = lds_quad(k, S::LDK, r0, 16 * m, lane), k1 = lds_quad(k, S::LDK, r0, 16 * m + 16, lane);
 #pragma unroll
       for (int t = 0; t < Terms<E>::N; ++t) ks[i] = mma2(k0, k1, a.t[t], b.t[t], ks[i]);
@@ -354,17 +391,35 @@ __device__ inline void delta_state_products(const E* k, const E* q, int row0, co
   }
 }
 
-// e = (I + A)^-1 x over the block's tiles, from the inverse's tiles or with REVERSE its transpose's
+// e = (I + A)^-1 x, or with REVERSE (I + A')^-T x, over the block's tiles, from what delta_setup left
 template <typename S, bool REVERSE>
-__device__ inline void delta_solve(const float* tiles, const f32x4 (&x)[S::NB], f32x4 (&e)[S::NB], int lane) {
-  const float* at = tiles + (lane & 15) * S::LDT + 4 * (lane >> 4);
-#pragma unroll
-  for (int i = 0; i < S::NB; ++i) {
-    e[i] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < S::NB; ++j)
-      if (REVERSE ? j >= i : j <= i) e[i] = mma16(lds_f4(at + (REVERSE ? tri(j, i) : tri(i, j)) * S::TILE), x[j], e[i]);
+__device__ inline void delta_solve(const float* inv, f32x4 (&x)[S::NB], f32x4 (&e)[S::NB], int lane) {
+  const float* at = inv + (lane & 15) * S::LDT + 4 * (lane >> 4);
+  const f32x4 zero = {0, 0, 0, 0};
+  if constexpr (S::NB == 2) {
+    constexpr int first = REVERSE ? 1 : 0, second = 1 - first;
+    const f32x4 t0 = lds_f4(at + tri(first, first) * S::TILE), corner = lds_f4(at + tri(1, 0) * S::TILE);
+    const f32x4 t1 = lds_f4(at + tri(second, second) * S::TILE);
+    e[first] = mma16(t0, x[first], zero);
+    x[second] = mma16(corner, e[first], x[second]);
+    e[second] = mma16(t1, x[second], zero);
+  } else {
+    e[0] = mma16(lds_f4(at), x[0], zero);
   }
+}
+
+// K^T as operands, and s := total s + K^T w
+template <typename E, typename S, int KA>
+__device__ inline void transposed_rows(const E* k, quad_t<E> (&kt)[KA][S::NB], int lane) {
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+#pragma unroll
+    for (int i = 0; i < S::NB; ++i) kt[m][i] = lds_quad_t(k, S::LDK, 16 * i, 16 * m, lane);
+}
+template <typename E, int KA, int NB>
+__device__ inline void delta_state_update(const quad_t<E> (&kt)[KA][NB], const Terms<E> (&w)[NB], float total, f32x4 (&s)[KA][1]) {
+#pragma unroll
+  for (int m = 0; m < KA; ++m) s[m][0] = mma_terms(kt[m], w, s[m][0] * total);
 }
 
 // A wave's columns of a history whose state is not finite in the end, by the definition, a step at
@@ -410,229 +465,341 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
   if (p.s_out && seg == (L - 1) / p.seg_len) store_state(s, p.s_out + bh * size, p.dk, p.dv, col0, lo, hi);
 }
 
-template <typename E, int DK, int DV>
-constexpr size_t delta_forward_lds() {
-  using S = DeltaShape<E, DK, DV>;
-  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::SCORES + 2 * S::C * S::LDK + S::C * S::LDV);
+// ---- backward ----
+// Three kernels.  The first walks forwards in time as the forward pass does and leaves e_t, the state
+// at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
+// which gives y = dv and dbeta, and leaves the gradient at each chunk's end: over a block,
+//   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_15 - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
+//   R := exp(G_15) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y,  Y = diag(beta) dU.
+// With the state and its gradient known at its ends every chunk then gives its dq and dk by itself:
+//   dq_i = scale exp(G_i) do_i S^T + sum_{j <= i} M_ij k_j,  M_ij = scale Gamma_ij (do_i . u_j),
+//   dk_j = exp(G_end - G_j) u_j R^T - exp(G_j) y_j S^T + sum_{i >= j} M_ij q_i
+//          - sum_{i > j} N_ij k_i - sum_{l < j} N_jl k_l,  N_ij = Gamma_ij (y_i . u_j).
+// log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>; what makes it change from step to step is
+// dg_t = dg_{t+1} + do_t . o_t - dv_t . v_t, so it is that sum from the end of each stretch of 256
+// steps, where both matrices are at hand in fp32, and o enters it unrounded.  (No values that are not
+// finite are looked for here: they may spoil the gradients of their whole history and head.)
+template <typename E>
+struct DeltaBwdArgs {
+  DeltaArgs<E> f;
+  const E* d_o;
+  int64_t dos[3];
+  const float* d_out;  // (B, H, dk, dv) or NULL
+  int chunks, stretches;  // of T
+  E *e;                // (B H, chunks C, DV)
+  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends
+  float *w, *z;        // (B H, chunks C): do . o, y . v
+  float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
+  float* dot;          // (B H, stretches): <R, S> there
+  E* y;                // as e, or dv's output (B, T, H, dv)
+  int64_t ys[2];       // its strides of (b h) and step, from b and h where it is the output
+  int y_width;
+  float* y_part;       // (B, T, H, dv) or NULL
+  E* dbeta;            // (B, T, H)
+  float* dg;           // (B, T, H)
+  float* d_in;         // (B, H, dk, dv) or NULL
+  float* r_seg;        // f.segs > 1: as f.seg_state, of the state's gradient at the runs' ends
+  void *dq, *dk;       // (B, T, H, dk) of E, or fp32 parts
+  int q_part, k_part;
+};
+// sum over the 16 lanes of a row
+__device__ inline float row16_sum(float v) {
+#define TMPC_ROR(n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + n, 0xf, 0xf, false))
+  v += TMPC_ROR(8);
+  v += TMPC_ROR(4);
+  v += TMPC_ROR(2);
+  v += TMPC_ROR(1);
+#undef TMPC_ROR
+  return v;
 }
 
-// A workgroup a run of a (problem, head).
-template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_FORWARD)) void delta_forward_kernel(
-    DeltaArgs<E> p) {
+// The wave's 16 columns of a state, rounded, as rows of a (DV, DK) matrix.
+template <typename E, int DK, int KA>
+__device__ inline void store_columns(E* dst, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
+#pragma unroll
+  for (int m = 0; m < KA; ++m)
+    *reinterpret_cast<quad_t<E>*>(dst + (col0 + lo) * DK + 16 * m + 4 * hi) = to_quad<E>(s[m][0]);
+}
+
+// Rows of a tile in LDS to memory: `n` of them, row t at dst + t pitch.
+template <typename R, typename E>
+__device__ inline void copy_out(const R& map, const E* tile, E* dst, int64_t pitch, int n, int width) {
+  constexpr int P = Elem<E>::PIECE;
+  if (map.row >= R::RS) return;
+#pragma unroll
+  for (int i = 0; i < R::N; ++i) {
+    const int row = map.row + i * R::RS;
+    if (row < n && map.c < width)
+      store_piece(dst + row * pitch, map.c, width, *reinterpret_cast<const piece_t<E>*>(tile + row * R::LD + map.c));
+  }
+  (void)P;
+}
+
+// A long history of few heads does not fill the chip: it is cut into runs.  A run is a linear map of the
+// state it starts from, S -> M S + N: a first pass (WALK_RUN) makes each run's M (its columns start from the
+// unit matrix, with values of zero) and N (from zero), a scan carries the states through, and the
+// outputs start from those.  There a wave has 16 columns of [N | M].
+enum DeltaWalk { WALK_OUT, WALK_STATES, WALK_RUN };
+
+template <typename E, int DK, int DV, int MODE>
+struct DeltaWalkLds {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP;
+  static constexpr bool SCORES = MODE != WALK_RUN, DO = MODE == WALK_STATES;
+  // a buffer's bytes: gates, inverses, scores (of E, or for the states fp32), sums, rows of K, V, Q, dO
+  static constexpr size_t inv = sizeof(float) * S::GATES, scores = inv + sizeof(float) * S::INV;
+  static constexpr size_t sums = scores + (MODE == WALK_OUT ? sizeof(E) * S::SCORES : DO ? sizeof(float) * S::INV : 0);
+  static constexpr size_t k = sums + (DO ? sizeof(float) * S::W * S::C : 0), v = k + sizeof(E) * S::C * S::LDK;
+  static constexpr size_t q = v + sizeof(E) * S::C * S::LDV, d_o = q + (SCORES ? sizeof(E) * S::C * S::LDK : 0);
+  static constexpr size_t bytes = d_o + (DO ? sizeof(E) * S::C * S::LDV : 0), all = 2 * bytes;
+};
+
+// A workgroup a run of a (problem, head).
+template <typename E, int DK, int DV, int MODE>
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_walk_kernel(
+    DeltaBwdArgs<E> a, int run_width) {
+  using S = DeltaShape<E, DK, DV>;
+  using M = DeltaWalkLds<E, DK, DV, MODE>;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDV = S::LDV, LDT = S::LDT, LDP = S::LDP, CK = AttnTile<E>::C;
   extern __shared__ __align__(16) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
+  const DeltaArgs<E>& p = a.f;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
   const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
-  const DeltaGates d = delta_gates<S>(smem);
-  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
-  E* tp = reinterpret_cast<E*>(inv + S::INV);  // the blocks' scores
-  E* tk = tp + S::SCORES;
-  E* tq = tk + C * LDK;
-  E* tv = tq + C * LDK;
-
-  DeltaRows<E, C, DK, S::THREADS> rk, rq;
-  DeltaRows<E, C, DV, S::THREADS> rv;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
-  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
-  auto fetch = [&](int t0) {
-    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rg.load(t0, L - t0, tid);
+  const int blocks = begin < L ? (L - begin + C - 1) / C : 0;
+  struct Buffer {
+    DeltaGates d;
+    float *inv, *sums;
+    char* scores;
+    E *k, *v, *q, *d_o;
   };
-  if (begin < L) fetch(begin);
-  f32x4 s[KA][1];
-  if (p.segs > 1) load_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
-  else load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
-  const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
-  const int oc = col0 + 4 * hi;
-  const unsigned ooff = oc < p.dv ? (unsigned)((lo * orow + oc) * sizeof(E)) : kNowhere;
-  const unsigned otile = (unsigned)(16 * orow * sizeof(E));
+  auto buffer = [&](int i) {
+    char* x = smem + (i & 1) * M::bytes;
+    return Buffer{delta_gates<S>((float*)x), (float*)(x + M::inv), (float*)(x + M::sums), x + M::scores, (E*)(x + M::k),
+                  (E*)(x + M::v), (E*)(x + M::q), (E*)(x + M::d_o)};
+  };
 
-  for (int t0 = begin; t0 < L; t0 += C) {
-    const int n = min(C, L - t0);
-    rk.store(tk), rq.store(tq), rv.store(tv), rg.store(d, tid);
-    __syncthreads();
-    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
-      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
-      if (r0 >= n) continue;
-      if (task < S::NBLK) {
-        delta_inverse<E, S, DK, false>(d, inv, tk, blk, lane);
-        continue;
+  if (wave >= S::W) {  // ---- a helper
+    constexpr int THREADS = 128;
+    const int helper = wave - S::W, htid = tid - S::WALKERS - 64;
+    if (helper == 0) {
+      __builtin_amdgcn_s_setprio(3);  // the longest way from meeting to meeting
+      DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+      rg.start(begin + lane, false);
+      auto fetch = [&](int c) { rg.load(L - begin - c * C, lane); };
+      auto setup = [&](int c) {
+        const Buffer x = buffer(c);
+        delta_setup<E, S, DK, false, true, false>(x.d, x.inv, x.k, x.q, p.scale, here(lane), [](int, f32x4) {});
+      };
+      if (blocks > 0) fetch(0), rg.scan(lane), rg.store(buffer(0).d, lane);
+      meet();
+      if (blocks > 1) fetch(1);
+      if (blocks > 0) setup(0);
+      if (blocks > 1) rg.scan(lane);
+      meet();
+      for (int c = 0; c < blocks; ++c) {
+        if (c + 1 < blocks) rg.store(buffer(c + 1).d, lane);
+        meet();
+        if (c + 2 < blocks) fetch(c + 2);
+        if (c + 1 < blocks) setup(c + 1);
+        if (c + 2 < blocks) rg.scan(lane);
+        meet();
       }
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j <= i; ++j) {
-          f32x4 x = row_products<E, DK>(tk, r0 + 16 * j, tq, r0 + 16 * i, LDK, lane);
-          const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r <= lo ? p.scale * (x[r] * __expf(lag[r])) : 0.0f;
-          *reinterpret_cast<quad_t<E>*>(tp + (blk * S::TRI + tri(i, j)) * S::TILE_P + lo * LDP + 4 * hi) = to_quad<E>(x);
-        }
+      return;
     }
-    __syncthreads();
-    if (t0 + C < L) fetch(t0 + C);
-    const __amdgpu_buffer_rsrc_t rs = buffer_at(p.o + obase + t0 * orow);
-#pragma unroll 1
-    for (int blk = 0; blk * S::BS < n; ++blk) {
-      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
-      f32x4 o[NB], x[NB], u[NB];
-      delta_state_products<E, S, KA, Terms<E>::N == 3 ? 2 : 1>(tk, tq, r0, s, x, o, lane);
+    DeltaRows<E, C, DK, THREADS> rk, rq;
+    DeltaRows<E, C, DV, THREADS> rv, rdo;
+    const int c0 = MODE == WALK_RUN ? blockIdx.y * DV : 0;  // the first of the workgroup's columns
+    rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, htid);
+    rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2] + min(c0, p.dv), p.vs[1], min(max(p.dv - c0, 0), DV), p.vec, htid);
+    if constexpr (M::SCORES) rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, htid);
+    if constexpr (M::DO) rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, htid);
+    auto fetch = [&](int c) {
+      const int t0 = begin + c * C;
+      rk.load(t0, L - t0), rv.load(t0, L - t0);
+      if constexpr (M::SCORES) rq.load(t0, L - t0);
+      if constexpr (M::DO) rdo.load(t0, L - t0);
+    };
+    auto stage = [&](int c) {
+      const Buffer x = buffer(c);
+      rk.store(x.k), rv.store(x.v);
+      if constexpr (M::SCORES) rq.store(x.q);
+      if constexpr (M::DO) rdo.store(x.d_o);
+    };
+    auto setup = [&](int c) {
+      const Buffer x = buffer(c);
+      [[maybe_unused]] const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+      auto put = [&](int tile, f32x4 s) {
+        if constexpr (M::DO) *reinterpret_cast<f32x4*>((float*)x.scores + tile * S::TILE + lo * LDT + 4 * hi) = s;
+        else *reinterpret_cast<quad_t<E>*>((E*)x.scores + tile * S::TILE_P + lo * LDP + 4 * hi) = to_quad<E>(s);
+      };
+      if constexpr (M::SCORES)
+        if (helper == 1) delta_setup<E, S, DK, false, false, true>(x.d, x.inv, x.k, x.q, p.scale, lane, put);
+    };
+    auto results = [&](int c) {  // of a block that the walkers have left
+      if constexpr (M::DO) {
+        const Buffer x = buffer(c);
+        const int t0 = begin + c * C, n = min(C, L - t0);
+        copy_out(rv, x.v, a.e + ((int64_t)bh * a.chunks * CK + t0) * DV, DV, n, DV);
+        if (htid < n) {
+          float w = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        x[i] = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane)) - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
-      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
-      Terms<E> w[NB];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        u[i] *= lds_f4(d.beta + r0 + 16 * i + 4 * hi);
-        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * u[i]);
+          for (int i = 0; i < S::W; ++i) w += x.sums[i * C + htid];
+          a.w[(int64_t)bh * a.chunks * CK + t0 + htid] = w;
+        }
       }
-      const float total = d.total[blk];
+    };
+    if (blocks > 0) fetch(0), stage(0);
+    meet();
+    if (blocks > 1) fetch(1);
+    if (blocks > 0) setup(0);
+    meet();
+    for (int c = 0; c < blocks; ++c) {
+      if (c > 0) results(c - 1);
+      if (c + 1 < blocks) stage(c + 1);
+      meet();
+      if (c + 2 < blocks) fetch(c + 2);
+      if (c + 1 < blocks) setup(c + 1);
+      meet();
+    }
+    if (blocks > 0) results(blocks - 1);
+    return;
+  }
+
+  // ---- a walker
+  f32x4 s[KA][1];
+  const int unit = MODE == WALK_RUN ? (blockIdx.y * S::W + wave) * 16 - run_width : 0;  // its first column of the unit matrix
+  {
+    const int lo = lane & 15, hi = lane >> 4;
+    if constexpr (MODE == WALK_RUN) {
 #pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        quad_t<E> kt[NB];
+      for (int m = 0; m < KA; ++m)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
-        s[m][0] = mma_terms(kt, w, s[m][0] * total);
-      }
-      // outputs, bf16: the scores are rounded, the state and u enter by two terms (16 bits)
+        for (int r = 0; r < 4; ++r) s[m][0][r] = 16 * m + 4 * hi + r == unit + lo ? 1.0f : 0.0f;
+    } else if (p.segs > 1) {
+      load_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, wave * 16, lo, hi);
+    } else {
+      load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, wave * 16, lo, hi);
+    }
+  }
+  const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
+  const int oc = wave * 16 + 4 * (lane >> 4);
+  const unsigned ooff = oc < p.dv ? (unsigned)(((lane & 15) * (int)orow + oc) * (int)sizeof(E)) : kNowhere;
+  const unsigned otile = (unsigned)(16 * (int)orow * (int)sizeof(E));
+  meet();
+  meet();
+  for (int c = 0; c < blocks; ++c) {
+    const int t0 = begin + c * C, n = min(C, L - t0);
+    const Buffer x = buffer(c);
+    if (M::DO && t0 % CK == 0)
+      store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + t0 / CK) * DK * DV, s, wave * 16, lane & 15, lane >> 4);
+    const __amdgpu_buffer_rsrc_t rs = buffer_at(MODE == WALK_OUT ? p.o + obase + t0 * orow : nullptr);
+    const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
+    f32x4 o[NB], e[NB], u[NB];
+    // the state and u enter outputs of bf16 by two terms (16 bits)
+    constexpr int OT = MODE == WALK_RUN ? 0 : M::DO ? Terms<E>::N : (Terms<E>::N + 1) / 2;
+    meet();
+    delta_state_products<E, S, KA, OT>(x.k, x.q, s, e, o, lane);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      e[i] = to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane)) - lds_f4(x.d.from + 16 * i + 4 * hi) * e[i];
+    quad_t<E> kt[KA][NB];  // read ahead of their use
+    transposed_rows<E, S, KA>(x.k, kt, lane);
+    f32x4 beta[NB], to[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) beta[i] = lds_f4(x.d.beta + 16 * i + 4 * hi), to[i] = lds_f4(x.d.to + 16 * i + 4 * hi);
+    const float total = *x.d.total;
+    delta_solve<S, false>(x.inv, e, u, lane);
+    Terms<E> w[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      // these columns of V are this wave's alone and have been read: e takes their place
+      if constexpr (M::DO)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x.v[(16 * i + 4 * hi + r) * LDV + col0 + lo] = (E)u[i][r];
+      u[i] *= beta[i];
+      w[i] = Terms<E>(to[i] * u[i]);
+    }
+    delta_state_update<E, KA, NB>(kt, w, total, s);
+    if constexpr (MODE == WALK_OUT) {
       Terms<E> ut[NB];
 #pragma unroll
       for (int i = 0; i < NB; ++i) ut[i] = Terms<E>(u[i]);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        o[i] *= p.scale * d.from[r0 + 16 * i + lo];
-        const E* pt = tp + (blk * S::TRI + tri(i, 0)) * S::TILE_P + lo * LDP + 4 * hi;
+        o[i] *= p.scale * x.d.from[16 * i + lo];
+        const E* pt = (const E*)x.scores + (tri(i, 0)) * S::TILE_P + lo * LDP + 4 * hi;
 #pragma unroll
         for (int j = 0; j <= i; ++j) {
-          const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(pt + j * S::TILE_P);
+          const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(pt + j * S::TILE_P);  // rounded, in bf16
           if constexpr (sizeof(E) == 2) o[i] = mma2(ut[j].t[0], ut[j].t[1], pq, pq, o[i]);
           else o[i] = mma16(u[j], pq, o[i]);
         }
-        const unsigned at = r0 + 16 * i + lo < n && ooff != kNowhere ? ooff + (blk * NB + i) * otile : kNowhere;
+        const unsigned at = 16 * i + lo < n ? ooff : kNowhere, past = i * otile;
         if (p.vec) {
-          if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i]), rs, at, 0, 0);
-          else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, to_bf16(o[i])), rs, at, 0, 0);
+          if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i]), rs, at, past, 0);
+          else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, to_bf16(o[i])), rs, at, past, 0);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned ae = oc + e < p.dv && at != kNowhere ? at + e * (unsigned)sizeof(E) : kNowhere;
-            const float f = o[i][e];
-            if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f), rs, ae, 0, 0);
-            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (bf16)f), rs, ae, 0, 0);
+          for (int r = 0; r < 4; ++r) {
+            const unsigned ae = oc + r < p.dv && at != kNowhere ? at + r * (unsigned)sizeof(E) : kNowhere;
+            const float f = o[i][r];
+            if constexpr (sizeof(E) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f), rs, ae, past, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (bf16)f), rs, ae, past, 0);
           }
         }
       }
     }
-    __syncthreads();
-  }
-  // What follows makes its indexes and reads its arguments again: they would be kept through every chunk.
-  auto* args = __builtin_amdgcn_kernarg_segment_ptr();
-  int etid = tid, block = blockIdx.x;
-  asm volatile("" : "+v"(etid), "+s"(args), "+s"(block));
-  const DeltaArgs<E>& a = *(const DeltaArgs<E>*)args;
-  const int ebh = block / a.segs, eseg = block - ebh * a.segs, eb = ebh / a.H, eL = delta_length(a, eb);
-  const int ebegin = eseg * a.seg_len;
-  zero_rows(a.o, false, sizeof(E), ((int64_t)eb * a.T * a.H + (ebh - eb * a.H)) * a.dv, (int64_t)a.H * a.dv, a.dv, max(eL, ebegin),
-            min((int64_t)a.T, (int64_t)ebegin + a.seg_len), etid, S::THREADS);
-  // An infinite or NaN value leaves the state so, to the end.
-  f32x4 zero = {0, 0, 0, 0};
-#pragma unroll
-  for (int m = 0; m < KA; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][0][r], 0.0f, zero[r]);
-  if (ebegin < eL && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
-    __threadfence_block();  // rows written above are written again
-    delta_by_step<E, KA, DV>(a, block, etid);
-  } else if (a.s_out && eseg == (eL > 0 ? (eL - 1) / a.seg_len : 0)) {  // the run that holds the last live step
-    store_state(s, a.s_out + ebh * ((int64_t)a.dk * a.dv), a.dk, a.dv, (etid >> 6) * 16, etid & 15, (etid & 63) >> 4);
-  }
-}
-
-// A long history of few heads does not fill the chip: it is cut into runs.  A run is a linear map of the
-// state it starts from, S -> M S + N: a first pass makes each run's M (its columns start from the unit
-// matrix, with values of zero) and N (from zero), a scan carries the states through, and the outputs
-// start from those.  A wave 16 columns of [N | M].
-template <typename E, int DK>
-constexpr size_t delta_run_lds() {
-  using S = DeltaShape<E, DK, 64>;
-  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (S::C * S::LDK + S::C * S::LDV);
-}
-template <typename E, int DK>
-__global__ __launch_bounds__(256, DK <= 64 ? 3 : 2) void delta_run_kernel(DeltaArgs<E> p, int DV) {
-  using S = DeltaShape<E, DK, 64>;
-  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV;
-  extern __shared__ __align__(16) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
-  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
-  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);
-  const int tile = blockIdx.y * 4 + wave, unit = tile * 16 - DV;  // the first of its columns of the unit matrix
-  const DeltaGates d = delta_gates<S>(smem);
-  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
-  E* tk = reinterpret_cast<E*>(inv + S::INV);
-  E* tv = tk + C * LDK;
-  DeltaRows<E, C, DK, 256> rk;
-  DeltaRows<E, C, 64, 256> rv;
-  const int c0 = blockIdx.y * 64;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2] + min(c0, p.dv), p.vs[1], min(max(p.dv - c0, 0), 64), p.vec, tid);
-  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
-  auto fetch = [&](int t0) { rk.load(t0, L - t0), rv.load(t0, L - t0), rg.load(t0, L - t0, tid); };
-  if (begin < L) fetch(begin);
-  f32x4 s[KA][1];
-#pragma unroll
-  for (int m = 0; m < KA; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s[m][0][r] = 16 * m + 4 * hi + r == unit + lo ? 1.0f : 0.0f;
-  for (int t0 = begin; t0 < L; t0 += C) {
-    const int n = min(C, L - t0);
-    rk.store(tk), rv.store(tv), rg.store(d, tid);
-    __syncthreads();
-    if (wave < S::NBLK && wave * S::BS < n) delta_inverse<E, S, DK, false>(d, inv, tk, wave, here(lane));
-    __syncthreads();
-    if (t0 + C < L) fetch(t0 + C);
-#pragma unroll 1
-    for (int blk = 0; blk * S::BS < n; ++blk) {
-      const int r0 = blk * S::BS, lane = here(tid & 63), hi = lane >> 4, col0 = here(wave) * 16;
-      f32x4 none[NB], x[NB], u[NB];
-      delta_state_products<E, S, KA, 0>(tk, tk, r0, s, x, none, lane);
+    if constexpr (M::DO) {  // do . o, unrounded
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const f32x4 v = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane));  // zeros for the unit matrix' columns
-        x[i] = v - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
-      }
-      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
-      Terms<E> w[NB];
+        o[i] *= p.scale * x.d.from[16 * i + lo];
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * (lds_f4(d.beta + r0 + 16 * i + 4 * hi) * u[i]));
-      const float total = d.total[blk];
-#pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        quad_t<E> kt[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
-        s[m][0] = mma_terms(kt, w, s[m][0] * total);
+        for (int j = 0; j <= i; ++j)
+          o[i] = mma16(u[j], lds_f4((const float*)x.scores + (tri(i, j)) * S::TILE + lo * LDT + 4 * hi), o[i]);
+        o[i] *= to_f32(lds_quad(x.d_o, LDV, 16 * i, col0, lane));
+        float w1 = o[i][0] + o[i][1] + o[i][2] + o[i][3];
+        w1 += __shfl_xor(w1, 16, 64), w1 += __shfl_xor(w1, 32, 64);
+        if (hi == 0) x.sums[wave * C + 16 * i + lo] = w1;
       }
     }
-    __syncthreads();
+    if (M::DO && ((t0 + C) % kDeltaSeg == 0 || t0 + C >= L)) {
+    f32x4* dst = reinterpret_cast<f32x4*>(a.s_seg + ((int64_t)bh * a.stretches + t0 / kDeltaSeg) * DK * DV) + wave * KA * 64 + lane;
+#pragma unroll
+    for (int m = 0; m < KA; ++m) dst[m * 64] = s[m][0];
+    }
+    meet();
   }
-  if (unit >= 0) {
-    if (unit < DK) store_state(s, p.seg_map + blockIdx.x * (int64_t)(DK * DK), DK, DK, unit, lo, hi);
-  } else {
-    store_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), DK, DV, tile * 16, lo, hi);
+  if constexpr (MODE == WALK_RUN) {
+    const int lo = lane & 15, hi = lane >> 4;
+    if (unit >= 0) {
+      if (unit < DK) store_state(s, p.seg_map + blockIdx.x * (int64_t)(DK * DK), DK, DK, unit, lo, hi);
+    } else {
+      store_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * run_width), DK, run_width, unit + run_width, lo, hi);
+    }
   }
-}
-
-// The same backwards in time: what a run adds to the gradient of the state that it starts from.
-template <typename E, int DK>
-constexpr size_t delta_reverse_run_lds() {
-  using S = DeltaShape<E, DK, 64>;
-  return sizeof(float) * (S::GATES + S::INV) + sizeof(E) * (Terms<E>::N * S::SCORES + 2 * S::C * S::LDK + S::C * S::LDV);
+  if constexpr (MODE == WALK_OUT) {
+    // What follows makes its indexes and reads its arguments again: they would be kept through every chunk.
+    auto* args = __builtin_amdgcn_kernarg_segment_ptr();
+    int etid = tid, block = blockIdx.x;
+    asm volatile("" : "+v"(etid), "+s"(args), "+s"(block));
+    const DeltaArgs<E>& f = ((const DeltaBwdArgs<E>*)args)->f;
+    const int ebh = block / f.segs, eseg = block - ebh * f.segs, eb = ebh / f.H, eL = delta_length(f, eb);
+    const int ebegin = eseg * f.seg_len;
+    zero_rows(f.o, false, sizeof(E), ((int64_t)eb * f.T * f.H + (ebh - eb * f.H)) * f.dv, (int64_t)f.H * f.dv, f.dv, max(eL, ebegin),
+              min((int64_t)f.T, (int64_t)ebegin + f.seg_len), etid, S::WALKERS);
+    // An infinite or NaN value leaves the state so, to the end.
+    f32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < KA; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) zero[r] = fmaf(s[m][0][r], 0.0f, zero[r]);
+    if (ebegin < eL && __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f))) {
+      __threadfence_block();  // rows written above are written again
+      delta_by_step<E, KA, DV>(f, block, etid);
+    } else if (f.s_out && eseg == (eL > 0 ? (eL - 1) / f.seg_len : 0)) {  // the run that holds the last live step
+      store_state(s, f.s_out + ebh * ((int64_t)f.dk * f.dv), f.dk, f.dv, (etid >> 6) * 16, etid & 15, (etid & 63) >> 4);
+    }
+  }
 }
 
 // Between the passes: each run's sum becomes the state it starts from (REVERSE: the state's gradient
@@ -703,236 +870,20 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const float* map, float
   }
 }
 
-// ---- backward ----
-// Three kernels.  The first walks forwards in time as the forward pass does and leaves e_t, the state
-// at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
-// which gives y = dv and dbeta, and leaves the gradient at each chunk's end: over a block,
-//   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_15 - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
-//   R := exp(G_15) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y,  Y = diag(beta) dU.
-// With the state and its gradient known at its ends every chunk then gives its dq and dk by itself:
-//   dq_i = scale exp(G_i) do_i S^T + sum_{j <= i} M_ij k_j,  M_ij = scale Gamma_ij (do_i . u_j),
-//   dk_j = exp(G_end - G_j) u_j R^T - exp(G_j) y_j S^T + sum_{i >= j} M_ij q_i
-//          - sum_{i > j} N_ij k_i - sum_{l < j} N_jl k_l,  N_ij = Gamma_ij (y_i . u_j).
-// log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>; what makes it change from step to step is
-// dg_t = dg_{t+1} + do_t . o_t - dv_t . v_t, so it is that sum from the end of each stretch of 256
-// steps, where both matrices are at hand in fp32, and o enters it unrounded.  (No values that are not
-// finite are looked for here: they may spoil the gradients of their whole history and head.)
-template <typename E>
-struct DeltaBwdArgs {
-  DeltaArgs<E> f;
-  const E* d_o;
-  int64_t dos[3];
-  const float* d_out;  // (B, H, dk, dv) or NULL
-  int chunks, segs;    // of T
-  E *e;                // (B H, chunks C, DV)
-  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends
-  float *w, *z;        // (B H, chunks C): do . o, y . v
-  float* s_seg;        // (B H, segs, the wave's registers): the states at the stretches' ends
-  float* dot;          // (B H, segs): <R, S> there
-  E* y;                // as e, or dv's output (B, T, H, dv)
-  int64_t ys[2];       // its strides of (b h) and step, from b and h where it is the output
-  int y_width;
-  float* y_part;       // (B, T, H, dv) or NULL
-  E* dbeta;            // (B, T, H)
-  float* dg;           // (B, T, H)
-  float* d_in;         // (B, H, dk, dv) or NULL
-  float* r_seg;        // f.segs > 1: as f.seg_state, of the state's gradient at the runs' ends
-  void *dq, *dk;       // (B, T, H, dk) of E, or fp32 parts
-  int q_part, k_part;
-};
-// sum over the 16 lanes of a row
-__device__ inline float row16_sum(float v) {
-#define TMPC_ROR(n) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + n, 0xf, 0xf, false))
-  v += TMPC_ROR(8);
-  v += TMPC_ROR(4);
-  v += TMPC_ROR(2);
-  v += TMPC_ROR(1);
-#undef TMPC_ROR
-  return v;
-}
-
-// The wave's 16 columns of a state, rounded, as rows of a (DV, DK) matrix.
-template <typename E, int DK, int KA>
-__device__ inline void store_columns(E* dst, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
-#pragma unroll
-  for (int m = 0; m < KA; ++m)
-    *reinterpret_cast<quad_t<E>*>(dst + (col0 + lo) * DK + 16 * m + 4 * hi) = to_quad<E>(s[m][0]);
-}
-
-// Rows of a tile in LDS to memory: `n` of them, row t at dst + t pitch.
-template <typename R, typename E>
-__device__ inline void copy_out(const R& map, const E* tile, E* dst, int64_t pitch, int n, int width) {
-  constexpr int P = Elem<E>::PIECE;
-  if (map.row >= R::RS) return;
-#pragma unroll
-  for (int i = 0; i < R::N; ++i) {
-    const int row = map.row + i * R::RS;
-    if (row < n && map.c < width)
-      store_piece(dst + row * pitch, map.c, width, *reinterpret_cast<const piece_t<E>*>(tile + row * R::LD + map.c));
-  }
-  (void)P;
-}
-
-template <typename E, int DK, int DV>
-constexpr size_t delta_states_lds() {
-  using S = DeltaShape<E, DK, DV>;
-  return sizeof(float) * (S::GATES + 2 * S::INV + S::W * S::C) + sizeof(E) * (2 * S::C * S::LDK + 2 * S::C * S::LDV);
-}
-
-template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_BACKWARD)) void delta_states_kernel(
-    DeltaBwdArgs<E> a) {
-  using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDT = S::LDT, SEG = kDeltaSeg / C;
-  extern __shared__ __align__(16) char smem[];
-  const DeltaArgs<E>& p = a.f;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
-  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
-  const DeltaGates d = delta_gates<S>(smem);
-  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
-  float* tp = inv + S::INV;   // the blocks' scores
-  float* sums = tp + S::INV;  // (waves, steps)
-  E* tk = reinterpret_cast<E*>(sums + S::W * C);
-  E* tq = tk + C * LDK;
-  E* tv = tq + C * LDK;
-  E* tdo = tv + C * LDV;
-
-  DeltaRows<E, C, DK, S::THREADS> rk, rq;
-  DeltaRows<E, C, DV, S::THREADS> rv, rdo;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
-  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
-  auto fetch = [&](int t0) {
-    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), rg.load(t0, L - t0, tid);
-  };
-  if (begin < L) fetch(begin);
-  f32x4 s[KA][1];
-  if (p.segs > 1) load_state(s, p.seg_state + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
-  else load_state(s, p.s_in ? p.s_in + bh * ((int64_t)p.dk * p.dv) : nullptr, false, p.dk, p.dv, col0, lo, hi);
-
-  for (int t0 = begin; t0 < L; t0 += C) {
-    const int n = min(C, L - t0), chunk = t0 / C;
-    rk.store(tk), rq.store(tq), rv.store(tv), rdo.store(tdo), rg.store(d, tid);
-    store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + chunk) * DK * DV, s, col0, lo, hi);
-    __syncthreads();
-    for (int task = wave; task < 2 * S::NBLK; task += S::W) {
-      const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
-      if (r0 >= n) continue;
-      if (task < S::NBLK) {
-        delta_inverse<E, S, DK, false>(d, inv, tk, blk, lane);
-        continue;
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int j = 0; j <= i; ++j) {
-          f32x4 x = row_products<E, DK>(tk, r0 + 16 * j, tq, r0 + 16 * i, LDK, lane);
-          const f32x4 lag = delta_lag(d, r0 + 16 * i, r0 + 16 * j, lane);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r <= lo ? p.scale * (x[r] * __expf(lag[r])) : 0.0f;
-          *reinterpret_cast<f32x4*>(tp + (blk * S::TRI + tri(i, j)) * S::TILE + lo * LDT + 4 * hi) = x;
-        }
-    }
-    __syncthreads();
-    if (t0 + C < L) fetch(t0 + C);
-#pragma unroll 1
-    for (int blk = 0; blk * S::BS < n; ++blk) {
-      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
-      f32x4 o[NB], x[NB], u[NB];
-      delta_state_products<E, S, KA, Terms<E>::N>(tk, tq, r0, s, x, o, lane);
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-        x[i] = to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane)) - lds_f4(d.from + r0 + 16 * i + 4 * hi) * x[i];
-      delta_solve<S, false>(inv + blk * S::TRI * S::TILE, x, u, lane);
-      Terms<E> w[NB];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        // these columns of V are this wave's alone and have been read: e takes their place
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tv[(r0 + 16 * i + 4 * hi + r) * LDV + col0 + lo] = (E)u[i][r];
-        u[i] *= lds_f4(d.beta + r0 + 16 * i + 4 * hi);
-        w[i] = Terms<E>(lds_f4(d.to + r0 + 16 * i + 4 * hi) * u[i]);
-      }
-      const float total = d.total[blk];
-#pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        quad_t<E> kt[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) kt[i] = lds_quad_t(tk, LDK, r0 + 16 * i, 16 * m, lane);
-        s[m][0] = mma_terms(kt, w, s[m][0] * total);
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        o[i] *= p.scale * d.from[r0 + 16 * i + lo];
-#pragma unroll
-        for (int j = 0; j <= i; ++j)
-          o[i] = mma16(u[j], lds_f4(tp + (blk * S::TRI + tri(i, j)) * S::TILE + lo * LDT + 4 * hi), o[i]);
-        o[i] *= to_f32(lds_quad(tdo, LDV, r0 + 16 * i, col0, lane));
-        float w1 = o[i][0] + o[i][1] + o[i][2] + o[i][3];
-        w1 += __shfl_xor(w1, 16, 64), w1 += __shfl_xor(w1, 32, 64);
-        if (hi == 0) sums[wave * C + r0 + 16 * i + lo] = w1;
-      }
-    }
-    if ((chunk + 1) % SEG == 0 || t0 + C >= L) {
-      f32x4* dst = reinterpret_cast<f32x4*>(a.s_seg + ((int64_t)bh * a.segs + chunk / SEG) * DK * DV) + wave * KA * 64 + lane;
-#pragma unroll
-      for (int m = 0; m < KA; ++m) dst[m * 64] = s[m][0];
-    }
-    __syncthreads();
-    copy_out(rv, tv, a.e + ((int64_t)bh * a.chunks + chunk) * C * DV, DV, n, DV);
-    if (tid < n) {
-      float w = 0.0f;
-#pragma unroll
-      for (int i = 0; i < S::W; ++i) w += sums[i * C + tid];
-      a.w[(int64_t)bh * a.chunks * C + t0 + tid] = w;
-    }
-  }
-}
-
-// The inverses' transposes and the scores, transposed and by their terms, of a chunk's blocks.
-template <typename E, typename S, int DK>
-__device__ inline void delta_reverse_setup(const DeltaGates& d, float* inv, E* tp, const E* tk, const E* tq, int n, float scale,
-                                           int wave, int tid) {
-  for (int task = wave; task < 2 * S::NBLK; task += S::W) {
-    const int blk = task % S::NBLK, r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
-    if (r0 >= n) continue;
-    if (task < S::NBLK) {
-      delta_inverse<E, S, DK, true>(d, inv, tk, blk, lane);
-      continue;
-    }
-#pragma unroll
-    for (int i = 0; i < S::NB; ++i)
-#pragma unroll
-      for (int j = 0; j <= i; ++j) {  // lane lo has the key's row
-        f32x4 x = row_products<E, DK>(tq, r0 + 16 * i, tk, r0 + 16 * j, S::LDK, lane);
-        const f32x4 lag = delta_lag(d, r0 + 16 * j, r0 + 16 * i, lane);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = i > j || 4 * hi + r >= lo ? scale * (x[r] * __expf(-lag[r])) : 0.0f;
-        const Terms<E> terms(x);
-#pragma unroll
-        for (int t = 0; t < Terms<E>::N; ++t)
-          *reinterpret_cast<quad_t<E>*>(tp + ((blk * S::TRI + tri(i, j)) * Terms<E>::N + t) * S::TILE_P + lo * S::LDP + 4 * hi) = terms.t[t];
-      }
-  }
-}
-
 // dU of a block, and dO's columns as operands
 template <typename E, typename S, int KA>
-__device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv, const E* tp, const E* tk, const E* tdo, int blk,
+__device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv, const E* tp, const E* tk, const E* tdo,
                                            const f32x4 (&s)[KA][1], quad_t<E> (&g)[S::NB], f32x4 (&du)[S::NB], int col0, int lane) {
   constexpr int NB = S::NB, TERMS = Terms<E>::N;
-  const int r0 = blk * S::BS, lo = lane & 15, hi = lane >> 4;
+  const int lo = lane & 15, hi = lane >> 4;
   f32x4 x[NB], none[NB];
-  delta_state_products<E, S, KA, 0>(tk, tk, r0, s, x, none, lane);
+  delta_state_products<E, S, KA, 0>(tk, tk, s, x, none, lane);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    g[i] = lds_quad_t(tdo, S::LDV, r0 + 16 * i, col0, lane);
-    x[i] *= lds_f4(d.to + r0 + 16 * i + 4 * hi);
+    g[i] = lds_quad_t(tdo, S::LDV, 16 * i, col0, lane);
+    x[i] *= lds_f4(d.to + 16 * i + 4 * hi);
   }
-  const E* pt = tp + blk * S::TRI * TERMS * S::TILE_P + lo * S::LDP + 4 * hi;
+  const E* pt = tp + lo * S::LDP + 4 * hi;
   auto score = [&](int i, int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * TERMS + t) * S::TILE_P); };
   if constexpr (NB == 2) {
     const quad_t<E> zero = to_quad<E>(f32x4{0, 0, 0, 0});
@@ -943,208 +894,244 @@ __device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv
   } else {
     x[0] = mma16(score(0, 0, 0), g[0], x[0]);
   }
-  delta_solve<S, true>(inv + blk * S::TRI * S::TILE, x, du, lane);
+  delta_solve<S, true>(inv, x, du, lane);
 }
 
 // R := exp(G_end) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y
 template <typename E, typename S, int KA>
-__device__ inline void delta_reverse_update(const DeltaGates& d, const E* tk, const E* tq, int blk, float scale,
+__device__ inline void delta_reverse_update(const DeltaGates& d, const E* tk, const E* tq, float scale,
                                             const quad_t<E> (&g)[S::NB], const f32x4 (&du)[S::NB], f32x4 (&s)[KA][1], int lane) {
   constexpr int NB = S::NB;
-  const int r0 = blk * S::BS, hi = lane >> 4;
+  const int hi = lane >> 4;
   Terms<E> wq[NB], wk[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    const f32x4 from = lds_f4(d.from + r0 + 16 * i + 4 * hi);
+    const f32x4 from = lds_f4(d.from + 16 * i + 4 * hi);
     wq[i] = Terms<E>(scale * from * to_f32(g[i]));
-    wk[i] = Terms<E>(-(from * (lds_f4(d.beta + r0 + 16 * i + 4 * hi) * du[i])));
+    wk[i] = Terms<E>(-(from * (lds_f4(d.beta + 16 * i + 4 * hi) * du[i])));
   }
-  const float total = d.total[blk];
+  const float total = *d.total;
 #pragma unroll
   for (int m = 0; m < KA; ++m) {
     quad_t<E> qt[NB], kt[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      qt[i] = lds_quad_t(tq, S::LDK, r0 + 16 * i, 16 * m, lane);
-      kt[i] = lds_quad_t(tk, S::LDK, r0 + 16 * i, 16 * m, lane);
+      qt[i] = lds_quad_t(tq, S::LDK, 16 * i, 16 * m, lane);
+      kt[i] = lds_quad_t(tk, S::LDK, 16 * i, 16 * m, lane);
     }
     s[m][0] = mma_terms(kt, wk, mma_terms(qt, wq, s[m][0] * total));
   }
 }
 
-template <typename E, int DK, int DV>
-constexpr size_t delta_reverse_lds() {
+template <typename E, int DK, int DV, bool RUN>
+struct DeltaReverseLds {
   using S = DeltaShape<E, DK, DV>;
-  return sizeof(float) * (S::GATES + S::INV + 2 * S::W * S::C + 8) +
-         sizeof(E) * (Terms<E>::N * S::SCORES + 2 * S::C * S::LDK + 3 * S::C * S::LDV);
-}
+  // a buffer's bytes: gates, inverses, scores by their terms, sums, rows of K, Q, dO, V, e
+  static constexpr size_t inv = sizeof(float) * S::GATES, scores = inv + sizeof(float) * S::INV;
+  static constexpr size_t sums = scores + sizeof(E) * Terms<E>::N * S::SCORES;
+  static constexpr size_t k = sums + (RUN ? 0 : sizeof(float) * (2 * S::W * S::C + 16)), q = k + sizeof(E) * S::C * S::LDK;
+  static constexpr size_t d_o = q + sizeof(E) * S::C * S::LDK, v = d_o + sizeof(E) * S::C * S::LDV;
+  static constexpr size_t e = v + (RUN ? 0 : sizeof(E) * S::C * S::LDV);
+  static constexpr size_t bytes = e + (RUN ? 0 : sizeof(E) * S::C * S::LDV), all = 2 * bytes;
+};
 
-template <typename E, int DK, int DV>
-__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_BACKWARD)) void delta_reverse_kernel(
-    DeltaBwdArgs<E> a) {
+// The walk backwards; RUN: what a run adds to the gradient of the state that it starts from, alone.
+template <typename E, int DK, int DV, bool RUN>
+__global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
+    DeltaBwdArgs<E> a, int run_width) {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, LDP = S::LDP, SEG = kDeltaSeg / C;
-  constexpr int TERMS = Terms<E>::N;
+  using M = DeltaReverseLds<E, DK, DV, RUN>;
+  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDV = S::LDV, LDP = S::LDP, TERMS = Terms<E>::N, CK = AttnTile<E>::C;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
   const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
-  const DeltaGates d = delta_gates<S>(smem);
-  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
-  float* sum_beta = inv + S::INV;     // (waves, steps)
-  float* sum_z = sum_beta + S::W * C;
-  float* sum_dot = sum_z + S::W * C;  // (waves)
-  E* tp = reinterpret_cast<E*>(sum_dot + 8);  // the blocks' scores, transposed, by their terms
-  E* tk = tp + TERMS * S::SCORES;
-  E* tq = tk + C * LDK;
-  E* tv = tq + C * LDK;
-  E* tdo = tv + C * LDV;
-  E* te = tdo + C * LDV;
-
-  DeltaRows<E, C, DK, S::THREADS> rk, rq;
-  DeltaRows<E, C, DV, S::THREADS> rv, rdo;
-  DeltaRows<E, C, DV, S::THREADS> re;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
-  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid);
-  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
-  auto fetch = [&](int t0) {
-    rk.load(t0, L - t0), rq.load(t0, L - t0), rv.load(t0, L - t0), rdo.load(t0, L - t0), re.load(t0, L - t0);
-    rg.load(t0, L - t0, tid);
+  const int blocks = begin < L ? (L - begin + C - 1) / C : 0, last = begin / C + blocks - 1;  // block `last` comes first
+  const int c0 = RUN ? blockIdx.y * DV : 0;  // the first of the workgroup's columns
+  struct Buffer {
+    DeltaGates d;
+    float *inv, *beta, *z, *dot;
+    E *scores, *k, *q, *d_o, *v, *e;
   };
-  const int last = begin < L ? (L - 1) / C : -1;
-  if (last >= 0) fetch(last * C);
+  auto buffer = [&](int i) {
+    char* x = smem + (i & 1) * M::bytes;
+    float* sums = (float*)(x + M::sums);
+    return Buffer{delta_gates<S>((float*)x), (float*)(x + M::inv), sums, sums + S::W * C, sums + 2 * S::W * C, (E*)(x + M::scores),
+                  (E*)(x + M::k), (E*)(x + M::q), (E*)(x + M::d_o), (E*)(x + M::v), (E*)(x + M::e)};
+  };
+  auto ends = [&](int t0, int of) { return (t0 + C) % of == 0 || t0 + C >= L; };
+
+  if (wave >= S::W) {  // ---- a helper
+    constexpr int THREADS = 128;
+    const int helper = wave - S::W, htid = tid - S::WALKERS - 64;
+    if (helper == 0) {
+      __builtin_amdgcn_s_setprio(3);  // the longest way from meeting to meeting
+      DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
+      rg.start((int64_t)last * C + lane, true);
+      auto fetch = [&](int c) { rg.load(L - (last - c) * C, lane); };
+      auto setup = [&](int c) {
+        const Buffer x = buffer(c);
+        delta_setup<E, S, DK, true, true, false>(x.d, x.inv, x.k, x.q, p.scale, here(lane), [](int, f32x4) {});
+      };
+      if (blocks > 0) fetch(0), rg.scan(lane), rg.store(buffer(0).d, lane);
+      meet();
+      if (blocks > 1) fetch(1);
+      if (blocks > 0) setup(0);
+      if (blocks > 1) rg.scan(lane);
+      meet();
+      for (int c = 0; c < blocks; ++c) {
+        if (c + 1 < blocks) rg.store(buffer(c + 1).d, lane);
+        meet();
+        if (c + 2 < blocks) fetch(c + 2);
+        if (c + 1 < blocks) setup(c + 1);
+        if (c + 2 < blocks) rg.scan(lane);
+        meet();
+      }
+      return;
+    }
+    DeltaRows<E, C, DK, THREADS> rk, rq;
+    DeltaRows<E, C, DV, THREADS> rdo, rv, re;
+    rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, htid);
+    rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, htid);
+    rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + min(c0, p.dv), a.dos[1], min(max(p.dv - c0, 0), DV), p.vec, htid);
+    if constexpr (!RUN) {
+      rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, htid);
+      re.init(a.e + (int64_t)bh * a.chunks * CK * DV, DV, DV, true, htid);
+    }
+    auto fetch = [&](int c) {
+      const int t0 = (last - c) * C;
+      rk.load(t0, L - t0), rq.load(t0, L - t0), rdo.load(t0, L - t0);
+      if constexpr (!RUN) rv.load(t0, L - t0), re.load(t0, L - t0);
+    };
+    auto stage = [&](int c) {
+      const Buffer x = buffer(c);
+      rk.store(x.k), rq.store(x.q), rdo.store(x.d_o);
+      if constexpr (!RUN) rv.store(x.v), re.store(x.e);
+    };
+    auto setup = [&](int c) {
+      const Buffer x = buffer(c);
+      [[maybe_unused]] const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
+      auto put = [&](int tile, f32x4 s) {
+        const Terms<E> terms(s);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+          *reinterpret_cast<quad_t<E>*>(x.scores + (tile * TERMS + t) * S::TILE_P + lo * LDP + 4 * hi) = terms.t[t];
+      };
+      if (helper == 1) delta_setup<E, S, DK, true, false, true>(x.d, x.inv, x.k, x.q, p.scale, lane, put);
+    };
+    E* yrow = a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv);
+    auto results = [&](int c) {  // of a block that the walkers have left
+      if constexpr (!RUN) {
+        const Buffer x = buffer(c);
+        const int t0 = (last - c) * C, n = min(C, L - t0);
+        copy_out(rdo, x.d_o, yrow + t0 * a.ys[1], a.ys[1], n, a.y_width);
+        if (htid < n) {
+          float sb = 0.0f, sz = 0.0f;
+#pragma unroll
+          for (int i = 0; i < S::W; ++i) sb += x.beta[i * C + htid], sz += x.z[i * C + htid];
+          a.dbeta[((int64_t)b * p.T + t0 + htid) * p.H + h] = (E)sb;
+          a.z[(int64_t)bh * a.chunks * CK + t0 + htid] = sz;
+        }
+        if (htid == 0 && ends(t0, kDeltaSeg)) {
+          float dot = 0.0f;
+          for (int i = 0; i < S::W; ++i) dot += x.dot[i];
+          a.dot[(int64_t)bh * a.stretches + t0 / kDeltaSeg] = dot;
+        }
+      }
+    };
+    if (blocks > 0) fetch(0), stage(0);
+    meet();
+    if (blocks > 1) fetch(1);
+    if (blocks > 0) setup(0);
+    meet();
+    for (int c = 0; c < blocks; ++c) {
+      if (c > 0) results(c - 1);
+      if (c + 1 < blocks) stage(c + 1);
+      meet();
+      if (c + 2 < blocks) fetch(c + 2);
+      if (c + 1 < blocks) setup(c + 1);
+      meet();
+    }
+    if (blocks > 0) results(blocks - 1);
+    return;
+  }
+
+  // ---- a walker
   const int64_t size = (int64_t)p.dk * p.dv;
   f32x4 s[KA][1];
-  if (p.segs > 1) load_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, col0, lo, hi);
-  else load_state(s, a.d_out ? a.d_out + bh * size : nullptr, false, p.dk, p.dv, col0, lo, hi);
-  E* yrow = a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv);
-
-  for (int chunk = last; chunk * C >= begin; --chunk) {
-    const int t0 = chunk * C, n = min(C, L - t0);
-    rk.store(tk), rq.store(tq), rv.store(tv), rdo.store(tdo), re.store(te), rg.store(d, tid);
-    store_columns<E, DK>(a.r + ((int64_t)bh * a.chunks + chunk) * DK * DV, s, col0, lo, hi);
-    const bool seg_end = (chunk + 1) % SEG == 0 || chunk == last;
-    if (seg_end) {
-      const f32x4* src = reinterpret_cast<const f32x4*>(a.s_seg + ((int64_t)bh * a.segs + chunk / SEG) * DK * DV) + wave * KA * 64 + lane;
-      float dot = 0.0f;
+  if constexpr (RUN) {
 #pragma unroll
-      for (int m = 0; m < KA; ++m) {
-        const f32x4 x = src[m * 64];
+    for (int m = 0; m < KA; ++m) s[m][0] = f32x4{0, 0, 0, 0};
+  } else if (p.segs > 1) {
+    load_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * DV), false, DK, DV, wave * 16, lane & 15, lane >> 4);
+  } else {
+    load_state(s, a.d_out ? a.d_out + bh * size : nullptr, false, p.dk, p.dv, wave * 16, lane & 15, lane >> 4);
+  }
+  meet();
+  meet();
+  for (int c = 0; c < blocks; ++c) {
+    const int t0 = (last - c) * C, n = min(C, L - t0);
+    const Buffer x = buffer(c);
+    if constexpr (!RUN) {
+      if (ends(t0, CK)) store_columns<E, DK>(a.r + ((int64_t)bh * a.chunks + t0 / CK) * DK * DV, s, wave * 16, lane & 15, lane >> 4);
+      if (ends(t0, kDeltaSeg)) {
+        const f32x4* src = reinterpret_cast<const f32x4*>(a.s_seg + ((int64_t)bh * a.stretches + t0 / kDeltaSeg) * DK * DV) + wave * KA * 64 + lane;
+        float dot = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dot += x[r] * s[m][0][r];
+        for (int m = 0; m < KA; ++m) {
+          const f32x4 y = src[m * 64];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dot += y[r] * s[m][0][r];
+        }
+#pragma unroll
+        for (int i = 32; i; i >>= 1) dot += __shfl_xor(dot, i, 64);
+        if (lane == 0) x.dot[wave] = dot;
       }
-#pragma unroll
-      for (int i = 32; i; i >>= 1) dot += __shfl_xor(dot, i, 64);
-      if (lane == 0) sum_dot[wave] = dot;
     }
-    __syncthreads();
-    if (seg_end && tid == 0) {
-      float dot = 0.0f;
-      for (int i = 0; i < S::W; ++i) dot += sum_dot[i];
-      a.dot[(int64_t)bh * a.segs + chunk / SEG] = dot;
-    }
-    delta_reverse_setup<E, S, DK>(d, inv, tp, tk, tq, n, p.scale, wave, tid);
-    __syncthreads();
-    if (t0 > begin) fetch(t0 - C);
-#pragma unroll 1
-    for (int blk = (n - 1) / S::BS; blk >= 0; --blk) {
-      const int r0 = blk * S::BS, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = here(wave) * 16;
-      f32x4 du[NB];
-      quad_t<E> g[NB];
-      delta_reverse_solve<E, S, KA>(d, inv, tp, tk, tdo, blk, s, g, du, col0, lane);
+    const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
+    f32x4 du[NB];
+    quad_t<E> g[NB];
+    meet();
+    delta_reverse_solve<E, S, KA>(x.d, x.inv, x.scores, x.k, x.d_o, s, g, du, col0, lane);
+    if constexpr (!RUN) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const f32x4 y = lds_f4(d.beta + r0 + 16 * i + 4 * hi) * du[i];
-        const f32x4 pe = du[i] * to_f32(lds_quad_t(te, LDV, r0 + 16 * i, col0, lane));
-        const f32x4 pv = y * to_f32(lds_quad_t(tv, LDV, r0 + 16 * i, col0, lane));
+        const f32x4 y = lds_f4(x.d.beta + 16 * i + 4 * hi) * du[i];
+        const f32x4 pe = du[i] * to_f32(lds_quad_t(x.e, LDV, 16 * i, col0, lane));
+        const f32x4 pv = y * to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int t = r0 + 16 * i + 4 * hi + r;
+          const int t = 16 * i + 4 * hi + r;
           const float sb = row16_sum(pe[r]), sz = row16_sum(pv[r]);
-          if (lo == 0) sum_beta[wave * C + t] = sb, sum_z[wave * C + t] = sz;
-          tdo[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
+          if (lo == 0) x.beta[wave * C + t] = sb, x.z[wave * C + t] = sz;
+          x.d_o[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
           if (a.y_part && t < n && col0 + lo < p.dv)
             a.y_part[(((int64_t)b * p.T + t0 + t) * p.H + h) * p.dv + col0 + lo] = y[r];
         }
       }
-      delta_reverse_update<E, S, KA>(d, tk, tq, blk, p.scale, g, du, s, lane);
     }
-    __syncthreads();
-    copy_out(rdo, tdo, yrow + t0 * a.ys[1], a.ys[1], n, a.y_width);
-    if (tid < n) {
-      float sb = 0.0f, sz = 0.0f;
-#pragma unroll
-      for (int i = 0; i < S::W; ++i) sb += sum_beta[i * C + tid], sz += sum_z[i * C + tid];
-      a.dbeta[((int64_t)b * p.T + t0 + tid) * p.H + h] = (E)sb;
-      a.z[(int64_t)bh * a.chunks * C + t0 + tid] = sz;
-    }
+    delta_reverse_update<E, S, KA>(x.d, x.k, x.q, p.scale, g, du, s, lane);
+    meet();
   }
-  if (a.d_in && seg == 0) store_state(s, a.d_in + bh * size, p.dk, p.dv, col0, lo, hi);
-  const int z0 = max(delta_length(p, b), begin), z1 = (int)min((int64_t)p.T, (int64_t)begin + p.seg_len);
-  for (int t = z0 + tid; t < z1; t += S::THREADS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
-  const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
-  if (a.y_part) zero_rows(a.y_part, true, 4, obase, orow, p.dv, z0, z1, tid, S::THREADS);
-  else zero_rows(a.y, false, sizeof(E), obase, orow, p.dv, z0, z1, tid, S::THREADS);
-}
-
-template <typename E, int DK>
-__global__ __launch_bounds__(256, DK <= 64 ? 3 : 2) void delta_reverse_run_kernel(DeltaBwdArgs<E> a, int DV) {
-  using S = DeltaShape<E, DK, 64>;
-  constexpr int C = S::C, NB = S::NB, KA = DK / 16, LDK = S::LDK, LDV = S::LDV, TERMS = Terms<E>::N;
-  extern __shared__ __align__(16) char smem[];
-  const DeltaArgs<E>& p = a.f;
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
-  const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);
-  const DeltaGates d = delta_gates<S>(smem);
-  float* inv = reinterpret_cast<float*>(smem) + S::GATES;
-  E* tp = reinterpret_cast<E*>(inv + S::INV);
-  E* tk = tp + TERMS * S::SCORES;
-  E* tq = tk + C * LDK;
-  E* tdo = tq + C * LDK;
-  DeltaRows<E, C, DK, 256> rk, rq;
-  DeltaRows<E, C, 64, 256> rdo;
-  const int c0 = blockIdx.y * 64;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + min(c0, p.dv), a.dos[1], min(max(p.dv - c0, 0), 64), p.vec, tid);
-  DeltaGateRows<E, S> rg{p.g + b * p.gs[0] + h * p.gs[2], p.beta + b * p.bs[0] + h * p.bs[2], p.gs[1], p.bs[1]};
-  auto fetch = [&](int t0) { rk.load(t0, L - t0), rq.load(t0, L - t0), rdo.load(t0, L - t0), rg.load(t0, L - t0, tid); };
-  const int last = begin < L ? (L - 1) / C : -1;
-  if (last >= 0) fetch(last * C);
-  f32x4 s[KA][1];
-#pragma unroll
-  for (int m = 0; m < KA; ++m) s[m][0] = f32x4{0, 0, 0, 0};
-  for (int chunk = last; chunk * C >= begin; --chunk) {
-    const int t0 = chunk * C, n = min(C, L - t0);
-    rk.store(tk), rq.store(tq), rdo.store(tdo), rg.store(d, tid);
-    __syncthreads();
-    delta_reverse_setup<E, S, DK>(d, inv, tp, tk, tq, n, p.scale, wave, tid);
-    __syncthreads();
-    if (t0 > begin) fetch(t0 - C);
-#pragma unroll 1
-    for (int blk = (n - 1) / S::BS; blk >= 0; --blk) {
-      f32x4 du[NB];
-      quad_t<E> g[NB];
-      const int lane = here(tid & 63), col0 = here(wave) * 16;
-      delta_reverse_solve<E, S, KA>(d, inv, tp, tk, tdo, blk, s, g, du, col0, lane);
-      delta_reverse_update<E, S, KA>(d, tk, tq, blk, p.scale, g, du, s, lane);
-    }
-    __syncthreads();
+  if constexpr (RUN) {
+    const int col0 = c0 + wave * 16;
+    if (col0 < run_width) store_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * run_width), DK, run_width, col0, lane & 15, lane >> 4);
+  } else {
+    if (a.d_in && seg == 0) store_state(s, a.d_in + bh * size, p.dk, p.dv, wave * 16, lane & 15, lane >> 4);
+    const int z0 = max(delta_length(p, b), begin), z1 = (int)min((int64_t)p.T, (int64_t)begin + p.seg_len);
+    for (int t = z0 + tid; t < z1; t += S::WALKERS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
+    const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
+    if (a.y_part) zero_rows(a.y_part, true, 4, obase, orow, p.dv, z0, z1, tid, S::WALKERS);
+    else zero_rows(a.y, false, sizeof(E), obase, orow, p.dv, z0, z1, tid, S::WALKERS);
   }
-  const int col0 = c0 + wave * 16;
-  if (col0 < DV) store_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * DV), DK, DV, col0, tid & 15, (tid & 63) >> 4);
 }
 
 // log_decay's gradient: a wave a stretch, four steps a lane; in 64 bits, for the terms are.
 template <typename E>
 __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows) {
   const DeltaArgs<E>& p = a.f;
-  const int seg = blockIdx.x % a.segs, bh = blockIdx.x / a.segs, b = bh / p.H, h = bh - b * p.H, lane = threadIdx.x;
+  const int seg = blockIdx.x % a.stretches, bh = blockIdx.x / a.stretches, b = bh / p.H, h = bh - b * p.H, lane = threadIdx.x;
   const int L = delta_length(p, b);
   const int t0 = seg * kDeltaSeg + lane * 4;
   const int64_t at = (int64_t)bh * rows + t0;
@@ -1161,7 +1148,7 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
     if (lane + i < 64) after += v;
   }
   after -= sum;
-  if (seg * kDeltaSeg < L) after += (double)a.dot[(int64_t)bh * a.segs + seg];
+  if (seg * kDeltaSeg < L) after += (double)a.dot[(int64_t)bh * a.stretches + seg];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = t0 + i;
@@ -1175,14 +1162,15 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
 template <typename E, int DK, int DV>
 constexpr size_t delta_dqk_lds() {
   using S = DeltaShape<E, DK, DV>;
-  return 8 * S::C + 4 * 3 * S::C + sizeof(E) * (2 * S::C * S::LDK + 3 * S::C * S::LDV + DV * S::LDK);
+  constexpr int C = AttnTile<E>::C;
+  return 8 * C + 4 * 3 * C + sizeof(E) * (2 * C * S::LDK + 3 * C * S::LDV + DV * S::LDK);
 }
 
 // dq and dk of a chunk: a wave 16 rows (and with fp32 chunks of 32 steps half of the columns).
 template <typename E, int DK, int DV>
 __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   using S = DeltaShape<E, DK, DV>;
-  constexpr int C = S::C, CT = C / 16, WC = 4 / CT, KT = DK / 16 / WC, VA = DV / 16, LDK = S::LDK, LDV = S::LDV;
+  constexpr int C = AttnTile<E>::C, CT = C / 16, WC = 4 / CT, KT = DK / 16 / WC, VA = DV / 16, LDK = S::LDK, LDV = S::LDV;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
