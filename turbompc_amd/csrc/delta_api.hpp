@@ -137,7 +137,7 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
 // The backward pass' arrays in the workspace, one after another.
 struct BackwardPlan {
   int chunks, stretches, DK, DV;
-  size_t e, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
+  size_t e, e_low, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
   RunPlan runs;
 };
 template <typename E>
@@ -154,6 +154,7 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
     return at;
   };
   p.e = take(rows * p.DV * sizeof(E));
+  if (sizeof(E) == 2) p.e_low = take(rows * p.DV * sizeof(E));
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
   p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
@@ -182,7 +183,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   a.d_o = (const E*)d_o, a.d_out = d_out;
   std::copy_n(dos, 3, a.dos);
   a.chunks = w.chunks, a.stretches = w.stretches;
-  a.e = (E*)(base + w.e), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
+  a.e = (E*)(base + w.e), a.e_low = (E*)(base + w.e_low), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
   a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot);
   if (x->Hv != x->H) {
     a.y = (E*)(base + w.y), a.y_part = (float*)(base + w.y_part), a.y_width = w.DV;
@@ -208,7 +209,8 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
     if (x->T > 0) launch_walk<E, dkw(), dvw(), WALK_STATES>(st, a, dvw(), 0);
     launch_reverse<E, dkw(), dvw(), false>(st, a, dvw(), 0);
     if (x->T > 0)
-      launch(st, delta_dqk_kernel<E, dkw(), dvw()>, dim3((unsigned)(bh * w.chunks)), 256, delta_dqk_lds<E, dkw(), dvw()>(), a);
+      launch(st, delta_dqk_kernel<E, dkw(), dvw()>, dim3((unsigned)(bh * w.chunks)), DeltaDqkShape<E, dkw(), dvw()>::THREADS,
+             DeltaDqkShape<E, dkw(), dvw()>::LDS, a);
   });
   if (x->T > 0) {
     hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.stretches)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);

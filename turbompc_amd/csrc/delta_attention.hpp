@@ -422,6 +422,14 @@ __device__ inline void delta_state_update(const quad_t<E> (&kt)[KA][NB], const T
   for (int m = 0; m < KA; ++m) s[m][0] = mma_terms(kt[m], w, s[m][0] * total);
 }
 
+// Zero rows [z0, z1) of an output, four columns a thread.
+template <typename T>
+__device__ inline void zero_quads(T* base, int64_t pitch, int d, int64_t z0, int64_t z1, int tid, int threads) {
+  const int q = (d + 3) / 4, per = threads / q, r = tid / q, c = (tid - r * q) * 4;
+  if (r >= per) return;
+  for (int64_t t = z0 + r; t < z1; t += per) store_quad(base + t * pitch, c, d, f32x4{0, 0, 0, 0});
+}
+
 // A wave's columns of a history whose state is not finite in the end, by the definition, a step at
 // a time: in a block such a step meets the earlier ones with factors of zero, which makes those NaN.
 template <typename E, int KA, int DV>
@@ -486,7 +494,7 @@ struct DeltaBwdArgs {
   int64_t dos[3];
   const float* d_out;  // (B, H, dk, dv) or NULL
   int chunks, stretches;  // of T
-  E *e;                // (B H, chunks C, DV)
+  E *e, *e_low;        // (B H, chunks C, DV): e_t, in bf16 by two terms
   E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends
   float *w, *z;        // (B H, chunks C): do . o, y . v
   float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
@@ -639,7 +647,9 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       if constexpr (M::DO) {
         const Buffer x = buffer(c);
         const int t0 = begin + c * C, n = min(C, L - t0);
-        copy_out(rv, x.v, a.e + ((int64_t)bh * a.chunks * CK + t0) * DV, DV, n, DV);
+        const int64_t at = ((int64_t)bh * a.chunks * CK + t0) * DV;
+        copy_out(rv, x.v, a.e + at, DV, n, DV);
+        if constexpr (sizeof(E) == 2) copy_out(rdo, x.d_o, a.e_low + at, DV, n, DV);
         if (htid < n) {
           float w = 0.0f;
 #pragma unroll
@@ -710,12 +720,16 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     const float total = *x.d.total;
     delta_solve<S, false>(x.inv, e, u, lane);
     Terms<E> w[NB];
+    [[maybe_unused]] bf16x4 low[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       // these columns of V are this wave's alone and have been read: e takes their place
       if constexpr (M::DO)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x.v[(16 * i + 4 * hi + r) * LDV + col0 + lo] = (E)u[i][r];
+        for (int r = 0; r < 4; ++r) {
+          const E high = (E)u[i][r];
+          x.v[(16 * i + 4 * hi + r) * LDV + col0 + lo] = high, low[i][r] = (bf16)(u[i][r] - (float)high);
+        }
       u[i] *= beta[i];
       w[i] = Terms<E>(to[i] * u[i]);
     }
@@ -760,6 +774,9 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         float w1 = o[i][0] + o[i][1] + o[i][2] + o[i][3];
         w1 += __shfl_xor(w1, 16, 64), w1 += __shfl_xor(w1, 32, 64);
         if (hi == 0) x.sums[wave * C + 16 * i + lo] = w1;
+        if constexpr (sizeof(E) == 2)  // and so for dO
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x.d_o[(16 * i + 4 * hi + r) * LDV + col0 + lo] = low[i][r];
       }
     }
     if (M::DO && ((t0 + C) % kDeltaSeg == 0 || t0 + C >= L)) {
@@ -785,8 +802,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     const DeltaArgs<E>& f = ((const DeltaBwdArgs<E>*)args)->f;
     const int ebh = block / f.segs, eseg = block - ebh * f.segs, eb = ebh / f.H, eL = delta_length(f, eb);
     const int ebegin = eseg * f.seg_len;
-    zero_rows(f.o, false, sizeof(E), ((int64_t)eb * f.T * f.H + (ebh - eb * f.H)) * f.dv, (int64_t)f.H * f.dv, f.dv, max(eL, ebegin),
-              min((int64_t)f.T, (int64_t)ebegin + f.seg_len), etid, S::WALKERS);
+    zero_quads(f.o + ((int64_t)eb * f.T * f.H + (ebh - eb * f.H)) * f.dv, (int64_t)f.H * f.dv, f.dv, max(eL, ebegin),
+               min((int64_t)f.T, (int64_t)ebegin + f.seg_len), etid, S::WALKERS);
     // An infinite or NaN value leaves the state so, to the end.
     f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
@@ -1122,8 +1139,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     const int z0 = max(delta_length(p, b), begin), z1 = (int)min((int64_t)p.T, (int64_t)begin + p.seg_len);
     for (int t = z0 + tid; t < z1; t += S::WALKERS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
     const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
-    if (a.y_part) zero_rows(a.y_part, true, 4, obase, orow, p.dv, z0, z1, tid, S::WALKERS);
-    else zero_rows(a.y, false, sizeof(E), obase, orow, p.dv, z0, z1, tid, S::WALKERS);
+    if (a.y_part) zero_quads(a.y_part + obase, orow, p.dv, z0, z1, tid, S::WALKERS);
+    else zero_quads(a.y + obase, orow, p.dv, z0, z1, tid, S::WALKERS);
   }
 }
 
@@ -1160,17 +1177,26 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
 }
 
 template <typename E, int DK, int DV>
-constexpr size_t delta_dqk_lds() {
-  using S = DeltaShape<E, DK, DV>;
-  constexpr int C = AttnTile<E>::C;
-  return 8 * C + 4 * 3 * C + sizeof(E) * (2 * C * S::LDK + 3 * C * S::LDV + DV * S::LDK);
-}
+struct DeltaDqkShape {
+  static constexpr int C = AttnTile<E>::C, CT = C / 16;
+  // waves that share 16 rows' columns, and tiles of each
+  static constexpr int WC = sizeof(E) == 2 ? (DK == 128 || DV == 128 ? 2 : 1) : DK == 32 ? 2 : 4, KT = DK / 16 / WC;
+  static constexpr int THREADS = 64 * CT * WC, HALF = DV < 64 ? DV : 64;  // values of a state in LDS at a time
+  static constexpr int LDK = DK + AttnTile<E>::PAD, LDV = DV + AttnTile<E>::PAD, TERMS = sizeof(E) == 2 ? 2 : 1;
+  // rows of e (by its terms), dO and y and a state's half; then rows of K and Q in their place
+  static constexpr size_t FIRST = sizeof(E) * ((2 + TERMS) * C * LDV + HALF * LDK), SECOND = sizeof(E) * 2 * C * LDK;
+  static constexpr size_t LDS = 8 * C + 4 * 3 * C + (FIRST > SECOND ? FIRST : SECOND);
+  static constexpr int FIT = 160 * 1024 / LDS * THREADS / 256, MOST = KT >= 4 ? 3 : 4, WAVES_PER_SIMD = FIT > MOST ? MOST : FIT;  // by LDS and registers
+};
 
-// dq and dk of a chunk: a wave 16 rows (and with fp32 chunks of 32 steps half of the columns).
+// dq and dk of a chunk.  beta_j stays out of the operands (u_j = beta_j e_j), and in bf16 e and the scores M and N
+// enter by two terms: y and the states are what is rounded, once each.  (With e by one term dk is 2.7e-3 off
+// where a rounding is 1.66e-3, with it by two 2.1e-3.)
 template <typename E, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
-  using S = DeltaShape<E, DK, DV>;
-  constexpr int C = AttnTile<E>::C, CT = C / 16, WC = 4 / CT, KT = DK / 16 / WC, VA = DV / 16, LDK = S::LDK, LDV = S::LDV;
+__global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
+  using S = DeltaDqkShape<E, DK, DV>;
+  constexpr int C = S::C, CT = S::CT, WC = S::WC, KT = S::KT, THREADS = S::THREADS, HALF = S::HALF, LDK = S::LDK, LDV = S::LDV;
+  constexpr int VA = DV / 16, HA = HALF / 16, P = Elem<E>::PIECE, TERMS = S::TERMS;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
@@ -1179,153 +1205,195 @@ __global__ __launch_bounds__(256) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   const int t0 = chunk * C, n = min(C, L - t0);
   const int64_t orow = (int64_t)p.H * p.dk, obase = ((int64_t)b * p.T * p.H + h) * p.dk;
   const int64_t z0 = max(L, t0), z1 = min(p.T, t0 + C);
-  zero_rows(a.dq, a.q_part, sizeof(E), obase, orow, p.dk, z0, z1, tid, 256);
-  zero_rows(a.dk, a.k_part, sizeof(E), obase, orow, p.dk, z0, z1, tid, 256);
+  auto zero = [&](void* out, bool part) {
+    if (part) zero_quads((float*)out + obase, orow, p.dk, z0, z1, tid, THREADS);
+    else zero_quads((E*)out + obase, orow, p.dk, z0, z1, tid, THREADS);
+  };
+  if (z0 < z1) zero(a.dq, a.q_part), zero(a.dk, a.k_part);
   if (n <= 0) return;
   double* G = reinterpret_cast<double*>(smem);
   float* beta = reinterpret_cast<float*>(G + C);
   float* from = beta + C;
   float* to = from + C;
+  E* tdo = reinterpret_cast<E*>(to + C);
+  E* ty = tdo + C * LDV;
+  E* te = ty + C * LDV;               // TERMS of them
+  E* ts = te + TERMS * C * LDV;       // half of a state or of its gradient, (HALF, DK)
   E* tk = reinterpret_cast<E*>(to + C);
   E* tq = tk + C * LDK;
-  E* tu = tq + C * LDK;
-  E* tdo = tu + C * LDV;
-  E* ty = tdo + C * LDV;
-  E* ts = ty + C * LDV;  // a state or its gradient, (DV, DK)
 
-  DeltaRows<E, C, DK, 256> rk, rq;
-  DeltaRows<E, C, DV, 256> rdo, re, ry;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
-  re.init(a.e + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid);
-  ry.init(a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv), a.ys[1], a.y_width, a.y_part || p.vec, tid);
-  rk.load(t0, n), rq.load(t0, n), rdo.load(t0, n), re.load(t0, n), ry.load(t0, n);
-  // rows of the state: DV of DK elements, whole pieces
-  constexpr int P = Elem<E>::PIECE, SP = (DV * DK / P + 255) / 256;
+  // the states' halves, rows of whole pieces, on their way to LDS: S's and R's first, then the second ones
+  constexpr int SP = (HALF * DK / P + THREADS - 1) / THREADS, PHASES = 2 * DV / HALF;
   piece_t<E> sp[SP];
-  const E* src = a.s + ((int64_t)bh * a.chunks + chunk) * DK * DV;
-  auto state_load = [&](const E* from_) {
+  const int64_t state = ((int64_t)bh * a.chunks + chunk) * DK * DV;
+  auto state_load = [&](int phase) {
+    const E* src = (phase & 1 ? a.r : a.s) + state + phase / 2 * HALF * DK;
 #pragma unroll
     for (int i = 0; i < SP; ++i)
-      if ((i * 256 + tid) * P < DV * DK) sp[i] = *reinterpret_cast<const piece_t<E>*>(from_ + (i * 256 + tid) * P);
+      if ((i * THREADS + tid) * P < HALF * DK) sp[i] = *reinterpret_cast<const piece_t<E>*>(src + (i * THREADS + tid) * P);
   };
   auto state_store = [&]() {
 #pragma unroll
     for (int i = 0; i < SP; ++i) {
-      const int e = (i * 256 + tid) * P;
-      if (e < DV * DK) *reinterpret_cast<piece_t<E>*>(ts + e / DK * LDK + e % DK) = sp[i];
+      const int e = (i * THREADS + tid) * P;
+      if (e < HALF * DK) *reinterpret_cast<piece_t<E>*>(ts + e / DK * LDK + e % DK) = sp[i];
     }
   };
-  state_load(src);
-  if (wave == 0) {
-    const bool live = lane < n;
-    float g = live ? p.g[b * p.gs[0] + (t0 + lane) * p.gs[1] + h * p.gs[2]] : 0.0f;
-    g = g < kNoDecay ? kNoDecay : g;
-    double sum = (double)g;
+  {
+    DeltaRows<E, C, DV, THREADS> rdo, re[TERMS], ry;
+    rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
+    ry.init(a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv), a.ys[1], a.y_width, a.y_part || p.vec, tid);
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-      const double v = __shfl_up(sum, i, 64);
-      if (lane >= i) sum += v;
+    for (int t = 0; t < TERMS; ++t) re[t].init((t ? a.e_low : a.e) + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid), re[t].load(t0, n);
+    rdo.load(t0, n), ry.load(t0, n);
+    state_load(0);
+    if (wave == 0) {
+      const bool live = lane < n;
+      float g = live ? p.g[b * p.gs[0] + (t0 + lane) * p.gs[1] + h * p.gs[2]] : 0.0f;
+      const float bt = live ? (float)p.beta[b * p.bs[0] + (t0 + lane) * p.bs[1] + h * p.bs[2]] : 0.0f;
+      g = g < kNoDecay ? kNoDecay : g;
+      double sum = (double)g;
+#pragma unroll
+      for (int i = 1; i < 64; i <<= 1) {
+        const double v = __shfl_up(sum, i, 64);
+        if (lane >= i) sum += v;
+      }
+      const double end = __shfl(sum, 63, 64);
+      if (lane < C) G[lane] = sum, from[lane] = __expf((float)sum), to[lane] = __expf((float)(end - sum)), beta[lane] = bt;
     }
-    const double end = __shfl(sum, 63, 64);
-    if (lane < C) {
-      G[lane] = sum, from[lane] = __expf((float)sum), to[lane] = __expf((float)(end - sum));
-      beta[lane] = live ? (float)p.beta[b * p.bs[0] + (t0 + lane) * p.bs[1] + h * p.bs[2]] : 0.0f;
-    }
-  }
-  rk.store(tk), rq.store(tq), rdo.store(tdo);
-  ry.store(ty);
-  state_store();
-  __syncthreads();
+    rdo.store(tdo), ry.store(ty);
 #pragma unroll
-  for (int i = 0; i < re.N; ++i) {
-    const float f = re.row < re.RS ? beta[re.row + i * re.RS] : 0.0f;
-#pragma unroll
-    for (int e = 0; e < P; ++e) re.r[i][e] = (E)((float)re.r[i][e] * f);
+    for (int t = 0; t < TERMS; ++t) re[t].store(te + t * C * LDV);
+    state_store();
   }
-  re.store(tu);
-  state_load(a.r + ((int64_t)bh * a.chunks + chunk) * DK * DV);
   __syncthreads();
+  state_load(1);
 
   const int it = wave / WC, kt0 = (wave % WC) * KT, row = 16 * it + lo;
-  const double mine = G[row];
-  // the scores as operands: outer index this wave's rows, contracted the chunk's steps
-  quad_t<E> m[CT], mt[CT], nn[CT];
+  // R's part is scaled by exp(G_end - G_j) beta_j, S's by -exp(G_j): kept apart until the sums are whole
+  f32x4 aq[KT], as[KT], ar[KT];
 #pragma unroll
-  for (int jt = 0; jt < CT; ++jt) {
-    f32x4 s1 = {0, 0, 0, 0}, s2 = {0, 0, 0, 0}, s3 = {0, 0, 0, 0}, s4 = {0, 0, 0, 0};
-    const bool below = jt <= it, above = jt >= it;
+  for (int kt = 0; kt < KT; ++kt) aq[kt] = as[kt] = ar[kt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int v = 0; v < VA; v += 2) {
-      auto two = [&](const E* x, int r0, quad_t<E>& x0, quad_t<E>& x1) {
-        x0 = lds_quad(x, LDV, r0, 16 * v, lane), x1 = lds_quad(x, LDV, r0, 16 * v + 16, lane);
-      };
-      quad_t<E> x0, x1, y0, y1;
-      if (below) {
-        two(tu, 16 * jt, x0, x1);
-        two(tdo, 16 * it, y0, y1), s1 = mma2(x0, x1, y0, y1, s1);
-        two(ty, 16 * it, y0, y1), s2 = mma2(x0, x1, y0, y1, s2);
+  for (int phase = 0; phase < PHASES; ++phase) {
+    if (phase > 0) {
+      __syncthreads();
+      state_store();
+      __syncthreads();
+      if (phase + 1 < PHASES) state_load(phase + 1);
+    }
+    if (16 * it >= n) continue;
+    const int lane = here(tid & 63);
+#pragma unroll
+    for (int v = 0; v < HA; v += 2) {
+      const int col = phase / 2 * HALF + 16 * v;
+      quad_t<E> x[2][2];  // this wave's rows of dO and y, or of e's terms
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if ((phase & 1) && t == TERMS) continue;
+        const E* z = phase & 1 ? te + t * C * LDV : t ? ty : tdo;
+        x[t][0] = lds_quad(z, LDV, 16 * it, col, lane), x[t][1] = lds_quad(z, LDV, 16 * it, col + 16, lane);
       }
-      if (above) {
-        two(tu, 16 * it, x0, x1);
-        two(tdo, 16 * jt, y0, y1), s3 = mma2(y0, y1, x0, x1, s3);
-        two(ty, 16 * jt, y0, y1), s4 = mma2(y0, y1, x0, x1, s4);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const quad_t<E> s0 = lds_quad_t(ts, LDK, 16 * v, 16 * (kt0 + kt), lane);
+        const quad_t<E> s1 = lds_quad_t(ts, LDK, 16 * v + 16, 16 * (kt0 + kt), lane);
+        if (phase & 1) {
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) ar[kt] = mma2(s0, s1, x[t][0], x[t][1], ar[kt]);
+        } else {
+          aq[kt] = mma2(s0, s1, x[0][0], x[0][1], aq[kt]);
+          as[kt] = mma2(s0, s1, x[1][0], x[1][1], as[kt]);
+        }
       }
     }
+  }
+  const float ff = from[row], ft = to[row], bt = beta[row];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) aq[kt] *= p.scale * ff, ar[kt] = ft * bt * ar[kt] - ff * as[kt];
+
+  DeltaRows<E, C, DK, THREADS> rk, rq;
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rk.load(t0, n), rq.load(t0, n);  // in flight while the scores are made
+
+  // the scores of this wave's rows with the chunk's steps, as operands
+  quad_t<E> m[CT][TERMS], mt[CT][TERMS], nn[CT][TERMS];
+  const double mine = G[row];
+#pragma unroll
+  for (int jt = 0; jt < CT; ++jt) {
+    const int j0 = 16 * jt, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, row = 16 * it + lo;
+    f32x4 s1 = {0, 0, 0, 0}, s2 = {0, 0, 0, 0}, s3 = {0, 0, 0, 0}, s4 = {0, 0, 0, 0};
+    const bool live = 16 * max(it, jt) < n, below = live && jt <= it, above = live && jt >= it;
+#pragma unroll
+    for (int v = 0; v < VA; v += 2) {
+      auto two = [&](const E* z, int r0, quad_t<E>& z0, quad_t<E>& z1) {
+        z0 = lds_quad(z, LDV, r0, 16 * v, lane), z1 = lds_quad(z, LDV, r0, 16 * v + 16, lane);
+      };
+      quad_t<E> e0, e1, g0, g1, y0, y1;
+      if (below) {
+        two(tdo, 16 * it, g0, g1), two(ty, 16 * it, y0, y1);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          two(te + t * C * LDV, j0, e0, e1);
+          s1 = mma2(e0, e1, g0, g1, s1), s2 = mma2(e0, e1, y0, y1, s2);
+        }
+      }
+      if (above) {
+        two(tdo, j0, g0, g1), two(ty, j0, y0, y1);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          two(te + t * C * LDV, 16 * it, e0, e1);
+          s3 = mma2(g0, g1, e0, e1, s3), s4 = mma2(y0, y1, e0, e1, s4);
+        }
+      }
+    }
+    const f32x4 bj = lds_f4(beta + j0 + 4 * hi);
     f32x4 nsum;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int j = 16 * jt + 4 * hi + r;
+      const int j = j0 + 4 * hi + r;
       const float lag = (float)(mine - G[j]);
-      const float back = __expf(lag), ahead = __expf(-lag);
-      s1[r] = below && j <= row ? p.scale * back * s1[r] : 0.0f;
-      s3[r] = above && j >= row ? p.scale * ahead * s3[r] : 0.0f;
-      nsum[r] = j < row ? -back * s2[r] : j > row ? -ahead * s4[r] : 0.0f;
+      const float ratio = __expf(j <= row ? lag : -lag);
+      s1[r] = j <= row ? p.scale * ratio * bj[r] * s1[r] : 0.0f;
+      s3[r] = j >= row ? p.scale * ratio * bt * s3[r] : 0.0f;
+      nsum[r] = j < row ? -ratio * bj[r] * s2[r] : j > row ? -ratio * bt * s4[r] : 0.0f;
     }
-    m[jt] = to_quad<E>(s1), mt[jt] = to_quad<E>(s3), nn[jt] = to_quad<E>(nsum);
-  }
-  f32x4 aq[KT], ak[KT];
-  const float ff = from[row], ft = to[row];
+    const Terms<E> a1(s1), a2(s3), a3(nsum);
+    __builtin_amdgcn_sched_barrier(0);  // the next tile's reads not yet: their registers
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    aq[kt] = ak[kt] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int v = 0; v < VA; v += 2) {
-      const quad_t<E> s0 = lds_quad_t(ts, LDK, 16 * v, 16 * (kt0 + kt), lane);
-      const quad_t<E> s1 = lds_quad_t(ts, LDK, 16 * v + 16, 16 * (kt0 + kt), lane);
-      aq[kt] = mma2(s0, s1, lds_quad(tdo, LDV, 16 * it, 16 * v, lane), lds_quad(tdo, LDV, 16 * it, 16 * v + 16, lane), aq[kt]);
-      ak[kt] = mma2(s0, s1, lds_quad(ty, LDV, 16 * it, 16 * v, lane), lds_quad(ty, LDV, 16 * it, 16 * v + 16, lane), ak[kt]);
-    }
-    aq[kt] *= p.scale * ff, ak[kt] *= -ff;
+    for (int t = 0; t < TERMS; ++t) m[jt][t] = a1.t[t], mt[jt][t] = a2.t[t], nn[jt][t] = a3.t[t];
   }
   __syncthreads();
-  state_store();
+  rk.store(tk), rq.store(tq);
   __syncthreads();
+  if (16 * it >= n) return;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
-    f32x4 r = {0, 0, 0, 0};
+    const int col = 16 * (kt0 + kt), lane = here(tid & 63);
 #pragma unroll
-    for (int v = 0; v < VA; v += 2)
-      r = mma2(lds_quad_t(ts, LDK, 16 * v, 16 * (kt0 + kt), lane), lds_quad_t(ts, LDK, 16 * v + 16, 16 * (kt0 + kt), lane),
-               lds_quad(tu, LDV, 16 * it, 16 * v, lane), lds_quad(tu, LDV, 16 * it, 16 * v + 16, lane), r);
-    ak[kt] += ft * r;
+    for (int jt = 0; jt < CT; jt += 2) {
+      if (16 * jt >= n) continue;
+      const quad_t<E> k0 = lds_quad_t(tk, LDK, 16 * jt, col, lane), k1 = lds_quad_t(tk, LDK, 16 * jt + 16, col, lane);
+      const quad_t<E> q0 = lds_quad_t(tq, LDK, 16 * jt, col, lane), q1 = lds_quad_t(tq, LDK, 16 * jt + 16, col, lane);
 #pragma unroll
-    for (int j = 0; j < CT; j += 2) {
-      const quad_t<E> k0 = lds_quad_t(tk, LDK, 16 * j, 16 * (kt0 + kt), lane), k1 = lds_quad_t(tk, LDK, 16 * j + 16, 16 * (kt0 + kt), lane);
-      const quad_t<E> q0 = lds_quad_t(tq, LDK, 16 * j, 16 * (kt0 + kt), lane), q1 = lds_quad_t(tq, LDK, 16 * j + 16, 16 * (kt0 + kt), lane);
-      aq[kt] = mma2(k0, k1, m[j], m[j + 1], aq[kt]);
-      ak[kt] = mma2(k0, k1, nn[j], nn[j + 1], ak[kt]);
-      ak[kt] = mma2(q0, q1, mt[j], mt[j + 1], ak[kt]);
+      for (int t = 0; t < TERMS; ++t) {
+        aq[kt] = mma2(k0, k1, m[jt][t], m[jt + 1][t], aq[kt]);
+        ar[kt] = mma2(k0, k1, nn[jt][t], nn[jt + 1][t], ar[kt]);
+        ar[kt] = mma2(q0, q1, mt[jt][t], mt[jt + 1][t], ar[kt]);
+      }
     }
-    if (row < n) {
-      const int64_t at = obase + (t0 + row) * orow;
-      const int c = 16 * (kt0 + kt) + 4 * hi;
-      if (a.q_part) store_quad((float*)a.dq + at, c, p.dk, aq[kt]);
-      else store_quad((E*)a.dq + at, c, p.dk, aq[kt]);
-      if (a.k_part) store_quad((float*)a.dk + at, c, p.dk, ak[kt]);
-      else store_quad((E*)a.dk + at, c, p.dk, ak[kt]);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (row >= n) return;
+  const int64_t at = obase + (t0 + row) * orow;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int c = 16 * (kt0 + kt) + 4 * hi;
+    if (a.q_part) store_quad((float*)a.dq + at, c, p.dk, aq[kt]);
+    else store_quad((E*)a.dq + at, c, p.dk, aq[kt]);
+    if (a.k_part) store_quad((float*)a.dk + at, c, p.dk, ar[kt]);
+    else store_quad((E*)a.dk + at, c, p.dk, ar[kt]);
   }
 }
 
