@@ -27,8 +27,9 @@ from turbompc_amd.solvers.turbompc_solver import DEFAULT_SOLVER_PARAMS, TurboMPC
 CONTROL, FINAL = "weights_penalization_control_squared", "weights_penalization_final_state"
 
 
-def run(B: int = 256, steps: int = 60, width: int = 64, dtype: torch.dtype = torch.float32, seed: int = 0, say=print):
-    """(losses, the model, histories, lengths) of a short training run."""
+def run(B: int = 256, steps: int = 60, width: int = 64, dtype: torch.dtype = torch.float32, seed: int = 0, say=print,
+        **options):
+    """(losses, the model, histories, lengths) of a short training run; options: the model's memory, norm and dropout."""
     dev = torch.device("cuda")
     gen = torch.Generator(device=dev).manual_seed(seed)
     torch.manual_seed(seed)
@@ -49,21 +50,23 @@ def run(B: int = 256, steps: int = 60, width: int = 64, dtype: torch.dtype = tor
     target = solver.solve(guess, start, expert).controls[:, :-1]
 
     model = HistoryWeights(history.shape[-1], {CONTROL: 2, FINAL: 4}, width=width, layers=2, heads=4, kv_heads=2,
-                           hidden=3 * width, dtype=dtype, device=dev)
+                           hidden=3 * width, dtype=dtype, device=dev, **options)
+    key = torch.tensor([seed, 0], device=dev)  # of the masks, where the model drops
     solve = solver.get_differentiable_solve_function()
     optimizer = torch.optim.Adam(model.parameters(), lr=3e-3)
     losses = []
     for i in range(steps):
-        weights = {k: w.double() for k, w in model(history, lengths).items()}
+        weights = {k: w.double() for k, w in model(history, lengths, key).items()}
         controls = solve(guess, start, weights).controls[:, :-1]
         loss = ((controls - target) ** 2).mean()
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
         optimizer.step()
+        key[1] += 1
         losses.append(loss.detach())
         if i % 10 == 0 or i + 1 == steps:
             say(f"step {i:4d}  mean squared control error {float(loss.detach()):.5f}")
-    return torch.stack(losses).tolist(), model, history, lengths
+    return torch.stack(losses).tolist(), model.eval(), history, lengths
 
 
 def control_loop(model, history, lengths):
