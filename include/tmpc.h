@@ -709,7 +709,8 @@ int tmpc_decay_attention_step_bf16(hipStream_t stream, const tmpc_decay_attentio
  * head or problem.  H is a multiple of each of Hq, Hk, Hv; head h reads head h / (H / Hq) of q, and so
  * on.  1 <= dk, dv <= 128.  q (B, T, Hq, dk), k (B, T, Hk, dk), v (B, T, Hv, dv) have contiguous rows;
  * beta (B, T, H) is of their type, log_decay (B, T, H) fp32.  Strides (elements) are those of
- * problem, step and head, that of a step at most 2^23 - 1; T <= 2^30, H <= 32768 and B H <= 2^23. */
+ * problem, step and head, that of a step at most 2^23 - 1; T <= 2^30, H <= 32768 and B H <= 2^22; the
+ * backward pass takes B H ceil(T / 32) < 2^31. */
 typedef struct tmpc_delta_attention {
   int32_t B, T, H, Hq, Hk, Hv, dk, dv;
   const void *q, *k, *v, *beta;

@@ -181,3 +181,26 @@ def test_differences(shape):
     for n, h in (("q", 2.0), ("k", 0.3), ("v", 2.0), ("state", 2.0), ("beta", 1.0), ("g", 0.3 if shape[2][0] > 1 else 0.5)):
         check_differences(lambda v: ours(n, v), lambda v: formula(n, v), lambda v: rounding, x[n], got["d" + n],
                           full["d" + n][0], h, 108)
+
+
+def test_more_chunks_than_a_row_of_workgroups():
+    """Past 2^22 chunks the gradients' launch has rows of workgroups; the last problems are those of a
+    call of their own."""
+    B, T, H, d = (1 << 20) + 3, 65, 2, 4
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    normal = lambda *s: torch.randn(s, generator=gen, device=DEV, dtype=torch.bfloat16)  # noqa: E731
+    x = {n: normal(B, T, H, d) for n in "qkv"}
+    x["g"] = -0.1 * torch.rand((B, T, H), generator=gen, device=DEV)
+    x["beta"] = torch.rand((B, T, H), generator=gen, device=DEV).bfloat16()
+    do = normal(B, T, H, d)
+
+    def grads(b0):
+        z = [x[n][b0:].detach().requires_grad_(True) for n in ("q", "k", "v", "g", "beta")]
+        o, _ = learning.delta_attention(*z)
+        return torch.autograd.grad(o, z, do[b0:])
+
+    whole, part = grads(0), grads(B - 300)
+    for name, got, want in zip(("q", "k", "v", "g", "beta"), whole, part):
+        assert torch.equal(got[-300:], want), name
+    del whole, part
+    torch.cuda.empty_cache()

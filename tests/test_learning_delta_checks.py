@@ -60,6 +60,24 @@ def test_refusals(lib, sfx):
     assert fwd(None, ctypes.byref(empty), None, None, None, 0) == 0 and back(empty) == 0
 
 
+@pytest.mark.parametrize("sfx", SFX)
+def test_launches_stay_within_32_bits(lib, sfx):
+    """Problems times heads past 2^22, and chunks of the backward pass past 2^31."""
+    fwd, bwd = (getattr(lib, f"tmpc_delta_attention_{n}_{sfx}") for n in ("forward", "backward"))
+    st, eb = (ctypes.c_int64 * 3)(1, 1, 1), 2 if sfx == "bf16" else 4
+    back = lambda a: bwd(None, ctypes.byref(a), X, st, None, X, X, X, X, X, X, None, 0)  # noqa: E731
+    most = attention(B=1 << 20, H=4, T=1, **DATA)
+    assert fwd(None, ctypes.byref(most), None, None, None, 0) == 2 and back(most) == 3
+    more = attention(B=(1 << 20) + 1, H=4, T=1, **DATA)
+    assert fwd(None, ctypes.byref(more), X, X, None, 0) == 1 and back(more) == 1
+    query = lambda **kw: lib.tmpc_delta_attention_workspace_bytes(eb, ctypes.byref(attention(**kw)), 1)  # noqa: E731
+    long = dict(B=64, H=4, T=8388576)  # just below 2^26 chunks
+    assert long["B"] * long["H"] * -(-long["T"] // 32) < 1 << 31
+    assert back(attention(**long, **DATA)) == 3 and query(**long) > 0
+    long = dict(B=1024, H=4, T=1 << 24)
+    assert back(attention(**long, **DATA)) == 1 and query(**long) == 0
+
+
 @pytest.mark.parametrize("eb", [2, 4])
 def test_workspaces(lib, eb):
     query = lib.tmpc_delta_attention_workspace_bytes

@@ -12,12 +12,17 @@ namespace {
 
 constexpr int64_t kMaxStep = (1 << 23) - 1;  // elements between steps: 64 fp32 steps within 31 bits
 constexpr int kMaxHeads = 32768, kMaxSteps = 1 << 30;
+constexpr int64_t kMaxBatchHeads = 1 << 22;  // workgroups of a walk, of up to 704 threads: a launch has less than 2^32
 
 bool shape_ok(const tmpc_delta_attention* a) {
   auto heads = [&](int n) { return n >= 1 && a->H % n == 0; };
   return a && a->B >= 0 && a->T >= 0 && a->T <= kMaxSteps && a->H >= 1 && a->H <= kMaxHeads && heads(a->Hq) &&
          heads(a->Hk) && heads(a->Hv) && a->dk >= 1 && a->dk <= 128 && a->dv >= 1 && a->dv <= 128 &&
-         (int64_t)a->B * a->H <= 1 << 23;
+         (int64_t)a->B * a->H <= kMaxBatchHeads;
+}
+// the backward pass' chunks, counted in 31 bits
+bool chunks_ok(const tmpc_delta_attention* a) {
+  return (int64_t)a->B * a->H * ceil_div(a->T, 32) < int64_t(1) << 31;
 }
 bool steps_ok(const tmpc_delta_attention* a) {
   for (const int64_t* s : {a->q_stride, a->k_stride, a->v_stride, a->log_decay_stride, a->beta_stride})
@@ -99,6 +104,8 @@ void launch_reverse(hipStream_t st, const DeltaBwdArgs<E>& a, int columns, int r
   const dim3 grid((unsigned)((int64_t)a.f.B * a.f.H * a.f.segs), (unsigned)ceil_div(columns, DV));
   launch(st, delta_reverse_kernel<E, DK, DV, RUN>, grid, DeltaShape<E, DK, DV>::THREADS, DeltaReverseLds<E, DK, DV, RUN>::all, a, run_width);
 }
+// A launch of n workgroups: the kernel's `flat_block()` tells them.
+inline dim3 flat_grid(int64_t n) { return dim3((unsigned)std::min(n, kFlatGrid), (unsigned)ceil_div(n, kFlatGrid)); }
 // the runs' starts, from the pass before the outputs'
 template <typename E, int DK>
 void launch_runs(hipStream_t st, const DeltaBwdArgs<E>& a, int DV) {
@@ -170,7 +177,7 @@ template <typename E>
 int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o, const int64_t* dos,
                   const float* d_out, void* dq, void* dk, void* dv, float* dg, void* dbeta, float* d_in, void* ws,
                   size_t wsb) {
-  if (!shape_ok(x)) return TMPC_EBADSHAPE;
+  if (!shape_ok(x) || !chunks_ok(x)) return TMPC_EBADSHAPE;
   if (x->B == 0) return TMPC_OK;
   if (!steps_ok(x) || (dos && (dos[1] < 0 || dos[1] > kMaxStep))) return TMPC_EBADSHAPE;
   if (!dos || !data_ok(x) || (x->T > 0 && (!d_o || !dq || !dk || !dv || !dg || !dbeta))) return TMPC_EBADARG;
@@ -209,11 +216,11 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
     if (x->T > 0) launch_walk<E, dkw(), dvw(), WALK_STATES>(st, a, dvw(), 0);
     launch_reverse<E, dkw(), dvw(), false>(st, a, dvw(), 0);
     if (x->T > 0)
-      launch(st, delta_dqk_kernel<E, dkw(), dvw()>, dim3((unsigned)(bh * w.chunks)), DeltaDqkShape<E, dkw(), dvw()>::THREADS,
+      launch(st, delta_dqk_kernel<E, dkw(), dvw()>, flat_grid(bh * w.chunks), DeltaDqkShape<E, dkw(), dvw()>::THREADS,
              DeltaDqkShape<E, dkw(), dvw()>::LDS, a);
   });
   if (x->T > 0) {
-    hipLaunchKernelGGL((delta_dgate_kernel<E>), dim3((unsigned)(bh * w.stretches)), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
+    hipLaunchKernelGGL((delta_dgate_kernel<E>), flat_grid(bh * w.stretches), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
     auto sum = [&](const void* in, int heads, int d, void* out) {
       const int64_t rows = (int64_t)x->B * x->T * heads;
       const int q = (d + 3) / 4;

@@ -109,6 +109,10 @@ __device__ inline void meet() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
+// A launch's threads stay within 32 bits: many workgroups lie in rows of kFlatGrid.
+constexpr int64_t kFlatGrid = 1 << 22;
+__device__ inline int64_t flat_block() { return blockIdx.y * kFlatGrid + blockIdx.x; }
+
 template <int CTRL>
 __device__ inline double dpp_f64(double v) {  // zero where there is no such lane
   const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -1148,7 +1152,9 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 template <typename E>
 __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows) {
   const DeltaArgs<E>& p = a.f;
-  const int seg = blockIdx.x % a.stretches, bh = blockIdx.x / a.stretches, b = bh / p.H, h = bh - b * p.H, lane = threadIdx.x;
+  const int block = (int)flat_block(), bh = block / a.stretches, seg = block - bh * a.stretches;
+  if (bh >= p.B * p.H) return;
+  const int b = bh / p.H, h = bh - b * p.H, lane = threadIdx.x;
   const int L = delta_length(p, b);
   const int t0 = seg * kDeltaSeg + lane * 4;
   const int64_t at = (int64_t)bh * rows + t0;
@@ -1200,7 +1206,8 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
-  const int chunk = blockIdx.x % a.chunks, bh = blockIdx.x / a.chunks, b = bh / p.H, h = bh - b * p.H;
+  const int block = (int)flat_block(), bh = block / a.chunks, chunk = block - bh * a.chunks, b = bh / p.H, h = bh - b * p.H;
+  if (b >= p.B) return;
   const int L = delta_length(p, b);
   const int t0 = chunk * C, n = min(C, L - t0);
   const int64_t orow = (int64_t)p.H * p.dk, obase = ((int64_t)b * p.T * p.H + h) * p.dk;

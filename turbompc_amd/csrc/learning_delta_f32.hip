@@ -11,6 +11,7 @@ size_t tmpc_delta_attention_workspace_bytes(int elem_bytes, const tmpc_delta_att
     const RunPlan runs = run_plan(a);
     return runs.state + runs.map;
   }
+  if (!chunks_ok(a)) return 0;
   return elem_bytes == 2 ? backward_plan<bf16>(a).bytes : backward_plan<float>(a).bytes;
 }
 

@@ -11,9 +11,10 @@ from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from .. import _lib
-from .ops import (MAX_BATCH_HEADS, MAX_HEAD_WIDTH, MAX_HEADS, MAX_STEPS, _call, _check, _first, _ptr, _rows,
+from .ops import (MAX_HEAD_WIDTH, MAX_HEADS, MAX_STEPS, _call, _check, _first, _ptr, _rows,
                   _step_strides, _steps, _wants_grad, _workspace)
 
+MAX_BATCH_HEADS = 1 << 22
 _DELTA = struct.Struct("@8i5P15q2Pd")  # tmpc_delta_attention, packed
 assert _DELTA.size == ctypes.sizeof(_lib.DeltaAttention)
 
@@ -32,37 +33,39 @@ def _gate_strides(t: torch.Tensor) -> Tuple[int, int, int]:
 
 def _delta_args(q, k, v, log_decay, beta, lengths, state, scale):
     B, T, H = log_decay.shape if log_decay.dim() == 3 else (log_decay.shape[0], 1, log_decay.shape[1])
-    p = lambda t: t.data_ptr() if t is not None else 0  # noqa: E731
+    *_, Hv, dv = v.shape
     return _lib.DeltaAttention.from_buffer_copy(_DELTA.pack(
-        B, T, H, q.shape[-2], k.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1], p(q), p(k), p(v), p(beta),
-        p(log_decay), *_step_strides(q), *_step_strides(k), *_step_strides(v), *_gate_strides(beta),
-        *_gate_strides(log_decay), p(lengths), p(state), scale))
+        B, T, H, q.shape[-2], k.shape[-2], Hv, q.shape[-1], dv, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        beta.data_ptr(), log_decay.data_ptr(), *_step_strides(q), *_step_strides(k), *_step_strides(v),
+        *_gate_strides(beta), *_gate_strides(log_decay), _ptr(lengths) or 0, _ptr(state) or 0, scale))
 
 
 def _check_delta(q, k, v, log_decay, beta, scale, step):
     sfx = _first("q", q, (3,) if step else (4,))
     _check("k", k, q)
     _check("v", v, q)
-    lead, dk = tuple(q.shape[:-2]), q.shape[-1]
-    if k.dim() != q.dim() or tuple(k.shape[:-2]) != lead or k.shape[-1] != dk:
-        raise ValueError(f"k has shape {tuple(k.shape)}, expected {lead + ('Hk', dk)}")
-    if v.dim() != q.dim() or tuple(v.shape[:-2]) != lead:
-        raise ValueError(f"v has shape {tuple(v.shape)}, expected {lead + ('Hv', 'dv')}")
     _check("log_decay", log_decay, q, None, torch.float32)
-    if tuple(log_decay.shape[:-1]) != lead or log_decay.dim() != q.dim() - 1:
-        raise ValueError(f"log_decay has shape {tuple(log_decay.shape)}, expected {lead + ('H',)}")
+    *lead, Hq, dk = q.shape
+    *klead, Hk, kd = k.shape if k.dim() == q.dim() else (None, 0, 0)
+    *vlead, Hv, dv = v.shape if v.dim() == q.dim() else (None, 0, 0)
+    *glead, H = log_decay.shape if log_decay.dim() else (None,)
+    if klead != lead or kd != dk:
+        raise ValueError(f"k has shape {tuple(k.shape)}, expected {(*lead, 'Hk', dk)}")
+    if vlead != lead:
+        raise ValueError(f"v has shape {tuple(v.shape)}, expected {(*lead, 'Hv', 'dv')}")
+    if glead != lead:
+        raise ValueError(f"log_decay has shape {tuple(log_decay.shape)}, expected {(*lead, 'H')}")
     _check("beta", beta, q, log_decay.shape)
-    H = log_decay.shape[-1]
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.shape[-2] < 1 or H < 1 or H % t.shape[-2]:
-            raise ValueError(f"the {H} heads of log_decay are not a multiple of the {t.shape[-2]} heads of {name}")
+    for name, n in (("q", Hq), ("k", Hk), ("v", Hv)):
+        if n < 1 or H < 1 or H % n:
+            raise ValueError(f"the {H} heads of log_decay are not a multiple of the {n} heads of {name}")
     if H > MAX_HEADS:
         raise ValueError(f"log_decay has {H} heads, expected at most {MAX_HEADS}")
     if lead[0] * H > MAX_BATCH_HEADS:
         raise ValueError(f"log_decay has {lead[0]} problems of {H} heads, expected at most {MAX_BATCH_HEADS} together")
     if not step and lead[1] > MAX_STEPS:
         raise ValueError(f"q has {lead[1]} steps, expected at most {MAX_STEPS}")
-    for name, d in (("q and k", dk), ("v", v.shape[-1])):
+    for name, d in (("q and k", dk), ("v", dv)):
         if not 1 <= d <= MAX_HEAD_WIDTH:
             raise ValueError(f"{name} have heads of {d} elements, expected 1 to {MAX_HEAD_WIDTH}")
     return sfx, float(dk ** -0.5 if scale is None else scale)
@@ -152,7 +155,7 @@ def delta_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if _wants_grad(q, k, v, log_decay, beta, state):
         raise ValueError("delta_attention_step has no gradient; use delta_attention, or torch.no_grad()")
     q, k, v = _rows(q), _rows(k), _rows(v)
-    o = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
+    o = q.new_empty((B, H, dv))
     a = _delta_args(q, k, v, log_decay, beta, None, None, scale)
     _call(f"tmpc_delta_attention_step_{sfx}", q.device, a, _ptr(active), _ptr(state), _ptr(o))
     increment_version(state)  # a backward pass that saved it has to see the change
