@@ -186,8 +186,17 @@ __global__ __launch_bounds__(256) void layer_norm_dweight_kernel(const float* __
   __shared__ float t[16][17];
   const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
   float v = 0.0f;
-  if (c < 2 * width)
-    for (int b = k; b < nblocks; b += 16) v += part[(int64_t)b * 2 * width + c];
+  if (c < 2 * width) {
+    int b = k;
+    for (; b + 7 * 16 < nblocks; b += 8 * 16) {  // eight reads on their way at a time
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = part[(int64_t)(b + i * 16) * 2 * width + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += x[i];
+    }
+    for (; b < nblocks; b += 16) v += part[(int64_t)b * 2 * width + c];
+  }
   t[k][threadIdx.x % 16] = v;
   __syncthreads();
   if (k == 0 && c < 2 * width) {

@@ -43,7 +43,7 @@ def _check_dropout(x, p, key, call, what):
 # --------------------------------------------------------------- dropout --
 def _dropout_run(x, p, key, call, sfx):
     xm, ldx = _matrix(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     _call(f"tmpc_dropout_{sfx}", x.device, xm.shape[0], xm.shape[1], _ptr(xm), ldx, p, _ptr(key), call, _ptr(y))
     return y
 
@@ -99,7 +99,7 @@ def _norm_forward(x, residual, weight, bias, eps, p, key, call, sfx, stats):
     """(y, s); stats: a (rows, 2) tensor to fill, or None."""
     xm, ldx = _matrix(x)
     rm, ldr = _matrix(residual) if residual is not None else (None, 0)
-    y, s = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    y, s = (torch.empty_like(x, memory_format=torch.contiguous_format) for _ in range(2))
     a = _norm_args(xm.shape[0], xm.shape[1], call, xm, rm, weight, bias, ldx, ldr, eps, p, key)
     _call(f"tmpc_layer_norm_forward_{sfx}", x.device, a, _ptr(y), _ptr(s), _ptr(stats))
     return y, s
