@@ -74,8 +74,7 @@ def _check_delta(q, k, v, log_decay, beta, scale, step):
 def _delta_forward(q, k, v, log_decay, beta, state, lengths, scale, sfx):
     B, T, H = log_decay.shape
     dk, dv = q.shape[-1], v.shape[-1]
-    o = torch.empty((B, T, H, dv), dtype=q.dtype, device=q.device)
-    out = torch.empty((B, H, dk, dv), dtype=torch.float32, device=q.device)
+    o, out = q.new_empty((B, T, H, dv)), log_decay.new_empty((B, H, dk, dv))
     a = _delta_args(q, k, v, log_decay, beta, lengths, state, scale)
     nbytes, ws = _workspace("tmpc_delta_attention_workspace_bytes", q.device, q.element_size(), a, 0)
     _call(f"tmpc_delta_attention_forward_{sfx}", q.device, a, _ptr(o), _ptr(out), _ptr(ws), nbytes)
@@ -97,7 +96,7 @@ class _DeltaAttention(torch.autograd.Function):
         dev = q.device
         d_o = _steps(d_o) if d_o is not None else torch.zeros(log_decay.shape + v.shape[-1:], dtype=q.dtype, device=dev)
         d_out = d_out.contiguous() if d_out is not None else None
-        empty = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+        empty = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dq, dk, dv, dg, dbeta = (empty(t) for t in (q, k, v, log_decay, beta))
         d_state = empty(state) if state is not None and ctx.needs_input_grad[5] else None
         a = _delta_args(q, k, v, log_decay, beta, lengths, state, ctx.scale)

@@ -126,9 +126,9 @@ class _LayerNorm(torch.autograd.Function):
         dsm, ldds = _matrix(ds) if ds is not None else (None, 0)
         sm, lds = _matrix(s)
         w = w.contiguous()
-        empty = lambda *shape: torch.empty(shape, dtype=s.dtype, device=dev)  # noqa: E731
-        dx, dw, db = empty(*s.shape), empty(D), empty(D) if has_bias else None
-        dr = empty(*s.shape) if has_residual and p > 0.0 else None  # else it is dx
+        like = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
+        dx, dw, db = like(s), like(w), like(w) if has_bias else None
+        dr = like(s) if has_residual and p > 0.0 else None  # else it is dx
         nbytes, ws = _workspace("tmpc_layer_norm_backward_workspace_bytes", dev, s.element_size(), M, D)
         a = _norm_args(M, D, call, None, None, w, None, 0, 0, eps, p, key)
         _call(f"tmpc_layer_norm_backward_{sfx}", dev, a, _ptr(dym), lddy, _ptr(dsm), ldds, _ptr(sm), lds,
