@@ -77,7 +77,7 @@ struct RunPlan {
 inline int tile_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 inline RunPlan run_plan(const tmpc_delta_attention* x) {
   const int64_t bh = std::max<int64_t>(1, (int64_t)x->B * x->H), stretches = std::max<int64_t>(1, ceil_div(x->T, kDeltaSeg));
-  const int64_t fill = 2 * kCUs / bh;
+  const int64_t fill = (x->dv > 64 ? 1 : 2) * kCUs / bh;
   int64_t want = std::min(fill, stretches);
   while (want > 8 && want * want > 40 * stretches) --want;
   if (want < 4) want = 1;
@@ -110,7 +110,7 @@ inline dim3 flat_grid(int64_t n) { return dim3((unsigned)std::min(n, kFlatGrid),
 template <typename E, int DK>
 void launch_runs(hipStream_t st, const DeltaBwdArgs<E>& a, int DV) {
   const DeltaArgs<E>& p = a.f;
-  launch_walk<E, DK, 64, WALK_RUN>(st, a, DV + DK, DV);
+  launch_walk<E, DK, DK == 128 ? 128 : 64, WALK_RUN>(st, a, DV + DK, DV);
   launch(st, delta_scan_kernel<DK, false>, dim3((unsigned)((int64_t)p.B * p.H * (DV / 16))), 256, 0, (const float*)p.seg_map, p.seg_state,
          p.segs, DV, p.s_in, p.dk, p.dv);
 }
@@ -209,7 +209,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   with_widths(x->dk, x->dv, [&](auto dkw, auto dvw) {
     if (a.f.segs > 1) {
       launch_runs<E, dkw()>(st, a, dvw());
-      launch_reverse<E, dkw(), 64, true>(st, a, dvw(), dvw());
+      launch_reverse<E, dkw(), dvw(), true>(st, a, dvw(), dvw());
       launch(st, delta_scan_kernel<dkw(), true>, dim3((unsigned)(bh * (dvw() / 16))), 256, 0, (const float*)a.f.seg_map, a.r_seg,
              a.f.segs, (int)dvw(), d_out, x->dk, x->dv);
     }

@@ -578,6 +578,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
   const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
   const int blocks = begin < L ? (L - begin + C - 1) / C : 0;
+  if (MODE == WALK_RUN && seg == p.segs - 1 && !a.r_seg) return;  // no run starts from it, nor has its gradient at its end
   struct Buffer {
     DeltaGates d;
     float *inv, *sums;
@@ -826,7 +827,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 // Between the passes: each run's sum becomes the state it starts from (REVERSE: the state's gradient
 // that it ends with, through the maps' transposes), for 16 columns a workgroup; its waves share the rows out.
 template <int DK, bool REVERSE>
-__global__ __launch_bounds__(256) void delta_scan_kernel(const float* map, float* state, int segs, int DV, const float* start,
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(const float* map, float* state, int segs, int DV, const float* start,
                                                          int dk, int dv) {
   constexpr int KA = DK / 16, MT = (KA + 3) / 4, LD = DK + 4;
   __shared__ __align__(16) float ts[2][16 * LD];  // (column, row)
@@ -834,27 +835,30 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const float* map, float
   const int tiles = DV / 16, bh = blockIdx.x / tiles, col = (blockIdx.x - bh * tiles) * 16 + lo;
   map += (int64_t)bh * segs * DK * DK, state += (int64_t)bh * segs * DK * DV;
   const int first = REVERSE ? segs - 1 : 0, dir = REVERSE ? -1 : 1;
-  f32x4 a[MT][KA], n[MT], s[MT];
-  auto load = [&](int seg) {
+  struct Run {
+    f32x4 map[MT][KA], sum[MT];
+  } even, odd;  // a run's and, on its way meanwhile, the next one's
+  f32x4 s[MT];
+  auto load = [&](int seg, Run& run) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int m = wave + 4 * i;
-      if (m >= KA) continue;
+      if (KA % 4 != 0 && m >= KA) continue;
 #pragma unroll
       for (int k = 0; k < KA; ++k) {
         const float* x = map + (int64_t)seg * DK * DK;
         if constexpr (REVERSE) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[i][k][r] = x[(16 * k + 4 * hi + r) * DK + 16 * m + lo];
+          for (int r = 0; r < 4; ++r) run.map[i][k][r] = x[(16 * k + 4 * hi + r) * DK + 16 * m + lo];
         } else {
-          a[i][k] = *reinterpret_cast<const f32x4*>(x + (16 * m + lo) * DK + 16 * k + 4 * hi);
+          run.map[i][k] = *reinterpret_cast<const f32x4*>(x + (16 * m + lo) * DK + 16 * k + 4 * hi);
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) n[i][r] = state[(int64_t)seg * DK * DV + (16 * m + 4 * hi + r) * DV + col];
+      for (int r = 0; r < 4; ++r) run.sum[i][r] = state[(int64_t)seg * DK * DV + (16 * m + 4 * hi + r) * DV + col];
     }
   };
-  load(first);
+  load(first, even);
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -862,32 +866,34 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const float* map, float
       const int row = 16 * (wave + 4 * i) + 4 * hi + r;
       s[i][r] = start && row < dk && col < dv ? start[((int64_t)bh * dk + row) * dv + col] : 0.0f;
     }
-  for (int j = 0; j < segs; ++j) {
+  auto step = [&](int j, const Run& run, Run& ahead) {
     const int seg = first + dir * j;
     float* t = ts[j & 1];
+    load(first + dir * min(j + 1, segs - 2), ahead);  // the last run's own are nobody's start; no branch, whose end waits for all
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int m = wave + 4 * i;
-      if (m < KA) *reinterpret_cast<f32x4*>(t + lo * LD + 16 * m + 4 * hi) = s[i];
+      if (KA % 4 == 0 || m < KA) *reinterpret_cast<f32x4*>(t + lo * LD + 16 * m + 4 * hi) = s[i];
     }
     __syncthreads();
     f32x4 all[KA];
 #pragma unroll
     for (int k = 0; k < KA; ++k) all[k] = lds_f4(t + lo * LD + 16 * k + 4 * hi);
-    f32x4 next[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int m = wave + 4 * i;
-      if (m >= KA) continue;
+      if (KA % 4 != 0 && m >= KA) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) state[(int64_t)seg * DK * DV + (16 * m + 4 * hi + r) * DV + col] = s[i][r];
-      next[i] = n[i];
+      f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < KA; ++k) next[i] = mma16(a[i][k], all[k], next[i]);
+      for (int k = 0; k < KA; ++k) acc = mma16(run.map[i][k], all[k], acc);
+      s[i] = acc + run.sum[i];
     }
-    if (j + 1 < segs) load(seg + dir);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) s[i] = next[i];
+  };
+  for (int j = 0; j < segs; j += 2) {
+    step(j, even, odd);
+    if (j + 1 < segs) step(j + 1, odd, even);
   }
 }
 
@@ -969,6 +975,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   const int bh = blockIdx.x / p.segs, seg = blockIdx.x - bh * p.segs, b = bh / p.H, h = bh - b * p.H;
   const int begin = seg * p.seg_len, L = min(delta_length(p, b), begin + p.seg_len);  // the run's end
   const int blocks = begin < L ? (L - begin + C - 1) / C : 0, last = begin / C + blocks - 1;  // block `last` comes first
+  if (RUN && seg == 0) return;  // no run ends where it starts
   const int c0 = RUN ? blockIdx.y * DV : 0;  // the first of the workgroup's columns
   struct Buffer {
     DeltaGates d;
