@@ -69,7 +69,16 @@ bool vec_ok(const DeltaArgs<E>& p) {
   return rows_ok(p.q, p.qs, p.dk) && rows_ok(p.k, p.ks, p.dk) && rows_ok(p.v, p.vs, p.dv) && ((uintptr_t)p.o & 15) == 0;
 }
 
-// How a history is cut into runs, and their arrays in the workspace.  (Both passes' runs: see below.)
+// How a history is cut into runs, and their arrays in the workspace.  A run costs its columns of the unit matrix
+// beside its own, twice the work and more, so a history is cut only where its heads leave CUs empty, into as many
+// runs as workgroups fill the CUs once: one a CU where the values are wider than 64 (eleven waves), else two.  (Two
+// histories of 200000 steps, 8 heads of 128: 3.9 ms with two a CU, 3.4 with one; 4 of 4096, 8 heads of 64,
+// with gradients: 327 us with one a CU, 315 with two.)  The runs' states are joined one after another, so
+// the best number goes by the root of the length, that of 40 times its stretches (10, 40, 160: 113, 97, 106 us for
+// 20000 steps of 4 heads of 64, 211, 199, 271 for 2 of 128, 66, 47, 47 for 4096 steps of 4 of 64).
+// Fewer than four runs are not worth their maps: two cost 447 us where whole histories take 261 (16 of 4096, 16
+// heads of 64) and 551 where they take 408 (8 of 4096, 16 of 128); three 421 and 402 (5 of 4096), but 1.43 ms
+// and 1.58 at 16384 steps.
 struct RunPlan {
   int segs, len;
   size_t state, map;  // bytes of a head's states and maps of all runs, of all heads
@@ -110,6 +119,7 @@ inline dim3 flat_grid(int64_t n) { return dim3((unsigned)std::min(n, kFlatGrid),
 template <typename E, int DK>
 void launch_runs(hipStream_t st, const DeltaBwdArgs<E>& a, int DV) {
   const DeltaArgs<E>& p = a.f;
+  // 128 wide keys: one set of helpers a CU in place of two (16 heads of 128 / 128, 50001 steps: 1.02 against 1.0 ms)
   launch_walk<E, DK, DK == 128 ? 128 : 64, WALK_RUN>(st, a, DV + DK, DV);
   launch(st, delta_scan_kernel<DK, false>, dim3((unsigned)((int64_t)p.B * p.H * (DV / 16))), 256, 0, (const float*)p.seg_map, p.seg_state,
          p.segs, DV, p.s_in, p.dk, p.dv);

@@ -20,6 +20,13 @@
 // result, enters products as three bf16 terms (24 bits); a block has two tiles there, so that they are
 // formed half as often.
 //
+// What bounds it: a walker's vector instructions and the latency of its chain (4000 to 4900 cycles a block of
+// 32 steps with two workgroups on a CU, the vector units busy for 70% of them), not memory.  Forward, 64
+// problems of 1024 steps, 8 heads of 64 / 64, bf16, whose bytes take 58 us at a copy's rate: with blocks of 16
+// steps 214 us, of 32 145 us, their inverses by whole rows 137 us, with helpers 103 to 120 us.  The helpers cost where workgroups are
+// many and short (2048 ragged histories of 101, 4 heads of 64 / 128: 297 us without them, 333 with; 1024 of
+// 51 in fp32, 4 heads of 33 / 57: 84 and 101), and a second form of every kernel was not worth that.
+//
 // Backward.  With R_t = dL/dS_t from later steps, D_t = R_t + scale q_t^T do_t:
 //   du_t = k_t D_t,  y_t = dv_t = beta_t du_t,  R_{t-1} = a_t (D_t - k_t^T y_t),  dbeta_t = du_t . e_t,
 //   dq_t = scale do_t S_t^T,  dk_t = u_t D_t^T - a_t y_t S_{t-1}^T,  dg_t = <R_{t-1}, S_{t-1}>.
@@ -49,7 +56,9 @@ struct DeltaArgs {
   float* seg_state;   // segs > 1: (B H, segs, DK, DV): each run's own sum, then the state it starts from
   float* seg_map;     // segs > 1: (B H, segs, DK, DK): what a run does to the state it starts from
 };
-constexpr int kDeltaSeg = 256;  // steps
+// Steps of a stretch: a state kept in fp32 each (1/4 of the bytes of the bf16 states at every 64 steps), and at
+// most so many terms of the gates' gradients summed up from one exact value.  Runs are whole stretches.
+constexpr int kDeltaSeg = 256;
 
 template <typename E>
 __device__ inline int delta_length(const DeltaArgs<E>& p, int b) {
@@ -280,8 +289,8 @@ __device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk,
   }
 }
 
-// A chunk's rows of one operand on their way from memory through registers to LDS, as AttnRows moves
-// them; whether they are whole pieces at 4-byte addresses is asked at run time (a variant of every kernel for
+// A block's rows of one operand on their way from memory through registers to LDS, by two helpers; whether
+// they are whole pieces at 4-byte addresses is asked at run time (a variant of every kernel for
 // it would double what there is to compile).
 template <typename E, int C, int D, int THREADS>
 struct DeltaRows {
@@ -478,7 +487,7 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
 }
 
 // ---- backward ----
-// Three kernels.  The first walks forwards in time as the forward pass does and leaves e_t, the state
+// Four kernels (and the sums over heads that share one of q's, k's or v's).  The first walks forwards in time as the forward pass does and leaves e_t, the state
 // at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
 // which gives y = dv and dbeta, and leaves the gradient at each chunk's end: over a block,
 //   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_15 - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
@@ -487,7 +496,7 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
 //   dq_i = scale exp(G_i) do_i S^T + sum_{j <= i} M_ij k_j,  M_ij = scale Gamma_ij (do_i . u_j),
 //   dk_j = exp(G_end - G_j) u_j R^T - exp(G_j) y_j S^T + sum_{i >= j} M_ij q_i
 //          - sum_{i > j} N_ij k_i - sum_{l < j} N_jl k_l,  N_ij = Gamma_ij (y_i . u_j).
-// log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>; what makes it change from step to step is
+// The last: log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>; what makes it change from step to step is
 // dg_t = dg_{t+1} + do_t . o_t - dv_t . v_t, so it is that sum from the end of each stretch of 256
 // steps, where both matrices are at hand in fp32, and o enters it unrounded.  (No values that are not
 // finite are looked for here: they may spoil the gradients of their whole history and head.)
@@ -826,6 +835,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 
 // Between the passes: each run's sum becomes the state it starts from (REVERSE: the state's gradient
 // that it ends with, through the maps' transposes), for 16 columns a workgroup; its waves share the rows out.
+// Bound by the chain: 2.9 us a run of 128 x 128 (64 dependent matrix instructions, a meeting, the states'
+// stores), with the next run's map and sum on their way meanwhile.  16 heads, 16 runs: 46 us.
 template <int DK, bool REVERSE>
 __global__ __launch_bounds__(256, 1) void delta_scan_kernel(const float* map, float* state, int segs, int DV, const float* start,
                                                          int dk, int dv) {
@@ -962,7 +973,8 @@ struct DeltaReverseLds {
   static constexpr size_t bytes = e + (RUN ? 0 : sizeof(E) * S::C * S::LDV), all = 2 * bytes;
 };
 
-// The walk backwards; RUN: what a run adds to the gradient of the state that it starts from, alone.
+// The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 156 to 189 us, where the walk for
+// the states takes 145 to 171; both are bound as the forward walk); RUN: what a run adds to the gradient of the state that it starts from, alone.
 template <typename E, int DK, int DV, bool RUN>
 __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
     DeltaBwdArgs<E> a, int run_width) {
@@ -1205,6 +1217,9 @@ struct DeltaDqkShape {
 // dq and dk of a chunk.  beta_j stays out of the operands (u_j = beta_j e_j), and in bf16 e and the scores M and N
 // enter by two terms: y and the states are what is rounded, once each.  (With e by one term dk is 2.7e-3 off
 // where a rounding is 1.66e-3, with it by two 2.1e-3.)
+// Every chunk is a workgroup of its own, so this is bound by what a CU holds: LDS for the rows by their terms
+// and half of a state at a time, registers for the scores as operands.  64 problems of 1024 steps, 8 heads
+// of 64 / 64: 153 to 174 us; 2048 ragged histories of 101, 4 heads of 64 / 128: 576 us for 1.24 GB.
 template <typename E, int DK, int DV>
 __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   using S = DeltaDqkShape<E, DK, DV>;
@@ -1414,7 +1429,8 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
 // One step, S := a S + k^T u, u = beta (v - a k S), o = scale q S, in place: a (problem, head) a workgroup, thread
 // (row group, 4 columns) with NR rows of S in registers between its one read and its write;
 // k S and q S are summed over the row groups in LDS together, o = scale (a q S + (q . k) u).
-// Bound by the state's read and write.
+// Bound by the state's read and write: 4096 problems, a quarter of them idle, 8 heads of 64 x 64: 148 to 153
+// us, 5.2 TB/s.
 template <typename E>
 struct DeltaStepArgs {
   int B, H, gq, gk, gv, dk, dv;

@@ -5,7 +5,10 @@
 // (m: dropout.hpp, made again in the backward pass).  A row stays in registers from its one
 // read to its write, so the mean is subtracted before the squares are summed: no
 // cancellation, whatever the mean.  The backward pass reads s as the forward call returned
-// it, in bf16 rounded once.
+// it, in bf16 rounded once (dx, dw and db are 2.5e-3 off where a rounding is 1.7e-3); x and the residual read
+// again instead would be one tensor pass more.  Bound by memory, both passes: 206848 x 512, bf16, with
+// dropout: 157 to 172 us (4.9 to 5.4 TB/s over four tensor passes), the gradients 197 us (5.4 TB/s over
+// five) and 5 us for the weights' sums; 20705 x 1001, fp32: 57 to 63 us.
 #pragma once
 #include "dropout.hpp"
 #include "rms_norm.hpp"

@@ -36,7 +36,8 @@ int dropout_impl(hipStream_t st, int64_t rows, int32_t width, const void* x, int
   return launch_status();
 }
 
-// Blocks of the backward pass, whose rows meet in the blocks' partial sums.
+// Blocks of the backward pass, whose rows meet in the blocks' partial sums (206848 x 512, bf16: 237 to 267 us
+// with 512, 197 with 1024, 209 with 2048, the sums' kernel 4, 5 and 10 us beside them).
 constexpr int kNormBlocks = 1024;
 int64_t backward_blocks(int64_t rows, int width, int elem_bytes) {
   return std::min<int64_t>(ceil_div(rows, rows_per_block(width, elem_bytes)), kNormBlocks);
