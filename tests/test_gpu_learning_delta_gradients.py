@@ -63,6 +63,15 @@ def test_long_histories_in_runs(shape, dtype):
             assert not bool(want[n][b, L:].any()), n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1100, (1, 1, 1, 1), 128, 128), (1, 1050, (2, 1, 1, 2), 100, 24), (1, 2299, (64, 32, 64, 64), 8, 8)],
+                         ids=SHAPE_IDS)
+def test_runs_of_other_widths_and_lengths(shape, dtype):
+    """Heads of 128 and of up to 32, whose runs go by other columns a workgroup; runs of two stretches, the
+    last one of one."""
+    check(inputs(*shape, dtype, seed=127))
+
+
 def test_spoiled_values_in_runs():
     """A value that is not finite in one run of several: earlier runs' outputs stay, later ones are spoiled."""
     x = inputs(1, 1300, (2, 2, 2, 2), 32, 32, torch.float32, seed=111)

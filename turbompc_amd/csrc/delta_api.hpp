@@ -119,7 +119,7 @@ inline dim3 flat_grid(int64_t n) { return dim3((unsigned)std::min(n, kFlatGrid),
 template <typename E, int DK>
 void launch_runs(hipStream_t st, const DeltaBwdArgs<E>& a, int DV) {
   const DeltaArgs<E>& p = a.f;
-  // 128 wide keys: one set of helpers a CU in place of two (16 heads of 128 / 128, 50001 steps: 1.02 against 1.0 ms)
+  // 128 wide keys: one set of helpers a CU in place of two (16 heads of 128 / 128, 50001 steps: 1.00 ms against 1.02)
   launch_walk<E, DK, DK == 128 ? 128 : 64, WALK_RUN>(st, a, DV + DK, DV);
   launch(st, delta_scan_kernel<DK, false>, dim3((unsigned)((int64_t)p.B * p.H * (DV / 16))), 256, 0, (const float*)p.seg_map, p.seg_state,
          p.segs, DV, p.s_in, p.dk, p.dv);

@@ -76,6 +76,7 @@ struct DeltaShape {
   static constexpr int LDP = 20, TILE_P = 16 * LDP;  // one of E
   // of a buffer, of which there are two: floats of the gates and the inverses; elements of E of the scores
   static constexpr int GATES = 6 * C + 4, INV = TRI * TILE, SCORES = TRI * TILE_P;
+  // registers for two workgroups of seven waves on a CU, or one of eleven; five-wave ones are short of nothing
   static constexpr int WAVES_PER_SIMD = W == 2 ? 2 : 3;
 };
 // tile (i, j <= i) of a block
@@ -487,8 +488,8 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
 }
 
 // ---- backward ----
-// Four kernels (and the sums over heads that share one of q's, k's or v's).  The first walks forwards in time as the forward pass does and leaves e_t, the state
-// at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
+// Four kernels (and the sums over heads that share one of q's, k's or v's).  The first walks forwards in
+// time as the forward pass does and leaves e_t, the state at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
 // which gives y = dv and dbeta, and leaves the gradient at each chunk's end: over a block,
 //   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_15 - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
 //   R := exp(G_15) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y,  Y = diag(beta) dU.
@@ -880,7 +881,8 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(const float* map, fl
   auto step = [&](int j, const Run& run, Run& ahead) {
     const int seg = first + dir * j;
     float* t = ts[j & 1];
-    load(first + dir * min(j + 1, segs - 2), ahead);  // the last run's own are nobody's start; no branch, whose end waits for all
+    // the last run's own are nobody's start; a branch in place of the min would wait for all at its end
+    load(first + dir * min(j + 1, segs - 2), ahead);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int m = wave + 4 * i;
@@ -974,7 +976,8 @@ struct DeltaReverseLds {
 };
 
 // The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 156 to 189 us, where the walk for
-// the states takes 145 to 171; both are bound as the forward walk); RUN: what a run adds to the gradient of the state that it starts from, alone.
+// the states takes 145 to 171; both are bound as the forward walk); RUN: what a run adds to the gradient of the
+// state that it starts from, alone.
 template <typename E, int DK, int DV, bool RUN>
 __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
     DeltaBwdArgs<E> a, int run_width) {
