@@ -154,7 +154,7 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
 // The backward pass' arrays in the workspace, one after another.
 struct BackwardPlan {
   int chunks, stretches, DK, DV;
-  size_t e, e_low, s, r, w, z, s_seg, dot, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
+  size_t e, e_low, s, r, w, z, s_seg, dot, dot0, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
   RunPlan runs;
 };
 template <typename E>
@@ -175,6 +175,7 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
   p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
+  p.dot0 = take(bh * 8 * sizeof(float));
   if (x->Hv != x->H) p.y = take(rows * p.DV * sizeof(E)), p.y_part = take(tok * x->dv);
   if (x->Hq != x->H) p.q_part = take(tok * x->dk);
   if (x->Hk != x->H) p.k_part = take(tok * x->dk);
@@ -201,7 +202,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   std::copy_n(dos, 3, a.dos);
   a.chunks = w.chunks, a.stretches = w.stretches;
   a.e = (E*)(base + w.e), a.e_low = (E*)(base + w.e_low), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
-  a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot);
+  a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot), a.dot0 = (float*)(base + w.dot0);
   if (x->Hv != x->H) {
     a.y = (E*)(base + w.y), a.y_part = (float*)(base + w.y_part), a.y_width = w.DV;
     a.ys[0] = (int64_t)w.chunks * AttnTile<E>::C * w.DV, a.ys[1] = w.DV;
@@ -230,7 +231,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
              DeltaDqkShape<E, dkw(), dvw()>::LDS, a);
   });
   if (x->T > 0) {
-    hipLaunchKernelGGL((delta_dgate_kernel<E>), flat_grid(bh * w.stretches), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C);
+    hipLaunchKernelGGL((delta_dgate_kernel<E>), flat_grid(bh * w.stretches), dim3(64), 0, st, a, w.chunks * AttnTile<E>::C, w.DV / 16);
     auto sum = [&](const void* in, int heads, int d, void* out) {
       const int64_t rows = (int64_t)x->B * x->T * heads;
       const int q = (d + 3) / 4;

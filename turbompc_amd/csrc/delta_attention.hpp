@@ -513,6 +513,7 @@ struct DeltaBwdArgs {
   float *w, *z;        // (B H, chunks C): do . o, y . v
   float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
   float* dot;          // (B H, stretches): <R, S> there
+  float* dot0;         // (B H, 8): at the history's start, the walkers' parts
   E* y;                // as e, or dv's output (B, T, H, dv)
   int64_t ys[2];       // its strides of (b h) and step, from b and h where it is the output
   int y_width;
@@ -567,9 +568,10 @@ template <typename E, int DK, int DV, int MODE>
 struct DeltaWalkLds {
   using S = DeltaShape<E, DK, DV>;
   static constexpr bool SCORES = MODE != WALK_RUN, DO = MODE == WALK_STATES;
+  static constexpr int TERMS = (Terms<E>::N + 1) / 2;  // of the outputs' scores: in bf16 two
   // a buffer's bytes: gates, inverses, scores (of E, or for the states fp32), sums, rows of K, V, Q, dO
   static constexpr size_t inv = sizeof(float) * S::GATES, scores = inv + sizeof(float) * S::INV;
-  static constexpr size_t sums = scores + (MODE == WALK_OUT ? sizeof(E) * S::SCORES : DO ? sizeof(float) * S::INV : 0);
+  static constexpr size_t sums = scores + (MODE == WALK_OUT ? sizeof(E) * TERMS * S::SCORES : DO ? sizeof(float) * S::INV : 0);
   static constexpr size_t k = sums + (DO ? sizeof(float) * S::W * S::C : 0), v = k + sizeof(E) * S::C * S::LDK;
   static constexpr size_t q = v + sizeof(E) * S::C * S::LDV, d_o = q + (SCORES ? sizeof(E) * S::C * S::LDK : 0);
   static constexpr size_t bytes = d_o + (DO ? sizeof(E) * S::C * S::LDV : 0), all = 2 * bytes;
@@ -652,8 +654,14 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       const Buffer x = buffer(c);
       [[maybe_unused]] const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4;
       auto put = [&](int tile, f32x4 s) {
-        if constexpr (M::DO) *reinterpret_cast<f32x4*>((float*)x.scores + tile * S::TILE + lo * LDT + 4 * hi) = s;
-        else *reinterpret_cast<quad_t<E>*>((E*)x.scores + tile * S::TILE_P + lo * LDP + 4 * hi) = to_quad<E>(s);
+        if constexpr (M::DO) {
+          *reinterpret_cast<f32x4*>((float*)x.scores + tile * S::TILE + lo * LDT + 4 * hi) = s;
+        } else {
+          const Terms<E> terms(s);
+#pragma unroll
+          for (int t = 0; t < M::TERMS; ++t)
+            *reinterpret_cast<quad_t<E>*>((E*)x.scores + (tile * M::TERMS + t) * S::TILE_P + lo * LDP + 4 * hi) = terms.t[t];
+        }
       };
       if constexpr (M::SCORES)
         if (helper == 1) delta_setup<E, S, DK, false, false, true>(x.d, x.inv, x.k, x.q, p.scale, lane, put);
@@ -720,7 +728,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     const __amdgpu_buffer_rsrc_t rs = buffer_at(MODE == WALK_OUT ? p.o + obase + t0 * orow : nullptr);
     const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
     f32x4 o[NB], e[NB], u[NB];
-    // the state and u enter outputs of bf16 by two terms (16 bits)
+    // the state, u and the scores enter outputs of bf16 by two terms (16 bits: the scores by one made outputs of
+    // heads of 16, or of short histories, 2.5e-3 off where a rounding is 1.66e-3)
     constexpr int OT = MODE == WALK_RUN ? 0 : M::DO ? Terms<E>::N : (Terms<E>::N + 1) / 2;
     meet();
     delta_state_products<E, S, KA, OT>(x.k, x.q, s, e, o, lane);
@@ -756,12 +765,17 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         o[i] *= p.scale * x.d.from[16 * i + lo];
-        const E* pt = (const E*)x.scores + (tri(i, 0)) * S::TILE_P + lo * LDP + 4 * hi;
+        const E* pt = (const E*)x.scores + lo * LDP + 4 * hi;
+        auto score = [&](int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * M::TERMS + t) * S::TILE_P); };
+        if constexpr (sizeof(E) == 2) {
 #pragma unroll
-        for (int j = 0; j <= i; ++j) {
-          const quad_t<E> pq = *reinterpret_cast<const quad_t<E>*>(pt + j * S::TILE_P);  // rounded, in bf16
-          if constexpr (sizeof(E) == 2) o[i] = mma2(ut[j].t[0], ut[j].t[1], pq, pq, o[i]);
-          else o[i] = mma16(u[j], pq, o[i]);
+          for (int j = 0; j <= i; ++j) o[i] = mma2(ut[j].t[0], ut[j].t[1], score(j, 0), score(j, 0), o[i]);
+          const quad_t<E> zero = to_quad<E>(f32x4{0, 0, 0, 0});
+          if (i == 0) o[i] = mma2(ut[0].t[0], zero, score(0, 1), zero, o[i]);
+          else o[i] = mma2(ut[0].t[0], ut[1].t[0], score(0, 1), score(1, 1), o[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j <= i; ++j) o[i] = mma16(u[j], score(j, 0), o[i]);
         }
         const unsigned at = 16 * i + lo < n ? ooff : kNowhere, past = i * otile;
         if (p.vec) {
@@ -966,13 +980,14 @@ __device__ inline void delta_reverse_update(const DeltaGates& d, const E* tk, co
 template <typename E, int DK, int DV, bool RUN>
 struct DeltaReverseLds {
   using S = DeltaShape<E, DK, DV>;
-  // a buffer's bytes: gates, inverses, scores by their terms, sums, rows of K, Q, dO, V, e
+  static constexpr int TERMS = sizeof(E) == 2 ? 2 : 1;  // of e
+  // a buffer's bytes: gates, inverses, scores by their terms, sums, rows of K, Q, dO, V, e by its terms
   static constexpr size_t inv = sizeof(float) * S::GATES, scores = inv + sizeof(float) * S::INV;
   static constexpr size_t sums = scores + sizeof(E) * Terms<E>::N * S::SCORES;
   static constexpr size_t k = sums + (RUN ? 0 : sizeof(float) * (2 * S::W * S::C + 16)), q = k + sizeof(E) * S::C * S::LDK;
   static constexpr size_t d_o = q + sizeof(E) * S::C * S::LDK, v = d_o + sizeof(E) * S::C * S::LDV;
   static constexpr size_t e = v + (RUN ? 0 : sizeof(E) * S::C * S::LDV);
-  static constexpr size_t bytes = e + (RUN ? 0 : sizeof(E) * S::C * S::LDV), all = 2 * bytes;
+  static constexpr size_t bytes = e + (RUN ? 0 : sizeof(E) * TERMS * S::C * S::LDV), all = 2 * bytes;
 };
 
 // The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 156 to 189 us, where the walk for
@@ -1034,23 +1049,32 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       return;
     }
     DeltaRows<E, C, DK, THREADS> rk, rq;
-    DeltaRows<E, C, DV, THREADS> rdo, rv, re;
+    DeltaRows<E, C, DV, THREADS> rdo, rv, re[M::TERMS];
     rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, htid);
     rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, htid);
     rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + min(c0, p.dv), a.dos[1], min(max(p.dv - c0, 0), DV), p.vec, htid);
     if constexpr (!RUN) {
       rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, htid);
-      re.init(a.e + (int64_t)bh * a.chunks * CK * DV, DV, DV, true, htid);
+#pragma unroll
+      for (int t = 0; t < M::TERMS; ++t) re[t].init((t ? a.e_low : a.e) + (int64_t)bh * a.chunks * CK * DV, DV, DV, true, htid);
     }
     auto fetch = [&](int c) {
       const int t0 = (last - c) * C;
       rk.load(t0, L - t0), rq.load(t0, L - t0), rdo.load(t0, L - t0);
-      if constexpr (!RUN) rv.load(t0, L - t0), re.load(t0, L - t0);
+      if constexpr (!RUN) {
+        rv.load(t0, L - t0);
+#pragma unroll
+        for (int t = 0; t < M::TERMS; ++t) re[t].load(t0, L - t0);
+      }
     };
     auto stage = [&](int c) {
       const Buffer x = buffer(c);
       rk.store(x.k), rq.store(x.q), rdo.store(x.d_o);
-      if constexpr (!RUN) rv.store(x.v), re.store(x.e);
+      if constexpr (!RUN) {
+        rv.store(x.v);
+#pragma unroll
+        for (int t = 0; t < M::TERMS; ++t) re[t].store(x.e + t * C * LDV);
+      }
     };
     auto setup = [&](int c) {
       const Buffer x = buffer(c);
@@ -1141,7 +1165,10 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const f32x4 y = lds_f4(x.d.beta + 16 * i + 4 * hi) * du[i];
-        const f32x4 pe = du[i] * to_f32(lds_quad_t(x.e, LDV, 16 * i, col0, lane));
+        f32x4 et = to_f32(lds_quad_t(x.e, LDV, 16 * i, col0, lane));
+        // (by one term dbeta is 2.4e-3 off)
+        if constexpr (M::TERMS == 2) et += to_f32(lds_quad_t(x.e + C * LDV, LDV, 16 * i, col0, lane));
+        const f32x4 pe = du[i] * et;
         const f32x4 pv = y * to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -1162,6 +1189,20 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     if (col0 < run_width) store_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * run_width), DK, run_width, col0, lane & 15, lane >> 4);
   } else {
     if (a.d_in && seg == 0) store_state(s, a.d_in + bh * size, p.dk, p.dv, wave * 16, lane & 15, lane >> 4);
+    if (seg == 0) {
+      float dot = 0.0f;
+      if (p.s_in) {
+        f32x4 y[KA][1];
+        load_state(y, p.s_in + bh * size, false, p.dk, p.dv, wave * 16, lane & 15, lane >> 4);
+#pragma unroll
+        for (int m = 0; m < KA; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) dot += y[m][0][r] * s[m][0][r];
+#pragma unroll
+        for (int i = 32; i; i >>= 1) dot += __shfl_xor(dot, i, 64);
+      }
+      if (lane == 0) a.dot0[bh * (int64_t)8 + wave] = dot;
+    }
     const int z0 = max(delta_length(p, b), begin), z1 = (int)min((int64_t)p.T, (int64_t)begin + p.seg_len);
     for (int t = z0 + tid; t < z1; t += S::WALKERS) a.dbeta[((int64_t)b * p.T + t) * p.H + h] = E(0.0f);
     const int64_t orow = (int64_t)p.H * p.dv, obase = ((int64_t)b * p.T * p.H + h) * p.dv;
@@ -1170,9 +1211,11 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   }
 }
 
-// log_decay's gradient: a wave a stretch, four steps a lane; in 64 bits, for the terms are.
+// log_decay's gradient: a wave a stretch, four steps a lane; in 64 bits, for the terms are.  It is known at both
+// ends of a stretch from the states there.  What the terms' errors leave between the two is shared out by the
+// terms' squares, as independent errors of their size would be (6e-7 off in place of up to 1.1e-6).
 template <typename E>
-__global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows) {
+__global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows, int walkers) {
   const DeltaArgs<E>& p = a.f;
   const int block = (int)flat_block(), bh = block / a.stretches, seg = block - bh * a.stretches;
   if (bh >= p.B * p.H) return;
@@ -1180,27 +1223,38 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
   const int L = delta_length(p, b);
   const int t0 = seg * kDeltaSeg + lane * 4;
   const int64_t at = (int64_t)bh * rows + t0;
-  double x[4], sum = 0.0;
+  double x[4], y[4], sum = 0.0, squares = 0.0;
 #pragma unroll
   for (int i = 3; i >= 0; --i) {
-    if (t0 + i < L) sum += (double)a.w[at + i] - (double)a.z[at + i];
-    x[i] = sum;
+    if (t0 + i < L) {
+      const double w = a.w[at + i], z = a.z[at + i];
+      sum += w - z, squares += w * w + z * z;
+    }
+    x[i] = sum, y[i] = squares;
   }
-  double after = sum;  // this lane's and the later ones' terms
+  double later = sum, more = squares;  // this lane's and the later ones' terms
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) {
-    const double v = __shfl_down(after, i, 64);
-    if (lane + i < 64) after += v;
+    const double v = __shfl_down(later, i, 64), u = __shfl_down(more, i, 64);
+    if (lane + i < 64) later += v, more += u;
   }
-  after -= sum;
-  if (seg * kDeltaSeg < L) after += (double)a.dot[(int64_t)bh * a.stretches + seg];
+  double after = 0.0, share = 0.0;
+  if (seg * kDeltaSeg < L) {
+    const float* dot = a.dot + (int64_t)bh * a.stretches + seg;
+    double start = 0.0;
+    if (seg > 0) start = dot[-1];
+    else for (int i = 0; i < walkers; ++i) start += (double)a.dot0[bh * (int64_t)8 + i];
+    after = dot[0];
+    const double all = __shfl(more, 0, 64);
+    if (all > 0.0) share = (start - after - __shfl(later, 0, 64)) / all;
+  }
+  later -= sum, more -= squares;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = t0 + i;
     if (t >= p.T) break;
-    float v = 0.0f;
-    if (t < L && !(p.g[b * p.gs[0] + t * p.gs[1] + h * p.gs[2]] < kNoDecay)) v = (float)(after + x[i]);
-    a.dg[((int64_t)b * p.T + t) * p.H + h] = v;
+    const bool decays = t < L && !(p.g[b * p.gs[0] + t * p.gs[1] + h * p.gs[2]] < kNoDecay);
+    a.dg[((int64_t)b * p.T + t) * p.H + h] = decays ? (float)(after + (later + x[i]) + share * (more + y[i])) : 0.0f;
   }
 }
 
