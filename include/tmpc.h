@@ -645,9 +645,10 @@ typedef struct tmpc_layer_norm {
  * pass reads. */
 int tmpc_layer_norm_forward_f32(hipStream_t stream, const tmpc_layer_norm* args, void* y, void* s, float* stats);
 int tmpc_layer_norm_forward_bf16(hipStream_t stream, const tmpc_layer_norm* args, void* y, void* s, float* stats);
-/* Its gradients from dy (pitch lddy), ds (pitch ldds, or NULL: zero), s (pitch lds) and stats:
- * dx and dresidual (rows, width; dresidual NULL: not wanted; equal to dx where p is 0), dweight and
- * dbias (width; dbias NULL: not wanted).  x, residual and bias are not read. */
+/* Its gradients from dy (pitch lddy), ds (pitch ldds, or NULL: zero), stats and s (pitch lds): dx and
+ * dresidual (rows, width; dresidual NULL: not wanted; equal to dx where p is 0), dweight and
+ * dbias (width; dbias NULL: not wanted).  s NULL: it is made again from x and residual, unrounded, which are
+ * not read otherwise; bias never is. */
 size_t tmpc_layer_norm_backward_workspace_bytes(int elem_bytes, int64_t rows, int32_t width);
 int tmpc_layer_norm_backward_f32(hipStream_t stream, const tmpc_layer_norm* args, const void* dy, int64_t lddy,
                                  const void* ds, int64_t ldds, const void* s, int64_t lds, const float* stats,

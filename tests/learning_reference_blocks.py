@@ -57,8 +57,8 @@ def layer_norm(x, r, w, b, eps, dy=None, ds=None, p=0.0, key=None, call=0):
            "s": (s, 4 * F32 * parts + e * (s.abs() + 4 * F32 * parts))}
     if dy is None:
         return out
-    # the backward pass reads s as stored, and the forward pass' statistics
-    eh = eh + rstd * e * s.abs()
+    # the backward pass reads the forward pass' statistics, and s as stored where that is in 32 bits
+    eh = eh + rstd * (e if e == F32 else 4 * F32) * s.abs()
     a = dy * w
     ma, mah = a.mean(1, keepdim=True), (a * h).mean(1, keepdim=True)
     ema = (acc + 2 * F32) * a.abs().mean(1, keepdim=True)

@@ -5,10 +5,11 @@ written out, with bounds on a kernel's rounding.
 
 Roundings to the data's type (unit e, 2^-8 for bf16): half a unit of each result, and of operands of
 products whose result is of that type.  An output is a product of q with the state at the start of its
-block of 16 steps and of scores with the block's u, each with two rounded operands at most; a
+block of 16 steps and of scores with the block's u, whose inexact operands keep 16 bits (two terms of 8,
+cut off: 2^-15 each, two a product at most); a
 gradient of q or k has up to three roundings a product (u, the score, a state), with the states at the
 ends of its chunk of 64 steps.  Each is e times the sum of the products' magnitudes; beta's
-gradient reads e_t rounded.  These are elementwise tolerances, zero in fp32.
+gradient reads e_t by two rounded terms.  These are elementwise tolerances, zero in fp32.
 
 Roundings in fp32: a step's map of the state, a (I - beta k^T k), lengthens nothing where beta |k|^2
 is from 0 to 2, so that errors made at one step are carried on and not raised, and add up as
@@ -123,7 +124,7 @@ def delta(q, k, v, g, beta, state=None, lengths=None, scale=None, do=None, dstat
     dk, dv = q.shape[-1], v.shape[-1]
     lim = lambda c: norm_limit(T, dk, dv, c)  # noqa: E731
     # 1.02: what is of second order, and the exponentials' own error
-    out = {"o": (x["o"], r * x["o"].abs() + 1.02 * 2 * r * mo, lim(3), None), "state": (x["state"], 0.0, lim(3), None)}
+    out = {"o": (x["o"], r * x["o"].abs() + 1.02 * 4 * r * r * mo, lim(3), None), "state": (x["state"], 0.0, lim(3), None)}
     if do is None:
         return out
     group = lambda z, key: z.reshape(B, T, heads[key], H // heads[key], -1).sum(3)  # noqa: E731
@@ -132,7 +133,7 @@ def delta(q, k, v, g, beta, state=None, lengths=None, scale=None, do=None, dstat
         out[key] = (total, r * total.abs() + 1.02 * 3 * r * group(mag, key), lim(6), None)
     total = group(x["y"], "dv")
     out["dv"] = (total, r * total.abs(), lim(5), None)
-    out["dbeta"] = (x["dbeta"], r * x["dbeta"].abs() + 1.02 * r * (x["du"].abs() * x["e"].abs()).sum(-1), lim(6), None)
+    out["dbeta"] = (x["dbeta"], r * x["dbeta"].abs() + 1.02 * r * r * (x["du"].abs() * x["e"].abs()).sum(-1), lim(6), None)
     # log_decay's gradient is summed up from terms do . o - dv . v: its errors are units of those too
     terms = torch.stack([(do.abs() * x["o"].abs()).sum(-1), (x["y"].abs() * f[2].abs()).sum(-1)], -1)
     out["dg"] = (x["dg"], 0.0, lim(6), terms)

@@ -38,17 +38,25 @@ struct Philox {
   }
 };
 
-// the piece of a row from column c on (a multiple of the piece): what is kept, times the factor
+// the piece of a row from column c on (a multiple of the piece): a bit an element, set where it is kept
 template <int P>
-__device__ inline void drop_piece(const Philox& rng, const DropKey& d, uint32_t row, int c, float (&v)[P]) {
+__device__ inline uint32_t drop_mask(const Philox& rng, const DropKey& d, uint32_t row, int c) {
   const uint4 w = rng((uint32_t)c / 8, row);
   const bool second = P == 4 && (c & 4);
   const uint32_t bits[4] = {second ? w.z : w.x, second ? w.w : w.y, w.z, w.w};
+  uint32_t kept = 0;
 #pragma unroll
   for (int e = 0; e < P; ++e) {
     const uint32_t h = e & 1 ? bits[e / 2] >> 16 : bits[e / 2] & 0xffffu;
-    v[e] = h >= d.least ? v[e] * d.factor : 0.0f;
+    kept |= (h >= d.least ? 1u : 0u) << e;
   }
+  return kept;
+}
+// what is kept, times the factor
+template <int P>
+__device__ inline void drop_piece(uint32_t kept, const DropKey& d, float (&v)[P]) {
+#pragma unroll
+  for (int e = 0; e < P; ++e) v[e] = kept >> e & 1 ? v[e] * d.factor : 0.0f;
 }
 
 // A thread a piece, `pieces` a row.
@@ -64,7 +72,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(uint32_t n, int width, uin
     float v[P];
 #pragma unroll
     for (int e = 0; e < P; ++e) v[e] = (float)in[e];
-    drop_piece(rng, d, row, c, v);
+    drop_piece(drop_mask<P>(rng, d, row, c), d, v);
     piece_t<E> out;
 #pragma unroll
     for (int e = 0; e < P; ++e) out[e] = (E)v[e];

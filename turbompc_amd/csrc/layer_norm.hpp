@@ -5,10 +5,10 @@
 // (m: dropout.hpp, made again in the backward pass).  A row stays in registers from its one
 // read to its write, so the mean is subtracted before the squares are summed: no
 // cancellation, whatever the mean.  The backward pass reads s as the forward call returned
-// it, in bf16 rounded once (dx, dw and db are 2.5e-3 off where a rounding is 1.7e-3); x and the residual read
-// again instead would be one tensor pass more.  Bound by memory, both passes: 206848 x 512, bf16, with
-// dropout: 157 to 172 us (4.9 to 5.4 TB/s over four tensor passes), the gradients 197 us (5.4 TB/s over
-// five) and 5 us for the weights' sums; 20705 x 1001, fp32: 57 to 63 us.
+// it, or, where that was rounded (bf16), x and r again: s rounded made dw 2.4e-3 off, for narrow rows 3e-3,
+// where a rounding is 1.7e-3.  Bound by memory, both passes: 206848 x 512, bf16, with
+// dropout: 157 to 172 us (4.9 to 5.4 TB/s over four tensor passes), the gradients 237 us (5.4 TB/s over
+// six; 197 with s rounded) and 5 us for the weights' sums; 20705 x 1001, fp32: 57 to 63 us.
 #pragma once
 #include "dropout.hpp"
 #include "rms_norm.hpp"
@@ -31,8 +31,10 @@ template <typename E>
 struct LayerNormBwdArgs {
   int64_t rows;
   int width;
-  const E *dy, *ds, *s, *w;  // ds NULL: zero
+  const E *dy, *ds, *s, *w;  // ds NULL: zero; s NULL: x and r are read
   int64_t lddy, ldds, lds_;
+  const E *x, *r;  // r NULL: zero
+  int64_t ldx, ldr;
   const float* stats;
   DropKey drop;
   E *dx, *dr;   // dr NULL: not wanted
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(256) void layer_norm_forward_kernel(LayerNormArgs<E
       const piece_t<E> px = load_piece(a.x + row * a.ldx, c, a.width, live);
 #pragma unroll
       for (int e = 0; e < P; ++e) v[i][e] = (float)px[e];
-      if (a.drop.key) drop_piece(rng, a.drop, (uint32_t)row, c, v[i]);
+      if (a.drop.key) drop_piece(drop_mask<P>(rng, a.drop, (uint32_t)row, c), a.drop, v[i]);
       if (a.r) {
         const piece_t<E> pr = load_piece(a.r + row * a.ldr, c, a.width, live);
 #pragma unroll
@@ -114,14 +116,27 @@ __global__ __launch_bounds__(256) void layer_norm_backward_kernel(LayerNormBwdAr
     const bool live = row < a.rows;
     const float mean = live ? a.stats[2 * row] : 0.0f, rstd = live ? a.stats[2 * row + 1] : 0.0f;
     float h[NP][P], g[NP][P], sa = 0.0f, sah = 0.0f;
+    uint32_t kept[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = (i * TPR + lane) * P;
-      const piece_t<E> ps = load_piece(a.s + row * a.lds_, c, a.width, live);
+      const piece_t<E> ps = a.s ? load_piece(a.s + row * a.lds_, c, a.width, live) : load_piece(a.x + row * a.ldx, c, a.width, live);
       const piece_t<E> pg = load_piece(a.dy + row * a.lddy, c, a.width, live);
+      float s[P];
+#pragma unroll
+      for (int e = 0; e < P; ++e) s[e] = (float)ps[e];
+      if (a.drop.key) kept[i] = drop_mask<P>(rng, a.drop, (uint32_t)row, c);
+      if (!a.s) {
+        if (a.drop.key) drop_piece(kept[i], a.drop, s);
+        if (a.r) {
+          const piece_t<E> pr = load_piece(a.r + row * a.ldr, c, a.width, live);
+#pragma unroll
+          for (int e = 0; e < P; ++e) s[e] += (float)pr[e];
+        }
+      }
 #pragma unroll
       for (int e = 0; e < P; ++e) {
-        h[i][e] = ((float)ps[e] - mean) * rstd, g[i][e] = (float)pg[e];  // g is zero past the row's end
+        h[i][e] = (s[e] - mean) * rstd, g[i][e] = (float)pg[e];  // g is zero past the row's end
         dw[i][e] += g[i][e] * h[i][e], db[i][e] += g[i][e];
         g[i][e] *= w[i][e];
         sa += g[i][e], sah += g[i][e] * h[i][e];
@@ -145,7 +160,7 @@ __global__ __launch_bounds__(256) void layer_norm_backward_kernel(LayerNormBwdAr
       }
       if (a.dr) store_piece(a.dr + row * a.width, c, a.width, px);
       if (a.drop.key) {
-        drop_piece(rng, a.drop, (uint32_t)row, c, d);
+        drop_piece(kept[i], a.drop, d);
 #pragma unroll
         for (int e = 0; e < P; ++e) px[e] = (E)d[e];
       }

@@ -36,8 +36,8 @@ int dropout_impl(hipStream_t st, int64_t rows, int32_t width, const void* x, int
   return launch_status();
 }
 
-// Blocks of the backward pass, whose rows meet in the blocks' partial sums (206848 x 512, bf16: 237 to 267 us
-// with 512, 197 with 1024, 209 with 2048, the sums' kernel 4, 5 and 10 us beside them).
+// Blocks of the backward pass, whose rows meet in the blocks' partial sums (206848 x 512, bf16, reading s: 237
+// to 267 us with 512, 197 with 1024, 209 with 2048, the sums' kernel 4, 5 and 10 us beside them).
 constexpr int kNormBlocks = 1024;
 int64_t backward_blocks(int64_t rows, int width, int elem_bytes) {
   return std::min<int64_t>(ceil_div(rows, rows_per_block(width, elem_bytes)), kNormBlocks);
@@ -69,7 +69,8 @@ int backward_impl(hipStream_t st, const tmpc_layer_norm* a, const void* dy, int6
                   const void* s, int64_t lds, const float* stats, void* dx, void* dr, void* dw, void* db, void* ws,
                   size_t wsb) {
   if (!args_ok(a)) return TMPC_EBADSHAPE;
-  if (!dw || (a->rows > 0 && (!dy || !s || !a->weight || !stats || !dx)) || lddy < 0 || ldds < 0 || lds < 0 ||
+  if (!dw || (a->rows > 0 && (!dy || (!s && !a->x) || !a->weight || !stats || !dx)) || lddy < 0 || ldds < 0 ||
+      lds < 0 || a->ldx < 0 || a->ldr < 0 ||
       !drop_ok(a->p, a->key))
     return TMPC_EBADARG;
   const int64_t blocks = backward_blocks(a->rows, a->width, sizeof(E));
@@ -79,7 +80,8 @@ int backward_impl(hipStream_t st, const tmpc_layer_norm* a, const void* dy, int6
   float* part = (float*)ws;
   if (a->rows > 0) {
     const LayerNormBwdArgs<E> k{a->rows, a->width, (const E*)dy, (const E*)ds, (const E*)s, (const E*)a->weight, lddy,
-                                ldds, lds, stats, drop_key(a->p, a->key, a->call), (E*)dx, (E*)dr, part};
+                                ldds, lds, (const E*)a->x, (const E*)a->residual, a->ldx, a->ldr, stats,
+                                drop_key(a->p, a->key, a->call), (E*)dx, (E*)dr, part};
     with_row<E>(a->width, [&](auto tpr, auto np) {
       hipLaunchKernelGGL((layer_norm_backward_kernel<E, tpr(), np()>), dim3((unsigned)blocks), dim3(256), 0, st, k);
     });

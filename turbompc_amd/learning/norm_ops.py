@@ -111,26 +111,31 @@ class _LayerNorm(torch.autograd.Function):
         stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=x.device)
         y, s = _norm_forward(x, residual, weight, bias, eps, p, key, call, sfx, stats)
         ctx.args = eps, p, call, sfx, residual is not None, bias is not None
-        ctx.save_for_backward(s, weight, stats, key if p > 0.0 else None)
+        if x.dtype is torch.bfloat16 and (residual is not None or p > 0.0):  # s was rounded
+            saved = None, x, residual
+        else:
+            saved = s, None, None
+        ctx.save_for_backward(*saved, weight, stats, key if p > 0.0 else None)
         ctx.set_materialize_grads(False)
         return y, s
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds):
-        s, w, stats, key = ctx.saved_tensors
+        s, x, residual, w, stats, key = ctx.saved_tensors
         eps, p, call, sfx, has_residual, has_bias = ctx.args
-        D, dev = s.shape[-1], s.device
-        M = s.numel() // D
-        dym, lddy = _matrix(dy) if dy is not None else (torch.zeros((M, D), dtype=s.dtype, device=dev), D)
-        dsm, ldds = _matrix(ds) if ds is not None else (None, 0)
-        sm, lds = _matrix(s)
+        first = s if s is not None else x
+        D, dev = first.shape[-1], first.device
+        M = first.numel() // D
+        matrix = lambda t: _matrix(t) if t is not None else (None, 0)  # noqa: E731
+        dym, lddy = _matrix(dy) if dy is not None else (torch.zeros((M, D), dtype=w.dtype, device=dev), D)
+        (dsm, ldds), (sm, lds), (xm, ldx), (rm, ldr) = matrix(ds), matrix(s), matrix(x), matrix(residual)
         w = w.contiguous()
         like = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
-        dx, dw, db = like(s), like(w), like(w) if has_bias else None
-        dr = like(s) if has_residual and p > 0.0 else None  # else it is dx
-        nbytes, ws = _workspace("tmpc_layer_norm_backward_workspace_bytes", dev, s.element_size(), M, D)
-        a = _norm_args(M, D, call, None, None, w, None, 0, 0, eps, p, key)
+        dx, dw, db = like(first), like(w), like(w) if has_bias else None
+        dr = like(first) if has_residual and p > 0.0 else None  # else it is dx
+        nbytes, ws = _workspace("tmpc_layer_norm_backward_workspace_bytes", dev, w.element_size(), M, D)
+        a = _norm_args(M, D, call, xm, rm, w, None, ldx, ldr, eps, p, key)
         _call(f"tmpc_layer_norm_backward_{sfx}", dev, a, _ptr(dym), lddy, _ptr(dsm), ldds, _ptr(sm), lds,
               _ptr(stats.contiguous()), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, (dx if dr is None else dr) if has_residual else None, dw, db, None, None, None, None, None
@@ -142,7 +147,7 @@ def layer_norm_residual(x: torch.Tensor, residual: Optional[torch.Tensor], weigh
     """(y, s): s = d(x) + residual (d(x) where residual is None) and
     y = (s - mean(s)) / sqrt(mean((s - mean(s))^2) + eps) * weight + bias over the last axis (at
     most 8192 wide), d(x) being `dropout(x, dropout, key, call)`.  y is formed from the unrounded
-    sum; the backward pass reads s."""
+    sum, and so are the gradients."""
     sfx = _first("x", x, range(1, 9))
     D = x.shape[-1]
     if not 1 <= D <= MAX_NORM_WIDTH:
