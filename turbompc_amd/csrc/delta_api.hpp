@@ -175,7 +175,7 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
   p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
-  p.dot0 = take(bh * 8 * sizeof(float));
+  if (x->T > 0) p.dot0 = take(bh * 8 * sizeof(float));
   if (x->Hv != x->H) p.y = take(rows * p.DV * sizeof(E)), p.y_part = take(tok * x->dv);
   if (x->Hq != x->H) p.q_part = take(tok * x->dk);
   if (x->Hk != x->H) p.k_part = take(tok * x->dk);

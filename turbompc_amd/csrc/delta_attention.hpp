@@ -1189,7 +1189,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     if (col0 < run_width) store_state(s, a.r_seg + blockIdx.x * (int64_t)(DK * run_width), DK, run_width, col0, lane & 15, lane >> 4);
   } else {
     if (a.d_in && seg == 0) store_state(s, a.d_in + bh * size, p.dk, p.dv, wave * 16, lane & 15, lane >> 4);
-    if (seg == 0) {
+    if (seg == 0 && L > 0) {
       float dot = 0.0f;
       if (p.s_in) {
         f32x4 y[KA][1];
