@@ -1,0 +1,39 @@
+"""The history model's operators under saved-tensor hooks that give tensors back with equal values and other
+layouts: equal gradients."""
+import pytest
+import torch
+from torch.autograd.graph import saved_tensors_hooks
+
+from test_gpu_learning_delta import inputs
+from test_gpu_learning_delta_gradients import run
+from test_learning_saved import spread, turned
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16]
+LAYOUTS = [spread, turned]
+
+
+def given_back(layout, fn):
+    with saved_tensors_hooks(lambda t: t, layout):
+        return fn()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_delta_attention(layout, dtype):
+    x = inputs(3, 40, (4, 2, 4, 1), 16, 24, dtype, lengths=[40, 0, 17])
+    want = run(x)
+    got = given_back(layout, lambda: run(x))
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+def test_delta_attention_with_repeated_values():
+    """A tensor of one value may come back as one element, expanded."""
+    x = inputs(2, 40, (2, 2, 2, 2), 16, 24, torch.float32)
+    x = dict(x, q=torch.ones_like(x["q"]), state=torch.ones_like(x["state"]))
+    want = run(x)
+    got = given_back(lambda t: t.flatten()[:1].reshape((1,) * t.dim()).expand(t.shape) if bool((t == 1).all()) else t, lambda: run(x))
+    for n in want:
+        assert torch.equal(got[n], want[n]), n

@@ -1,0 +1,88 @@
+"""What the backward passes of the history model's operators hand to their kernels where a saved-tensor hook has
+given a tensor back with equal values and another layout: the kernels' view of the memory has the values.  On
+the CPU, the calls being recorded and not made."""
+import ctypes
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from turbompc_amd.learning import delta_ops, norm_ops, ops
+
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def spread(t):
+    """t's values, three elements apart."""
+    wide = torch.full(t.shape + (3,), 7, dtype=t.dtype, device=t.device)
+    wide[..., 1] = t
+    return wide[..., 1]
+
+
+def turned(t):
+    """t's values with its axes in memory the other way round."""
+    axes = tuple(range(t.dim()))[::-1]
+    return t.permute(axes).contiguous().permute(axes)
+
+
+def given_back(tensors, layout):
+    return tuple(layout(t) if t is not None else None for t in tensors)
+
+
+def at(address, shape, strides, dtype):
+    """The values that a kernel reads from an address by these strides (elements)."""
+    size = torch.empty((), dtype=dtype).element_size()
+    n = 1 + sum((d - 1) * s for d, s in zip(shape, strides))
+    raw = bytearray(ctypes.string_at(address, n * size))
+    return torch.frombuffer(raw, dtype=dtype).as_strided(shape, strides).clone()
+
+
+def rows_at(address, t):
+    strides = torch.empty(t.shape).stride()
+    return at(address, t.shape, strides, t.dtype)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The operators' calls of the library, each read by the function that a test puts here."""
+    readers = []
+
+    def call(fn, device, *args):
+        readers[0](fn, *args)
+
+    for module in (ops, delta_ops, norm_ops):
+        monkeypatch.setattr(module, "_call", call)
+        monkeypatch.setattr(module, "_workspace", lambda *a: (0, None))
+    return readers
+
+
+def history(B, T, heads, d, dtype, seed):
+    return torch.randn((B, T, heads, d), generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("layout", [spread, turned])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_delta_attention(calls, dtype, layout):
+    B, T, H, dk, dv = 3, 5, 4, 8, 6
+    gen = torch.Generator().manual_seed(1)
+    saved = (history(B, T, 2, dk, dtype, 2), history(B, T, 4, dk, dtype, 3), history(B, T, 1, dv, dtype, 4),
+             -torch.rand((B, T, H), generator=gen), torch.rand((B, T, H), generator=gen).to(dtype),
+             torch.randn((B, H, dk, dv), generator=gen), torch.tensor([5, 2, 0], dtype=torch.int32))
+    seen = []
+
+    def read(fn, a, *rest):
+        heads = lambda t, p, s: at(p, t.shape, (s[0], s[1], s[2], 1)[:t.dim()], t.dtype)  # noqa: E731
+        q, k, v, g, beta, state, lengths = saved
+        for t, p, s in ((q, a.q, a.q_stride), (k, a.k, a.k_stride), (v, a.v, a.v_stride), (g, a.log_decay, a.log_decay_stride),
+                        (beta, a.beta, a.beta_stride)):
+            assert torch.equal(heads(t, p, list(s)), t)
+        assert torch.equal(rows_at(a.state_in, state), state) and torch.equal(rows_at(a.lengths, lengths), lengths)
+        seen.append(fn)
+
+    calls.append(read)
+    ctx = SimpleNamespace(saved_tensors=given_back(saved, layout), scale=0.5, sfx="f32", needs_input_grad=(True,) * 9)
+    with torch.no_grad():
+        grads = delta_ops._DeltaAttention.backward(ctx, torch.zeros((B, T, H, dv), dtype=dtype), None)
+    assert seen
+    for g, t in zip(grads, saved[:6]):
+        assert g.shape == t.shape and g.is_contiguous()
