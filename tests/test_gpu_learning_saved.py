@@ -6,6 +6,7 @@ from torch.autograd.graph import saved_tensors_hooks
 
 from test_gpu_learning_delta import inputs
 from test_gpu_learning_delta_gradients import run
+from test_gpu_learning_norm import key, norm_inputs, norm_run
 from test_learning_saved import spread, turned
 
 pytestmark = pytest.mark.gpu
@@ -35,5 +36,15 @@ def test_delta_attention_with_repeated_values():
     x = dict(x, q=torch.ones_like(x["q"]), state=torch.ones_like(x["state"]))
     want = run(x)
     got = given_back(lambda t: t.flatten()[:1].reshape((1,) * t.dim()).expand(t.shape) if bool((t == 1).all()) else t, lambda: run(x))
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_layer_norm(layout, dtype):
+    x = norm_inputs(9, 200, dtype, seed=14)
+    want = norm_run(x, p=0.2, k=key())
+    got = given_back(layout, lambda: norm_run(x, p=0.2, k=key()))
     for n in want:
         assert torch.equal(got[n], want[n]), n

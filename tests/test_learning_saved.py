@@ -86,3 +86,33 @@ def test_delta_attention(calls, dtype, layout):
     assert seen
     for g, t in zip(grads, saved[:6]):
         assert g.shape == t.shape and g.is_contiguous()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_norm_and_dropout(calls, dtype):
+    """All that is saved, the key's two words among it."""
+    M, D = 5, 12
+    gen = torch.Generator().manual_seed(5)
+    x, r, dy = (torch.randn((M, D), generator=gen).to(dtype) for _ in range(3))
+    w, stats, key = torch.randn(D, generator=gen).to(dtype), torch.rand((M, 2), generator=gen), torch.tensor([11, 12])
+    seen = []
+
+    def read(fn, *args):
+        seen.append(fn)
+        if "dropout" in fn:
+            assert torch.equal(rows_at(args[5], key), key)
+            return
+        a, stats_at = args[0], args[7]
+        assert torch.equal(at(a.x, (M, D), (a.ldx, 1), dtype), x) and torch.equal(at(a.residual, (M, D), (a.ldr, 1), dtype), r)
+        assert torch.equal(rows_at(a.weight, w), w) and torch.equal(rows_at(stats_at, stats), stats)
+        assert torch.equal(rows_at(a.key, key), key)
+
+    calls.append(read)
+    for layout in (spread, turned):
+        saved = given_back((None, x, r, w, stats, key), layout)
+        ctx = SimpleNamespace(saved_tensors=saved, args=(1e-5, 0.5, 0, "f32", True, True))
+        with torch.no_grad():
+            for g, t in zip(norm_ops._LayerNorm.backward(ctx, dy, None), (x, r, w, w)):
+                assert g.shape == t.shape and g.is_contiguous()
+            norm_ops._Dropout.backward(SimpleNamespace(saved_tensors=(layout(key),), args=(0.5, 0, "f32")), dy)
+    assert len(seen) == 4

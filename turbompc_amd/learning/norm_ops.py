@@ -130,14 +130,15 @@ class _LayerNorm(torch.autograd.Function):
         matrix = lambda t: _matrix(t) if t is not None else (None, 0)  # noqa: E731
         dym, lddy = _matrix(dy) if dy is not None else (torch.zeros((M, D), dtype=w.dtype, device=dev), D)
         (dsm, ldds), (sm, lds), (xm, ldx), (rm, ldr) = matrix(ds), matrix(s), matrix(x), matrix(residual)
-        w = w.contiguous()
+        # a hook may give a tensor back in another layout
+        w, stats, key = w.contiguous(), stats.contiguous(), key.contiguous() if key is not None else None
         like = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format)  # noqa: E731
         dx, dw, db = like(first), like(w), like(w) if has_bias else None
         dr = like(first) if has_residual and p > 0.0 else None  # else it is dx
         nbytes, ws = _workspace("tmpc_layer_norm_backward_workspace_bytes", dev, w.element_size(), M, D)
         a = _norm_args(M, D, call, xm, rm, w, None, ldx, ldr, eps, p, key)
         _call(f"tmpc_layer_norm_backward_{sfx}", dev, a, _ptr(dym), lddy, _ptr(dsm), ldds, _ptr(sm), lds,
-              _ptr(stats.contiguous()), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+              _ptr(stats), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, (dx if dr is None else dr) if has_residual else None, dw, db, None, None, None, None, None
 
 
