@@ -4,10 +4,12 @@ import pytest
 import torch
 from torch.autograd.graph import saved_tensors_hooks
 
+from test_gpu_learning_calls import attention_inputs
 from test_gpu_learning_delta import inputs
 from test_gpu_learning_delta_gradients import run
 from test_gpu_learning_norm import key, norm_inputs, norm_run
 from test_learning_saved import spread, turned
+from turbompc_amd import learning
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -48,3 +50,18 @@ def test_layer_norm(layout, dtype):
     got = given_back(layout, lambda: norm_run(x, p=0.2, k=key()))
     for n in want:
         assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_decay_attention(layout, dtype):
+    q, k, v, g, state = attention_inputs(3, 40, 4, 2, 16, 24, dtype, seed=2)
+    lengths = torch.tensor([40, 0, 17], dtype=torch.int32, device=DEV)
+
+    def grads():
+        leaf = [t.detach().requires_grad_(True) for t in (q, k, v, state)]
+        o, s = learning.decay_attention(leaf[0], leaf[1], leaf[2], g, leaf[3], lengths)
+        return torch.autograd.grad((o.float() ** 2).sum() + s.sum(), leaf)
+
+    for a, b in zip(given_back(layout, grads), grads()):
+        assert torch.equal(a, b)

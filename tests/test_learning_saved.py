@@ -116,3 +116,29 @@ def test_layer_norm_and_dropout(calls, dtype):
                 assert g.shape == t.shape and g.is_contiguous()
             norm_ops._Dropout.backward(SimpleNamespace(saved_tensors=(layout(key),), args=(0.5, 0, "f32")), dy)
     assert len(seen) == 4
+
+
+@pytest.mark.parametrize("layout", [spread, turned])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decay_attention(calls, dtype, layout):
+    B, T, H, dk, dv = 3, 5, 4, 8, 6
+    gen = torch.Generator().manual_seed(6)
+    saved = (history(B, T, H, dk, dtype, 7), history(B, T, 2, dk, dtype, 8), history(B, T, 2, dv, dtype, 9),
+             -torch.rand(H, generator=gen), torch.randn((B, H, dk, dv), generator=gen), torch.tensor([5, 2, 0], dtype=torch.int32))
+    seen = []
+
+    def read(fn, a, *rest):
+        q, k, v, g, state, lengths = saved
+        for t, p, s in ((q, a.q, a.q_stride), (k, a.k, a.k_stride), (v, a.v, a.v_stride)):
+            assert torch.equal(at(p, t.shape, (*s, 1), dtype), t)
+        for t, p in ((g, a.log_decay), (state, a.state_in), (lengths, a.lengths)):
+            assert torch.equal(rows_at(p, t), t)
+        seen.append(fn)
+
+    calls.append(read)
+    ctx = SimpleNamespace(saved_tensors=given_back(saved, layout), scale=0.5, sfx="f32", needs_input_grad=(True,) * 8)
+    with torch.no_grad():
+        grads = ops._DecayAttention.backward(ctx, torch.zeros((B, T, H, dv), dtype=dtype), None)
+    assert seen
+    for g, t in zip(grads[:3], saved):
+        assert g.shape == t.shape and g.is_contiguous()

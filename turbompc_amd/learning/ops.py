@@ -249,6 +249,10 @@ class _DecayAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_o, d_out):
         q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        # a hook may give a tensor back in another layout
+        q, k, v, log_decay = _steps(q), _steps(k), _steps(v), log_decay.contiguous()
+        state = state.contiguous() if state is not None else None
+        lengths = lengths.contiguous() if lengths is not None else None
         dev = q.device
         d_o = _steps(d_o) if d_o is not None else torch.zeros(q.shape[:-1] + v.shape[-1:], dtype=q.dtype, device=dev)
         d_out = d_out.contiguous() if d_out is not None else None
