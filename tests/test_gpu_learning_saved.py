@@ -65,3 +65,16 @@ def test_decay_attention(layout, dtype):
 
     for a, b in zip(given_back(layout, grads), grads()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_rms_norm(layout, dtype):
+    x = norm_inputs(9, 200, dtype, seed=15)
+
+    def grads():
+        leaf = [x[n].detach().requires_grad_(True) for n in ("x", "r", "w")]
+        return torch.autograd.grad(learning.rms_norm_residual(*leaf), leaf, [x["dy"], x["ds"]])
+
+    for a, b in zip(given_back(layout, grads), grads()):
+        assert torch.equal(a, b)

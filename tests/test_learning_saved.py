@@ -142,3 +142,24 @@ def test_decay_attention(calls, dtype, layout):
     assert seen
     for g, t in zip(grads[:3], saved):
         assert g.shape == t.shape and g.is_contiguous()
+
+
+@pytest.mark.parametrize("layout", [spread, turned])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rms_norm(calls, dtype, layout):
+    M, D = 5, 12
+    gen = torch.Generator().manual_seed(10)
+    s, dy = (torch.randn((M, D), generator=gen).to(dtype) for _ in range(2))
+    w, rstd = torch.randn(D, generator=gen).to(dtype), torch.rand(M, generator=gen)
+    seen = []
+
+    def read(fn, dev, rows, width, dy_at, lddy, ds_at, ldds, s_at, lds, w_at, rstd_at, *rest):
+        assert torch.equal(at(s_at, (M, D), (lds, 1), dtype), s)
+        assert torch.equal(rows_at(w_at, w), w) and torch.equal(rows_at(rstd_at, rstd), rstd)
+        seen.append(fn)
+
+    calls.append(lambda fn, *args: read(fn, None, *args))
+    ctx = SimpleNamespace(saved_tensors=given_back((s, w, rstd), layout), sfx="f32", has_residual=True)
+    with torch.no_grad():
+        dx, dr, dw, *_ = ops._RmsNorm.backward(ctx, dy, None)
+    assert seen and dx.is_contiguous() and dx.shape == s.shape and dw.is_contiguous() and dr is dx

@@ -152,7 +152,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds):
-        s, w, rstd = ctx.saved_tensors
+        s, w, rstd = (t.contiguous() for t in ctx.saved_tensors)  # a hook may give one back in another layout
         D = s.shape[-1]
         M = s.numel() // D
         dym, lddy = _matrix(dy) if dy is not None else (torch.zeros((M, D), dtype=s.dtype, device=s.device), D)
