@@ -78,3 +78,17 @@ def test_rms_norm(layout, dtype):
 
     for a, b in zip(given_back(layout, grads), grads()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_gated_feed_forward(layout, dtype):
+    gen = torch.Generator().manual_seed(16)
+    data = [torch.randn(s, generator=gen).to(dtype).to(DEV) * 0.3 for s in ((9, 40), (72, 40), (72, 40), (24, 72), (9, 24))]
+
+    def grads():
+        leaf = [t.detach().requires_grad_(True) for t in data[:4]]
+        return torch.autograd.grad(learning.gated_feed_forward(*leaf), leaf, data[4])
+
+    for a, b in zip(given_back(layout, grads), grads()):
+        assert torch.equal(a, b)

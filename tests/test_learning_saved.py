@@ -163,3 +163,28 @@ def test_rms_norm(calls, dtype, layout):
     with torch.no_grad():
         dx, dr, dw, *_ = ops._RmsNorm.backward(ctx, dy, None)
     assert seen and dx.is_contiguous() and dx.shape == s.shape and dw.is_contiguous() and dr is dx
+
+
+@pytest.mark.parametrize("layout", [spread, turned])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_feed_forward(calls, dtype, layout):
+    M, D, F, out = 5, 12, 7, 6
+    gen = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(s, generator=gen).to(dtype)  # noqa: E731
+    x, w_gate, w_up, w_down = r(M, D), r(F, D), r(F, D), r(out, F)
+    gate, up = torch.randn((M, F), generator=gen), torch.randn((M, F), generator=gen)
+    seen = []
+
+    def read(fn, a, gate_at, up_at, *rest):
+        assert torch.equal(at(a.x, (M, D), (a.ldx, 1), dtype), x)
+        for t, p in ((w_gate, a.w_gate), (w_up, a.w_up), (w_down, a.w_down), (gate, gate_at), (up, up_at)):
+            assert torch.equal(rows_at(p, t), t)
+        seen.append(fn)
+
+    calls.append(read)
+    ctx = SimpleNamespace(saved_tensors=given_back((x, w_gate, w_up, w_down, gate, up), layout), shape=x.shape, act=0, sfx="f32")
+    with torch.no_grad():
+        grads = ops._GatedFF.backward(ctx, r(M, out))
+    assert seen
+    for g, t in zip(grads, (x, w_gate, w_up, w_down)):
+        assert g.shape == t.shape and g.is_contiguous()

@@ -351,8 +351,9 @@ class _GatedFF(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xm, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
+        xm, *rest = ctx.saved_tensors
         xm, ldx = _matrix(xm)
+        w_gate, w_up, w_down, gate, up = (t.contiguous() for t in rest)  # a hook may give one back in another layout
         a = _ff_args(xm, ldx, w_gate, w_up, w_down, ctx.act)
         dym, lddy = _matrix(dy)
         dx = torch.empty(ctx.shape, dtype=xm.dtype, device=xm.device)
