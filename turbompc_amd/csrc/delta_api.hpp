@@ -76,9 +76,12 @@ bool vec_ok(const DeltaArgs<E>& p) {
 // with gradients: 327 us with one a CU, 315 with two.)  The runs' states are joined one after another, so
 // the best number goes by the root of the length, that of 40 times its stretches (10, 40, 160: 113, 97, 106 us for
 // 20000 steps of 4 heads of 64, 211, 199, 271 for 2 of 128, 66, 47, 47 for 4096 steps of 4 of 64).
-// Fewer than four runs are not worth their maps: two cost 447 us where whole histories take 261 (16 of 4096, 16
-// heads of 64) and 551 where they take 408 (8 of 4096, 16 of 128); three 421 and 402 (5 of 4096), but 1.43 ms
-// and 1.58 at 16384 steps.
+// Fewer than four runs are not worth their maps and not asked for: two cost 447 us where whole histories take
+// 261 (16 of 4096, 16 heads of 64) and 551 where they take 408 (8 of 4096, 16 of 128); three 421 and 402 (5 of
+// 4096), but 1.43 ms and 1.58 at 16384 steps.  Runs are whole stretches, so four of five, six or
+// nine stretches come out as three: forwards 93 and 92 us where whole histories take 76 and 90 (16 of 1280 and 1536, 8
+// heads of 64, bf16), with gradients 390 and 414 against 373 and 441; 128 wide, 8 of 1280 and 1500, 168 and 168
+// against 139 and 163, with gradients 667 and 685 against 712 and 840.
 struct RunPlan {
   int segs, len;
   size_t state, map;  // bytes of a head's states and maps of all runs, of all heads
