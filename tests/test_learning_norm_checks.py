@@ -78,3 +78,11 @@ def test_host_tensors_and_wrong_types_are_refused():
                  lambda: learning.layer_norm_residual(x.half(), None, w)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("p", [float("inf"), -float("inf"), float("nan"), 1e300, 1.0, 1.0 - 2.0 ** -18, -1e-9])
+def test_probabilities_out_of_range_are_value_errors(p):
+    from turbompc_amd.learning.norm_ops import _check_dropout
+
+    with pytest.raises(ValueError, match="at least 0"):
+        _check_dropout(torch.zeros(2, 8), p, torch.zeros(2, dtype=torch.int64), 0, "p")

@@ -26,7 +26,7 @@ MAX_DROPOUT_ROWS = (1 << 31) - 1
 
 def _check_dropout(x, p, key, call, what):
     """p as a float; the key's and call's checks where something is dropped."""
-    if not (0.0 <= p and round(p * 65536) < 65536):
+    if not (0.0 <= p < 1.0 and round(p * 65536) < 65536):
         raise ValueError(f"{what} must be at least 0 and less than 1 - 2^-17, got {p}")
     if isinstance(call, bool) or not isinstance(call, int) or not 0 <= call < 1 << 32:
         raise ValueError(f"call must be a whole number from 0 to 2^32 - 1, got {call!r}")
