@@ -728,8 +728,10 @@ int tmpc_delta_attention_forward_f32(hipStream_t stream, const tmpc_delta_attent
 int tmpc_delta_attention_forward_bf16(hipStream_t stream, const tmpc_delta_attention* args, void* o, float* state_out,
                                       void* workspace, size_t workspace_bytes);
 /* Gradients from those of o (d_o, strides d_o_stride) and of the final state (d_state_out, or NULL:
- * zero): dq (B, T, Hq, dk), dk (B, T, Hk, dk), dv (B, T, Hv, dv), dlog_decay (B, T, H, fp32; zero where the decay
- * is), dbeta (B, T, H) and d_state_in (B, H, dk, dv, or NULL), contiguous; zero past a length.  The state is
+ * zero): dq (B, T, Hq, dk), dk (B, T, Hk, dk), dv (B, T, Hv, dv), dlog_decay (B, T, H, fp32: zero
+ * where exp(log_decay) is below 2^-126, and off by last bits of the gradients within 256 steps of it, so that a step
+ * which forgets nearly all between steps which do not has few bits of its own), dbeta (B, T, H) and d_state_in (B, H,
+ * dk, dv, or NULL), contiguous; zero past a length.  The state is
  * formed again; nothing of the forward call is kept.  Values that are not finite may spoil the
  * gradients of their whole history and head. */
 int tmpc_delta_attention_backward_f32(hipStream_t stream, const tmpc_delta_attention* args, const void* d_o,

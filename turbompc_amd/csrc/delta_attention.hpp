@@ -226,12 +226,19 @@ __device__ inline f32x4 row_products(const quad_t<E> (&x)[KA], const quad_t<E> (
   return t;
 }
 
-// What the walkers need of a block, by one wave.  INVERSE: the tiles on the diagonal of (I + A)^-1, or with
-// REVERSE of (I + A')^-T, and the other tile of -A, or of -A'^T; each has beta of the column.  SCORES: put(tile (i, j),
-// values) with scale (q_i . k_j) Gamma_ij, a lane having i = lo and j = 4 hi + r, or with REVERSE j = lo and
-// i = 4 hi + r.
-template <typename E, typename S, int DK, bool REVERSE, bool INVERSE, bool SCORES, typename Put>
-__device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk, const E* tq, float scale, int lane, Put put) {
+// Which of a block's scores are made: none, those of j <= i, or those of j < i and apart from them each step's own.
+enum DeltaScores { NO_SCORES, ALL_SCORES, EARLIER_SCORES };
+struct DeltaNone {
+  template <typename... A>
+  __device__ void operator()(A...) const {}
+};
+
+// What the walkers need of a block, by one wave.  INVERSE: the tiles on the diagonal of (I + A)^-1 - I, or with
+// REVERSE of (I + A')^-T - I, and the other tile of -A, or of -A'^T; each has beta of the column.  SCORES: put(tile
+// (i, j), values) with scale (q_i . k_j) Gamma_ij, a lane having i = lo and j = 4 hi + r, or with REVERSE j = lo and
+// i = 4 hi + r; own(i, scale (q_i . k_i)).
+template <typename E, typename S, int DK, bool REVERSE, bool INVERSE, DeltaScores SCORES, typename Put, typename Own>
+__device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk, const E* tq, float scale, int lane, Put put, Own own) {
   constexpr int NB = S::NB, LDT = S::LDT, KA = DK / 16;
   const int lo = lane & 15, hi = lane >> 4;
   quad_t<E> k[NB][KA];
@@ -239,7 +246,8 @@ __device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk,
   for (int i = 0; i < NB; ++i)
 #pragma unroll
     for (int m = 0; m < KA; ++m) k[i][m] = lds_quad(tk, S::LDK, 16 * i, 16 * m, lane);
-  if constexpr (SCORES) {
+  if constexpr (SCORES != NO_SCORES) {
+    constexpr int AFTER = SCORES == EARLIER_SCORES ? 1 : 0;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       quad_t<E> q[KA];
@@ -250,8 +258,11 @@ __device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk,
         f32x4 x = REVERSE ? row_products<E, KA>(q, k[j]) : row_products<E, KA>(k[j], q);
         const f32x4 ratio = delta_ratio<REVERSE>(d, REVERSE ? 16 * j : 16 * i, REVERSE ? 16 * i : 16 * j, lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[r] = i > j || (REVERSE ? 4 * hi + r >= lo : 4 * hi + r <= lo) ? scale * (x[r] * ratio[r]) : 0.0f;
+        for (int r = 0; r < 4; ++r) {
+          const int at = 4 * hi + r;
+          if (AFTER && i == j && at == lo) own(16 * i + lo, scale * x[r]);
+          x[r] = i > j || (REVERSE ? at >= lo + AFTER : at + AFTER <= lo) ? scale * (x[r] * ratio[r]) : 0.0f;
+        }
         put(tri(i, j), x);
       }
     }
@@ -286,7 +297,11 @@ __device__ inline void delta_setup(const DeltaGates& d, float* inv, const E* tk,
     });
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < NB; ++i) *rows(tri(i, i)) = t[i];
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[i][r] = 4 * hi + r == lo ? 0.0f : t[i][r];
+      *rows(tri(i, i)) = t[i];
+    }
   }
 }
 
@@ -365,6 +380,17 @@ struct Terms<bf16> {
   }
 };
 
+// An fp32 value where elements of E are kept: itself, or its bits as two halves.
+template <typename E>
+__device__ inline E upper(float v) {
+  if constexpr (sizeof(E) == 4) return v;
+  else return __builtin_bit_cast(bf16, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16));
+}
+__device__ inline bf16 lower(float v) { return __builtin_bit_cast(bf16, (uint16_t)__builtin_bit_cast(uint32_t, v)); }
+__device__ inline float joined(bf16 high, bf16 low) {
+  return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, high) << 16 | __builtin_bit_cast(uint16_t, low));
+}
+
 // acc += sum over NB tiles of A_i x_i, 16 contracted entries each, x by its terms
 template <int NB>
 __device__ inline f32x4 mma_terms(const bf16x4 (&a)[NB], const Terms<bf16> (&x)[NB], f32x4 acc) {
@@ -405,20 +431,28 @@ __device__ inline void delta_state_products(const E* k, const E* q, const f32x4 
   }
 }
 
-// e = (I + A)^-1 x, or with REVERSE (I + A')^-T x, over the block's tiles, from what delta_setup left
-template <typename S, bool REVERSE>
-__device__ inline void delta_solve(const float* inv, f32x4 (&x)[S::NB], f32x4 (&e)[S::NB], int lane) {
+// e = (I + A)^-1 (w + c), or with REVERSE by (I + A')^-T, over the block's tiles, from what delta_setup left.  With PARTS
+// c := e - w, summed up by itself (where w is far larger, c would be lost in it); without, w is not used.  (PARTS
+// everywhere: 315 in place of 304 us for the outputs of 2048 ragged histories of 101, 4 heads of 64 / 128.)
+template <typename S, bool REVERSE, bool PARTS>
+__device__ inline void delta_solve(const float* inv, const f32x4 (&w)[S::NB], f32x4 (&c)[S::NB], f32x4 (&e)[S::NB], int lane) {
   const float* at = inv + (lane & 15) * S::LDT + 4 * (lane >> 4);
-  const f32x4 zero = {0, 0, 0, 0};
+  auto tile = [&](int i, f32x4 t) {
+    if constexpr (PARTS) {
+      c[i] = mma16(t, c[i] + w[i], c[i]), e[i] = c[i] + w[i];
+    } else {
+      e[i] = mma16(t, c[i], c[i]);
+    }
+  };
   if constexpr (S::NB == 2) {
     constexpr int first = REVERSE ? 1 : 0, second = 1 - first;
     const f32x4 t0 = lds_f4(at + tri(first, first) * S::TILE), corner = lds_f4(at + tri(1, 0) * S::TILE);
     const f32x4 t1 = lds_f4(at + tri(second, second) * S::TILE);
-    e[first] = mma16(t0, x[first], zero);
-    x[second] = mma16(corner, e[first], x[second]);
-    e[second] = mma16(t1, x[second], zero);
+    tile(first, t0);
+    c[second] = mma16(corner, e[first], c[second]);
+    tile(second, t1);
   } else {
-    e[0] = mma16(lds_f4(at), x[0], zero);
+    tile(0, lds_f4(at));
   }
 }
 
@@ -489,18 +523,24 @@ __device__ __attribute__((always_inline)) inline void delta_by_step(const DeltaA
 
 // ---- backward ----
 // Four kernels (and the sums over heads that share one of q's, k's or v's).  The first walks forwards in
-// time as the forward pass does and leaves e_t, the state at each chunk's start and do_t . o_t.  The second walks backwards with the state's gradient,
-// which gives y = dv and dbeta, and leaves the gradient at each chunk's end: over a block,
-//   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_15 - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
-//   R := exp(G_15) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y,  Y = diag(beta) dU.
+// time as the forward pass does and leaves x_t = a_t k_t S_{t-1} (so e_t = v_t - x_t), the state at each chunk's start
+// and the first of dg's terms below.  The second walks backwards with the state's gradient,
+// which gives y = dv and dbeta, and leaves the gradient at each chunk's end and dg's other terms: over a block,
+//   dU = (I + A')^-T (scale (Q K^T o Gamma)^T dO + diag(exp(G_end - G)) K R),  A'_ij = beta_i Gamma_ij (k_i . k_j),
+//   R := exp(G_end) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y,  Y = diag(beta) dU.
 // With the state and its gradient known at its ends every chunk then gives its dq and dk by itself:
 //   dq_i = scale exp(G_i) do_i S^T + sum_{j <= i} M_ij k_j,  M_ij = scale Gamma_ij (do_i . u_j),
 //   dk_j = exp(G_end - G_j) u_j R^T - exp(G_j) y_j S^T + sum_{i >= j} M_ij q_i
 //          - sum_{i > j} N_ij k_i - sum_{l < j} N_jl k_l,  N_ij = Gamma_ij (y_i . u_j).
-// The last: log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>; what makes it change from step to step is
-// dg_t = dg_{t+1} + do_t . o_t - dv_t . v_t, so it is that sum from the end of each stretch of 256
-// steps, where both matrices are at hand in fp32, and o enters it unrounded.  (No values that are not
-// finite are looked for here: they may spoil the gradients of their whole history and head.)
+// The last: log_decay's gradient is dg_t = <R_{t-1}, S_{t-1}>, known from fp32 matrices at the ends of each stretch of
+// 256 steps, and from step to step dg_t - dg_{t+1} = do_t . o_t - y_t . v_t.  Taken so, what a step has in o_t
+// from itself and in v_t from itself cancels, and where decays are strong that is nearly all: at
+// log_decay -8 dg was 1e-4 off, at -20 it was lost.  With both parts left out
+//   dg_t = dg_{t+1} + w_t - z_t,  w_t = scale a_t do_t . (q_t S_{t-1}),  z_t = y_t . x_t + u_t . (k_t R_t),
+// whose terms have the decays of the gradients that they lead to or from.  They come by themselves from the
+// block's sums: w_t with the scores of j < t, and with T = (I + A)^-1, c = diag(exp G) K S and what the tiles before
+// add to it, x = c - (T - I) (V - c), so that e = V - x; k_t R_t = du_t - scale (q_t . k_t) do_t likewise.
+// (No values that are not finite are looked for here: they may spoil the gradients of their whole history and head.)
 template <typename E>
 struct DeltaBwdArgs {
   DeltaArgs<E> f;
@@ -508,9 +548,9 @@ struct DeltaBwdArgs {
   int64_t dos[3];
   const float* d_out;  // (B, H, dk, dv) or NULL
   int chunks, stretches;  // of T
-  E *e, *e_low;        // (B H, chunks C, DV): e_t, in bf16 by two terms
+  E *x, *x_low;        // (B H, chunks C, DV): x_t, fp32 (in bf16 its upper and its lower halves)
   E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends
-  float *w, *z;        // (B H, chunks C): do . o, y . v
+  float *w, *z;        // (B H, chunks C): the parts of dg_t - dg_{t+1}
   float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
   float* dot;          // (B H, stretches): <R, S> there
   float* dot0;         // (B H, 8): at the history's start, the walkers' parts
@@ -613,7 +653,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       auto fetch = [&](int c) { rg.load(L - begin - c * C, lane); };
       auto setup = [&](int c) {
         const Buffer x = buffer(c);
-        delta_setup<E, S, DK, false, true, false>(x.d, x.inv, x.k, x.q, p.scale, here(lane), [](int, f32x4) {});
+        delta_setup<E, S, DK, false, true, NO_SCORES>(x.d, x.inv, x.k, x.q, p.scale, here(lane), DeltaNone(), DeltaNone());
       };
       if (blocks > 0) fetch(0), rg.scan(lane), rg.store(buffer(0).d, lane);
       meet();
@@ -664,15 +704,16 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         }
       };
       if constexpr (M::SCORES)
-        if (helper == 1) delta_setup<E, S, DK, false, false, true>(x.d, x.inv, x.k, x.q, p.scale, lane, put);
+        if (helper == 1)
+          delta_setup<E, S, DK, false, false, M::DO ? EARLIER_SCORES : ALL_SCORES>(x.d, x.inv, x.k, x.q, p.scale, lane, put, DeltaNone());
     };
     auto results = [&](int c) {  // of a block that the walkers have left
       if constexpr (M::DO) {
         const Buffer x = buffer(c);
         const int t0 = begin + c * C, n = min(C, L - t0);
         const int64_t at = ((int64_t)bh * a.chunks * CK + t0) * DV;
-        copy_out(rv, x.v, a.e + at, DV, n, DV);
-        if constexpr (sizeof(E) == 2) copy_out(rdo, x.d_o, a.e_low + at, DV, n, DV);
+        copy_out(rv, x.v, a.x + at, DV, n, DV);
+        if constexpr (sizeof(E) == 2) copy_out(rdo, x.d_o, a.x_low + at, DV, n, DV);
         if (htid < n) {
           float w = 0.0f;
 #pragma unroll
@@ -727,33 +768,32 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + t0 / CK) * DK * DV, s, wave * 16, lane & 15, lane >> 4);
     const __amdgpu_buffer_rsrc_t rs = buffer_at(MODE == WALK_OUT ? p.o + obase + t0 * orow : nullptr);
     const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-    f32x4 o[NB], e[NB], u[NB];
+    f32x4 o[NB], v[NB], held[NB], u[NB];  // held: - a_t k_t S_{t-1}, where the outputs alone are made v_t less that
     // the state, u and the scores enter outputs of bf16 by two terms (16 bits: the scores by one made outputs of
     // heads of 16, or of short histories, 2.5e-3 off where a rounding is 1.66e-3)
     constexpr int OT = MODE == WALK_RUN ? 0 : M::DO ? Terms<E>::N : (Terms<E>::N + 1) / 2;
     meet();
-    delta_state_products<E, S, KA, OT>(x.k, x.q, s, e, o, lane);
+    delta_state_products<E, S, KA, OT>(x.k, x.q, s, held, o, lane);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-      e[i] = to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane)) - lds_f4(x.d.from + 16 * i + 4 * hi) * e[i];
+    for (int i = 0; i < NB; ++i) {
+      v[i] = to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane));
+      held[i] *= -lds_f4(x.d.from + 16 * i + 4 * hi);
+      if constexpr (!M::DO) held[i] += v[i];
+    }
     quad_t<E> kt[KA][NB];  // read ahead of their use
     transposed_rows<E, S, KA>(x.k, kt, lane);
     f32x4 beta[NB], to[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) beta[i] = lds_f4(x.d.beta + 16 * i + 4 * hi), to[i] = lds_f4(x.d.to + 16 * i + 4 * hi);
     const float total = *x.d.total;
-    delta_solve<S, false>(x.inv, e, u, lane);
+    delta_solve<S, false, M::DO>(x.inv, v, held, u, lane);
     Terms<E> w[NB];
-    [[maybe_unused]] bf16x4 low[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      // these columns of V are this wave's alone and have been read: e takes their place
+      // these columns of V are this wave's alone and have been read: x takes their place
       if constexpr (M::DO)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const E high = (E)u[i][r];
-          x.v[(16 * i + 4 * hi + r) * LDV + col0 + lo] = high, low[i][r] = (bf16)(u[i][r] - (float)high);
-        }
+        for (int r = 0; r < 4; ++r) x.v[(16 * i + 4 * hi + r) * LDV + col0 + lo] = upper<E>(-held[i][r]);
       u[i] *= beta[i];
       w[i] = Terms<E>(to[i] * u[i]);
     }
@@ -792,7 +832,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         }
       }
     }
-    if constexpr (M::DO) {  // do . o, unrounded
+    if constexpr (M::DO) {  // a_t do_t . (scale q_t S_{t-1}), unrounded
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         o[i] *= p.scale * x.d.from[16 * i + lo];
@@ -805,13 +845,13 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         if (hi == 0) x.sums[wave * C + 16 * i + lo] = w1;
         if constexpr (sizeof(E) == 2)  // and so for dO
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x.d_o[(16 * i + 4 * hi + r) * LDV + col0 + lo] = low[i][r];
+          for (int r = 0; r < 4; ++r) x.d_o[(16 * i + 4 * hi + r) * LDV + col0 + lo] = lower(-held[i][r]);
       }
     }
     if (M::DO && ((t0 + C) % kDeltaSeg == 0 || t0 + C >= L)) {
-    f32x4* dst = reinterpret_cast<f32x4*>(a.s_seg + ((int64_t)bh * a.stretches + t0 / kDeltaSeg) * DK * DV) + wave * KA * 64 + lane;
+      f32x4* dst = reinterpret_cast<f32x4*>(a.s_seg + ((int64_t)bh * a.stretches + t0 / kDeltaSeg) * DK * DV) + wave * KA * 64 + lane;
 #pragma unroll
-    for (int m = 0; m < KA; ++m) dst[m * 64] = s[m][0];
+      for (int m = 0; m < KA; ++m) dst[m * 64] = s[m][0];
     }
     meet();
   }
@@ -924,18 +964,19 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(const float* map, fl
   }
 }
 
-// dU of a block, and dO's columns as operands
-template <typename E, typename S, int KA>
-__device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv, const E* tp, const E* tk, const E* tdo,
-                                           const f32x4 (&s)[KA][1], quad_t<E> (&g)[S::NB], f32x4 (&du)[S::NB], int col0, int lane) {
+// dU of a block, dO's columns as operands, and with PARTS x_t = k_t R_t
+template <typename E, typename S, int KA, bool PARTS>
+__device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv, const float* own, const E* tp, const E* tk,
+                                           const E* tdo, const f32x4 (&s)[KA][1], quad_t<E> (&g)[S::NB], f32x4 (&du)[S::NB],
+                                           f32x4 (&x)[S::NB], int col0, int lane) {
   constexpr int NB = S::NB, TERMS = Terms<E>::N;
   const int lo = lane & 15, hi = lane >> 4;
-  f32x4 x[NB], none[NB];
+  f32x4 w[NB], none[NB];
   delta_state_products<E, S, KA, 0>(tk, tk, s, x, none, lane);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     g[i] = lds_quad_t(tdo, S::LDV, 16 * i, col0, lane);
-    x[i] *= lds_f4(d.to + 16 * i + 4 * hi);
+    x[i] *= lds_f4(d.to + 16 * i + 4 * hi), w[i] = lds_f4(own + 16 * i + 4 * hi) * to_f32(g[i]);
   }
   const E* pt = tp + lo * S::LDP + 4 * hi;
   auto score = [&](int i, int j, int t) { return *reinterpret_cast<const quad_t<E>*>(pt + (tri(i, j) * TERMS + t) * S::TILE_P); };
@@ -948,7 +989,10 @@ __device__ inline void delta_reverse_solve(const DeltaGates& d, const float* inv
   } else {
     x[0] = mma16(score(0, 0, 0), g[0], x[0]);
   }
-  delta_solve<S, true>(inv, x, du, lane);
+  if constexpr (!PARTS)
+#pragma unroll
+    for (int i = 0; i < NB; ++i) x[i] += w[i];
+  delta_solve<S, true, PARTS>(inv, w, x, du, lane);
 }
 
 // R := exp(G_end) R + (diag(exp G) scale Q)^T dO - (diag(exp G) K)^T Y
@@ -980,14 +1024,14 @@ __device__ inline void delta_reverse_update(const DeltaGates& d, const E* tk, co
 template <typename E, int DK, int DV, bool RUN>
 struct DeltaReverseLds {
   using S = DeltaShape<E, DK, DV>;
-  static constexpr int TERMS = sizeof(E) == 2 ? 2 : 1;  // of e
-  // a buffer's bytes: gates, inverses, scores by their terms, sums, rows of K, Q, dO, V, e by its terms
+  static constexpr int TERMS = sizeof(E) == 2 ? 2 : 1;  // elements of E that hold an x
+  // a buffer's bytes: gates, inverses, scores by their terms, the steps' own and sums, rows of K, Q, dO, V, x
   static constexpr size_t inv = sizeof(float) * S::GATES, scores = inv + sizeof(float) * S::INV;
   static constexpr size_t sums = scores + sizeof(E) * Terms<E>::N * S::SCORES;
-  static constexpr size_t k = sums + (RUN ? 0 : sizeof(float) * (2 * S::W * S::C + 16)), q = k + sizeof(E) * S::C * S::LDK;
+  static constexpr size_t k = sums + sizeof(float) * (S::C + (RUN ? 0 : 2 * S::W * S::C + 16)), q = k + sizeof(E) * S::C * S::LDK;
   static constexpr size_t d_o = q + sizeof(E) * S::C * S::LDK, v = d_o + sizeof(E) * S::C * S::LDV;
-  static constexpr size_t e = v + (RUN ? 0 : sizeof(E) * S::C * S::LDV);
-  static constexpr size_t bytes = e + (RUN ? 0 : sizeof(E) * TERMS * S::C * S::LDV), all = 2 * bytes;
+  static constexpr size_t x = v + (RUN ? 0 : sizeof(E) * S::C * S::LDV);
+  static constexpr size_t bytes = x + (RUN ? 0 : sizeof(E) * TERMS * S::C * S::LDV), all = 2 * bytes;
 };
 
 // The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 163 to 190 us, where the walk for
@@ -1009,14 +1053,14 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   const int c0 = RUN ? blockIdx.y * DV : 0;  // the first of the workgroup's columns
   struct Buffer {
     DeltaGates d;
-    float *inv, *beta, *z, *dot;
-    E *scores, *k, *q, *d_o, *v, *e;
+    float *inv, *own, *beta, *z, *dot;
+    E *scores, *k, *q, *d_o, *v, *x;
   };
   auto buffer = [&](int i) {
     char* x = smem + (i & 1) * M::bytes;
-    float* sums = (float*)(x + M::sums);
-    return Buffer{delta_gates<S>((float*)x), (float*)(x + M::inv), sums, sums + S::W * C, sums + 2 * S::W * C, (E*)(x + M::scores),
-                  (E*)(x + M::k), (E*)(x + M::q), (E*)(x + M::d_o), (E*)(x + M::v), (E*)(x + M::e)};
+    float *own = (float*)(x + M::sums), *sums = own + C;
+    return Buffer{delta_gates<S>((float*)x), (float*)(x + M::inv), own, sums, sums + S::W * C, sums + 2 * S::W * C, (E*)(x + M::scores),
+                  (E*)(x + M::k), (E*)(x + M::q), (E*)(x + M::d_o), (E*)(x + M::v), (E*)(x + M::x)};
   };
   auto ends = [&](int t0, int of) { return (t0 + C) % of == 0 || t0 + C >= L; };
 
@@ -1030,7 +1074,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       auto fetch = [&](int c) { rg.load(L - (last - c) * C, lane); };
       auto setup = [&](int c) {
         const Buffer x = buffer(c);
-        delta_setup<E, S, DK, true, true, false>(x.d, x.inv, x.k, x.q, p.scale, here(lane), [](int, f32x4) {});
+        delta_setup<E, S, DK, true, true, NO_SCORES>(x.d, x.inv, x.k, x.q, p.scale, here(lane), DeltaNone(), DeltaNone());
       };
       if (blocks > 0) fetch(0), rg.scan(lane), rg.store(buffer(0).d, lane);
       meet();
@@ -1049,14 +1093,14 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       return;
     }
     DeltaRows<E, C, DK, THREADS> rk, rq;
-    DeltaRows<E, C, DV, THREADS> rdo, rv, re[M::TERMS];
+    DeltaRows<E, C, DV, THREADS> rdo, rv, rx[M::TERMS];
     rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, htid);
     rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, htid);
     rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + min(c0, p.dv), a.dos[1], min(max(p.dv - c0, 0), DV), p.vec, htid);
     if constexpr (!RUN) {
       rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, htid);
 #pragma unroll
-      for (int t = 0; t < M::TERMS; ++t) re[t].init((t ? a.e_low : a.e) + (int64_t)bh * a.chunks * CK * DV, DV, DV, true, htid);
+      for (int t = 0; t < M::TERMS; ++t) rx[t].init((t ? a.x_low : a.x) + (int64_t)bh * a.chunks * CK * DV, DV, DV, true, htid);
     }
     auto fetch = [&](int c) {
       const int t0 = (last - c) * C;
@@ -1064,7 +1108,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       if constexpr (!RUN) {
         rv.load(t0, L - t0);
 #pragma unroll
-        for (int t = 0; t < M::TERMS; ++t) re[t].load(t0, L - t0);
+        for (int t = 0; t < M::TERMS; ++t) rx[t].load(t0, L - t0);
       }
     };
     auto stage = [&](int c) {
@@ -1073,7 +1117,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       if constexpr (!RUN) {
         rv.store(x.v);
 #pragma unroll
-        for (int t = 0; t < M::TERMS; ++t) re[t].store(x.e + t * C * LDV);
+        for (int t = 0; t < M::TERMS; ++t) rx[t].store(x.x + t * C * LDV);
       }
     };
     auto setup = [&](int c) {
@@ -1085,7 +1129,8 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         for (int t = 0; t < TERMS; ++t)
           *reinterpret_cast<quad_t<E>*>(x.scores + (tile * TERMS + t) * S::TILE_P + lo * LDP + 4 * hi) = terms.t[t];
       };
-      if (helper == 1) delta_setup<E, S, DK, true, false, true>(x.d, x.inv, x.k, x.q, p.scale, lane, put);
+      auto own = [&](int i, float v) { x.own[i] = v; };
+      if (helper == 1) delta_setup<E, S, DK, true, false, EARLIER_SCORES>(x.d, x.inv, x.k, x.q, p.scale, lane, put, own);
     };
     E* yrow = a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv);
     auto results = [&](int c) {  // of a block that the walkers have left
@@ -1157,23 +1202,27 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
       }
     }
     const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
-    f32x4 du[NB];
+    f32x4 du[NB], kr[NB];
     quad_t<E> g[NB];
     meet();
-    delta_reverse_solve<E, S, KA>(x.d, x.inv, x.scores, x.k, x.d_o, s, g, du, col0, lane);
+    delta_reverse_solve<E, S, KA, !RUN>(x.d, x.inv, x.own, x.scores, x.k, x.d_o, s, g, du, kr, col0, lane);
     if constexpr (!RUN) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const f32x4 y = lds_f4(x.d.beta + 16 * i + 4 * hi) * du[i];
-        f32x4 et = to_f32(lds_quad_t(x.e, LDV, 16 * i, col0, lane));
-        // (by one term dbeta is 2.4e-3 off)
-        if constexpr (M::TERMS == 2) et += to_f32(lds_quad_t(x.e + C * LDV, LDV, 16 * i, col0, lane));
-        const f32x4 pe = du[i] * et;
-        const f32x4 pv = y * to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane));
+        const f32x4 beta = lds_f4(x.d.beta + 16 * i + 4 * hi), y = beta * du[i];
+        const quad_t<E> high = lds_quad_t(x.x, LDV, 16 * i, col0, lane);
+        f32x4 held = to_f32(high);
+        if constexpr (M::TERMS == 2) {
+          const quad_t<E> low = lds_quad_t(x.x + C * LDV, LDV, 16 * i, col0, lane);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) held[r] = joined(high[r], low[r]);
+        }
+        const f32x4 e = to_f32(lds_quad_t(x.v, LDV, 16 * i, col0, lane)) - held;
+        const f32x4 pe = du[i] * e, pz = y * held + beta * e * kr[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = 16 * i + 4 * hi + r;
-          const float sb = row16_sum(pe[r]), sz = row16_sum(pv[r]);
+          const float sb = row16_sum(pe[r]), sz = row16_sum(pz[r]);
           if (lo == 0) x.beta[wave * C + t] = sb, x.z[wave * C + t] = sz;
           x.d_o[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
           if (a.y_part && t < n && col0 + lo < p.dv)
@@ -1211,10 +1260,24 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   }
 }
 
+// sum over the lanes behind this one, or before it
+template <bool BEHIND>
+__device__ inline double other_lanes(double v, int lane) {
+  double sum = v;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const double u = BEHIND ? __shfl_down(sum, i, 64) : __shfl_up(sum, i, 64);
+    if (BEHIND ? lane + i < 64 : lane >= i) sum += u;
+  }
+  const double u = BEHIND ? __shfl_down(sum, 1, 64) : __shfl_up(sum, 1, 64);
+  return (BEHIND ? lane < 63 : lane > 0) ? u : 0.0;
+}
+
 // log_decay's gradient: a wave a stretch, four steps a lane; in 64 bits, for the terms are.  It is known at both
-// ends of a stretch from the states there.  What the terms' errors leave between the two is shared out by the
-// terms' squares, as independent errors of their size would be (more than 1e-6 off for one of 1771 shapes in place
-// of six of 1482; 3e-7 to 7e-7 as a rule).
+// ends of a stretch from the states there, and the terms w - z lead from step to step; each of these numbers is
+// off by some of its own last bits.  So the two sums, from either end, are weighted by the squares of what
+// has gone into the other one: a large end (a final state's gradient behind decays that leave nothing of it)
+// spoils nothing beyond its own step.
 template <typename E>
 __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int rows, int walkers) {
   const DeltaArgs<E>& p = a.f;
@@ -1224,38 +1287,36 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
   const int L = delta_length(p, b);
   const int t0 = seg * kDeltaSeg + lane * 4;
   const int64_t at = (int64_t)bh * rows + t0;
-  double x[4], y[4], sum = 0.0, squares = 0.0;
+  double term[4], square[4], sum = 0.0, squares = 0.0;
 #pragma unroll
-  for (int i = 3; i >= 0; --i) {
-    if (t0 + i < L) {
-      const double w = a.w[at + i], z = a.z[at + i];
-      sum += w - z, squares += w * w + z * z;
-    }
-    x[i] = sum, y[i] = squares;
+  for (int i = 0; i < 4; ++i) {
+    const double w = t0 + i < L ? a.w[at + i] : 0.0, z = t0 + i < L ? a.z[at + i] : 0.0;
+    term[i] = w - z, square[i] = w * w + z * z;
+    sum += term[i], squares += square[i];
   }
-  double later = sum, more = squares;  // this lane's and the later ones' terms
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    const double v = __shfl_down(later, i, 64), u = __shfl_down(more, i, 64);
-    if (lane + i < 64) later += v, more += u;
-  }
-  double after = 0.0, share = 0.0;
+  double start = 0.0, end = 0.0;
   if (seg * kDeltaSeg < L) {
     const float* dot = a.dot + (int64_t)bh * a.stretches + seg;
-    double start = 0.0;
+    end = dot[0];
     if (seg > 0) start = dot[-1];
     else for (int i = 0; i < walkers; ++i) start += (double)a.dot0[bh * (int64_t)8 + i];
-    after = dot[0];
-    const double all = __shfl(more, 0, 64);
-    if (all > 0.0) share = (start - after - __shfl(later, 0, 64)) / all;
   }
-  later -= sum, more -= squares;
+  // from the start to before this lane's steps, and from the end to behind them
+  double from_start = start - other_lanes<false>(sum, lane), weight_end = start * start + other_lanes<false>(squares, lane);
+  double from_end[4], weight_start[4], later = end + other_lanes<true>(sum, lane);
+  double more = end * end + other_lanes<true>(squares, lane);
+#pragma unroll
+  for (int i = 3; i >= 0; --i) from_end[i] = later += term[i], weight_start[i] = more += square[i];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = t0 + i;
     if (t >= p.T) break;
-    const bool decays = t < L && !(p.g[b * p.gs[0] + t * p.gs[1] + h * p.gs[2]] < kNoDecay);
-    a.dg[((int64_t)b * p.T + t) * p.H + h] = decays ? (float)(after + (later + x[i]) + share * (more + y[i])) : 0.0f;
+    const double all = weight_start[i] + weight_end;
+    const double dg = all > 0.0 ? (from_start * weight_start[i] + from_end[i] * weight_end) / all : from_end[i];
+    // it has a_t as a factor: zero where that is below the least normal number
+    const bool decays = t < L && !(__expf(p.g[b * p.gs[0] + t * p.gs[1] + h * p.gs[2]]) < 0x1p-126f);
+    a.dg[((int64_t)b * p.T + t) * p.H + h] = decays ? (float)dg : 0.0f;
+    from_start -= term[i], weight_end += square[i];
   }
 }
 
@@ -1327,12 +1388,13 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
     }
   };
   {
-    DeltaRows<E, C, DV, THREADS> rdo, re[TERMS], ry;
+    DeltaRows<E, C, DV, THREADS> rdo, re[TERMS], ry, rv;
     rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
     ry.init(a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv), a.ys[1], a.y_width, a.y_part || p.vec, tid);
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t) re[t].init((t ? a.e_low : a.e) + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid), re[t].load(t0, n);
-    rdo.load(t0, n), ry.load(t0, n);
+    for (int t = 0; t < TERMS; ++t) re[t].init((t ? a.x_low : a.x) + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid), re[t].load(t0, n);
+    rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
+    rv.load(t0, n), rdo.load(t0, n), ry.load(t0, n);
     state_load(0);
     if (wave == 0) {
       const bool live = lane < n;
@@ -1349,6 +1411,17 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
       if (lane < C) G[lane] = sum, from[lane] = __expf((float)sum), to[lane] = __expf((float)(end - sum)), beta[lane] = bt;
     }
     rdo.store(tdo), ry.store(ty);
+#pragma unroll
+    for (int i = 0; i < rv.N; ++i)
+#pragma unroll
+      for (int c = 0; c < P; ++c) {  // e = v - x
+        if constexpr (TERMS == 2) {
+          const float e = (float)rv.r[i][c] - joined(re[0].r[i][c], re[1].r[i][c]);
+          re[0].r[i][c] = (bf16)e, re[1].r[i][c] = (bf16)(e - (float)re[0].r[i][c]);
+        } else {
+          re[0].r[i][c] = rv.r[i][c] - re[0].r[i][c];
+        }
+      }
 #pragma unroll
     for (int t = 0; t < TERMS; ++t) re[t].store(te + t * C * LDV);
     state_store();

@@ -126,7 +126,10 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     recurrence is stable for beta_t |k_t|^2 from 0 to 2: keys of unit length with beta from 0 to 1 are
     usual.  An infinite or NaN value at a live step spoils what it has a part in: no earlier step's output,
     other head or problem.  scale is dk^-1/2 where None.  Returns o (B, T, H, dv) and the state after
-    each history's last step (float32)."""
+    each history's last step (float32).
+
+    log_decay's gradient has the decay as a factor: it is zero where exp(log_decay) is below 2^-126, and off by
+    last bits of the gradients within 256 steps of it."""
     sfx, scale = _check_delta(q, k, v, log_decay, beta, scale, False)
     B, _, H = log_decay.shape
     if state is not None:
