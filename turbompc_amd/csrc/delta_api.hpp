@@ -157,7 +157,7 @@ int forward_impl(hipStream_t st, const tmpc_delta_attention* x, void* o, float* 
 // The backward pass' arrays in the workspace, one after another.
 struct BackwardPlan {
   int chunks, stretches, DK, DV;
-  size_t x, x_low, s, r, w, z, s_seg, dot, dot0, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
+  size_t x, x_low, y_low, s, s_low, r, r_low, w, z, s_seg, dot, dot0, y, y_part, q_part, k_part, run_state, run_map, run_grad, bytes;
   RunPlan runs;
 };
 template <typename E>
@@ -174,8 +174,11 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
     return at;
   };
   p.x = take(rows * p.DV * sizeof(E));
-  if (sizeof(E) == 2) p.x_low = take(rows * p.DV * sizeof(E));
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
+  if (sizeof(E) == 2) {
+    p.x_low = take(rows * p.DV * sizeof(E)), p.y_low = take(rows * p.DV * sizeof(E));
+    p.s_low = take(bh * p.chunks * state * sizeof(E)), p.r_low = take(bh * p.chunks * state * sizeof(E));
+  }
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
   p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
   if (x->T > 0) p.dot0 = take(bh * 8 * sizeof(float));
@@ -205,6 +208,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   std::copy_n(dos, 3, a.dos);
   a.chunks = w.chunks, a.stretches = w.stretches;
   a.x = (E*)(base + w.x), a.x_low = (E*)(base + w.x_low), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
+  a.y_low = (E*)(base + w.y_low), a.s_low = (E*)(base + w.s_low), a.r_low = (E*)(base + w.r_low);
   a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot), a.dot0 = (float*)(base + w.dot0);
   if (x->Hv != x->H) {
     a.y = (E*)(base + w.y), a.y_part = (float*)(base + w.y_part), a.y_width = w.DV;

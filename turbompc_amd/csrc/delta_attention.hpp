@@ -549,7 +549,8 @@ struct DeltaBwdArgs {
   const float* d_out;  // (B, H, dk, dv) or NULL
   int chunks, stretches;  // of T
   E *x, *x_low;        // (B H, chunks C, DV): x_t, fp32 (in bf16 its upper and its lower halves)
-  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends
+  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends,
+  E *s_low, *r_low;    // in bf16 with what a rounding leaves of them
   float *w, *z;        // (B H, chunks C): the parts of dg_t - dg_{t+1}
   float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
   float* dot;          // (B H, stretches): <R, S> there
@@ -557,6 +558,7 @@ struct DeltaBwdArgs {
   E* y;                // as e, or dv's output (B, T, H, dv)
   int64_t ys[2];       // its strides of (b h) and step, from b and h where it is the output
   int y_width;
+  E* y_low;            // in bf16 what y's rounding leaves, laid out as x
   float* y_part;       // (B, T, H, dv) or NULL
   E* dbeta;            // (B, T, H)
   float* dg;           // (B, T, H)
@@ -576,18 +578,21 @@ __device__ inline float row16_sum(float v) {
   return v;
 }
 
-// The wave's 16 columns of a state, rounded, as rows of a (DV, DK) matrix.
+// The wave's 16 columns of a state as rows of a (DV, DK) matrix, in bf16 by two terms.
 template <typename E, int DK, int KA>
-__device__ inline void store_columns(E* dst, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
+__device__ inline void store_columns(E* dst, E* low, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
 #pragma unroll
-  for (int m = 0; m < KA; ++m)
-    *reinterpret_cast<quad_t<E>*>(dst + (col0 + lo) * DK + 16 * m + 4 * hi) = to_quad<E>(s[m][0]);
+  for (int m = 0; m < KA; ++m) {
+    const int at = (col0 + lo) * DK + 16 * m + 4 * hi;
+    const quad_t<E> top = to_quad<E>(s[m][0]);
+    *reinterpret_cast<quad_t<E>*>(dst + at) = top;
+    if constexpr (sizeof(E) == 2) *reinterpret_cast<quad_t<E>*>(low + at) = to_quad<E>(s[m][0] - to_f32(top));
+  }
 }
 
 // Rows of a tile in LDS to memory: `n` of them, row t at dst + t pitch.
 template <typename R, typename E>
 __device__ inline void copy_out(const R& map, const E* tile, E* dst, int64_t pitch, int n, int width) {
-  constexpr int P = Elem<E>::PIECE;
   if (map.row >= R::RS) return;
 #pragma unroll
   for (int i = 0; i < R::N; ++i) {
@@ -595,7 +600,6 @@ __device__ inline void copy_out(const R& map, const E* tile, E* dst, int64_t pit
     if (row < n && map.c < width)
       store_piece(dst + row * pitch, map.c, width, *reinterpret_cast<const piece_t<E>*>(tile + row * R::LD + map.c));
   }
-  (void)P;
 }
 
 // A long history of few heads does not fill the chip: it is cut into runs.  A run is a linear map of the
@@ -764,8 +768,10 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
   for (int c = 0; c < blocks; ++c) {
     const int t0 = begin + c * C, n = min(C, L - t0);
     const Buffer x = buffer(c);
-    if (M::DO && t0 % CK == 0)
-      store_columns<E, DK>(a.s + ((int64_t)bh * a.chunks + t0 / CK) * DK * DV, s, wave * 16, lane & 15, lane >> 4);
+    if (M::DO && t0 % CK == 0) {
+      const int64_t at = ((int64_t)bh * a.chunks + t0 / CK) * DK * DV;
+      store_columns<E, DK>(a.s + at, a.s_low + at, s, wave * 16, lane & 15, lane >> 4);
+    }
     const __amdgpu_buffer_rsrc_t rs = buffer_at(MODE == WALK_OUT ? p.o + obase + t0 * orow : nullptr);
     const int lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, col0 = wave * 16;
     f32x4 o[NB], v[NB], held[NB], u[NB];  // held: - a_t k_t S_{t-1}, where the outputs alone are made v_t less that
@@ -1138,6 +1144,7 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
         const Buffer x = buffer(c);
         const int t0 = (last - c) * C, n = min(C, L - t0);
         copy_out(rdo, x.d_o, yrow + t0 * a.ys[1], a.ys[1], n, a.y_width);
+        if constexpr (sizeof(E) == 2) copy_out(rv, x.v, a.y_low + ((int64_t)bh * a.chunks * CK + t0) * DV, DV, n, DV);
         if (htid < n) {
           float sb = 0.0f, sz = 0.0f;
 #pragma unroll
@@ -1186,7 +1193,10 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
     const int t0 = (last - c) * C, n = min(C, L - t0);
     const Buffer x = buffer(c);
     if constexpr (!RUN) {
-      if (ends(t0, CK)) store_columns<E, DK>(a.r + ((int64_t)bh * a.chunks + t0 / CK) * DK * DV, s, wave * 16, lane & 15, lane >> 4);
+      if (ends(t0, CK)) {
+        const int64_t at = ((int64_t)bh * a.chunks + t0 / CK) * DK * DV;
+        store_columns<E, DK>(a.r + at, a.r_low + at, s, wave * 16, lane & 15, lane >> 4);
+      }
       if (ends(t0, kDeltaSeg)) {
         const f32x4* src = reinterpret_cast<const f32x4*>(a.s_seg + ((int64_t)bh * a.stretches + t0 / kDeltaSeg) * DK * DV) + wave * KA * 64 + lane;
         float dot = 0.0f;
@@ -1224,7 +1234,10 @@ __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK
           const int t = 16 * i + 4 * hi + r;
           const float sb = row16_sum(pe[r]), sz = row16_sum(pz[r]);
           if (lo == 0) x.beta[wave * C + t] = sb, x.z[wave * C + t] = sz;
-          x.d_o[t * LDV + col0 + lo] = (E)y[r];  // these columns of dO are this wave's alone and have been read
+          // these columns of dO and V are this wave's alone and have been read
+          const E top = (E)y[r];
+          x.d_o[t * LDV + col0 + lo] = top;
+          if constexpr (sizeof(E) == 2) x.v[t * LDV + col0 + lo] = (E)(y[r] - (float)top);
           if (a.y_part && t < n && col0 + lo < p.dv)
             a.y_part[(((int64_t)b * p.T + t0 + t) * p.H + h) * p.dv + col0 + lo] = y[r];
         }
@@ -1322,31 +1335,35 @@ __global__ __launch_bounds__(64) void delta_dgate_kernel(DeltaBwdArgs<E> a, int 
 
 template <typename E, int DK, int DV>
 struct DeltaDqkShape {
-  static constexpr int C = AttnTile<E>::C, CT = C / 16;
-  // waves that share 16 rows' columns, and tiles of each
-  static constexpr int WC = sizeof(E) == 2 ? (DK == 128 || DV == 128 ? 2 : 1) : DK == 32 ? 2 : 4, KT = DK / 16 / WC;
-  static constexpr int THREADS = 64 * CT * WC, HALF = DV < 64 ? DV : 64;  // values of a state in LDS at a time
-  static constexpr int LDK = DK + AttnTile<E>::PAD, LDV = DV + AttnTile<E>::PAD, TERMS = sizeof(E) == 2 ? 2 : 1;
-  // rows of e (by its terms), dO and y and a state's half; then rows of K and Q in their place
-  static constexpr size_t FIRST = sizeof(E) * ((2 + TERMS) * C * LDV + HALF * LDK), SECOND = sizeof(E) * 2 * C * LDK;
+  static constexpr int C = AttnTile<E>::C, CT = C / 16, PAD = AttnTile<E>::PAD, TERMS = sizeof(E) == 2 ? 2 : 1;
+  static constexpr int WC = sizeof(E) == 2 || DK == 32 ? 2 : 4, KT = DK / 16 / WC;  // waves that share 16 rows' columns, tiles of each
+  static constexpr int WAVES = CT * WC, THREADS = 64 * WAVES;
+  static constexpr int HV = DV < 64 ? DV : 64;                                // values in LDS at a time
+  static constexpr int SV = sizeof(E) == 2 && DK == 128 && HV == 64 ? 32 : HV;  // of these, of a state
+  static constexpr int LDK = DK + PAD, LDV = HV + PAD, LDC = C + PAD;
+  // tiles of the scores on and below the diagonal, and those right of it that a pair of tiles begins with
+  static constexpr int LOWER = CT * (CT + 1) / 2, TILES = LOWER + CT / 2, MINE = (TILES + WAVES - 1) / WAVES;
+  // rows of dO, y and e (these by their terms) and a state's part; then the scores by theirs, K and Q in their place
+  static constexpr size_t FIRST = sizeof(E) * ((1 + 2 * TERMS) * C * LDV + TERMS * SV * LDK);
+  static constexpr size_t SECOND = sizeof(E) * (2 * TERMS * C * LDC + 2 * C * LDK);
   static constexpr size_t LDS = 8 * C + 4 * 3 * C + (FIRST > SECOND ? FIRST : SECOND);
-  static constexpr int FIT = 160 * 1024 / LDS * THREADS / 256, MOST = KT >= 4 ? 3 : 4, WAVES_PER_SIMD = FIT > MOST ? MOST : FIT;  // by LDS and registers
+  static constexpr int FIT = 160 * 1024 / LDS * THREADS / 256, WAVES_PER_SIMD = FIT > 4 ? 4 : FIT;  // by LDS and registers
 };
 
-// dq and dk of a chunk.  beta_j stays out of the operands (u_j = beta_j e_j), and in bf16 e and the scores M and N
-// enter by two terms: y and the states are what is rounded, once each.  (With e by one term dk is 2.7e-3 off
-// where a rounding is 1.66e-3, with it by two 2.1e-3.)
-// Every chunk is a workgroup of its own, so this is bound by what a CU holds: LDS for the rows by their terms
-// and half of a state at a time, registers for the scores as operands.  64 problems of 1024 steps, 8 heads
-// of 64 / 64: 153 to 174 us; 2048 ragged histories of 101, 4 heads of 64 / 128: 576 us for 1.24 GB.
+// dq and dk of a chunk.  beta_j stays out of the operands (u_j = beta_j e_j).  In bf16 the states, y, e and the scores M
+// and N enter by two terms, so that dq and dk are off by their own rounding (1.66e-3; with y and the states by one
+// term 2.1e-3 and 2.3e-3).  The waves share the scores out and exchange them in LDS, half of the values' columns at a
+// time where they are 128: every wave for itself needed more registers than there are.  Bound by memory
+// where heads are 64 wide: 64 problems of 1024 steps, 8 heads of 64 / 64, 195 us for 0.94 GB, of which the second terms
+// are 0.20; 2048 ragged histories of 101, 4 heads of 64 / 128, 512 us for 1.5 GB; 256 of 41, 4 of 32 / 49, fp32, 31 us.
 template <typename E, int DK, int DV>
 __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   using S = DeltaDqkShape<E, DK, DV>;
-  constexpr int C = S::C, CT = S::CT, WC = S::WC, KT = S::KT, THREADS = S::THREADS, HALF = S::HALF, LDK = S::LDK, LDV = S::LDV;
-  constexpr int VA = DV / 16, HA = HALF / 16, P = Elem<E>::PIECE, TERMS = S::TERMS;
+  constexpr int C = S::C, CT = S::CT, WC = S::WC, KT = S::KT, THREADS = S::THREADS, HV = S::HV, SV = S::SV;
+  constexpr int LDK = S::LDK, LDV = S::LDV, LDC = S::LDC, P = Elem<E>::PIECE, TERMS = S::TERMS;
   extern __shared__ __align__(16) char smem[];
   const DeltaArgs<E>& p = a.f;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lo = lane & 15, hi = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lo = lane & 15, hi = lane >> 4;
   const int block = (int)flat_block(), bh = block / a.chunks, chunk = block - bh * a.chunks, b = bh / p.H, h = bh - b * p.H;
   if (b >= p.B) return;
   const int L = delta_length(p, b);
@@ -1364,186 +1381,234 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
   float* from = beta + C;
   float* to = from + C;
   E* tdo = reinterpret_cast<E*>(to + C);
-  E* ty = tdo + C * LDV;
-  E* te = ty + C * LDV;               // TERMS of them
-  E* ts = te + TERMS * C * LDV;       // half of a state or of its gradient, (HALF, DK)
-  E* tk = reinterpret_cast<E*>(to + C);
+  E* ty = tdo + C * LDV;              // TERMS of them
+  E* te = ty + TERMS * C * LDV;       // and of these
+  E* ts = te + TERMS * C * LDV;       // a state's or its gradient's, (SV, DK) each
+  E* tm = reinterpret_cast<E*>(to + C);  // M by its terms, -N by its terms
+  E* tk = tm + 2 * TERMS * C * LDC;
   E* tq = tk + C * LDK;
 
-  // the states' halves, rows of whole pieces, on their way to LDS: S's and R's first, then the second ones
-  constexpr int SP = (HALF * DK / P + THREADS - 1) / THREADS, PHASES = 2 * DV / HALF;
-  piece_t<E> sp[SP];
-  const int64_t state = ((int64_t)bh * a.chunks + chunk) * DK * DV;
-  auto state_load = [&](int phase) {
-    const E* src = (phase & 1 ? a.r : a.s) + state + phase / 2 * HALF * DK;
+  DeltaRows<E, C, HV, THREADS> rdo, rv, ry[TERMS], rx[TERMS];
+  const int64_t rows = ((int64_t)bh * a.chunks * C + t0) * DV;
+  auto rows_load = [&](int v0) {  // columns v0 ... of the values
+    const int left = min(max(p.dv - v0, 0), HV), from0 = min(v0, p.dv);
+    rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2] + from0, a.dos[1], left, p.vec, tid);
+    rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2] + from0, p.vs[1], left, p.vec, tid);
+    if (a.y_part) ry[0].init(a.y + bh * a.ys[0] + v0, a.ys[1], HV, true, tid);
+    else ry[0].init(a.y + b * a.ys[0] + (int64_t)h * p.dv + from0, a.ys[1], left, p.vec, tid);
+    rdo.load(t0, n), rv.load(t0, n), ry[0].load(t0, n);
 #pragma unroll
-    for (int i = 0; i < SP; ++i)
-      if ((i * THREADS + tid) * P < HALF * DK) sp[i] = *reinterpret_cast<const piece_t<E>*>(src + (i * THREADS + tid) * P);
+    for (int t = 0; t < TERMS; ++t) rx[t].init((t ? a.x_low : a.x) + rows + v0, DV, HV, true, tid), rx[t].load(0, n);
+    if constexpr (TERMS == 2) ry[1].init(a.y_low + rows + v0, DV, HV, true, tid), ry[1].load(0, n);
   };
-  auto state_store = [&]() {
-#pragma unroll
-    for (int i = 0; i < SP; ++i) {
-      const int e = (i * THREADS + tid) * P;
-      if (e < HALF * DK) *reinterpret_cast<piece_t<E>*>(ts + e / DK * LDK + e % DK) = sp[i];
-    }
-  };
-  {
-    DeltaRows<E, C, DV, THREADS> rdo, re[TERMS], ry, rv;
-    rdo.init(a.d_o + b * a.dos[0] + h * a.dos[2], a.dos[1], p.dv, p.vec, tid);
-    ry.init(a.y + (a.y_part ? bh * a.ys[0] : b * a.ys[0] + (int64_t)h * p.dv), a.ys[1], a.y_width, a.y_part || p.vec, tid);
-#pragma unroll
-    for (int t = 0; t < TERMS; ++t) re[t].init((t ? a.x_low : a.x) + (int64_t)bh * a.chunks * C * DV, DV, DV, true, tid), re[t].load(t0, n);
-    rv.init(p.v + b * p.vs[0] + (h / p.gv) * p.vs[2], p.vs[1], p.dv, p.vec, tid);
-    rv.load(t0, n), rdo.load(t0, n), ry.load(t0, n);
-    state_load(0);
-    if (wave == 0) {
-      const bool live = lane < n;
-      float g = live ? p.g[b * p.gs[0] + (t0 + lane) * p.gs[1] + h * p.gs[2]] : 0.0f;
-      const float bt = live ? (float)p.beta[b * p.bs[0] + (t0 + lane) * p.bs[1] + h * p.bs[2]] : 0.0f;
-      g = g < kNoDecay ? kNoDecay : g;
-      double sum = (double)g;
-#pragma unroll
-      for (int i = 1; i < 64; i <<= 1) {
-        const double v = __shfl_up(sum, i, 64);
-        if (lane >= i) sum += v;
-      }
-      const double end = __shfl(sum, 63, 64);
-      if (lane < C) G[lane] = sum, from[lane] = __expf((float)sum), to[lane] = __expf((float)(end - sum)), beta[lane] = bt;
-    }
-    rdo.store(tdo), ry.store(ty);
+  auto rows_store = [&]() {
+    rdo.store(tdo);
 #pragma unroll
     for (int i = 0; i < rv.N; ++i)
 #pragma unroll
       for (int c = 0; c < P; ++c) {  // e = v - x
         if constexpr (TERMS == 2) {
-          const float e = (float)rv.r[i][c] - joined(re[0].r[i][c], re[1].r[i][c]);
-          re[0].r[i][c] = (bf16)e, re[1].r[i][c] = (bf16)(e - (float)re[0].r[i][c]);
+          const float e = (float)rv.r[i][c] - joined(rx[0].r[i][c], rx[1].r[i][c]);
+          rx[0].r[i][c] = (bf16)e, rx[1].r[i][c] = (bf16)(e - (float)rx[0].r[i][c]);
         } else {
-          re[0].r[i][c] = rv.r[i][c] - re[0].r[i][c];
+          rx[0].r[i][c] = rv.r[i][c] - rx[0].r[i][c];
         }
       }
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t) re[t].store(te + t * C * LDV);
-    state_store();
+    for (int t = 0; t < TERMS; ++t) rx[t].store(te + t * C * LDV), ry[t].store(ty + t * C * LDV);
+  };
+  // SV rows of a state (by its terms) on their way to LDS: S's, then R's, then the next ones
+  constexpr int SP = (SV * DK / P + THREADS - 1) / THREADS, PARTS = 2 * DV / SV;
+  piece_t<E> sp[TERMS][SP];
+  const int64_t state = ((int64_t)bh * a.chunks + chunk) * DK * DV;
+  auto state_load = [&](int part) {
+    const int64_t at = state + part / 2 * SV * DK;
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      const E* src = (part & 1 ? t ? a.r_low : a.r : t ? a.s_low : a.s) + at;
+#pragma unroll
+      for (int i = 0; i < SP; ++i)
+        if ((i * THREADS + tid) * P < SV * DK) sp[t][i] = *reinterpret_cast<const piece_t<E>*>(src + (i * THREADS + tid) * P);
+    }
+  };
+  auto state_store = [&]() {
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+      for (int i = 0; i < SP; ++i) {
+        const int e = (i * THREADS + tid) * P;
+        if (e < SV * DK) *reinterpret_cast<piece_t<E>*>(ts + t * SV * LDK + e / DK * LDK + e % DK) = sp[t][i];
+      }
+  };
+  rows_load(0);
+  state_load(0);
+  if (wave == 0) {
+    const bool live = lane < n;
+    float g = live ? p.g[b * p.gs[0] + (t0 + lane) * p.gs[1] + h * p.gs[2]] : 0.0f;
+    const float bt = live ? (float)p.beta[b * p.bs[0] + (t0 + lane) * p.bs[1] + h * p.bs[2]] : 0.0f;
+    g = g < kNoDecay ? kNoDecay : g;
+    double sum = (double)g;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+      const double v = __shfl_up(sum, i, 64);
+      if (lane >= i) sum += v;
+    }
+    const double end = __shfl(sum, 63, 64);
+    if (lane < C) G[lane] = sum, from[lane] = __expf((float)sum), to[lane] = __expf((float)(end - sum)), beta[lane] = bt;
   }
-  __syncthreads();
-  state_load(1);
 
   const int it = wave / WC, kt0 = (wave % WC) * KT, row = 16 * it + lo;
   // R's part is scaled by exp(G_end - G_j) beta_j, S's by -exp(G_j): kept apart until the sums are whole
-  f32x4 aq[KT], as[KT], ar[KT];
+  f32x4 aq[KT], as[KT], ar[KT], s1[S::MINE], s2[S::MINE];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) aq[kt] = as[kt] = ar[kt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int phase = 0; phase < PHASES; ++phase) {
-    if (phase > 0) {
-      __syncthreads();
+  for (int k = 0; k < S::MINE; ++k) s1[k] = s2[k] = f32x4{0, 0, 0, 0};
+  // this wave's tiles of the scores: rows 16 ti, columns 16 tj; not live: all zeros
+  int ti[S::MINE], tj[S::MINE];
+  bool live[S::MINE];
+#pragma unroll
+  for (int k = 0; k < S::MINE; ++k) {
+    const int t = wave + k * S::WAVES;
+    ti[k] = t >= S::LOWER ? 2 * (t - S::LOWER) : t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+    tj[k] = t >= S::LOWER ? ti[k] + 1 : t - tri(ti[k], 0);
+    live[k] = t < S::LOWER && 16 * ti[k] < n;
+  }
+  DeltaRows<E, C, DK, THREADS> rk, rq;
+  // two quads of each of an operand's terms
+  auto two = [&](const E* z, int ld, int r0, int c0, int lane, quad_t<E> (&x)[2]) {
+    x[0] = lds_quad(z, ld, r0, c0, lane), x[1] = lds_quad(z, ld, r0, c0 + 16, lane);
+  };
+#pragma unroll 1
+  for (int part = 0; part < PARTS; part += 2 * HV / SV) {  // HV values
+    if (part > 0) rows_load(part / 2 * SV);  // (not ahead of their use: held in registers they cost 566 us for 512)
+    __syncthreads();
+    rows_store();
+#pragma unroll
+    for (int sub = 0; sub < 2 * HV / SV; ++sub) {
+      if (sub > 0) __syncthreads();
       state_store();
       __syncthreads();
-      if (phase + 1 < PHASES) state_load(phase + 1);
-    }
-    if (16 * it >= n) continue;
-    const int lane = here(tid & 63);
+      if (part + sub + 1 < PARTS) state_load(part + sub + 1);
+      if (16 * it >= n) continue;
+      const int lane = here(tid & 63);
 #pragma unroll
-    for (int v = 0; v < HA; v += 2) {
-      const int col = phase / 2 * HALF + 16 * v;
-      quad_t<E> x[2][2];  // this wave's rows of dO and y, or of e's terms
+      for (int v = 0; v < SV; v += 32) {
+        const int col = sub / 2 * SV + v;
+        quad_t<E> x[3][2];  // this wave's rows of dO and y (by its terms), or of e's terms
+        if (sub & 1) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if ((phase & 1) && t == TERMS) continue;
-        const E* z = phase & 1 ? te + t * C * LDV : t ? ty : tdo;
-        x[t][0] = lds_quad(z, LDV, 16 * it, col, lane), x[t][1] = lds_quad(z, LDV, 16 * it, col + 16, lane);
-      }
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const quad_t<E> s0 = lds_quad_t(ts, LDK, 16 * v, 16 * (kt0 + kt), lane);
-        const quad_t<E> s1 = lds_quad_t(ts, LDK, 16 * v + 16, 16 * (kt0 + kt), lane);
-        if (phase & 1) {
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t) ar[kt] = mma2(s0, s1, x[t][0], x[t][1], ar[kt]);
+          for (int t = 0; t < TERMS; ++t) two(te + t * C * LDV, LDV, 16 * it, col, lane, x[t]);
         } else {
-          aq[kt] = mma2(s0, s1, x[0][0], x[0][1], aq[kt]);
-          as[kt] = mma2(s0, s1, x[1][0], x[1][1], as[kt]);
+          two(tdo, LDV, 16 * it, col, lane, x[0]);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) two(ty + t * C * LDV, LDV, 16 * it, col, lane, x[1 + t]);
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) {  // the state's first term with all of theirs, the second with their first
+            const quad_t<E> s0 = lds_quad_t(ts + t * SV * LDK, LDK, v, 16 * (kt0 + kt), lane);
+            const quad_t<E> s1 = lds_quad_t(ts + t * SV * LDK, LDK, v + 16, 16 * (kt0 + kt), lane);
+            if (sub & 1) {
+#pragma unroll
+              for (int u = 0; u < (t ? 1 : TERMS); ++u) ar[kt] = mma2(s0, s1, x[u][0], x[u][1], ar[kt]);
+            } else {
+              aq[kt] = mma2(s0, s1, x[0][0], x[0][1], aq[kt]);
+#pragma unroll
+              for (int u = 0; u < (t ? 1 : TERMS); ++u) as[kt] = mma2(s0, s1, x[1 + u][0], x[1 + u][1], as[kt]);
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < S::MINE; ++k) {
+      if (!live[k]) continue;
+      const int lane = here(tid & 63);
+#pragma unroll
+      for (int v = 0; v < HV; v += 32) {
+        quad_t<E> g[2], y[TERMS][2], e[TERMS][2];
+        two(tdo, LDV, 16 * ti[k], v, lane, g);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) two(ty + t * C * LDV, LDV, 16 * ti[k], v, lane, y[t]), two(te + t * C * LDV, LDV, 16 * tj[k], v, lane, e[t]);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          s1[k] = mma2(e[t][0], e[t][1], g[0], g[1], s1[k]);
+#pragma unroll
+          for (int u = 0; u < (t ? 1 : TERMS); ++u) s2[k] = mma2(e[t][0], e[t][1], y[u][0], y[u][1], s2[k]);
         }
       }
     }
   }
+  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
+  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
+  rk.load(t0, n), rq.load(t0, n);
   const float ff = from[row], ft = to[row], bt = beta[row];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) aq[kt] *= p.scale * ff, ar[kt] = ft * bt * ar[kt] - ff * as[kt];
-
-  DeltaRows<E, C, DK, THREADS> rk, rq;
-  rk.init(p.k + b * p.ks[0] + (h / p.gk) * p.ks[2], p.ks[1], p.dk, p.vec, tid);
-  rq.init(p.q + b * p.qs[0] + (h / p.gq) * p.qs[2], p.qs[1], p.dk, p.vec, tid);
-  rk.load(t0, n), rq.load(t0, n);  // in flight while the scores are made
-
-  // the scores of this wave's rows with the chunk's steps, as operands
-  quad_t<E> m[CT][TERMS], mt[CT][TERMS], nn[CT][TERMS];
-  const double mine = G[row];
-#pragma unroll
-  for (int jt = 0; jt < CT; ++jt) {
-    const int j0 = 16 * jt, lane = here(tid & 63), lo = lane & 15, hi = lane >> 4, row = 16 * it + lo;
-    f32x4 s1 = {0, 0, 0, 0}, s2 = {0, 0, 0, 0}, s3 = {0, 0, 0, 0}, s4 = {0, 0, 0, 0};
-    const bool live = 16 * max(it, jt) < n, below = live && jt <= it, above = live && jt >= it;
-#pragma unroll
-    for (int v = 0; v < VA; v += 2) {
-      auto two = [&](const E* z, int r0, quad_t<E>& z0, quad_t<E>& z1) {
-        z0 = lds_quad(z, LDV, r0, 16 * v, lane), z1 = lds_quad(z, LDV, r0, 16 * v + 16, lane);
-      };
-      quad_t<E> e0, e1, g0, g1, y0, y1;
-      if (below) {
-        two(tdo, 16 * it, g0, g1), two(ty, 16 * it, y0, y1);
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
-          two(te + t * C * LDV, j0, e0, e1);
-          s1 = mma2(e0, e1, g0, g1, s1), s2 = mma2(e0, e1, y0, y1, s2);
-        }
-      }
-      if (above) {
-        two(tdo, j0, g0, g1), two(ty, j0, y0, y1);
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
-          two(te + t * C * LDV, 16 * it, e0, e1);
-          s3 = mma2(g0, g1, e0, e1, s3), s4 = mma2(y0, y1, e0, e1, s4);
-        }
-      }
-    }
-    const f32x4 bj = lds_f4(beta + j0 + 4 * hi);
-    f32x4 nsum;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = j0 + 4 * hi + r;
-      const float lag = (float)(mine - G[j]);
-      const float ratio = __expf(j <= row ? lag : -lag);
-      s1[r] = j <= row ? p.scale * ratio * bj[r] * s1[r] : 0.0f;
-      s3[r] = j >= row ? p.scale * ratio * bt * s3[r] : 0.0f;
-      nsum[r] = j < row ? -ratio * bj[r] * s2[r] : j > row ? -ratio * bt * s4[r] : 0.0f;
-    }
-    const Terms<E> a1(s1), a2(s3), a3(nsum);
-    __builtin_amdgcn_sched_barrier(0);  // the next tile's reads not yet: their registers
-#pragma unroll
-    for (int t = 0; t < TERMS; ++t) m[jt][t] = a1.t[t], mt[jt][t] = a2.t[t], nn[jt][t] = a3.t[t];
-  }
   __syncthreads();
+#pragma unroll
+  for (int k = 0; k < S::MINE; ++k) {
+    if (wave + k * S::WAVES >= S::TILES) continue;
+    const int i = 16 * ti[k] + lo, j0 = 16 * tj[k] + 4 * hi;
+    f32x4 m = {0, 0, 0, 0}, nn = {0, 0, 0, 0};
+    if (live[k]) {
+      const f32x4 bj = lds_f4(beta + j0);
+      const double mine = G[i];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = j0 + r;
+        const float ratio = __expf((float)(mine - G[j])) * bj[r];
+        m[r] = j <= i ? p.scale * ratio * s1[k][r] : 0.0f;
+        nn[r] = j < i ? -ratio * s2[k][r] : 0.0f;
+      }
+    }
+    const Terms<E> m_terms(m), n_terms(nn);
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      *reinterpret_cast<quad_t<E>*>(tm + t * C * LDC + i * LDC + j0) = m_terms.t[t];
+      *reinterpret_cast<quad_t<E>*>(tm + (TERMS + t) * C * LDC + i * LDC + j0) = n_terms.t[t];
+    }
+  }
   rk.store(tk), rq.store(tq);
   __syncthreads();
   if (16 * it >= n) return;
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int col = 16 * (kt0 + kt), lane = here(tid & 63);
+  for (int jt = 0; jt < CT; jt += 2) {
+    if (16 * jt >= n) continue;
+    const bool below = jt <= it, above = jt + 1 >= it;  // tiles left of the diagonal, or below it and read across
+    const int lane = here(tid & 63);
+    quad_t<E> m[TERMS][2], mt[TERMS][2], nl[TERMS][2], nt[TERMS][2];
 #pragma unroll
-    for (int jt = 0; jt < CT; jt += 2) {
-      if (16 * jt >= n) continue;
-      const quad_t<E> k0 = lds_quad_t(tk, LDK, 16 * jt, col, lane), k1 = lds_quad_t(tk, LDK, 16 * jt + 16, col, lane);
-      const quad_t<E> q0 = lds_quad_t(tq, LDK, 16 * jt, col, lane), q1 = lds_quad_t(tq, LDK, 16 * jt + 16, col, lane);
+    for (int t = 0; t < TERMS; ++t) {
+      const E *zm = tm + t * C * LDC, *zn = tm + (TERMS + t) * C * LDC;
+      if (below) two(zm, LDC, 16 * it, 16 * jt, lane, m[t]), two(zn, LDC, 16 * it, 16 * jt, lane, nl[t]);
+      if (above) {
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        aq[kt] = mma2(k0, k1, m[jt][t], m[jt + 1][t], aq[kt]);
-        ar[kt] = mma2(k0, k1, nn[jt][t], nn[jt + 1][t], ar[kt]);
-        ar[kt] = mma2(q0, q1, mt[jt][t], mt[jt + 1][t], ar[kt]);
+        for (int u = 0; u < 2; ++u)
+          mt[t][u] = lds_quad_t(zm, LDC, 16 * (jt + u), 16 * it, lane), nt[t][u] = lds_quad_t(zn, LDC, 16 * (jt + u), 16 * it, lane);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int col = 16 * (kt0 + kt);
+      const quad_t<E> k0 = lds_quad_t(tk, LDK, 16 * jt, col, lane), k1 = lds_quad_t(tk, LDK, 16 * jt + 16, col, lane);
+      if (below) {
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          aq[kt] = mma2(k0, k1, m[t][0], m[t][1], aq[kt]);
+          ar[kt] = mma2(k0, k1, nl[t][0], nl[t][1], ar[kt]);
+        }
+      }
+      if (above) {
+        const quad_t<E> q0 = lds_quad_t(tq, LDK, 16 * jt, col, lane), q1 = lds_quad_t(tq, LDK, 16 * jt + 16, col, lane);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          ar[kt] = mma2(k0, k1, nt[t][0], nt[t][1], ar[kt]);
+          ar[kt] = mma2(q0, q1, mt[t][0], mt[t][1], ar[kt]);
+        }
+      }
+    }
   }
   if (row >= n) return;
   const int64_t at = obase + (t0 + row) * orow;
