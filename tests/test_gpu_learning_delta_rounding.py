@@ -3,10 +3,11 @@ else by fewer than two terms.
 
 An error above half a step of the result (2^-8 of it) is at most that of operands with two terms of 8 bits, in units of
 e^2 = 2^-16 of the products' magnitudes.  Rounded to nearest an operand of two terms is off by e^2, cut off by 2 e^2;
-where both of a product have two, that of the second ones is left out: another e^2.  So, at most, a product has
+where both of a product have two, that of the second ones is left out: another e^2, or two where one of them is what a
+cut of the first term left.  So, at most, a product has
   o:   the state or u, cut off, with q exact or with a score, cut off:                        2 + 2 = 4,
   dq:  do, exact, with the state: 1; the score M, cut off, made from e and do: 2 + 1 =            3,
-  dk:  e with the state's gradient, y with the state: 1 + 1 + 1 = 3; M as above; N from y and e: 2 + 1 + 1 + 1 = 5.
+  dk:  e with the state's gradient, y with the state: 1 + 1 + 2 = 4; M as above; N from y and e: 2 + 1 + 1 + 1 = 5.
 The magnitudes are summed up over blocks of 32 steps for o, as they are in bf16, and chunks of 64 for dq and dk."""
 import pytest
 import torch

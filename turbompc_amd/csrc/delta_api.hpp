@@ -177,7 +177,7 @@ BackwardPlan backward_plan(const tmpc_delta_attention* x) {
   p.s = take(bh * p.chunks * state * sizeof(E)), p.r = take(bh * p.chunks * state * sizeof(E));
   if (sizeof(E) == 2) {
     p.x_low = take(rows * p.DV * sizeof(E)), p.y_low = take(rows * p.DV * sizeof(E));
-    p.s_low = take(bh * p.chunks * state * sizeof(E)), p.r_low = take(bh * p.chunks * state * sizeof(E));
+    p.s_low = take(bh * p.chunks * state), p.r_low = take(bh * p.chunks * state);
   }
   p.w = take(rows * sizeof(float)), p.z = take(rows * sizeof(float));
   p.s_seg = take(bh * p.stretches * state * sizeof(float)), p.dot = take(bh * p.stretches * sizeof(float));
@@ -208,7 +208,7 @@ int backward_impl(hipStream_t st, const tmpc_delta_attention* x, const void* d_o
   std::copy_n(dos, 3, a.dos);
   a.chunks = w.chunks, a.stretches = w.stretches;
   a.x = (E*)(base + w.x), a.x_low = (E*)(base + w.x_low), a.s = (E*)(base + w.s), a.r = (E*)(base + w.r), a.w = (float*)(base + w.w);
-  a.y_low = (E*)(base + w.y_low), a.s_low = (E*)(base + w.s_low), a.r_low = (E*)(base + w.r_low);
+  a.y_low = (E*)(base + w.y_low), a.s_low = (uint8_t*)(base + w.s_low), a.r_low = (uint8_t*)(base + w.r_low);
   a.z = (float*)(base + w.z), a.s_seg = (float*)(base + w.s_seg), a.dot = (float*)(base + w.dot), a.dot0 = (float*)(base + w.dot0);
   if (x->Hv != x->H) {
     a.y = (E*)(base + w.y), a.y_part = (float*)(base + w.y_part), a.y_width = w.DV;

@@ -549,8 +549,8 @@ struct DeltaBwdArgs {
   const float* d_out;  // (B, H, dk, dv) or NULL
   int chunks, stretches;  // of T
   E *x, *x_low;        // (B H, chunks C, DV): x_t, fp32 (in bf16 its upper and its lower halves)
-  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends,
-  E *s_low, *r_low;    // in bf16 with what a rounding leaves of them
+  E *s, *r;            // (B H, chunks, DV, DK): the states at the chunks' starts, their gradients at the ends; in
+  uint8_t *s_low, *r_low;  // bf16 the upper halves of fp32, and the next 8 bits here
   float *w, *z;        // (B H, chunks C): the parts of dg_t - dg_{t+1}
   float* s_seg;        // (B H, stretches, the walkers' registers): the states at their ends
   float* dot;          // (B H, stretches): <R, S> there
@@ -578,16 +578,35 @@ __device__ inline float row16_sum(float v) {
   return v;
 }
 
-// The wave's 16 columns of a state as rows of a (DV, DK) matrix, in bf16 by two terms.
+// The wave's 16 columns of a state as rows of a (DV, DK) matrix; in bf16 rounded to 24 bits, which are two terms.
 template <typename E, int DK, int KA>
-__device__ inline void store_columns(E* dst, E* low, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
+__device__ inline void store_columns(E* dst, uint8_t* low, const f32x4 (&s)[KA][1], int col0, int lo, int hi) {
 #pragma unroll
   for (int m = 0; m < KA; ++m) {
     const int at = (col0 + lo) * DK + 16 * m + 4 * hi;
-    const quad_t<E> top = to_quad<E>(s[m][0]);
-    *reinterpret_cast<quad_t<E>*>(dst + at) = top;
-    if constexpr (sizeof(E) == 2) *reinterpret_cast<quad_t<E>*>(low + at) = to_quad<E>(s[m][0] - to_f32(top));
+    if constexpr (sizeof(E) == 4) {
+      *reinterpret_cast<f32x4*>(dst + at) = s[m][0];
+    } else {
+      const u32x4 b = __builtin_bit_cast(u32x4, s[m][0]) + 0x80u;
+      *reinterpret_cast<u32x2*>(dst + at) = u32x2{__builtin_amdgcn_perm(b[1], b[0], 0x07060302u), __builtin_amdgcn_perm(b[3], b[2], 0x07060302u)};
+      const uint32_t b01 = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0501u), b23 = __builtin_amdgcn_perm(b[3], b[2], 0x05010c0cu);
+      *reinterpret_cast<uint32_t*>(low + at) = b01 | b23;
+    }
   }
+}
+// The second terms of 8 elements kept so: exact in bf16.
+__device__ inline bf16x8 second_terms(bf16x8 upper, u32x2 low) {
+  const u32x4 u = __builtin_bit_cast(u32x4, upper);
+  u32x4 r;
+  steps<4>([&](auto n) {
+    constexpr int i = n();
+    const uint32_t b = low[i / 2];
+    const uint32_t x0 = __builtin_amdgcn_perm(u[i], b, 0x0504000cu | (2 * i % 4) << 8), x1 = __builtin_amdgcn_perm(u[i], b, 0x0706000cu | (2 * i % 4 + 1) << 8);
+    const float t0 = __builtin_bit_cast(float, x0) - __builtin_bit_cast(float, u[i] << 16);
+    const float t1 = __builtin_bit_cast(float, x1) - __builtin_bit_cast(float, u[i] & 0xffff0000u);
+    r[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, t1), __builtin_bit_cast(uint32_t, t0), 0x07060302u);
+  });
+  return __builtin_bit_cast(bf16x8, r);
 }
 
 // Rows of a tile in LDS to memory: `n` of them, row t at dst + t pitch.
@@ -1354,8 +1373,9 @@ struct DeltaDqkShape {
 // and N enter by two terms, so that dq and dk are off by their own rounding (1.66e-3; with y and the states by one
 // term 2.1e-3 and 2.3e-3).  The waves share the scores out and exchange them in LDS, half of the values' columns at a
 // time where they are 128: every wave for itself needed more registers than there are.  Bound by memory
-// where heads are 64 wide: 64 problems of 1024 steps, 8 heads of 64 / 64, 195 us for 0.94 GB, of which the second terms
-// are 0.20; 2048 ragged histories of 101, 4 heads of 64 / 128, 512 us for 1.5 GB; 256 of 41, 4 of 32 / 49, fp32, 31 us.
+// where heads are 64 wide: 64 problems of 1024 steps, 8 heads of 64 / 64, 190 to 215 us for 0.87 GB, of which the second
+// terms are 0.13 (the states' as whole bf16 0.20 GB and 198 to 220); 2048 ragged histories of 101, 4 heads of 64 / 128,
+// 504 to 518 us; 256 of 41, 4 of 32 / 49, fp32, 31 us.
 template <typename E, int DK, int DV>
 __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_dqk_kernel(DeltaBwdArgs<E> a) {
   using S = DeltaDqkShape<E, DK, DV>;
@@ -1419,26 +1439,28 @@ __global__ __launch_bounds__((DeltaDqkShape<E, DK, DV>::THREADS), (DeltaDqkShape
   };
   // SV rows of a state (by its terms) on their way to LDS: S's, then R's, then the next ones
   constexpr int SP = (SV * DK / P + THREADS - 1) / THREADS, PARTS = 2 * DV / SV;
-  piece_t<E> sp[TERMS][SP];
+  piece_t<E> sp[SP];
+  [[maybe_unused]] u32x2 sp_low[SP];
   const int64_t state = ((int64_t)bh * a.chunks + chunk) * DK * DV;
   auto state_load = [&](int part) {
     const int64_t at = state + part / 2 * SV * DK;
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t) {
-      const E* src = (part & 1 ? t ? a.r_low : a.r : t ? a.s_low : a.s) + at;
-#pragma unroll
-      for (int i = 0; i < SP; ++i)
-        if ((i * THREADS + tid) * P < SV * DK) sp[t][i] = *reinterpret_cast<const piece_t<E>*>(src + (i * THREADS + tid) * P);
+    for (int i = 0; i < SP; ++i) {
+      const int e = (i * THREADS + tid) * P;
+      if (e >= SV * DK) continue;
+      sp[i] = *reinterpret_cast<const piece_t<E>*>((part & 1 ? a.r : a.s) + at + e);
+      if constexpr (TERMS == 2) sp_low[i] = *reinterpret_cast<const u32x2*>((part & 1 ? a.r_low : a.s_low) + at + e);
     }
   };
   auto state_store = [&]() {
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-      for (int i = 0; i < SP; ++i) {
-        const int e = (i * THREADS + tid) * P;
-        if (e < SV * DK) *reinterpret_cast<piece_t<E>*>(ts + t * SV * LDK + e / DK * LDK + e % DK) = sp[t][i];
-      }
+    for (int i = 0; i < SP; ++i) {
+      const int e = (i * THREADS + tid) * P;
+      if (e >= SV * DK) continue;
+      E* dst = ts + e / DK * LDK + e % DK;
+      *reinterpret_cast<piece_t<E>*>(dst) = sp[i];
+      if constexpr (TERMS == 2) *reinterpret_cast<piece_t<E>*>(dst + SV * LDK) = second_terms(sp[i], sp_low[i]);
+    }
   };
   rows_load(0);
   state_load(0);
