@@ -23,7 +23,7 @@
 // What bounds it: a walker's vector instructions and the latency of its chain (4000 to 4900 cycles a block of
 // 32 steps with two workgroups on a CU, the vector units busy for 70% of them), not memory.  Forward, 64
 // problems of 1024 steps, 8 heads of 64 / 64, bf16, whose bytes take 58 us at a copy's rate: with blocks of 16
-// steps 214 us, of 32 145 us, their inverses by whole rows 137 us, with helpers 105 to 123 us.  The helpers cost where workgroups are
+// steps 214 us, of 32 145 us, their inverses by whole rows 137 us, with helpers 104 to 126 us.  The helpers cost where workgroups are
 // many and short (2048 ragged histories of 101, 4 heads of 64 / 128: 297 us without them, 304 to 333 with; 1024 of
 // 51 in fp32, 4 heads of 33 / 57: 84 and 101), and a second form of every kernel was not worth that.
 //
@@ -1059,8 +1059,8 @@ struct DeltaReverseLds {
   static constexpr size_t bytes = x + (RUN ? 0 : sizeof(E) * TERMS * S::C * S::LDV), all = 2 * bytes;
 };
 
-// The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 163 to 190 us, where the walk for
-// the states takes 143 to 167; both are bound as the forward walk); RUN: what a run adds to the gradient of the
+// The walk backwards (64 problems of 1024 steps, 8 heads of 64 / 64, bf16: 189 to 224 us, where the walk for
+// the states takes 151 to 176; both are bound as the forward walk); RUN: what a run adds to the gradient of the
 // state that it starts from, alone.
 template <typename E, int DK, int DV, bool RUN>
 __global__ __launch_bounds__((DeltaShape<E, DK, DV>::THREADS), (DeltaShape<E, DK, DV>::WAVES_PER_SIMD)) void delta_reverse_kernel(
